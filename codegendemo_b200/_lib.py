@@ -25,6 +25,8 @@ EXPORTED_SYMBOLS = (
     "kcg_load_binary", "kcg_unload", "kcg_device_properties", "kcg_launch_gemm",
     "kcg_launch_gemm_ex", "kcg_launch_gemm_batched", "kcg_launch_gemm_strided", "kcg_softmax_rows", "kcg_softmax_rows_ex",
     "kcg_attention_fwd", "kcg_attention_status",
+    "kcg_rms_norm", "kcg_rms_norm_fp8", "kcg_rms_norm_backward_workspace", "kcg_rms_norm_backward", "kcg_quantize_fp8",
+    "kcg_matmul_fp8", "kcg_matmul_fp8_status",
     "kcg_launch_gemm_allgather", "kcg_peer_alloc", "kcg_peer_open", "kcg_peer_close",
     "kcg_peer_free", "kcg_check_status", "kcg_matmul_host", "kcg_launch_count", "kcg_trim", "kcg_shutdown",
     "kcg_last_error", "kcg_version", "kcg_gemm_bf16_splitk_noalloc",
@@ -95,6 +97,14 @@ class Epilogue(ctypes.Structure):
     """``kcg_epilogue``: C = act(alpha * A.B + beta * C + bias[col])."""
     _fields_ = [("alpha", ctypes.c_float), ("beta", ctypes.c_float), ("bias", ctypes.c_uint64),
                 ("relu", ctypes.c_int32), ("reserved", ctypes.c_int32 * 3)]
+
+
+class Fp8Product(ctypes.Structure):
+    """``kcg_fp8_product``."""
+    _fields_ = [(name, ctypes.c_uint64) for name in ("A", "scale_a", "B", "scale_b", "C", "bias")] + \
+               [(name, ctypes.c_int64) for name in ("lda", "ld_scale_a", "ldb", "ld_scale_b", "ldc")] + \
+               [(name, ctypes.c_int32) for name in ("m", "n", "k", "block_b", "dtype_a", "dtype_b", "dtype_c")] + \
+               [("beta", ctypes.c_float), ("relu", ctypes.c_int32), ("reserved", ctypes.c_int32 * 3)]
 
 
 class DeviceProps(ctypes.Structure):
@@ -169,6 +179,18 @@ def get_lib() -> ctypes.CDLL:
     lib.kcg_attention_fwd.restype = ctypes.c_int
     lib.kcg_attention_status.argtypes = [ctypes.c_int, ctypes.POINTER(ctypes.c_uint32)]
     lib.kcg_attention_status.restype = ctypes.c_int
+    i64, i32, f32 = ctypes.c_int64, ctypes.c_int, ctypes.c_float
+    lib.kcg_rms_norm.argtypes = [i32, u64, u64, i64, u64, i64, u64, u64, i64, u64, i64, i64, i32, f32, i32]
+    lib.kcg_rms_norm_fp8.argtypes = [i32, u64, u64, i64, u64, i64, u64, u64, i64, u64, u64, i64, i64, i32, f32, i32]
+    lib.kcg_rms_norm_backward_workspace.argtypes = [i32, i64, i32]
+    lib.kcg_rms_norm_backward_workspace.restype = i64
+    lib.kcg_rms_norm_backward.argtypes = [i32, u64, u64, i64, u64, i64, u64, u64, i64, u64, i64, u64, u64, i64, i64, i32, f32, i32]
+    lib.kcg_quantize_fp8.argtypes = [i32, u64, u64, i64, u64, i64, u64, i64, i32, i32, i32, i32, i32]
+    lib.kcg_matmul_fp8.argtypes = [i32, u64, ctypes.POINTER(Fp8Product)]
+    lib.kcg_matmul_fp8_status.argtypes = [i32, ctypes.POINTER(ctypes.c_uint32)]
+    for name in ("kcg_rms_norm", "kcg_rms_norm_fp8", "kcg_rms_norm_backward", "kcg_quantize_fp8", "kcg_matmul_fp8",
+                 "kcg_matmul_fp8_status"):
+        getattr(lib, name).restype = i32
     lib.kcg_peer_alloc.argtypes = [ctypes.c_int, u64, ctypes.POINTER(u64), ctypes.c_char_p]
     lib.kcg_peer_open.argtypes = [ctypes.c_int, ctypes.c_char_p, ctypes.POINTER(u64)]
     lib.kcg_peer_close.argtypes = [ctypes.c_int, u64]

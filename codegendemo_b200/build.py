@@ -96,13 +96,14 @@ def build_library(force: bool = False) -> str:
     deps = srcs + [os.path.join(kdir, f) for f in sorted(os.listdir(kdir))] + [
         os.path.join(os.path.dirname(HERE), "include", "kcg_b200.h")]
     # device code linked into the library itself: the allocation-free split-K entry, the row softmax, the fused attention
-    # and the split of fp32 operands
-    extra = [os.path.join(HERE, "csrc", f) for f in ("kcg_noalloc.cu", "kcg_softmax.cu", "kcg_attention.cu", "kcg_f32split.cu")]
-    deps += extra
+    # the split of fp32 operands, and the 8-bit linear layer
+    extra = [os.path.join(HERE, "csrc", f) for f in ("kcg_noalloc.cu", "kcg_softmax.cu", "kcg_attention.cu", "kcg_f32split.cu",
+                                                     "kcg_norm.cu", "kcg_quantize.cu", "kcg_fp8.cu")]
+    deps += extra + [os.path.join(HERE, "csrc", "fp8_common.cuh")]
     if not force and _newer(out, deps):
         return out
     nvcc = os.path.join(CUDA_HOME, "bin", "nvcc")
-    cmd = [nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-shared",
+    cmd = [nvcc, "-t", "0", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-shared",
            "-Xcompiler", "-fPIC", "-cudart", "static", "-I" + os.path.join(HERE, "csrc", "kernels"),
            "-o", out, *srcs, *extra, "-ldl", "-lpthread"]
     subprocess.check_call(cmd)

@@ -1,0 +1,778 @@
+// Product of 8-bit matrices with a scale for each block of 128 values along K:
+//     C[m, n] = sum over blocks kb of  sa[m, kb] * sb[n, kb] * sum over k in kb of a[m, k] * b[n, k],
+// a and b in e4m3 or e5m2 (each its own), rows of K values; sa a scale per row and block; sb one per 128 rows and block (a weight's
+// 128 x 128 blocks) or per row and block (both operands of a weight's gradient). fp32 accumulation, then beta * C + bias, ReLU, one
+// rounding to bf16, fp16 or fp32.
+//
+// The scales change with every 128 values of K, so the tensor core sums 128 values only (kind::f8f6f4, four instructions of 32),
+// into one of two accumulators in tensor memory; while it fills the other, warps read the first, one row of the tile a thread, and add
+// it to fp32 registers, times its scales.
+//
+// Two kernels. Fp8Tile: one CTA a tile of 128 rows by kBN columns, K split over the CTAs of a cluster, which add their tiles through
+// distributed shared memory (in the order of their ranks). With few tokens the weight's rows are the tile's rows and the tokens its
+// columns, 16 to 64 of them, so that a tile streams weights and little else. Fp8Pair: CTA pairs, 256 x 256 tiles, persistent.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cfloat>
+#include <cstdint>
+#include <mutex>
+#include <string>
+
+#include "../../include/kcg_b200.h"
+#include "fp8_common.cuh"
+#include "kernels/ptx_sm100.cuh"
+
+namespace {
+
+using namespace kcg;
+using namespace kcg8;
+
+__device__ unsigned int g_fp8_status[4];  // {code, block, detail, detail}; 0 = no wait ran out
+enum : uint32_t { FP8_TIMEOUT_PRODUCER = 1, FP8_TIMEOUT_MMA = 2, FP8_TIMEOUT_ACCUMULATE = 3 };
+
+// D[tmem] (+)= A[smem] * B[smem], 8-bit operands; issued by ONE thread (of the leader CTA, kCtas = 2).
+template <int kCtas>
+__device__ __forceinline__ void umma_fp8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+#define KCG_UMMA_FP8(group)                                                                \
+  asm volatile(                                                                            \
+      "{\n\t"                                                                              \
+      ".reg .pred p;\n\t"                                                                  \
+      "setp.ne.b32 p, %4, 0;\n\t"                                                          \
+      "tcgen05.mma.cta_group::" group ".kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"             \
+      "}\n"                                                                                \
+      :                                                                                    \
+      : "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)                   \
+      : "memory")
+  if constexpr (kCtas == 2) {
+    KCG_UMMA_FP8("2");
+  } else {
+    KCG_UMMA_FP8("1");
+  }
+#undef KCG_UMMA_FP8
+}
+
+// TMEM -> registers: 16 consecutive columns of this thread's lane
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+  return v;
+}
+
+struct Fp8Params {
+  CUtensorMap tmP, tmQ;  // {K, rows}: the operand whose rows are the tile's rows, and the one whose rows are its columns
+  const float *sp, *sq;  // scale of row i at block kb: s[(i >> shift) * ld + kb]
+  long long ldsp, ldsq;
+  int sp_shift, sq_shift;
+  int rows_p, rows_q, num_kb;
+  uint32_t fmt_p, fmt_q;  // 0 = e4m3, 1 = e5m2
+  void* C;
+  long long ldc;
+  const void* bias;
+  float beta;
+  int relu;
+  int vector_store;  // rows of C start on 16-byte boundaries
+  int splits;        // Fp8Tile: CTAs that share a tile's K
+};
+
+// The product of two scales, of which only the result of the sum decides whether it is out of range: no 0 * infinity.
+__device__ __forceinline__ float scale_product(float a, float b) {
+  const float f = a * b;
+  return f == INFINITY && a != INFINITY && b != INFINITY ? FLT_MAX : f;
+}
+
+// acc[i] += part[i] * f, for kN columns whose scale is the same.
+template <int kN>
+__device__ __forceinline__ void add_scaled(float* acc, const uint32_t (&part)[kN], float f) {
+#pragma unroll
+  for (int i = 0; i < kN; i += 2) {
+    const float2 y = __ffma2_rn(make_float2(__uint_as_float(part[i]), __uint_as_float(part[i + 1])), make_float2(f, f),
+                                make_float2(acc[i], acc[i + 1]));
+    acc[i] = y.x, acc[i + 1] = y.y;
+  }
+}
+// acc[i] += part[i] * scale[i] * f, scales of the columns in shared memory.
+template <int kN>
+__device__ __forceinline__ void add_scaled(float* acc, const uint32_t (&part)[kN], const float* scale, float f) {
+#pragma unroll
+  for (int i = 0; i < kN; i += 4) {
+    const float4 s = *reinterpret_cast<const float4*>(scale + i);
+    const float2 t0 = __fmul2_rn(make_float2(__uint_as_float(part[i]), __uint_as_float(part[i + 1])), make_float2(s.x, s.y));
+    const float2 t1 = __fmul2_rn(make_float2(__uint_as_float(part[i + 2]), __uint_as_float(part[i + 3])), make_float2(s.z, s.w));
+    const float2 y0 = __ffma2_rn(t0, make_float2(f, f), make_float2(acc[i], acc[i + 1]));
+    const float2 y1 = __ffma2_rn(t1, make_float2(f, f), make_float2(acc[i + 2], acc[i + 3]));
+    acc[i] = y0.x, acc[i + 1] = y0.y, acc[i + 2] = y1.x, acc[i + 3] = y1.y;
+  }
+}
+
+// One value of C from its sum.
+template <typename T>
+__device__ __forceinline__ float finish(const Fp8Params& p, float v, const T* c, float bias) {
+  if (p.beta != 0.f) v = fmaf(p.beta, to_f32(*c), v);
+  v += bias;
+  return p.relu ? fmaxf(v, 0.f) : v;
+}
+template <typename T>
+__device__ __forceinline__ float bias_at(const Fp8Params& p, int n) {
+  return p.bias ? to_f32(static_cast<const T*>(p.bias)[n]) : 0.f;
+}
+
+// Eight columns of one row of C from column n on.
+template <typename T>
+__device__ __forceinline__ void store_span8(const Fp8Params& p, const float* v, long long m, int n, int cols) {
+  T* c = static_cast<T*>(p.C) + m * p.ldc + n;
+  if (p.vector_store && n + 8 <= cols) {
+    float out[8];
+    float old[8];
+    if (p.beta != 0.f) load8(c, old);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      out[j] = v[j];
+      if (p.beta != 0.f) out[j] = fmaf(p.beta, old[j], out[j]);
+      out[j] += bias_at<T>(p, n + j);
+      if (p.relu) out[j] = fmaxf(out[j], 0.f);
+    }
+    store8(c, out);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (n + j < cols) c[j] = from_f32<T>(finish<T>(p, v[j], c + j, bias_at<T>(p, n + j)));
+  }
+}
+
+template <typename Bars>
+__device__ __forceinline__ void report(Bars* bars, uint32_t code, uint32_t d0, uint32_t d1) {
+  bars->abort_flag = 1u;
+  if (atomicCAS(&g_fp8_status[0], 0u, code) == 0u) {
+    g_fp8_status[1] = blockIdx.x;
+    g_fp8_status[2] = d0;
+    g_fp8_status[3] = d1;
+  }
+}
+
+// kBN: columns of a tile. kVector: each column has a scale of its own, else the tile's columns share one (kBN <= 128).
+// kSwap: the tile's rows are columns of C (weights), its columns rows of C (tokens).
+template <int kBN, bool kVector, bool kSwap, typename T>
+struct Fp8Tile {
+  static constexpr int NUM_THREADS = 192;  // producer, issuer, four accumulating warps
+  static constexpr int P_BYTES = 128 * 128, STAGE_BYTES = P_BYTES + kBN * 128;
+  static constexpr int STAGES = kBN == 16 ? 6 : kBN == 32 ? 5 : kBN == 64 ? 4 : 6;
+  static constexpr int CTAS_PER_SM = kBN <= 64 ? 2 : 1;
+  static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
+  static constexpr int PIECE = kBN < 32 ? 16 : 32;
+  static constexpr uint32_t TMEM_COLS = 2 * kBN;  // (32 at least, a power of two)
+  static constexpr int SMEM_BYTES = RING_BYTES + 1024 + 2048;
+  static_assert(kBN * 128 * 4 <= RING_BYTES, "the joining lays a tile over the ring");
+
+  struct Barriers {
+    uint64_t full[STAGES], empty[STAGES];
+    uint64_t tmem_full[2], tmem_empty[2];
+    uint32_t tmem_base;
+    volatile uint32_t abort_flag;
+    alignas(16) float scale[2][kVector ? kBN : 4];
+  };
+  static_assert(sizeof(Barriers) <= 2048, "barrier block exceeds its shared-memory slot");
+
+  __device__ static void run(const Fp8Params& p) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    Barriers* bars = reinterpret_cast<Barriers*>(smem + RING_BYTES);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = p.splits > 1 ? static_cast<int>(cluster_cta_rank()) : 0;
+    const int tile = static_cast<int>(blockIdx.x) / p.splits;
+    const int tiles_q = (p.rows_q + kBN - 1) / kBN;
+    const int p0 = tile / tiles_q * 128, q0 = tile % tiles_q * kBN;
+    // (splits <= num_kb: every CTA has at least one block)
+    const int kb0 = static_cast<int>(static_cast<long long>(p.num_kb) * rank / p.splits);
+    const int n = static_cast<int>(static_cast<long long>(p.num_kb) * (rank + 1) / p.splits) - kb0;
+
+    if (threadIdx.x == 0) {
+      tma_prefetch_desc(&p.tmP);
+      tma_prefetch_desc(&p.tmQ);
+      for (int s = 0; s < STAGES; ++s) {
+        mbar_init(&bars->full[s], 1);
+        mbar_init(&bars->empty[s], 1);
+      }
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&bars->tmem_full[b], 1);
+        mbar_init(&bars->tmem_empty[b], 4);
+      }
+      bars->abort_flag = 0u;
+      fence_mbar_init();
+      fence_proxy_async_smem();
+    }
+    if (warp == 1) {
+      tmem_alloc(&bars->tmem_base, TMEM_COLS);
+      tmem_relinquish();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem_base = bars->tmem_base;
+    griddep_wait();
+
+    float acc[kBN];
+    const int q = warp & 3, row = q * 32 + lane;  // (accumulating warps) TMEM lane quarter, row of the tile
+    bool ok = true;
+    if (warp == 0) {
+      if (lane == 0) {
+        for (int i = 0; i < n; ++i) {
+          const int s = i % STAGES;
+          if (!mbar_wait(&bars->empty[s], ((i / STAGES) & 1u) ^ 1u, &bars->abort_flag)) {
+            report(bars, FP8_TIMEOUT_PRODUCER, i, s);
+            break;
+          }
+          mbar_expect_tx(&bars->full[s], STAGE_BYTES);
+          tma_load_2d(smem + s * STAGE_BYTES, &p.tmP, &bars->full[s], (kb0 + i) * 128, p0);
+          tma_load_2d(smem + s * STAGE_BYTES + P_BYTES, &p.tmQ, &bars->full[s], (kb0 + i) * 128, q0);
+        }
+      }
+      __syncwarp();
+      griddep_launch_dependents();
+    } else if (warp == 1) {
+      const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+      const uint64_t pdesc = make_smem_desc(smem_u32(smem), 16, 1024, SWZ_128B);
+      const uint64_t qdesc = make_smem_desc(smem_u32(smem) + P_BYTES, 16, 1024, SWZ_128B);
+      const uint32_t idesc = make_instr_desc(0u, 0u, 0u, 128u, kBN) | p.fmt_p << 7 | p.fmt_q << 10;
+      for (int i = 0; i < n; ++i) {
+        const uint32_t s = i % STAGES, b = i & 1u;
+        if (!mbar_wait_warp(&bars->tmem_empty[b], ((i >> 1) & 1u) ^ 1u, &bars->abort_flag) ||
+            !mbar_wait_warp(&bars->full[s], (i / STAGES) & 1u, &bars->abort_flag)) {
+          if (lane == 0) report(bars, FP8_TIMEOUT_MMA, i, s);
+          break;
+        }
+        tc_fence_after_sync();
+        if (elect_one()) {
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)  // 32 values = 32 bytes of a row
+            umma_fp8<1>(tmem + b * kBN, pdesc + s * (STAGE_BYTES >> 4) + ks * 2, qdesc + s * (STAGE_BYTES >> 4) + ks * 2, idesc,
+                        ks > 0 ? 1u : 0u);
+          umma_commit(&bars->empty[s]);
+          umma_commit(&bars->tmem_full[b]);
+        }
+        __syncwarp();
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kBN; ++i) acc[i] = 0.f;
+      const int t = threadIdx.x - 64;  // also: column whose scale this thread fetches
+      const float* sp = p.sp + (static_cast<long long>(min(p0 + row, p.rows_p - 1)) >> p.sp_shift) * p.ldsp + kb0;
+      const float* sq = p.sq + (static_cast<long long>(min(q0 + (kVector ? t : 0), p.rows_q - 1)) >> p.sq_shift) * p.ldsq + kb0;
+      const bool fetches = !kVector || t < kBN;
+      float next_p = __ldg(sp), next_q = fetches ? __ldg(sq) : 0.f;
+      for (int i = 0; i < n; ++i) {
+        const uint32_t b = i & 1u;
+        const float f = kVector ? next_p : scale_product(next_p, next_q);
+        if constexpr (kVector) {
+          // (two buffers: a thread that writes one again has passed the meeting behind which all have read it)
+          if (fetches) bars->scale[b][t] = next_q;
+          named_bar_sync(1, 128);
+        }
+        if (i + 1 < n) {
+          next_p = __ldg(sp + i + 1);
+          if (fetches) next_q = __ldg(sq + i + 1);
+        }
+        if (ok) {
+          const bool got = mbar_wait(&bars->tmem_full[b], (i >> 1) & 1u, &bars->abort_flag);
+          if (!__all_sync(0xffffffffu, got)) {
+            if (lane == 0) report(bars, FP8_TIMEOUT_ACCUMULATE, i, b);
+            ok = false;
+          }
+        }
+        if (!ok) continue;  // (the meetings go on)
+        tc_fence_after_sync();
+        const uint32_t col = tmem_base + b * kBN + (static_cast<uint32_t>(q * 32) << 16);
+#pragma unroll
+        for (int c = 0; c < kBN; c += PIECE) {
+          uint32_t r[PIECE];
+          if constexpr (PIECE == 16) {
+            tmem_ld_32x32b_x16(col + c, r);
+          } else {
+            tmem_ld_32x32b_x32(col + c, r);
+          }
+          tmem_ld_wait();
+          if constexpr (kVector) {
+            add_scaled<PIECE>(acc + c, r, &bars->scale[b][c], f);
+          } else {
+            add_scaled<PIECE>(acc + c, r, f);
+          }
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->tmem_empty[b]);
+      }
+    }
+
+    if (p.splits > 1) {
+      // Every product has been read, so the ring is idle: the CTA's tile goes there, column after column of 128 rows.
+      float* part = reinterpret_cast<float*>(smem);
+      if (warp >= 2 && ok) {
+#pragma unroll
+        for (int c = 0; c < kBN; ++c) part[c * 128 + row] = acc[c];
+      }
+      __syncwarp();
+      cluster_sync_all();
+      if (warp >= 2 && ok) {
+        const int per = kBN / p.splits, c0 = rank * per;  // (splits: a power of two, at most 8)
+        const uint32_t mine = smem_u32(part + row);
+        for (int c = c0; c < c0 + per; ++c) {
+          float v = 0.f;
+          for (int r = 0; r < p.splits; ++r) v += ld_cluster_f32(map_to_cta(mine + c * 512, r));
+          const int gp = p0 + row, gq = q0 + c;
+          if (gp < p.rows_p && gq < p.rows_q) {
+            T* out = static_cast<T*>(p.C) + (kSwap ? gq * p.ldc + gp : gp * p.ldc + gq);
+            *out = from_f32<T>(finish<T>(p, v, out, bias_at<T>(p, kSwap ? gp : gq)));
+          }
+        }
+      }
+      __syncwarp();
+      cluster_sync_all();  // shared memory stays until the others have read it
+    } else if (warp >= 2 && ok && p0 + row < p.rows_p) {
+      if constexpr (kSwap) {
+        const float bias = bias_at<T>(p, p0 + row);
+#pragma unroll
+        for (int c = 0; c < kBN; ++c)
+          if (q0 + c < p.rows_q) {
+            T* out = static_cast<T*>(p.C) + static_cast<long long>(q0 + c) * p.ldc + p0 + row;
+            *out = from_f32<T>(finish<T>(p, acc[c], out, bias));
+          }
+      } else {
+#pragma unroll
+        for (int c = 0; c < kBN; c += 8) store_span8<T>(p, acc + c, p0 + row, q0 + c, p.rows_q);
+      }
+    }
+
+    // ---------------------------------------------------------------- common exit
+    __syncwarp();
+    if (bars->abort_flag != 0u) {
+      // give loads / products still in flight time to land before shared memory and TMEM are released
+      const uint64_t t0 = global_timer_ns();
+      while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 1) {
+      tc_fence_after_sync();
+      tmem_dealloc(tmem_base, TMEM_COLS);
+    }
+  }
+};
+
+template <int kBN, bool kVector, bool kSwap, typename T>
+__global__ void __launch_bounds__(192, Fp8Tile<kBN, kVector, kSwap, T>::CTAS_PER_SM) fp8_tile_kernel(const __grid_constant__ Fp8Params p) {
+  Fp8Tile<kBN, kVector, kSwap, T>::run(p);
+}
+
+// CTA pairs, tiles of 256 x 256, one after another. Each CTA holds 128 rows of A and 128 of B a stage; its eight accumulating warps
+// a row of the tile a thread, 128 columns each: warps 4-7 the first half, warps 8-11 the second.
+template <bool kVector, typename T>
+struct Fp8Pair {
+  static constexpr int NUM_THREADS = 384, kBM = 256, kBN = 256;
+  static constexpr int HALF_BYTES = 128 * 128, STAGE_BYTES = 2 * HALF_BYTES;
+  static constexpr int STAGES = 6;
+  static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
+  static constexpr int SMEM_BYTES = RING_BYTES + 1024 + 4096;
+  static constexpr int GROUP = 8;  // tile rows that are walked together, column after column
+  static constexpr uint32_t TMEM_COLS = 512;
+
+  struct Barriers {
+    uint64_t full[STAGES], empty[STAGES];
+    uint64_t tmem_full[2], tmem_empty[2];
+    uint32_t tmem_base;
+    volatile uint32_t abort_flag;
+    alignas(16) float scale[2][2][kVector ? 128 : 4];  // [half][buffer][column]
+  };
+  static_assert(sizeof(Barriers) <= 4096, "barrier block exceeds its shared-memory slot");
+
+  // Rows and columns of C at which tile i starts.
+  __device__ static __forceinline__ void tile_at(int i, int tiles_m, int tiles_n, int& m0, int& n0) {
+    const int per_group = GROUP * tiles_n, group = i / per_group, first = group * GROUP;
+    const int rows = min(GROUP, tiles_m - first), in = i - group * per_group;
+    m0 = (first + in % rows) * kBM;
+    n0 = in / rows * kBN;
+  }
+
+  __device__ static void run(const Fp8Params& p) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    Barriers* bars = reinterpret_cast<Barriers*>(smem + RING_BYTES);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_cta_rank();  // 0 = leader
+    const int tiles_m = (p.rows_p + kBM - 1) / kBM, tiles_n = (p.rows_q + kBN - 1) / kBN, tiles = tiles_m * tiles_n;
+    const int tile0 = static_cast<int>(blockIdx.x >> 1), stride = static_cast<int>(gridDim.x >> 1);
+
+    if (threadIdx.x == 0) {
+      tma_prefetch_desc(&p.tmP);
+      tma_prefetch_desc(&p.tmQ);
+      for (int s = 0; s < STAGES; ++s) {
+        mbar_init(&bars->full[s], 1);
+        mbar_init(&bars->empty[s], 1);
+      }
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&bars->tmem_full[b], 1);
+        mbar_init(&bars->tmem_empty[b], 16);  // one arrival per accumulating warp of each CTA
+      }
+      bars->abort_flag = 0u;
+      fence_mbar_init();
+      fence_proxy_async_smem();
+    }
+    if (warp == 1) {
+      tmem_alloc_pair(&bars->tmem_base, TMEM_COLS);
+      tmem_relinquish_pair();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync_all();  // the peer's barriers exist before anyone signals them
+    tc_fence_after_sync();
+    const uint32_t tmem_base = bars->tmem_base;
+    griddep_wait();
+
+    // Registers: 384 threads are launched with 168 each; 56 + 2 * 224 = 3 * 168.
+    if (warp < 4) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+      if (warp == 0) {
+        if (lane == 0) {
+          uint32_t it = 0;
+          bool ok = true;
+          for (int tile = tile0; tile < tiles && ok; tile += stride) {
+            int m0, n0;
+            tile_at(tile, tiles_m, tiles_n, m0, n0);
+            for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
+              const uint32_t s = it % STAGES;
+              if (!mbar_wait(&bars->empty[s], ((it / STAGES) & 1u) ^ 1u, &bars->abort_flag)) {
+                report(bars, FP8_TIMEOUT_PRODUCER, it, s);
+                ok = false;
+                break;
+              }
+              // completion bytes of both CTAs land on the leader's barrier
+              const uint32_t full_leader = map_to_cta(smem_u32(&bars->full[s]), 0u);
+              if (rank == 0u) mbar_expect_tx(&bars->full[s], 2 * STAGE_BYTES);
+              tma_load_2d_pair(smem + s * STAGE_BYTES, &p.tmP, full_leader, kb * 128, m0 + static_cast<int>(rank) * 128);
+              tma_load_2d_pair(smem + s * STAGE_BYTES + HALF_BYTES, &p.tmQ, full_leader, kb * 128, n0 + static_cast<int>(rank) * 128);
+            }
+          }
+        }
+        __syncwarp();
+        griddep_launch_dependents();
+      } else if (warp == 1 && rank == 0u) {
+        const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+        const uint64_t adesc = make_smem_desc(smem_u32(smem), 16, 1024, SWZ_128B);
+        const uint64_t bdesc = make_smem_desc(smem_u32(smem) + HALF_BYTES, 16, 1024, SWZ_128B);
+        const uint32_t idesc = make_instr_desc(0u, 0u, 0u, 256u, kBN) | p.fmt_p << 7 | p.fmt_q << 10;
+        uint32_t it = 0;
+        bool ok = true;
+        for (int tile = tile0; tile < tiles && ok; tile += stride) {
+          for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
+            const uint32_t s = it % STAGES, b = it & 1u;
+            if (!mbar_wait_warp(&bars->tmem_empty[b], ((it >> 1) & 1u) ^ 1u, &bars->abort_flag) ||
+                !mbar_wait_warp(&bars->full[s], (it / STAGES) & 1u, &bars->abort_flag)) {
+              if (lane == 0) report(bars, FP8_TIMEOUT_MMA, it, s);
+              ok = false;
+              break;
+            }
+            tc_fence_after_sync();
+            if (elect_one()) {
+#pragma unroll
+              for (int ks = 0; ks < 4; ++ks)
+                umma_fp8<2>(tmem + b * kBN, adesc + s * (STAGE_BYTES >> 4) + ks * 2, bdesc + s * (STAGE_BYTES >> 4) + ks * 2, idesc,
+                            ks > 0 ? 1u : 0u);
+              umma_commit_pair(smem_u32(&bars->empty[s]));
+              umma_commit_pair(map_to_cta(smem_u32(&bars->empty[s]), 1u));
+              umma_commit_pair(smem_u32(&bars->tmem_full[b]));
+              umma_commit_pair(map_to_cta(smem_u32(&bars->tmem_full[b]), 1u));
+            }
+            __syncwarp();
+          }
+        }
+      }
+    } else {
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+      const int q = warp & 3, half = (warp - 4) >> 2, row = q * 32 + lane;
+      const int t = threadIdx.x & 127;  // column of the half whose scale this thread fetches
+      uint32_t it = 0;
+      bool ok = true;
+      for (int tile = tile0; tile < tiles; tile += stride) {
+        int m0, n0;
+        tile_at(tile, tiles_m, tiles_n, m0, n0);
+        m0 += static_cast<int>(rank) * 128;
+        n0 += half * 128;
+        float acc[128];
+#pragma unroll
+        for (int i = 0; i < 128; ++i) acc[i] = 0.f;
+        const float* sp = p.sp + (static_cast<long long>(min(m0 + row, p.rows_p - 1)) >> p.sp_shift) * p.ldsp;
+        const float* sq = p.sq + (static_cast<long long>(min(n0 + (kVector ? t : 0), p.rows_q - 1)) >> p.sq_shift) * p.ldsq;
+        float next_p = __ldg(sp), next_q = __ldg(sq);
+        for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
+          const uint32_t b = it & 1u;
+          const float f = kVector ? next_p : scale_product(next_p, next_q);
+          if constexpr (kVector) {
+            bars->scale[half][b][t] = next_q;
+            named_bar_sync(1 + half, 128);
+          }
+          if (kb + 1 < p.num_kb) {
+            next_p = __ldg(sp + kb + 1);
+            next_q = __ldg(sq + kb + 1);
+          }
+          if (ok) {
+            const bool got = mbar_wait(&bars->tmem_full[b], (it >> 1) & 1u, &bars->abort_flag);
+            if (!__all_sync(0xffffffffu, got)) {
+              if (lane == 0) report(bars, FP8_TIMEOUT_ACCUMULATE, it, b);
+              ok = false;
+            }
+          }
+          if (!ok) continue;  // (the meetings go on)
+          tc_fence_after_sync();
+          const uint32_t col = tmem_base + b * kBN + half * 128 + (static_cast<uint32_t>(q * 32) << 16);
+#pragma unroll
+          for (int c = 0; c < 128; c += 32) {
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(col + c, r);
+            tmem_ld_wait();
+            if constexpr (kVector) {
+              add_scaled<32>(acc + c, r, &bars->scale[half][b][c], f);
+            } else {
+              add_scaled<32>(acc + c, r, f);
+            }
+          }
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster_cta(map_to_cta(smem_u32(&bars->tmem_empty[b]), 0u));  // (the reads are complete)
+        }
+        if (ok && m0 + row < p.rows_p) {
+#pragma unroll
+          for (int c = 0; c < 128; c += 8) store_span8<T>(p, acc + c, m0 + row, n0 + c, p.rows_q);
+        }
+      }
+    }
+
+    // ------------------------------------------------------------ common exit
+    __syncwarp();
+    if (bars->abort_flag != 0u) {
+      const uint64_t t0 = global_timer_ns();
+      while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    __syncwarp();
+    cluster_sync_all();  // the peer's shared memory and TMEM stay valid until both CTAs are done
+    if (warp == 1) {
+      __syncwarp();
+      tc_fence_after_sync();
+      tmem_dealloc_pair(tmem_base, TMEM_COLS);
+    }
+  }
+};
+
+template <bool kVector, typename T>
+__global__ void __launch_bounds__(384, 1) fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
+  Fp8Pair<kVector, T>::run(p);
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+std::mutex g_mutex;
+EncodeFn g_encode = nullptr;
+
+int encoder(EncodeFn* out) {
+  std::lock_guard<std::mutex> lock(g_mutex);
+  if (!g_encode) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult qres;
+    const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &qres);
+    if (e != cudaSuccess || qres != cudaDriverEntryPointSuccess || !fn)
+      return fail(KCG_E_NO_DRIVER, "cuTensorMapEncodeTiled not available from the driver");
+    g_encode = reinterpret_cast<EncodeFn>(fn);
+  }
+  *out = g_encode;
+  return 0;
+}
+
+// Rows of K bytes, `ld` apart; boxes of 128 bytes x `box_rows` rows. What lies past the matrix reads as zero.
+int encode(EncodeFn fn, CUtensorMap* tm, uint64_t ptr, int k, int64_t ld, int rows, int box_rows) {
+  cuuint64_t gdim[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)};
+  cuuint64_t gstride[1] = {static_cast<cuuint64_t>(ld)};
+  cuuint32_t box[2] = {128, static_cast<cuuint32_t>(box_rows)}, estr[2] = {1, 1};
+  const CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, reinterpret_cast<void*>(ptr), gdim, gstride, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : fail(static_cast<int>(r), "cuTensorMapEncodeTiled failed");
+}
+
+// Once per device: the kernel may use more than 48 KB of shared memory.
+template <typename K>
+int opt_in(K kernel, int device, int smem, bool (&ready)[64]) {
+  std::lock_guard<std::mutex> lock(g_mutex);
+  if (!ready[device]) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(MaxDynamicSharedMemorySize)");
+    ready[device] = true;
+  }
+  return 0;
+}
+
+struct Plan {
+  int pair;    // Fp8Pair
+  int swap;    // Fp8Tile: the weight's rows are the tile's rows
+  int bn;      // columns of a tile
+  int splits;  // CTAs that share a tile's K
+};
+
+// Which kernel takes a product.
+Plan plan_of(int m, int n, int k, int sms) {
+  const int num_kb = (k + 127) / 128;
+  Plan plan{0, 0, 128, 1};
+  long long tiles;
+  int at_once;
+  if (m <= 64) {
+    plan.swap = 1;
+    plan.bn = m <= 16 ? 16 : m <= 32 ? 32 : 64;
+    tiles = (n + 127) / 128;
+    at_once = 2 * sms;
+  } else {
+    const long long large = static_cast<long long>((m + 255) / 256) * ((n + 255) / 256);
+    if (large >= sms / 2) {
+      plan.pair = 1;
+      plan.bn = 256;
+      return plan;
+    }
+    tiles = static_cast<long long>((m + 127) / 128) * ((n + 127) / 128);
+    at_once = sms;
+  }
+  while (plan.splits < 8 && tiles * plan.splits * 2 <= at_once && num_kb >= plan.splits * 4) plan.splits *= 2;
+  return plan;
+}
+
+template <int kBN, bool kVector, bool kSwap, typename T>
+int launch_tile(int device, cudaStream_t st, const Fp8Params& p) {
+  using Kern = Fp8Tile<kBN, kVector, kSwap, T>;
+  static bool ready[64];
+  const auto kernel = fp8_tile_kernel<kBN, kVector, kSwap, T>;
+  if (int e = opt_in(kernel, device, Kern::SMEM_BYTES, ready)) return e;
+  const long long ctas = static_cast<long long>((p.rows_p + 127) / 128) * ((p.rows_q + kBN - 1) / kBN) * p.splits;
+  if (ctas > 0x7fffffffLL) return fail(KCG_E_TOO_LARGE, "too many tiles for one launch");
+  Launch l(st);
+  l.shape(static_cast<unsigned>(ctas), Kern::NUM_THREADS, Kern::SMEM_BYTES, p.splits);
+  return l(kernel, "8-bit product launch", p);
+}
+
+template <bool kVector, typename T>
+int launch_pair(int device, int sms, cudaStream_t st, const Fp8Params& p) {
+  using Kern = Fp8Pair<kVector, T>;
+  static bool ready[64];
+  const auto kernel = fp8_pair_kernel<kVector, T>;
+  if (int e = opt_in(kernel, device, Kern::SMEM_BYTES, ready)) return e;
+  const long long tiles = static_cast<long long>((p.rows_p + 255) / 256) * ((p.rows_q + 255) / 256);
+  if (tiles > 0x3fffffffLL) return fail(KCG_E_TOO_LARGE, "too many tiles for one launch");
+  const int pairs = static_cast<int>(tiles < sms / 2 ? tiles : sms / 2);
+  Launch l(st);
+  l.shape(2 * pairs, Kern::NUM_THREADS, Kern::SMEM_BYTES, 2);
+  return l(kernel, "8-bit product launch", p);
+}
+
+template <typename T>
+int launch(const Plan& plan, int device, int sms, cudaStream_t st, const Fp8Params& p, bool vector) {
+  if (plan.pair) return vector ? launch_pair<true, T>(device, sms, st, p) : launch_pair<false, T>(device, sms, st, p);
+  if (!plan.swap) return vector ? launch_tile<128, true, false, T>(device, st, p) : launch_tile<128, false, false, T>(device, st, p);
+  switch (plan.bn) {
+    case 16: return launch_tile<16, true, true, T>(device, st, p);
+    case 32: return launch_tile<32, true, true, T>(device, st, p);
+    default: return launch_tile<64, true, true, T>(device, st, p);
+  }
+}
+
+}  // namespace
+
+// For tests of the host logic: the plan of a product as {pair, swap, columns of a tile, splits}.
+extern "C" int kcg_internal_fp8_plan(int m, int n, int k, int sms, int out[4]) {
+  const Plan plan = plan_of(m, n, k, sms);
+  out[0] = plan.pair, out[1] = plan.swap, out[2] = plan.bn, out[3] = plan.splits;
+  return 0;
+}
+
+extern "C" int kcg_matmul_fp8(int device, uint64_t stream, const kcg_fp8_product* a) {
+  if (!a) return fail(KCG_E_BAD_ARG, "null argument");
+  if (a->m < 0 || a->n <= 0 || a->k <= 0) return fail(KCG_E_BAD_ARG, "shape out of range");
+  if (a->m == 0) return 0;
+  if (!a->A || !a->B || !a->C || !a->scale_a || !a->scale_b) return fail(KCG_E_BAD_ARG, "null device pointer");
+  if ((a->dtype_a != KCG_FP8_E4M3 && a->dtype_a != KCG_FP8_E5M2) || (a->dtype_b != KCG_FP8_E4M3 && a->dtype_b != KCG_FP8_E5M2))
+    return fail(KCG_E_BAD_ARG, "operands are e4m3 or e5m2");
+  if (!known_dtype(a->dtype_c)) return fail(KCG_E_BAD_ARG, "the result is float16, bfloat16 or float32");
+  if (a->block_b != 1 && a->block_b != 128) return fail(KCG_E_BAD_ARG, "blocks of b have 1 or 128 rows");
+  const int kb = (a->k - 1) / 128 + 1;
+  int64_t lda = a->lda ? a->lda : a->k, ldb = a->ldb ? a->ldb : a->k;
+  if (a->m == 1) lda = (lda + 15) / 16 * 16;  // (there is no second row)
+  if (a->n == 1) ldb = (ldb + 15) / 16 * 16;
+  const int64_t ldc = a->ldc ? a->ldc : a->n;
+  const int64_t ldsa = a->ld_scale_a ? a->ld_scale_a : kb, ldsb = a->ld_scale_b ? a->ld_scale_b : kb;
+  if (lda < a->k || ldb < a->k || ldc < a->n || ldsa < kb || ldsb < kb)
+    return fail(KCG_E_BAD_ARG, "leading dimension below the row length");
+  if (a->A % 16 || a->B % 16 || lda % 16 || ldb % 16)
+    return fail(KCG_E_BAD_ARG, "rows of 8-bit operands must start on 16-byte boundaries");
+  const int eb = a->dtype_c == KCG_DTYPE_FLOAT32 ? 4 : 2;
+  if (a->C % eb || a->bias % eb || a->scale_a % 4 || a->scale_b % 4) return fail(KCG_E_BAD_ARG, "operands must be aligned to their values");
+  int sms = 0;
+  if (int e = sm_count(device, &sms)) return e;
+  DeviceGuard guard;
+  const cudaError_t e = guard.enter(device);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaSetDevice");
+  EncodeFn enc = nullptr;
+  if (int r = encoder(&enc)) return r;
+  const Plan plan = plan_of(a->m, a->n, a->k, sms);
+  Fp8Params p{};
+  const int rows_box = plan.pair ? 128 : plan.bn;
+  const uint32_t fa = a->dtype_a == KCG_FP8_E5M2, fb = a->dtype_b == KCG_FP8_E5M2;
+  const int shift_b = a->block_b == 128 ? 7 : 0;
+  const float *sa = reinterpret_cast<const float*>(a->scale_a), *sb = reinterpret_cast<const float*>(a->scale_b);
+  if (plan.swap) {
+    if (int r = encode(enc, &p.tmP, a->B, a->k, ldb, a->n, 128)) return r;
+    if (int r = encode(enc, &p.tmQ, a->A, a->k, lda, a->m, rows_box)) return r;
+    p.sp = sb, p.ldsp = ldsb, p.sp_shift = shift_b, p.sq = sa, p.ldsq = ldsa, p.sq_shift = 0;
+    p.rows_p = a->n, p.rows_q = a->m, p.fmt_p = fb, p.fmt_q = fa;
+  } else {
+    if (int r = encode(enc, &p.tmP, a->A, a->k, lda, a->m, 128)) return r;
+    if (int r = encode(enc, &p.tmQ, a->B, a->k, ldb, a->n, rows_box)) return r;
+    p.sp = sa, p.ldsp = ldsa, p.sp_shift = 0, p.sq = sb, p.ldsq = ldsb, p.sq_shift = shift_b;
+    p.rows_p = a->m, p.rows_q = a->n, p.fmt_p = fa, p.fmt_q = fb;
+  }
+  p.num_kb = kb;
+  p.C = reinterpret_cast<void*>(a->C), p.ldc = ldc, p.bias = reinterpret_cast<const void*>(a->bias);
+  p.beta = a->beta, p.relu = a->relu, p.splits = plan.splits;
+  p.vector_store = a->C % 16 == 0 && ldc * eb % 16 == 0;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const bool vector = a->block_b == 1;
+  if (a->dtype_c == KCG_DTYPE_FLOAT32) return launch<float>(plan, device, sms, st, p, vector);
+  return a->dtype_c == KCG_DTYPE_FLOAT16 ? launch<__half>(plan, device, sms, st, p, vector)
+                                         : launch<__nv_bfloat16>(plan, device, sms, st, p, vector);
+}
+
+// Reads (and clears) the status word of the 8-bit products on `device`: out = {code, block, detail, detail}; code 0 = no bounded
+// wait has run out since the last call. Synchronises the device.
+extern "C" int kcg_matmul_fp8_status(int device, uint32_t out[4]) {
+  if (!out) return fail(KCG_E_BAD_ARG, "null argument");
+  DeviceGuard guard;
+  cudaError_t e = guard.enter(device);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaSetDevice");
+  e = cudaDeviceSynchronize();
+  if (e != cudaSuccess) return cuda_fail(e, "cudaDeviceSynchronize");
+  e = cudaMemcpyFromSymbol(out, g_fp8_status, sizeof(uint32_t) * 4);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaMemcpyFromSymbol");
+  if (out[0] != 0u) {
+    const uint32_t zero[4] = {0u, 0u, 0u, 0u};
+    e = cudaMemcpyToSymbol(g_fp8_status, zero, sizeof(zero));
+    if (e != cudaSuccess) return cuda_fail(e, "cudaMemcpyToSymbol");
+    return fail(KCG_E_DEVICE_TIMEOUT, "a bounded wait of an 8-bit product ran out");
+  }
+  return 0;
+}

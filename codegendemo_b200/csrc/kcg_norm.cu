@@ -1,0 +1,448 @@
+// Root-mean-square norm of rows, forward (with the residual's addition in front of it, its result in the rows' type or as 8-bit
+// values with a scale for each 128 of a row) and backward, for fp16, bf16 and fp32:
+//     h = x + residual,   y = h * r * w,   r = 1 / sqrt(mean(h^2) + eps)
+//     with g = dy * w:    dx = dh + r * g - h * r^3 * mean(g * h),   dw = sum over the rows of dy * h * r
+// (dh: the gradient that reaches h past the norm, along the residual stream.) Sums and products in fp32, one rounding at the end:
+// y comes from the unrounded sum h, which is rounded only where it is stored.
+//
+// Bound by HBM: a row is read once, into registers, and written once. Widths of whole 16-byte pieces take the kernels below
+// (a warp a row up to 1024 values, a CTA a row beyond), others a kernel that reads single values, twice.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <mutex>
+#include <string>
+
+#include "../../include/kcg_b200.h"
+#include "fp8_common.cuh"
+#include "kernels/ptx_sm100.cuh"
+
+namespace {
+
+using namespace kcg;
+using namespace kcg8;
+
+struct NormArgs {
+  const void *x, *residual, *w;
+  void *y, *h;       // y: 8-bit values where there are scales
+  float* scales;     // rows x ceil(width / 128)
+  long long ldx, ldr, ldy, ldh, rows;
+  int width, blocks;  // blocks: scales of a row
+  float eps;
+};
+
+// Sum over the threads of a row: a warp's, or the CTA's.
+template <bool kWarpRow, int kN>
+__device__ __forceinline__ void row_sum(float (&v)[kN], float* scratch) {
+#pragma unroll
+  for (int n = 0; n < kN; ++n)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+  if constexpr (!kWarpRow) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    if (lane == 0)
+#pragma unroll
+      for (int n = 0; n < kN; ++n) scratch[n * 32 + warp] = v[n];
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      v[n] = lane < warps ? scratch[n * 32 + lane] : 0.f;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+    }
+  }
+}
+
+// kVPT: pieces of 8 values a thread holds of a row.
+template <typename T, int kVPT, bool kWarpRow, bool kRes, bool kFp8>
+__global__ void __launch_bounds__(kWarpRow ? 256 : 1024) norm_kernel(const NormArgs a) {
+  __shared__ float scratch[32];
+  griddep_launch_dependents();
+  griddep_wait();
+  const int tid = kWarpRow ? threadIdx.x & 31 : threadIdx.x, threads = kWarpRow ? 32 : blockDim.x;
+  const long long row = kWarpRow ? static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+  if (kWarpRow && row >= a.rows) return;
+  const int pieces = a.width / 8;
+  const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+  const T* res = kRes ? static_cast<const T*>(a.residual) + row * a.ldr : nullptr;
+  float h[kVPT][8];
+  float sum[1] = {0.f};
+#pragma unroll
+  for (int i = 0; i < kVPT; ++i) {
+    const int v = i * threads + tid;
+    if (v < pieces) {
+      load8(x + 8 * v, h[i]);
+      if constexpr (kRes) {
+        float r[8];
+        load8(res + 8 * v, r);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[i][j] += r[j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) h[i][j] = 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum[0] = fmaf(h[i][j], h[i][j], sum[0]);
+  }
+  row_sum<kWarpRow>(sum, scratch);
+  const float r = rsqrtf(sum[0] / static_cast<float>(a.width) + a.eps);
+#pragma unroll
+  for (int i = 0; i < kVPT; ++i) {
+    const int v = i * threads + tid;
+    const bool in = v < pieces;
+    if (kRes && in) store8(static_cast<T*>(a.h) + row * a.ldh + 8 * v, h[i]);
+    float y[8];
+    if (in) {
+      float w[8];
+      load8(static_cast<const T*>(a.w) + 8 * v, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = h[i][j] * r * w[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = 0.f;
+    }
+    if constexpr (kFp8) {
+      // 16 neighbouring threads hold 128 values of the row
+      uint32_t top = abs_max(y);
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float scale = block_scale<false>(top);
+      if (in) {
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.y) + row * a.ldy + 8 * v) = quantize8<false>(y, 1.f / scale);
+        if ((tid & 15) == 0) a.scales[row * a.blocks + v / 16] = scale;
+      }
+    } else if (in) {
+      store8(static_cast<T*>(a.y) + row * a.ldy + 8 * v, y);
+    }
+  }
+}
+
+// Rows of any width, pitch and alignment: single values, a warp to 128 of them at a time, read twice (the second time from a cache).
+template <typename T, bool kRes, bool kFp8>
+__global__ void __launch_bounds__(256) norm_any_kernel(const NormArgs a) {
+  __shared__ float scratch[32];
+  griddep_launch_dependents();
+  griddep_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long row = blockIdx.x;
+  const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+  const T* res = kRes ? static_cast<const T*>(a.residual) + row * a.ldr : nullptr;
+  const T* w = static_cast<const T*>(a.w);
+  auto value = [&](int c) { return kRes ? to_f32(x[c]) + to_f32(res[c]) : to_f32(x[c]); };
+  float sum[1] = {0.f};
+  for (int c = threadIdx.x; c < a.width; c += blockDim.x) {
+    const float v = value(c);
+    sum[0] = fmaf(v, v, sum[0]);
+  }
+  row_sum<false>(sum, scratch);
+  const float r = rsqrtf(sum[0] / static_cast<float>(a.width) + a.eps);
+  for (int b = warp; b * 128 < a.width; b += blockDim.x >> 5) {
+    float y[4];
+    uint32_t top = 0u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = b * 128 + j * 32 + lane;
+      y[j] = 0.f;
+      if (c < a.width) {
+        const float v = value(c);
+        y[j] = v * r * to_f32(w[c]);
+        // (where h is written over x or the residual, each value has been read by the thread that writes it)
+        if constexpr (kRes) static_cast<T*>(a.h)[row * a.ldh + c] = from_f32<T>(v);
+        if constexpr (!kFp8) static_cast<T*>(a.y)[row * a.ldy + c] = from_f32<T>(y[j]);
+      }
+      top = max(top, __float_as_uint(y[j]) & 0x7fffffffu);
+    }
+    if constexpr (kFp8) {
+      const float scale = block_scale<false>(__reduce_max_sync(0xffffffffu, top)), inv = 1.f / scale;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int c = b * 128 + j * 32 + lane;
+        if (c < a.width) static_cast<uint8_t*>(a.y)[row * a.ldy + c] = quantize1<false>(y[j], inv);
+      }
+      if (lane == 0) a.scales[row * a.blocks + b] = scale;
+    }
+  }
+}
+
+struct GradArgs {
+  const void *dy, *h, *w, *dh;
+  void *dx, *dw;
+  float* partial;  // one row of `width` sums for each CTA
+  long long lddy, ldh, lddh, lddx, rows;
+  int width;
+  float eps;
+};
+
+// Each CTA walks rows blockIdx.x, + gridDim.x, ...; a thread keeps its columns' share of dw in registers.
+template <typename T, int kVPT, bool kDh>
+__global__ void __launch_bounds__(1024) norm_grad_kernel(const GradArgs a) {
+  __shared__ float scratch[2][64];
+  griddep_launch_dependents();
+  griddep_wait();
+  const int tid = threadIdx.x, threads = blockDim.x, pieces = a.width / 8;
+  float dw[kVPT][8];
+#pragma unroll
+  for (int i = 0; i < kVPT; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dw[i][j] = 0.f;
+  int turn = 0;
+  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+    float h[kVPT][8], dy[kVPT][8];
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kVPT; ++i) {
+      const int v = i * threads + tid;
+      if (v < pieces) {
+        load8(static_cast<const T*>(a.h) + row * a.ldh + 8 * v, h[i]);
+        load8(static_cast<const T*>(a.dy) + row * a.lddy + 8 * v, dy[i]);
+        float w[8];
+        load8(static_cast<const T*>(a.w) + 8 * v, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          sum[0] = fmaf(h[i][j], h[i][j], sum[0]);
+          sum[1] = fmaf(dy[i][j] * w[j], h[i][j], sum[1]);
+        }
+      }
+    }
+    row_sum<false>(sum, scratch[turn]);  // (two scratches: one barrier a row)
+    const float inv = 1.f / static_cast<float>(a.width);
+    const float r = rsqrtf(fmaf(sum[0], inv, a.eps));
+    const float back = r * r * (sum[1] * inv);  // dx = r * (g - h * back)
+#pragma unroll
+    for (int i = 0; i < kVPT; ++i) {
+      const int v = i * threads + tid;
+      if (v < pieces) {
+        float w[8], d[8];
+        load8(static_cast<const T*>(a.w) + 8 * v, w);
+        if constexpr (kDh) {
+          load8(static_cast<const T*>(a.dh) + row * a.lddh + 8 * v, d);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float dx = r * (dy[i][j] * w[j] - h[i][j] * back);
+          dw[i][j] = fmaf(dy[i][j], h[i][j] * r, dw[i][j]);
+          d[j] = kDh ? d[j] + dx : dx;
+        }
+        store8(static_cast<T*>(a.dx) + row * a.lddx + 8 * v, d);
+      }
+    }
+  }
+  float* mine = a.partial + static_cast<long long>(blockIdx.x) * a.width;
+#pragma unroll
+  for (int i = 0; i < kVPT; ++i) {
+    const int v = i * threads + tid;
+    if (v < pieces) store8(mine + 8 * v, dw[i]);
+  }
+}
+
+// Any width, pitch and alignment: the CTA's share of dw in shared memory, each value owned by one thread.
+template <typename T, bool kDh>
+__global__ void __launch_bounds__(512) norm_grad_any_kernel(const GradArgs a) {
+  extern __shared__ float dw[];
+  __shared__ float scratch[2][64];
+  griddep_launch_dependents();
+  griddep_wait();
+  const T* w = static_cast<const T*>(a.w);
+  for (int c = threadIdx.x; c < a.width; c += blockDim.x) dw[c] = 0.f;
+  int turn = 0;
+  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+    const T *h = static_cast<const T*>(a.h) + row * a.ldh, *dy = static_cast<const T*>(a.dy) + row * a.lddy;
+    float sum[2] = {0.f, 0.f};
+    for (int c = threadIdx.x; c < a.width; c += blockDim.x) {
+      const float v = to_f32(h[c]);
+      sum[0] = fmaf(v, v, sum[0]);
+      sum[1] = fmaf(to_f32(dy[c]) * to_f32(w[c]), v, sum[1]);
+    }
+    row_sum<false>(sum, scratch[turn]);
+    const float inv = 1.f / static_cast<float>(a.width);
+    const float r = rsqrtf(fmaf(sum[0], inv, a.eps)), back = r * r * (sum[1] * inv);
+    for (int c = threadIdx.x; c < a.width; c += blockDim.x) {
+      const float v = to_f32(h[c]), g = to_f32(dy[c]);
+      float dx = r * (g * to_f32(w[c]) - v * back);
+      if constexpr (kDh) dx += to_f32(static_cast<const T*>(a.dh)[row * a.lddh + c]);
+      static_cast<T*>(a.dx)[row * a.lddx + c] = from_f32<T>(dx);
+      dw[c] = fmaf(g, v * r, dw[c]);
+    }
+  }
+  float* mine = a.partial + static_cast<long long>(blockIdx.x) * a.width;
+  for (int c = threadIdx.x; c < a.width; c += blockDim.x) mine[c] = dw[c];
+}
+
+// dw = sum of the CTAs' shares, in their order.
+template <typename T>
+__global__ void __launch_bounds__(512) norm_grad_sum_kernel(const float* partial, int parts, int width, T* dw) {
+  __shared__ float sums[16][33];
+  griddep_launch_dependents();
+  griddep_wait();
+  const int lane = threadIdx.x & 31, part = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  float s = 0.f;
+  if (c < width)
+    for (int p = part; p < parts; p += 16) s += partial[static_cast<long long>(p) * width + c];
+  sums[part][lane] = s;
+  __syncthreads();
+  if (part == 0 && c < width) {
+    s = 0.f;
+#pragma unroll
+    for (int p = 0; p < 16; ++p) s += sums[p][lane];
+    dw[c] = from_f32<T>(s);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ launches
+template <typename T, bool kRes, bool kFp8>
+int launch_norm(const NormArgs& a, bool vectors, cudaStream_t st) {
+  Launch l(st);
+  if (!vectors) {
+    l.shape(static_cast<unsigned>(a.rows), 256);
+    return l(norm_any_kernel<T, kRes, kFp8>, "norm launch", a);
+  }
+  const int pieces = a.width / 8;
+  if (pieces <= 128) {
+    l.shape(static_cast<unsigned>((a.rows + 7) / 8), 256);
+    if (pieces <= 32) return l(norm_kernel<T, 1, true, kRes, kFp8>, "norm launch", a);
+    if (pieces <= 64) return l(norm_kernel<T, 2, true, kRes, kFp8>, "norm launch", a);
+    return l(norm_kernel<T, 4, true, kRes, kFp8>, "norm launch", a);
+  }
+  const int vpt = pieces <= 2048 ? 2 : 4;
+  l.shape(static_cast<unsigned>(a.rows), ((pieces + vpt - 1) / vpt + 31) / 32 * 32);
+  if (vpt == 2) return l(norm_kernel<T, 2, false, kRes, kFp8>, "norm launch", a);
+  return l(norm_kernel<T, 4, false, kRes, kFp8>, "norm launch", a);
+}
+
+template <typename T>
+int launch_norm(const NormArgs& a, bool vectors, cudaStream_t st) {
+  if (a.residual) return a.scales ? launch_norm<T, true, true>(a, vectors, st) : launch_norm<T, true, false>(a, vectors, st);
+  return a.scales ? launch_norm<T, false, true>(a, vectors, st) : launch_norm<T, false, false>(a, vectors, st);
+}
+
+constexpr int kMaxWidth = 32768;  // a row in a CTA's registers, its share of dw in shared memory
+
+// CTAs that walk the rows of the backward pass, each with its own share of dw.
+int grad_ctas(int sms, long long rows, int width) {
+  const long long most = static_cast<long long>(sms) * (width <= 4096 ? 4 : width <= 8192 ? 2 : 1);
+  return static_cast<int>(rows < most ? rows : most);
+}
+
+template <typename T, bool kDh>
+int launch_grad(const GradArgs& a, int ctas, bool vectors, cudaStream_t st) {
+  Launch l(st);
+  if (!vectors) {
+    const size_t smem = static_cast<size_t>(a.width) * sizeof(float);
+    if (smem > 40 * 1024) {
+      const cudaError_t e = cudaFuncSetAttribute(norm_grad_any_kernel<T, kDh>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 kMaxWidth * static_cast<int>(sizeof(float)));
+      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(MaxDynamicSharedMemorySize)");
+    }
+    l.shape(ctas, 512, smem);
+    return l(norm_grad_any_kernel<T, kDh>, "norm gradient launch", a);
+  }
+  const int pieces = a.width / 8, vpt = pieces <= 1024 ? 1 : pieces <= 2048 ? 2 : 4;
+  l.shape(ctas, ((pieces + vpt - 1) / vpt + 31) / 32 * 32);
+  if (vpt == 1) return l(norm_grad_kernel<T, 1, kDh>, "norm gradient launch", a);
+  if (vpt == 2) return l(norm_grad_kernel<T, 2, kDh>, "norm gradient launch", a);
+  return l(norm_grad_kernel<T, 4, kDh>, "norm gradient launch", a);
+}
+
+template <typename T>
+int launch_grad(const GradArgs& a, int ctas, bool vectors, cudaStream_t st) {
+  if (int e = a.dh ? launch_grad<T, true>(a, ctas, vectors, st) : launch_grad<T, false>(a, ctas, vectors, st)) return e;
+  Launch l(st);
+  l.shape((a.width + 31) / 32, 512);
+  return l(norm_grad_sum_kernel<T>, "norm gradient launch", static_cast<const float*>(a.partial), ctas, a.width,
+           static_cast<T*>(a.dw));
+}
+
+// Whether all rows of a matrix start on 16-byte boundaries and hold whole pieces of 8 values.
+bool pieces_of_8(uint64_t p, int64_t ld, int bytes) { return p % 16 == 0 && ld * bytes % 16 == 0; }
+
+int norm_checks(int64_t rows, int width, int dtype, float eps) {
+  if (rows < 0 || rows > 0x7fffffffLL) return fail(KCG_E_BAD_ARG, "number of rows out of range");
+  if (width <= 0 || width > kMaxWidth) return fail(KCG_E_BAD_ARG, "row width must be 1 to 32768");
+  if (!known_dtype(dtype)) return fail(KCG_E_BAD_ARG, "the norm takes float16, bfloat16 or float32 data");
+  if (!(eps >= 0.f) || eps > 3e38f) return fail(KCG_E_BAD_ARG, "eps must be finite and not negative");
+  return 0;
+}
+
+int norm_forward(int device, uint64_t stream, NormArgs a, uint64_t X, uint64_t R, uint64_t W, uint64_t Y, uint64_t H, int dtype) {
+  if (int e = norm_checks(a.rows, a.width, dtype, a.eps)) return e;
+  if (a.rows == 0) return 0;
+  if (!X || !W || !Y || !R != !H) return fail(KCG_E_BAD_ARG, "null matrix, or a residual without a place for the sum");
+  const bool fp8 = a.scales != nullptr;
+  if (a.ldx == 0) a.ldx = a.width;
+  if (a.ldr == 0) a.ldr = a.width;
+  if (a.ldy == 0) a.ldy = a.width;
+  if (a.ldh == 0) a.ldh = a.width;
+  if (a.ldx < a.width || a.ldr < a.width || a.ldy < a.width || a.ldh < a.width)
+    return fail(KCG_E_BAD_ARG, "leading dimension below the row length");
+  const int eb = dtype == KCG_DTYPE_FLOAT32 ? 4 : 2;
+  if ((X | R | W | H | (fp8 ? 0 : Y)) % eb) return fail(KCG_E_BAD_ARG, "operands must be aligned to their values");
+  const bool vectors = a.width % 8 == 0 && pieces_of_8(X, a.ldx, eb) && pieces_of_8(R, a.ldr, eb) && pieces_of_8(H, a.ldh, eb) &&
+                       W % 16 == 0 && (fp8 ? Y % 8 == 0 && a.ldy % 8 == 0 : pieces_of_8(Y, a.ldy, eb));
+  a.x = reinterpret_cast<const void*>(X), a.residual = reinterpret_cast<const void*>(R), a.w = reinterpret_cast<const void*>(W);
+  a.y = reinterpret_cast<void*>(Y), a.h = reinterpret_cast<void*>(H);
+  DeviceGuard guard;
+  const cudaError_t e = guard.enter(device);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaSetDevice");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (dtype == KCG_DTYPE_FLOAT32) return launch_norm<float>(a, vectors, st);
+  return dtype == KCG_DTYPE_FLOAT16 ? launch_norm<__half>(a, vectors, st) : launch_norm<__nv_bfloat16>(a, vectors, st);
+}
+
+}  // namespace
+
+extern "C" int kcg_rms_norm(int device, uint64_t stream, uint64_t X, int64_t ldx, uint64_t R, int64_t ldr, uint64_t W, uint64_t Y,
+                            int64_t ldy, uint64_t H, int64_t ldh, int64_t rows, int width, float eps, int dtype) {
+  NormArgs a{};
+  a.ldx = ldx, a.ldr = ldr, a.ldy = ldy, a.ldh = ldh, a.rows = rows, a.width = width, a.eps = eps;
+  return norm_forward(device, stream, a, X, R, W, Y, H, dtype);
+}
+
+extern "C" int kcg_rms_norm_fp8(int device, uint64_t stream, uint64_t X, int64_t ldx, uint64_t R, int64_t ldr, uint64_t W, uint64_t Q,
+                                int64_t ldq, uint64_t S, uint64_t H, int64_t ldh, int64_t rows, int width, float eps, int dtype) {
+  NormArgs a{};
+  if (!S || S % 4) return fail(KCG_E_BAD_ARG, "scales: null or not aligned to 4 bytes");
+  a.scales = reinterpret_cast<float*>(S), a.blocks = (width + 127) / 128;
+  a.ldx = ldx, a.ldr = ldr, a.ldy = ldq, a.ldh = ldh, a.rows = rows, a.width = width, a.eps = eps;
+  return norm_forward(device, stream, a, X, R, W, Q, H, dtype);
+}
+
+extern "C" int64_t kcg_rms_norm_backward_workspace(int device, int64_t rows, int width) {
+  if (rows <= 0 || width <= 0) return 0;
+  int sms = 0;
+  if (sm_count(device, &sms)) return -1;
+  return static_cast<int64_t>(grad_ctas(sms, rows, width)) * width * static_cast<int64_t>(sizeof(float));
+}
+
+extern "C" int kcg_rms_norm_backward(int device, uint64_t stream, uint64_t DY, int64_t lddy, uint64_t H, int64_t ldh, uint64_t W,
+                                     uint64_t DH, int64_t lddh, uint64_t DX, int64_t lddx, uint64_t DW, uint64_t workspace,
+                                     int64_t workspace_bytes, int64_t rows, int width, float eps, int dtype) {
+  if (int e = norm_checks(rows, width, dtype, eps)) return e;
+  if (rows == 0) return fail(KCG_E_BAD_ARG, "empty shape");
+  if (!DY || !H || !W || !DX || !DW || !workspace) return fail(KCG_E_BAD_ARG, "null matrix");
+  if (lddy == 0) lddy = width;
+  if (ldh == 0) ldh = width;
+  if (lddh == 0) lddh = width;
+  if (lddx == 0) lddx = width;
+  if (lddy < width || ldh < width || lddh < width || lddx < width) return fail(KCG_E_BAD_ARG, "leading dimension below the row length");
+  const int eb = dtype == KCG_DTYPE_FLOAT32 ? 4 : 2;
+  if ((DY | H | W | DH | DX | DW) % eb || workspace % 16) return fail(KCG_E_BAD_ARG, "operands must be aligned to their values");
+  int sms = 0;
+  if (int e = sm_count(device, &sms)) return e;
+  const int ctas = grad_ctas(sms, rows, width);
+  if (workspace_bytes < static_cast<int64_t>(ctas) * width * static_cast<int64_t>(sizeof(float)))
+    return fail(KCG_E_BAD_ARG, "workspace too small");
+  GradArgs a{};
+  a.dy = reinterpret_cast<const void*>(DY), a.h = reinterpret_cast<const void*>(H), a.w = reinterpret_cast<const void*>(W);
+  a.dh = reinterpret_cast<const void*>(DH), a.dx = reinterpret_cast<void*>(DX), a.dw = reinterpret_cast<void*>(DW);
+  a.partial = reinterpret_cast<float*>(workspace);
+  a.lddy = lddy, a.ldh = ldh, a.lddh = lddh, a.lddx = lddx, a.rows = rows, a.width = width, a.eps = eps;
+  const bool vectors = width % 8 == 0 && pieces_of_8(DY, lddy, eb) && pieces_of_8(H, ldh, eb) && pieces_of_8(DH, lddh, eb) &&
+                       pieces_of_8(DX, lddx, eb) && W % 16 == 0;
+  DeviceGuard guard;
+  const cudaError_t e = guard.enter(device);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaSetDevice");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (dtype == KCG_DTYPE_FLOAT32) return launch_grad<float>(a, ctas, vectors, st);
+  return dtype == KCG_DTYPE_FLOAT16 ? launch_grad<__half>(a, ctas, vectors, st) : launch_grad<__nv_bfloat16>(a, ctas, vectors, st);
+}

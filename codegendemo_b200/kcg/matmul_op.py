@@ -9,6 +9,8 @@ from codegendemo_b200.kcg.CompiledKernelFactory import CompiledKernelFactory, En
 from codegendemo_b200.kcg.KCGCompiler import KCGCompiler
 from codegendemo_b200.kcg.Operators.matmul import KernelArgMatmul
 from codegendemo_b200.kcg.Utils import DeviceInfo, EnumKernelDType, FromTorchType
+from codegendemo_b200.kcg.fp8_op import (matmul_fp8, matmul_fp8_status, quantize_fp8, rms_norm, rms_norm_backward,  # noqa: F401
+                                         rms_norm_fp8)
 
 
 def default_config(M: int, N: int, K: int, dtype: EnumKernelDType, out_dtype=None, **keys) -> KernelArgMatmul:

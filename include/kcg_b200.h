@@ -45,6 +45,9 @@ enum kcg_cfg_index {
 #define KCG_DTYPE_FLOAT16 2
 #define KCG_DTYPE_FLOAT32 4
 #define KCG_DTYPE_BFLOAT16 62
+/* 8-bit types of the block-scaled operands (below) */
+#define KCG_FP8_E4M3 1
+#define KCG_FP8_E5M2 2
 
 /* Kernel families. AUTO picks TCGEN05 when the tile shape is one the tensor-core
  * kernel can build and SIMT otherwise. */
@@ -221,6 +224,56 @@ int kcg_attention_fwd(int device, uint64_t stream, uint64_t Q, uint64_t K, uint6
 /* Synchronises `device` and reads (and clears) the status word of the kernel above: out = {code, block,
  * detail, detail}. Returns KCG_E_DEVICE_TIMEOUT when a bounded wait ran out since the last call, else 0. */
 int kcg_attention_status(int device, uint32_t out[4]);
+
+/* ---- the 8-bit linear layer -------------------------------------------------------------
+ * What stands in front of a linear layer, its 8-bit operands and its product; no counterpart in the reference (its type enum
+ * has a float8 that no kernel of it computes with). All are asynchronous on `stream`, allocate nothing and take matrices
+ * with a row pitch in elements (0 = contiguous). `dtype` is KCG_DTYPE_FLOAT16, _BFLOAT16 or _FLOAT32; sums are fp32.
+ *
+ * 8-bit operands come in blocks along the dimension that a product sums over: of each block scale = max(largest
+ * magnitude / 448 (e5m2: 57344), 2^-126), fp32, and values x / scale, rounded to nearest even. A NaN in a block
+ * makes its scale and its values NaN; an infinity makes the scale infinite and the infinite values NaN. Scales of a matrix lie row after row,
+ * ceil(columns / 128) to a row, one row for each block row.
+ *
+ * Root-mean-square norm: H = X + R, Y = H / sqrt(mean(H^2) + eps) * W, each row by itself. R = 0 (no residual): H = X, and H
+ * must be 0 too. Y and H are rounded once; Y comes from the unrounded sum. H may be X or R, Y may be X or R if H is not. Rows
+ * of up to 32768 values; whole 16-byte pieces (width a multiple of 8, aligned rows) are the fast case. */
+int kcg_rms_norm(int device, uint64_t stream, uint64_t X, int64_t ldx, uint64_t R, int64_t ldr, uint64_t W, uint64_t Y,
+                 int64_t ldy, uint64_t H, int64_t ldh, int64_t rows, int width, float eps, int dtype);
+/* The same with Y as e4m3 values Q in blocks of 1 x 128 and their scales S, from the unrounded Y. */
+int kcg_rms_norm_fp8(int device, uint64_t stream, uint64_t X, int64_t ldx, uint64_t R, int64_t ldr, uint64_t W, uint64_t Q,
+                     int64_t ldq, uint64_t S, uint64_t H, int64_t ldh, int64_t rows, int width, float eps, int dtype);
+/* Its gradient: with r = 1 / sqrt(mean(H^2) + eps) and g = DY * W, DX = DH + r * g - H * r^3 * mean(g * H) (DH = 0: no
+ * such term) and DW = sum over the rows of DY * H * r. DX may be DY or DH. The sums of DW go through `workspace` (16-byte aligned,
+ * as many bytes as the function below says, for these rows and this width; free again when the call's work is done) in an
+ * order that the shape and the device fix. */
+int64_t kcg_rms_norm_backward_workspace(int device, int64_t rows, int width);
+int kcg_rms_norm_backward(int device, uint64_t stream, uint64_t DY, int64_t lddy, uint64_t H, int64_t ldh, uint64_t W,
+                          uint64_t DH, int64_t lddh, uint64_t DX, int64_t lddx, uint64_t DW, uint64_t workspace,
+                          int64_t workspace_bytes, int64_t rows, int width, float eps, int dtype);
+/* 8-bit values and scales of a matrix in blocks of block_rows (1 or 128) x 128; `transposed`: of its transpose, whose rows (cols
+ * of them) are what is cut into blocks. `dtype8`: KCG_FP8_E4M3 or _E5M2. Rows of Q start on 16-byte boundaries, and a row's last
+ * 16-byte piece is written whole. */
+int kcg_quantize_fp8(int device, uint64_t stream, uint64_t X, int64_t ldx, uint64_t Q, int64_t ldq, uint64_t S, int64_t rows,
+                     int cols, int block_rows, int transposed, int dtype, int dtype8);
+/* C = act(sum over blocks of scale_a * scale_b * (A * B^T of the block) + beta * C + bias[col]): A is M x K in blocks of 1 x 128,
+ * B is N x K (a weight as linear layers keep it) in blocks of block_b (1 or 128) x 128. The scales' products have to
+ * be normal fp32 numbers. Rows of A and B start on 16-byte boundaries; C and bias are of dtype_c. beta * C is skipped when beta
+ * == 0. C must not overlap the operands. */
+typedef struct kcg_fp8_product {
+  uint64_t A, scale_a, B, scale_b, C, bias;
+  int64_t lda, ld_scale_a, ldb, ld_scale_b, ldc;
+  int32_t m, n, k;
+  int32_t block_b;
+  int32_t dtype_a, dtype_b; /* KCG_FP8_* */
+  int32_t dtype_c;          /* KCG_DTYPE_* */
+  float beta;
+  int32_t relu;
+  int32_t reserved[3];
+} kcg_fp8_product;
+int kcg_matmul_fp8(int device, uint64_t stream, const kcg_fp8_product* product);
+/* As kcg_attention_status, for kcg_matmul_fp8. */
+int kcg_matmul_fp8_status(int device, uint32_t out[4]);
 
 /* ---- M-sharded product with the all-gather of C fused into the kernel ---------------
  * No counterpart in the reference (it has no multi-GPU code). Rank r of G computes rows
