@@ -63,6 +63,27 @@ __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)
       : "memory");
 }
 
+// The same tensor memory spread as the products of mma.sync are: of 16 lanes (rows) and 8 columns a group, register 4 g + 2 h + e of a
+// thread holds row 8 h + lane / 4, column 8 g + 2 (lane % 4) + e.
+__device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+// Ties the registers of an earlier load to the wait before it: no use of them may be scheduled ahead of this.
+__device__ __forceinline__ void pin_32(uint32_t (&r)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i]));
+}
+__device__ __forceinline__ void pin_16(uint32_t (&r)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(r[i]));
+}
+
 __device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
@@ -71,6 +92,7 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr) {
 
 struct Fp8Params {
   CUtensorMap tmP, tmQ;  // {K, rows}: the operand whose rows are the tile's rows, and the one whose rows are its columns
+  CUtensorMap tmC;       // Fp8Pair, vector_store: {N, M}, blocks of 128 bytes x 32 rows
   const float *sp, *sq;  // scale of row i at block kb: s[(i >> shift) * ld + kb]
   long long ldsp, ldsq;
   int sp_shift, sq_shift;
@@ -82,6 +104,7 @@ struct Fp8Params {
   float beta;
   int relu;
   int vector_store;  // rows of C start on 16-byte boundaries
+  int vector_sp, vector_sq;  // so do those of the scales
   int splits;        // Fp8Tile: CTAs that share a tile's K
 };
 
@@ -373,26 +396,37 @@ __global__ void __launch_bounds__(192, Fp8Tile<kBN, kVector, kSwap, T>::CTAS_PER
   Fp8Tile<kBN, kVector, kSwap, T>::run(p);
 }
 
-// CTA pairs, tiles of 256 x 256, one after another. Each CTA holds 128 rows of A and 128 of B a stage; its eight accumulating warps
-// a row of the tile a thread, 128 columns each: warps 4-7 the first half, warps 8-11 the second.
+// CTA pairs, tiles of 256 x 256, one after another. Each CTA holds 128 rows of A and 128 of B a stage; of its eight accumulating
+// warps 4-7 take the first 128 columns, warps 8-11 the others. Warps 2 and 3 bring the scales of four blocks of K at a time into shared
+// memory.
+//
+// Where the columns of a half share a scale, a thread accumulates one row of 128 columns, times one factor. Where each has its own
+// (kVector), a thread takes two neighbouring columns of each eight of four rows, as tcgen05.ld.16x256b gives them: 32 scales
+// of columns and four of rows, where a row a thread would take 128 from shared memory, 16 bytes a lane, which alone is 1024
+// cycles of its port a block of K against 512 of the tensor pipe.
 template <bool kVector, typename T>
 struct Fp8Pair {
   static constexpr int NUM_THREADS = 384, kBM = 256, kBN = 256;
   static constexpr int HALF_BYTES = 128 * 128, STAGE_BYTES = 2 * HALF_BYTES;
-  static constexpr int STAGES = 6;
+  static constexpr int STAGES = 5;
   static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
-  static constexpr int SMEM_BYTES = RING_BYTES + 1024 + 4096;
+  static constexpr int STORE_BYTES = 8 * 32 * 128;  // a block of 32 rows of 128 bytes for each accumulating warp
+  static constexpr int SCALES = 128 + (kVector ? 256 : 4);  // of a block of K: the CTA's rows, the tile's columns (or halves)
+  static constexpr int GROUP_KB = 4;                        // blocks of K whose scales come together
+  static constexpr int SCALE_BYTES = 2 * GROUP_KB * SCALES * 4;
+  static constexpr int SMEM_BYTES = RING_BYTES + STORE_BYTES + SCALE_BYTES + 1024 + 512;
   static constexpr int GROUP = 8;  // tile rows that are walked together, column after column
   static constexpr uint32_t TMEM_COLS = 512;
+  static constexpr int COLS_BLOCK = 128 / static_cast<int>(sizeof(T));  // columns of a store
 
   struct Barriers {
     uint64_t full[STAGES], empty[STAGES];
     uint64_t tmem_full[2], tmem_empty[2];
+    uint64_t scale_full[2], scale_empty[2];
     uint32_t tmem_base;
     volatile uint32_t abort_flag;
-    alignas(16) float scale[2][2][kVector ? 128 : 4];  // [half][buffer][column]
   };
-  static_assert(sizeof(Barriers) <= 4096, "barrier block exceeds its shared-memory slot");
+  static_assert(sizeof(Barriers) <= 512, "barrier block exceeds its shared-memory slot");
 
   // Rows and columns of C at which tile i starts.
   __device__ static __forceinline__ void tile_at(int i, int tiles_m, int tiles_n, int& m0, int& n0) {
@@ -402,10 +436,108 @@ struct Fp8Pair {
     n0 = in / rows * kBN;
   }
 
+  // Four consecutive scales of a row (of an operand with `rows` of them, whose scales lie `ld` apart) from block kb on; those past
+  // the last block are not used.
+  __device__ static __forceinline__ float4 scales4(const float* s, long long ld, int shift, int row, int rows, int kb, int num_kb, bool vec) {
+    const float* at = s + (static_cast<long long>(min(row, rows - 1)) >> shift) * ld + kb;
+    if (vec && kb + 4 <= num_kb) return __ldg(reinterpret_cast<const float4*>(at));
+    const int left = num_kb - kb;
+    return make_float4(__ldg(at), left > 1 ? __ldg(at + 1) : 0.f, left > 2 ? __ldg(at + 2) : 0.f, left > 3 ? __ldg(at + 3) : 0.f);
+  }
+  __device__ static __forceinline__ void put4(float* slot, int i, const float4& v) {
+    slot[i] = v.x, slot[SCALES + i] = v.y, slot[2 * SCALES + i] = v.z, slot[3 * SCALES + i] = v.w;
+  }
+
+  // This warp's accumulators to C: `at(c)` is the row's (kVector: the rows') values of columns c on.
+  __device__ static __forceinline__ void store(const Fp8Params& p, float (&acc)[128], int row0, int col0, uint8_t* block) {
+    const int lane = threadIdx.x & 31;
+    if constexpr (!kVector) {
+      const int m = row0 + lane;
+      if (!p.vector_store) {
+        if (m < p.rows_p)
+#pragma unroll
+          for (int c = 0; c < 128; c += 8) store_span8<T>(p, acc + c, m, col0 + c, p.rows_q);
+        return;
+      }
+      T* out = static_cast<T*>(p.C) + static_cast<long long>(m) * p.ldc + col0;
+#pragma unroll
+      for (int c0 = 0; c0 < 128; c0 += COLS_BLOCK) {
+        if (row0 >= p.rows_p || col0 + c0 >= p.rows_q) break;
+        if (lane == 0) tma_store_wait_read<0>();
+        __syncwarp();
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {  // 16 bytes
+          constexpr int kN = 16 / static_cast<int>(sizeof(T));
+          float v[kN];
+#pragma unroll
+          for (int i = 0; i < kN; ++i) {
+            const int c = c0 + u * kN + i;
+            v[i] = acc[c];
+            const bool in = m < p.rows_p && col0 + c < p.rows_q;
+            if (p.beta != 0.f && in) v[i] = fmaf(p.beta, to_f32(out[c]), v[i]);
+            if (p.bias && in) v[i] += bias_at<T>(p, col0 + c);
+            if (p.relu) v[i] = fmaxf(v[i], 0.f);
+          }
+          uint4 raw;
+          if constexpr (kN == 4) {
+            raw = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+          } else {
+            raw = make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()), pack2(v[4], v[5], T()), pack2(v[6], v[7], T()));
+          }
+          *reinterpret_cast<uint4*>(block + lane * 128 + ((u ^ (lane & 7)) << 4)) = raw;
+        }
+        send(p, block, row0, col0 + c0);
+      }
+    } else {
+#pragma unroll
+      for (int c0 = 0; c0 < 128; c0 += COLS_BLOCK) {
+        if (row0 >= p.rows_p || col0 + c0 >= p.rows_q) break;
+        if (p.vector_store) {
+          if (lane == 0) tma_store_wait_read<0>();
+          __syncwarp();
+        }
+#pragma unroll
+        for (int j = c0 / 8; j < (c0 + COLS_BLOCK) / 8; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int row = r * 8 + (lane >> 2), m = row0 + row, c = j * 8 + (lane & 3) * 2, n = col0 + c;
+            float v[2] = {acc[j * 8 + r * 2], acc[j * 8 + r * 2 + 1]};
+            T* out = static_cast<T*>(p.C) + static_cast<long long>(m) * p.ldc + n;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (m < p.rows_p && n + i < p.rows_q) v[i] = finish<T>(p, v[i], out + i, bias_at<T>(p, n + i));
+            if (p.vector_store) {
+              const uint32_t byte = static_cast<uint32_t>(c - c0) * sizeof(T);
+              uint8_t* to = block + row * 128 + (((byte >> 4) ^ (row & 7)) << 4) + (byte & 15);
+              if constexpr (sizeof(T) == 4) {
+                *reinterpret_cast<float2*>(to) = make_float2(v[0], v[1]);
+              } else {
+                *reinterpret_cast<uint32_t*>(to) = pack2(v[0], v[1], T());
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+                if (m < p.rows_p && n + i < p.rows_q) out[i] = from_f32<T>(v[i]);
+            }
+          }
+        if (p.vector_store) send(p, block, row0, col0 + c0);
+      }
+    }
+  }
+  __device__ static __forceinline__ void send(const Fp8Params& p, uint8_t* block, int row, int col) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) {
+      tma_store_2d(&p.tmC, block, col, row);
+      tma_store_commit();
+    }
+  }
+
   __device__ static void run(const Fp8Params& p) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    Barriers* bars = reinterpret_cast<Barriers*>(smem + RING_BYTES);
+    float* scales = reinterpret_cast<float*>(smem + RING_BYTES + STORE_BYTES);
+    Barriers* bars = reinterpret_cast<Barriers*>(smem + RING_BYTES + STORE_BYTES + SCALE_BYTES);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_cta_rank();  // 0 = leader
     const int tiles_m = (p.rows_p + kBM - 1) / kBM, tiles_n = (p.rows_q + kBN - 1) / kBN, tiles = tiles_m * tiles_n;
@@ -421,6 +553,8 @@ struct Fp8Pair {
       for (int b = 0; b < 2; ++b) {
         mbar_init(&bars->tmem_full[b], 1);
         mbar_init(&bars->tmem_empty[b], 16);  // one arrival per accumulating warp of each CTA
+        mbar_init(&bars->scale_full[b], 64);
+        mbar_init(&bars->scale_empty[b], 8);
       }
       bars->abort_flag = 0u;
       fence_mbar_init();
@@ -464,95 +598,170 @@ struct Fp8Pair {
         }
         __syncwarp();
         griddep_launch_dependents();
-      } else if (warp == 1 && rank == 0u) {
-        const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
-        const uint64_t adesc = make_smem_desc(smem_u32(smem), 16, 1024, SWZ_128B);
-        const uint64_t bdesc = make_smem_desc(smem_u32(smem) + HALF_BYTES, 16, 1024, SWZ_128B);
-        const uint32_t idesc = make_instr_desc(0u, 0u, 0u, 256u, kBN) | p.fmt_p << 7 | p.fmt_q << 10;
-        uint32_t it = 0;
+      } else if (warp == 1) {
+        if (rank == 0u) {
+          const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+          const uint64_t adesc = make_smem_desc(smem_u32(smem), 16, 1024, SWZ_128B);
+          const uint64_t bdesc = make_smem_desc(smem_u32(smem) + HALF_BYTES, 16, 1024, SWZ_128B);
+          const uint32_t idesc = make_instr_desc(0u, 0u, 0u, 256u, kBN) | p.fmt_p << 7 | p.fmt_q << 10;
+          uint32_t it = 0;
+          bool ok = true;
+          for (int tile = tile0; tile < tiles && ok; tile += stride) {
+            for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
+              const uint32_t s = it % STAGES, b = it & 1u;
+              if (!mbar_wait_warp(&bars->tmem_empty[b], ((it >> 1) & 1u) ^ 1u, &bars->abort_flag) ||
+                  !mbar_wait_warp(&bars->full[s], (it / STAGES) & 1u, &bars->abort_flag)) {
+                if (lane == 0) report(bars, FP8_TIMEOUT_MMA, it, s);
+                ok = false;
+                break;
+              }
+              tc_fence_after_sync();
+              if (elect_one()) {
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks)
+                  umma_fp8<2>(tmem + b * kBN, adesc + s * (STAGE_BYTES >> 4) + ks * 2, bdesc + s * (STAGE_BYTES >> 4) + ks * 2, idesc,
+                              ks > 0 ? 1u : 0u);
+                umma_commit_pair(smem_u32(&bars->empty[s]));
+                umma_commit_pair(map_to_cta(smem_u32(&bars->empty[s]), 1u));
+                umma_commit_pair(smem_u32(&bars->tmem_full[b]));
+                umma_commit_pair(map_to_cta(smem_u32(&bars->tmem_full[b]), 1u));
+              }
+              __syncwarp();
+            }
+          }
+        }
+      } else {
+        // ------------------------------------------------------------ scales, GROUP_KB blocks at a time
+        const int t = threadIdx.x - 64;
+        uint32_t g = 0;
         bool ok = true;
         for (int tile = tile0; tile < tiles && ok; tile += stride) {
-          for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
-            const uint32_t s = it % STAGES, b = it & 1u;
-            if (!mbar_wait_warp(&bars->tmem_empty[b], ((it >> 1) & 1u) ^ 1u, &bars->abort_flag) ||
-                !mbar_wait_warp(&bars->full[s], (it / STAGES) & 1u, &bars->abort_flag)) {
-              if (lane == 0) report(bars, FP8_TIMEOUT_MMA, it, s);
+          int m0, n0;
+          tile_at(tile, tiles_m, tiles_n, m0, n0);
+          m0 += static_cast<int>(rank) * 128;
+          for (int kb = 0; kb < p.num_kb; kb += GROUP_KB, ++g) {
+            const uint32_t b = g & 1u;
+            float* slot = scales + b * GROUP_KB * SCALES;
+            const float4 p0 = scales4(p.sp, p.ldsp, p.sp_shift, m0 + t, p.rows_p, kb, p.num_kb, p.vector_sp);
+            const float4 p1 = scales4(p.sp, p.ldsp, p.sp_shift, m0 + 64 + t, p.rows_p, kb, p.num_kb, p.vector_sp);
+            float4 q[kVector ? 4 : 1];
+            if constexpr (kVector) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                q[i] = scales4(p.sq, p.ldsq, p.sq_shift, n0 + i * 64 + t, p.rows_q, kb, p.num_kb, p.vector_sq);
+            } else if (t < 2) {
+              q[0] = scales4(p.sq, p.ldsq, p.sq_shift, n0 + t * 128, p.rows_q, kb, p.num_kb, p.vector_sq);
+            }
+            if (!mbar_wait(&bars->scale_empty[b], ((g >> 1) & 1u) ^ 1u, &bars->abort_flag)) {
+              report(bars, FP8_TIMEOUT_PRODUCER, g, 100u);
               ok = false;
               break;
             }
-            tc_fence_after_sync();
-            if (elect_one()) {
+            put4(slot, t, p0);
+            put4(slot, 64 + t, p1);
+            if constexpr (kVector) {
 #pragma unroll
-              for (int ks = 0; ks < 4; ++ks)
-                umma_fp8<2>(tmem + b * kBN, adesc + s * (STAGE_BYTES >> 4) + ks * 2, bdesc + s * (STAGE_BYTES >> 4) + ks * 2, idesc,
-                            ks > 0 ? 1u : 0u);
-              umma_commit_pair(smem_u32(&bars->empty[s]));
-              umma_commit_pair(map_to_cta(smem_u32(&bars->empty[s]), 1u));
-              umma_commit_pair(smem_u32(&bars->tmem_full[b]));
-              umma_commit_pair(map_to_cta(smem_u32(&bars->tmem_full[b]), 1u));
+              for (int i = 0; i < 4; ++i) put4(slot, 128 + i * 64 + t, q[i]);
+            } else if (t < 2) {
+              put4(slot, 128 + t, q[0]);
             }
-            __syncwarp();
+            mbar_arrive(&bars->scale_full[b]);
           }
         }
       }
     } else {
       asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-      const int q = warp & 3, half = (warp - 4) >> 2, row = q * 32 + lane;
-      const int t = threadIdx.x & 127;  // column of the half whose scale this thread fetches
-      uint32_t it = 0;
+      const int q = warp & 3, half = (warp - 4) >> 2;
+      uint8_t* block = smem + RING_BYTES + (warp - 4) * 4096;
+      uint32_t it = 0, g = 0;
       bool ok = true;
-      for (int tile = tile0; tile < tiles; tile += stride) {
-        int m0, n0;
-        tile_at(tile, tiles_m, tiles_n, m0, n0);
-        m0 += static_cast<int>(rank) * 128;
-        n0 += half * 128;
+      auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t what) {
+        if (ok) {
+          ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, &bars->abort_flag));
+          if (!ok && lane == 0) report(bars, FP8_TIMEOUT_ACCUMULATE, it, what);
+        }
+        return ok;
+      };
+      for (int tile = tile0; tile < tiles && ok; tile += stride) {
         float acc[128];
 #pragma unroll
         for (int i = 0; i < 128; ++i) acc[i] = 0.f;
-        const float* sp = p.sp + (static_cast<long long>(min(m0 + row, p.rows_p - 1)) >> p.sp_shift) * p.ldsp;
-        const float* sq = p.sq + (static_cast<long long>(min(n0 + (kVector ? t : 0), p.rows_q - 1)) >> p.sq_shift) * p.ldsq;
-        float next_p = __ldg(sp), next_q = __ldg(sq);
-        for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
-          const uint32_t b = it & 1u;
-          const float f = kVector ? next_p : scale_product(next_p, next_q);
-          if constexpr (kVector) {
-            bars->scale[half][b][t] = next_q;
-            named_bar_sync(1 + half, 128);
-          }
-          if (kb + 1 < p.num_kb) {
-            next_p = __ldg(sp + kb + 1);
-            next_q = __ldg(sq + kb + 1);
-          }
-          if (ok) {
-            const bool got = mbar_wait(&bars->tmem_full[b], (it >> 1) & 1u, &bars->abort_flag);
-            if (!__all_sync(0xffffffffu, got)) {
-              if (lane == 0) report(bars, FP8_TIMEOUT_ACCUMULATE, it, b);
-              ok = false;
-            }
-          }
-          if (!ok) continue;  // (the meetings go on)
-          tc_fence_after_sync();
+        for (int kb = 0; kb < p.num_kb && ok; ++kb, ++it) {
+          const uint32_t b = it & 1u, sb = g & 1u;
+          if (kb % GROUP_KB == 0 && !wait(&bars->scale_full[sb], (g >> 1) & 1u, 2u)) break;
+          const float* slot = scales + (sb * GROUP_KB + kb % GROUP_KB) * SCALES;
           const uint32_t col = tmem_base + b * kBN + half * 128 + (static_cast<uint32_t>(q * 32) << 16);
+          auto release = [&]() {  // (the reads are complete)
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster_cta(map_to_cta(smem_u32(&bars->tmem_empty[b]), 0u));
+          };
+          if constexpr (!kVector) {
+            const float f = scale_product(slot[q * 32 + lane], slot[128 + half]);
+            if (!wait(&bars->tmem_full[b], (it >> 1) & 1u, 0u)) break;
+            tc_fence_after_sync();
+            uint32_t r[2][32];
+            tmem_ld_32x32b_x32(col, r[0]);
 #pragma unroll
-          for (int c = 0; c < 128; c += 32) {
-            uint32_t r[32];
-            tmem_ld_32x32b_x32(col + c, r);
-            tmem_ld_wait();
-            if constexpr (kVector) {
-              add_scaled<32>(acc + c, r, &bars->scale[half][b][c], f);
-            } else {
-              add_scaled<32>(acc + c, r, f);
+            for (int c = 0; c < 4; ++c) {
+              tmem_ld_wait();
+              pin_32(r[c & 1]);
+              if (c < 3) {
+                tmem_ld_32x32b_x32(col + (c + 1) * 32, r[(c + 1) & 1]);
+              } else {
+                release();
+              }
+              add_scaled<32>(acc + c * 32, r[c & 1], f);
+            }
+          } else {
+            float f[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = slot[q * 32 + i * 8 + (lane >> 2)];
+            const float* column = slot + 128 + half * 128 + (lane & 3) * 2;
+            if (!wait(&bars->tmem_full[b], (it >> 1) & 1u, 0u)) break;
+            tc_fence_after_sync();
+            // 32 columns at a time, rows 0-15 and 16-31 of the warp's lanes
+            uint32_t r[2][2][16];
+            tmem_ld_16x256b_x4(col, r[0][0]);
+            tmem_ld_16x256b_x4(col + (16u << 16), r[0][1]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              tmem_ld_wait();
+              pin_16(r[c & 1][0]);
+              pin_16(r[c & 1][1]);
+              if (c < 3) {
+                tmem_ld_16x256b_x4(col + (c + 1) * 32, r[(c + 1) & 1][0]);
+                tmem_ld_16x256b_x4(col + (c + 1) * 32 + (16u << 16), r[(c + 1) & 1][1]);
+              } else {
+                release();
+              }
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float2 s = *reinterpret_cast<const float2*>(column + c * 32 + j * 8);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {  // rows i * 8 + lane / 4
+                  const uint32_t* part = &r[c & 1][i >> 1][j * 4 + (i & 1) * 2];
+                  float* a = acc + (c * 4 + j) * 8 + i * 2;
+                  const float2 y = __ffma2_rn(__fmul2_rn(make_float2(__uint_as_float(part[0]), __uint_as_float(part[1])), s),
+                                              make_float2(f[i], f[i]), make_float2(a[0], a[1]));
+                  a[0] = y.x, a[1] = y.y;
+                }
+              }
             }
           }
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster_cta(map_to_cta(smem_u32(&bars->tmem_empty[b]), 0u));  // (the reads are complete)
+          if (kb % GROUP_KB == GROUP_KB - 1 || kb == p.num_kb - 1) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->scale_empty[sb]);
+            ++g;
+          }
         }
-        if (ok && m0 + row < p.rows_p) {
-#pragma unroll
-          for (int c = 0; c < 128; c += 8) store_span8<T>(p, acc + c, m0 + row, n0 + c, p.rows_q);
-        }
+        if (!ok) break;
+        int m0, n0;
+        tile_at(tile, tiles_m, tiles_n, m0, n0);
+        store(p, acc, m0 + static_cast<int>(rank) * 128 + q * 32, n0 + half * 128, block);
       }
+      if (lane == 0) tma_store_wait_read<0>();  // shared memory outlives the stores' reads
+      __syncwarp();
     }
 
     // ------------------------------------------------------------ common exit
@@ -607,6 +816,20 @@ int encode(EncodeFn fn, CUtensorMap* tm, uint64_t ptr, int k, int64_t ld, int ro
   const CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, reinterpret_cast<void*>(ptr), gdim, gstride, box, estr,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : fail(static_cast<int>(r), "cuTensorMapEncodeTiled failed");
+}
+
+// C, for stores of 128 bytes x 32 rows; what lies past it is not stored.
+int encode_c(EncodeFn fn, CUtensorMap* tm, uint64_t ptr, int dtype, int n, int64_t ld, int m) {
+  const int eb = dtype == KCG_DTYPE_FLOAT32 ? 4 : 2;
+  cuuint64_t gdim[2] = {static_cast<cuuint64_t>(n), static_cast<cuuint64_t>(m)};
+  cuuint64_t gstride[1] = {static_cast<cuuint64_t>(ld) * eb};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / eb), 32}, estr[2] = {1, 1};
+  const CUtensorMapDataType type = dtype == KCG_DTYPE_FLOAT32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : dtype == KCG_DTYPE_FLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUresult r = fn(tm, type, 2, reinterpret_cast<void*>(ptr), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : fail(static_cast<int>(r), "cuTensorMapEncodeTiled failed");
 }
 
@@ -750,6 +973,10 @@ extern "C" int kcg_matmul_fp8(int device, uint64_t stream, const kcg_fp8_product
   p.C = reinterpret_cast<void*>(a->C), p.ldc = ldc, p.bias = reinterpret_cast<const void*>(a->bias);
   p.beta = a->beta, p.relu = a->relu, p.splits = plan.splits;
   p.vector_store = a->C % 16 == 0 && ldc * eb % 16 == 0;
+  p.vector_sp = reinterpret_cast<uint64_t>(p.sp) % 16 == 0 && p.ldsp % 4 == 0;
+  p.vector_sq = reinterpret_cast<uint64_t>(p.sq) % 16 == 0 && p.ldsq % 4 == 0;
+  if (plan.pair && p.vector_store)
+    if (int r = encode_c(enc, &p.tmC, a->C, a->dtype_c, a->n, ldc, a->m)) return r;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool vector = a->block_b == 1;
   if (a->dtype_c == KCG_DTYPE_FLOAT32) return launch<float>(plan, device, sms, st, p, vector);
