@@ -65,14 +65,11 @@ __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)
 
 // The same tensor memory spread as the products of mma.sync are: of 16 lanes (rows) and 8 columns a group, register 4 g + 2 h + e of a
 // thread holds row 8 h + lane / 4, column 8 g + 2 (lane % 4) + e.
-__device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
-      : "memory");
+__device__ __forceinline__ void tmem_ld_16x256b_x2(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
 }
 // Ties the registers of an earlier load to the wait before it: no use of them may be scheduled ahead of this.
 __device__ __forceinline__ void pin_32(uint32_t (&r)[32]) {
@@ -82,6 +79,17 @@ __device__ __forceinline__ void pin_32(uint32_t (&r)[32]) {
 __device__ __forceinline__ void pin_16(uint32_t (&r)[16]) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(r[i]));
+}
+__device__ __forceinline__ void pin_8(uint32_t (&r)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) asm volatile("" : "+r"(r[i]));
+}
+
+// Completion of the pair's products issued so far -> one arrival on this barrier of both CTAs.
+__device__ __forceinline__ void umma_commit_both(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+               "h"(static_cast<uint16_t>(3))
+               : "memory");
 }
 
 __device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr) {
@@ -103,6 +111,7 @@ struct Fp8Params {
   const void* bias;
   float beta;
   int relu;
+  int fused;  // any of the three
   int vector_store;  // rows of C start on 16-byte boundaries
   int vector_sp, vector_sq;  // so do those of the scales
   int splits;        // Fp8Tile: CTAs that share a tile's K
@@ -396,9 +405,14 @@ __global__ void __launch_bounds__(192, Fp8Tile<kBN, kVector, kSwap, T>::CTAS_PER
   Fp8Tile<kBN, kVector, kSwap, T>::run(p);
 }
 
-// CTA pairs, tiles of 256 x 256, one after another. Each CTA holds 128 rows of A and 128 of B a stage; of its eight accumulating
-// warps 4-7 take the first 128 columns, warps 8-11 the others. Warps 2 and 3 bring the scales of four blocks of K at a time into shared
-// memory.
+// CTA pairs, tiles of 256 x 256, one after another. Each CTA holds 128 rows of A and 128 of B a stage. Eleven warps of up to 184
+// registers: warp 0 waits in the accumulating warps' place, warp 1 of the leader issues the products, warp 2 loads the operands and brings
+// the scales of four blocks of K at a time into shared memory, warps 3-6 accumulate the first 128 columns and warps 7-10 the others.
+//
+// A block of K takes 512 cycles of the tensor pipe, and its accumulator has to be read, and the leader's issuer to hear of it from both
+// CTAs, while the other fills. The products' operands and TMA fill the shared-memory port, where an access then takes
+// hundreds of cycles, so the accumulating warps look at no mbarrier and spill nothing: warp 0 looks, and meets them on two named barriers
+// a block. (With mbarriers of their own a block took 1070 cycles, with a few spilled registers 1300.)
 //
 // Where the columns of a half share a scale, a thread accumulates one row of 128 columns, times one factor. Where each has its own
 // (kVector), a thread takes two neighbouring columns of each eight of four rows, as tcgen05.ld.16x256b gives them: 32 scales
@@ -406,11 +420,11 @@ __global__ void __launch_bounds__(192, Fp8Tile<kBN, kVector, kSwap, T>::CTAS_PER
 // cycles of its port a block of K against 512 of the tensor pipe.
 template <bool kVector, typename T>
 struct Fp8Pair {
-  static constexpr int NUM_THREADS = 384, kBM = 256, kBN = 256;
+  static constexpr int NUM_THREADS = 352, kBM = 256, kBN = 256;
   static constexpr int HALF_BYTES = 128 * 128, STAGE_BYTES = 2 * HALF_BYTES;
-  static constexpr int STAGES = 5;
+  static constexpr int STAGES = 4;  // (three are as fast)
   static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
-  static constexpr int STORE_BYTES = 8 * 32 * 128;  // a block of 32 rows of 128 bytes for each accumulating warp
+  static constexpr int STORE_BYTES = 8 * 2 * 32 * 128;  // two blocks of 32 rows of 128 bytes for each accumulating warp
   static constexpr int SCALES = 128 + (kVector ? 256 : 4);  // of a block of K: the CTA's rows, the tile's columns (or halves)
   static constexpr int GROUP_KB = 4;                        // blocks of K whose scales come together
   static constexpr int SCALE_BYTES = 2 * GROUP_KB * SCALES * 4;
@@ -428,6 +442,10 @@ struct Fp8Pair {
   };
   static_assert(sizeof(Barriers) <= 512, "barrier block exceeds its shared-memory slot");
 
+  // Named barrier on which warp 0 and the accumulating warps meet in every block of K: the block's accumulator is complete, its scales
+  // and the next block's are in shared memory. All leave together where a wait of warp 0 ran out.
+  static constexpr uint32_t BAR_FULL = 1, MEETING = 32 + 256;
+
   // Rows and columns of C at which tile i starts.
   __device__ static __forceinline__ void tile_at(int i, int tiles_m, int tiles_n, int& m0, int& n0) {
     const int per_group = GROUP * tiles_n, group = i / per_group, first = group * GROUP;
@@ -436,92 +454,101 @@ struct Fp8Pair {
     n0 = in / rows * kBN;
   }
 
-  // Four consecutive scales of a row (of an operand with `rows` of them, whose scales lie `ld` apart) from block kb on; those past
-  // the last block are not used.
-  __device__ static __forceinline__ float4 scales4(const float* s, long long ld, int shift, int row, int rows, int kb, int num_kb, bool vec) {
-    const float* at = s + (static_cast<long long>(min(row, rows - 1)) >> shift) * ld + kb;
-    if (vec && kb + 4 <= num_kb) return __ldg(reinterpret_cast<const float4*>(at));
-    const int left = num_kb - kb;
-    return make_float4(__ldg(at), left > 1 ? __ldg(at + 1) : 0.f, left > 2 ? __ldg(at + 2) : 0.f, left > 3 ? __ldg(at + 3) : 0.f);
-  }
-  __device__ static __forceinline__ void put4(float* slot, int i, const float4& v) {
-    slot[i] = v.x, slot[SCALES + i] = v.y, slot[2 * SCALES + i] = v.z, slot[3 * SCALES + i] = v.w;
-  }
+  // The scales of GROUP_KB blocks of K, on their way through the registers of warp 2: four rows of the tile a lane (kVector: and
+  // eight columns).
+  struct Scales {
+    float4 p[4], q[kVector ? 8 : 1];
+    __device__ static __forceinline__ float4 four(const float* s, long long ld, int shift, int row, int rows, int kb, int num_kb, bool vec) {
+      const float* at = s + (static_cast<long long>(min(row, rows - 1)) >> shift) * ld + kb;
+      if (vec && kb + 4 <= num_kb) return __ldg(reinterpret_cast<const float4*>(at));
+      const int left = num_kb - kb;  // (those past the last block are not used)
+      return make_float4(__ldg(at), left > 1 ? __ldg(at + 1) : 0.f, left > 2 ? __ldg(at + 2) : 0.f, left > 3 ? __ldg(at + 3) : 0.f);
+    }
+    __device__ __forceinline__ void load(const Fp8Params& a, int m0, int n0, int kb) {
+      const int lane = threadIdx.x & 31;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = four(a.sp, a.ldsp, a.sp_shift, m0 + i * 32 + lane, a.rows_p, kb, a.num_kb, a.vector_sp);
+      if constexpr (kVector) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = four(a.sq, a.ldsq, a.sq_shift, n0 + i * 32 + lane, a.rows_q, kb, a.num_kb, a.vector_sq);
+      } else {
+        q[0] = four(a.sq, a.ldsq, a.sq_shift, n0 + (lane & 1) * 128, a.rows_q, kb, a.num_kb, a.vector_sq);
+      }
+    }
+    __device__ static __forceinline__ void put4(float* slot, int i, const float4& v) {
+      slot[i] = v.x, slot[SCALES + i] = v.y, slot[2 * SCALES + i] = v.z, slot[3 * SCALES + i] = v.w;
+    }
+    __device__ __forceinline__ void store(float* slot) const {
+      const int lane = threadIdx.x & 31;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) put4(slot, i * 32 + lane, p[i]);
+      if constexpr (kVector) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) put4(slot, 128 + i * 32 + lane, q[i]);
+      } else if (lane < 2) {
+        put4(slot, 128 + lane, q[0]);
+      }
+    }
+  };
 
-  // This warp's accumulators to C: `at(c)` is the row's (kVector: the rows') values of columns c on.
-  __device__ static __forceinline__ void store(const Fp8Params& p, float (&acc)[128], int row0, int col0, uint8_t* block) {
+  // This warp's accumulators to C: 32 rows of 128 columns, through blocks of shared memory (16-byte units XORed with the row, the
+  // swizzle of the tensor map) and TMA stores, two under way.
+  __device__ static __forceinline__ void store(const Fp8Params& p, float (&acc)[128], int row0, int col0, uint8_t* blocks) {
     const int lane = threadIdx.x & 31;
-    if constexpr (!kVector) {
-      const int m = row0 + lane;
-      if (!p.vector_store) {
-        if (m < p.rows_p)
+    // Row and column of accumulator i: kVector as tcgen05.ld.16x256b lays them out, else a row a thread.
+    auto row_of = [&](int i) { return kVector ? (i >> 1 & 3) * 8 + (lane >> 2) : lane; };
+    auto col_of = [&](int i) { return kVector ? (i >> 3) * 8 + (lane & 3) * 2 + (i & 1) : i; };
+    if (p.fused || !p.vector_store) {
 #pragma unroll
-          for (int c = 0; c < 128; c += 8) store_span8<T>(p, acc + c, m, col0 + c, p.rows_q);
-        return;
+      for (int i = 0; i < 128; ++i) {
+        const int m = row0 + row_of(i), n = col0 + col_of(i);
+        if (m < p.rows_p && n < p.rows_q) {
+          T* c = static_cast<T*>(p.C) + static_cast<long long>(m) * p.ldc + n;
+          acc[i] = finish<T>(p, acc[i], c, bias_at<T>(p, n));
+          if (!p.vector_store) *c = from_f32<T>(acc[i]);
+        }
       }
-      T* out = static_cast<T*>(p.C) + static_cast<long long>(m) * p.ldc + col0;
+      if (!p.vector_store) return;
+    }
 #pragma unroll
-      for (int c0 = 0; c0 < 128; c0 += COLS_BLOCK) {
-        if (row0 >= p.rows_p || col0 + c0 >= p.rows_q) break;
-        if (lane == 0) tma_store_wait_read<0>();
-        __syncwarp();
+    for (int b = 0; b < 128 / COLS_BLOCK; ++b) {
+      if (row0 >= p.rows_p || col0 + b * COLS_BLOCK >= p.rows_q) break;
+      uint8_t* block = blocks + (b & 1) * 4096;
+      if (lane == 0) tma_store_wait_read<1>();  // the store before the last has read its block
+      __syncwarp();
+      if constexpr (!kVector) {
+        uint8_t* to = block + lane * 128;
+        const float* v = acc + b * COLS_BLOCK;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {  // 16 bytes
-          constexpr int kN = 16 / static_cast<int>(sizeof(T));
-          float v[kN];
-#pragma unroll
-          for (int i = 0; i < kN; ++i) {
-            const int c = c0 + u * kN + i;
-            v[i] = acc[c];
-            const bool in = m < p.rows_p && col0 + c < p.rows_q;
-            if (p.beta != 0.f && in) v[i] = fmaf(p.beta, to_f32(out[c]), v[i]);
-            if (p.bias && in) v[i] += bias_at<T>(p, col0 + c);
-            if (p.relu) v[i] = fmaxf(v[i], 0.f);
-          }
+        for (int u = 0; u < 8; ++u) {
           uint4 raw;
-          if constexpr (kN == 4) {
-            raw = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+          if constexpr (sizeof(T) == 4) {
+            raw = make_uint4(__float_as_uint(v[4 * u]), __float_as_uint(v[4 * u + 1]), __float_as_uint(v[4 * u + 2]),
+                             __float_as_uint(v[4 * u + 3]));
           } else {
-            raw = make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()), pack2(v[4], v[5], T()), pack2(v[6], v[7], T()));
+            raw = make_uint4(pack2(v[8 * u], v[8 * u + 1], T()), pack2(v[8 * u + 2], v[8 * u + 3], T()),
+                             pack2(v[8 * u + 4], v[8 * u + 5], T()), pack2(v[8 * u + 6], v[8 * u + 7], T()));
           }
-          *reinterpret_cast<uint4*>(block + lane * 128 + ((u ^ (lane & 7)) << 4)) = raw;
+          *reinterpret_cast<uint4*>(to + ((u ^ (lane & 7)) << 4)) = raw;
         }
-        send(p, block, row0, col0 + c0);
-      }
-    } else {
+      } else {
+        const uint32_t x = lane >> 2, t = lane & 3;  // (row within eight, pair of columns within eight)
+        uint8_t* to = block + x * 128 + (sizeof(T) == 4 ? (t & 1) * 8 : t * 4);
+        const uint32_t swizzle = (sizeof(T) == 4 ? x ^ (t >> 1) : x) << 4;
 #pragma unroll
-      for (int c0 = 0; c0 < 128; c0 += COLS_BLOCK) {
-        if (row0 >= p.rows_p || col0 + c0 >= p.rows_q) break;
-        if (p.vector_store) {
-          if (lane == 0) tma_store_wait_read<0>();
-          __syncwarp();
-        }
-#pragma unroll
-        for (int j = c0 / 8; j < (c0 + COLS_BLOCK) / 8; ++j)
+        for (int j = 0; j < COLS_BLOCK / 8; ++j)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int row = r * 8 + (lane >> 2), m = row0 + row, c = j * 8 + (lane & 3) * 2, n = col0 + c;
-            float v[2] = {acc[j * 8 + r * 2], acc[j * 8 + r * 2 + 1]};
-            T* out = static_cast<T*>(p.C) + static_cast<long long>(m) * p.ldc + n;
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              if (m < p.rows_p && n + i < p.rows_q) v[i] = finish<T>(p, v[i], out + i, bias_at<T>(p, n + i));
-            if (p.vector_store) {
-              const uint32_t byte = static_cast<uint32_t>(c - c0) * sizeof(T);
-              uint8_t* to = block + row * 128 + (((byte >> 4) ^ (row & 7)) << 4) + (byte & 15);
-              if constexpr (sizeof(T) == 4) {
-                *reinterpret_cast<float2*>(to) = make_float2(v[0], v[1]);
-              } else {
-                *reinterpret_cast<uint32_t*>(to) = pack2(v[0], v[1], T());
-              }
+            const float* v = acc + (b * (COLS_BLOCK / 8) + j) * 8 + r * 2;
+            uint8_t* at = to + r * 1024 + ((j * (sizeof(T) == 4 ? 32 : 16)) ^ swizzle);
+            if constexpr (sizeof(T) == 4) {
+              *reinterpret_cast<float2*>(at) = make_float2(v[0], v[1]);
             } else {
-#pragma unroll
-              for (int i = 0; i < 2; ++i)
-                if (m < p.rows_p && n + i < p.rows_q) out[i] = from_f32<T>(v[i]);
+              *reinterpret_cast<uint32_t*>(at) = pack2(v[0], v[1], T());
             }
           }
-        if (p.vector_store) send(p, block, row0, col0 + c0);
       }
+      send(p, block, row0, col0 + b * COLS_BLOCK);
     }
   }
   __device__ static __forceinline__ void send(const Fp8Params& p, uint8_t* block, int row, int col) {
@@ -552,9 +579,9 @@ struct Fp8Pair {
       }
       for (int b = 0; b < 2; ++b) {
         mbar_init(&bars->tmem_full[b], 1);
-        mbar_init(&bars->tmem_empty[b], 16);  // one arrival per accumulating warp of each CTA
-        mbar_init(&bars->scale_full[b], 64);
-        mbar_init(&bars->scale_empty[b], 8);
+        mbar_init(&bars->tmem_empty[b], 16);  // one arrival for each accumulating warp of both CTAs
+        mbar_init(&bars->scale_full[b], 32);
+        mbar_init(&bars->scale_empty[b], 1);
       }
       bars->abort_flag = 0u;
       fence_mbar_init();
@@ -571,189 +598,185 @@ struct Fp8Pair {
     const uint32_t tmem_base = bars->tmem_base;
     griddep_wait();
 
-    // Registers: 384 threads are launched with 168 each; 56 + 2 * 224 = 3 * 168.
-    if (warp < 4) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-      if (warp == 0) {
-        if (lane == 0) {
-          uint32_t it = 0;
-          bool ok = true;
-          for (int tile = tile0; tile < tiles && ok; tile += stride) {
-            int m0, n0;
-            tile_at(tile, tiles_m, tiles_n, m0, n0);
-            for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
-              const uint32_t s = it % STAGES;
-              if (!mbar_wait(&bars->empty[s], ((it / STAGES) & 1u) ^ 1u, &bars->abort_flag)) {
-                report(bars, FP8_TIMEOUT_PRODUCER, it, s);
-                ok = false;
-                break;
-              }
-              // completion bytes of both CTAs land on the leader's barrier
-              const uint32_t full_leader = map_to_cta(smem_u32(&bars->full[s]), 0u);
-              if (rank == 0u) mbar_expect_tx(&bars->full[s], 2 * STAGE_BYTES);
-              tma_load_2d_pair(smem + s * STAGE_BYTES, &p.tmP, full_leader, kb * 128, m0 + static_cast<int>(rank) * 128);
-              tma_load_2d_pair(smem + s * STAGE_BYTES + HALF_BYTES, &p.tmQ, full_leader, kb * 128, n0 + static_cast<int>(rank) * 128);
-            }
-          }
-        }
-        __syncwarp();
-        griddep_launch_dependents();
-      } else if (warp == 1) {
-        if (rank == 0u) {
-          const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
-          const uint64_t adesc = make_smem_desc(smem_u32(smem), 16, 1024, SWZ_128B);
-          const uint64_t bdesc = make_smem_desc(smem_u32(smem) + HALF_BYTES, 16, 1024, SWZ_128B);
-          const uint32_t idesc = make_instr_desc(0u, 0u, 0u, 256u, kBN) | p.fmt_p << 7 | p.fmt_q << 10;
-          uint32_t it = 0;
-          bool ok = true;
-          for (int tile = tile0; tile < tiles && ok; tile += stride) {
-            for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
-              const uint32_t s = it % STAGES, b = it & 1u;
-              if (!mbar_wait_warp(&bars->tmem_empty[b], ((it >> 1) & 1u) ^ 1u, &bars->abort_flag) ||
-                  !mbar_wait_warp(&bars->full[s], (it / STAGES) & 1u, &bars->abort_flag)) {
-                if (lane == 0) report(bars, FP8_TIMEOUT_MMA, it, s);
-                ok = false;
-                break;
-              }
-              tc_fence_after_sync();
-              if (elect_one()) {
-#pragma unroll
-                for (int ks = 0; ks < 4; ++ks)
-                  umma_fp8<2>(tmem + b * kBN, adesc + s * (STAGE_BYTES >> 4) + ks * 2, bdesc + s * (STAGE_BYTES >> 4) + ks * 2, idesc,
-                              ks > 0 ? 1u : 0u);
-                umma_commit_pair(smem_u32(&bars->empty[s]));
-                umma_commit_pair(map_to_cta(smem_u32(&bars->empty[s]), 1u));
-                umma_commit_pair(smem_u32(&bars->tmem_full[b]));
-                umma_commit_pair(map_to_cta(smem_u32(&bars->tmem_full[b]), 1u));
-              }
-              __syncwarp();
-            }
-          }
-        }
-      } else {
-        // ------------------------------------------------------------ scales, GROUP_KB blocks at a time
-        const int t = threadIdx.x - 64;
-        uint32_t g = 0;
-        bool ok = true;
-        for (int tile = tile0; tile < tiles && ok; tile += stride) {
-          int m0, n0;
-          tile_at(tile, tiles_m, tiles_n, m0, n0);
-          m0 += static_cast<int>(rank) * 128;
-          for (int kb = 0; kb < p.num_kb; kb += GROUP_KB, ++g) {
-            const uint32_t b = g & 1u;
-            float* slot = scales + b * GROUP_KB * SCALES;
-            const float4 p0 = scales4(p.sp, p.ldsp, p.sp_shift, m0 + t, p.rows_p, kb, p.num_kb, p.vector_sp);
-            const float4 p1 = scales4(p.sp, p.ldsp, p.sp_shift, m0 + 64 + t, p.rows_p, kb, p.num_kb, p.vector_sp);
-            float4 q[kVector ? 4 : 1];
-            if constexpr (kVector) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                q[i] = scales4(p.sq, p.ldsq, p.sq_shift, n0 + i * 64 + t, p.rows_q, kb, p.num_kb, p.vector_sq);
-            } else if (t < 2) {
-              q[0] = scales4(p.sq, p.ldsq, p.sq_shift, n0 + t * 128, p.rows_q, kb, p.num_kb, p.vector_sq);
-            }
-            if (!mbar_wait(&bars->scale_empty[b], ((g >> 1) & 1u) ^ 1u, &bars->abort_flag)) {
-              report(bars, FP8_TIMEOUT_PRODUCER, g, 100u);
-              ok = false;
-              break;
-            }
-            put4(slot, t, p0);
-            put4(slot, 64 + t, p1);
-            if constexpr (kVector) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) put4(slot, 128 + i * 64 + t, q[i]);
-            } else if (t < 2) {
-              put4(slot, 128 + t, q[0]);
-            }
-            mbar_arrive(&bars->scale_full[b]);
-          }
-        }
-      }
-    } else {
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-      const int q = warp & 3, half = (warp - 4) >> 2;
-      uint8_t* block = smem + RING_BYTES + (warp - 4) * 4096;
+    if (warp == 0) {
+      // ------------------------------------------------ waits in the accumulating warps' place
       uint32_t it = 0, g = 0;
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t what) {
-        if (ok) {
-          ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, &bars->abort_flag));
-          if (!ok && lane == 0) report(bars, FP8_TIMEOUT_ACCUMULATE, it, what);
+        if (ok) ok = mbar_wait_warp(bar, parity, &bars->abort_flag);
+        if (!ok && lane == 0) report(bars, FP8_TIMEOUT_ACCUMULATE, it, what);
+      };
+      wait(&bars->scale_full[0], 0u, 2u);
+      ok = named_bar_all(BAR_FULL, MEETING, ok);  // the first block's scales
+      for (int tile = tile0; tile < tiles && ok; tile += stride) {
+        for (int kb = 0; kb < p.num_kb && ok; ++kb, ++it) {
+          if ((kb % GROUP_KB == GROUP_KB - 1 || kb == p.num_kb - 1) && (kb < p.num_kb - 1 || tile + stride < tiles))
+            wait(&bars->scale_full[(g + 1) & 1u], ((g + 1) >> 1) & 1u, 2u);
+          wait(&bars->tmem_full[it & 1u], (it >> 1) & 1u, 0u);
+          tc_fence_after_sync();
+          tc_fence_before_sync();
+          ok = named_bar_all(BAR_FULL, MEETING, ok);
+          if (kb % GROUP_KB == 0 && it > 0) {  // nobody reads the group before any more
+            if (lane == 0) mbar_arrive(&bars->scale_empty[g & 1u]);
+            ++g;
+          }
         }
+      }
+    } else if (warp == 1) {
+      if (rank == 0u) {
+        const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+        const uint64_t adesc = make_smem_desc(smem_u32(smem), 16, 1024, SWZ_128B);
+        const uint64_t bdesc = make_smem_desc(smem_u32(smem) + HALF_BYTES, 16, 1024, SWZ_128B);
+        const uint32_t idesc = make_instr_desc(0u, 0u, 0u, 256u, kBN) | p.fmt_p << 7 | p.fmt_q << 10;
+        uint32_t it = 0;
+        bool ok = true;
+        for (int tile = tile0; tile < tiles && ok; tile += stride) {
+          for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
+            const uint32_t s = it % STAGES, b = it & 1u;
+            // (the operands have mostly been there for long: what is waited for is the accumulator)
+            if (!mbar_wait_warp(&bars->full[s], (it / STAGES) & 1u, &bars->abort_flag) ||
+                !mbar_wait_warp(&bars->tmem_empty[b], ((it >> 1) & 1u) ^ 1u, &bars->abort_flag)) {
+              if (lane == 0) report(bars, FP8_TIMEOUT_MMA, it, s);
+              ok = false;
+              break;
+            }
+            tc_fence_after_sync();
+            if (elect_one()) {
+#pragma unroll
+              for (int ks = 0; ks < 4; ++ks)
+                umma_fp8<2>(tmem + b * kBN, adesc + s * (STAGE_BYTES >> 4) + ks * 2, bdesc + s * (STAGE_BYTES >> 4) + ks * 2, idesc,
+                            ks > 0 ? 1u : 0u);
+              umma_commit_both(&bars->tmem_full[b]);
+              umma_commit_both(&bars->empty[s]);
+            }
+            __syncwarp();
+          }
+        }
+      }
+    } else if (warp == 2) {
+      // ------------------------------------------------ operands, and scales GROUP_KB blocks at a time
+      uint32_t it = 0, g = 0;
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t what) {
+        ok = mbar_wait_warp(bar, parity, &bars->abort_flag);
+        if (!ok && lane == 0) report(bars, FP8_TIMEOUT_PRODUCER, it, what);
         return ok;
       };
+      for (int tile = tile0; tile < tiles && ok; tile += stride) {
+        int m0, n0;
+        tile_at(tile, tiles_m, tiles_n, m0, n0);
+        m0 += static_cast<int>(rank) * 128;
+        Scales held;
+        held.load(p, m0, n0, 0);
+        for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
+          const uint32_t s = it % STAGES;
+          if (!wait(&bars->empty[s], ((it / STAGES) & 1u) ^ 1u, s)) break;
+          if (lane == 0) {
+            // completion bytes of both CTAs land on the leader's barrier
+            const uint32_t full_leader = map_to_cta(smem_u32(&bars->full[s]), 0u);
+            if (rank == 0u) mbar_expect_tx(&bars->full[s], 2 * STAGE_BYTES);
+            tma_load_2d_pair(smem + s * STAGE_BYTES, &p.tmP, full_leader, kb * 128, m0);
+            tma_load_2d_pair(smem + s * STAGE_BYTES + HALF_BYTES, &p.tmQ, full_leader, kb * 128, n0 + static_cast<int>(rank) * 128);
+          }
+          __syncwarp();
+          if (kb % GROUP_KB == 0) {
+            if (!wait(&bars->scale_empty[g & 1u], ((g >> 1) & 1u) ^ 1u, 100u)) break;
+            held.store(scales + (g & 1u) * GROUP_KB * SCALES);
+            mbar_arrive(&bars->scale_full[g & 1u]);
+            ++g;
+            if (kb + GROUP_KB < p.num_kb) held.load(p, m0, n0, kb + GROUP_KB);
+          }
+        }
+      }
+      griddep_launch_dependents();
+    } else {
+      const int q = warp & 3, half = (warp - 3) >> 2;  // TMEM lane quarter of this warp, half of the tile's columns
+      uint8_t* block = smem + RING_BYTES + (warp - 3) * 8192;
+      // The scales of a block's rows (and of its half's columns, where they share one) are read when the block before has been added:
+      // read before its additions they cost a third of the speed.
+      const float* row_scales = scales + q * 32 + (kVector ? lane >> 2 : lane);
+      const float* column_scales = scales + 128 + half * (kVector ? 128 : 1) + (kVector ? (lane & 3) * 2 : 0);
+      const uint32_t empty_leader = map_to_cta(smem_u32(&bars->tmem_empty[0]), 0u);
+      constexpr int kF = kVector ? 4 : 2;
+      float f[kF];
+      uint32_t at = 0, it = 0;  // where the block's scales lie
+      auto fetch = [&]() {
+        if constexpr (kVector) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) f[i] = row_scales[at + i * 8];
+        } else {
+          f[0] = row_scales[at];
+          f[1] = column_scales[at];
+        }
+      };
+      bool ok = named_bar_all(BAR_FULL, MEETING, true);
+      fetch();
       for (int tile = tile0; tile < tiles && ok; tile += stride) {
         float acc[128];
 #pragma unroll
         for (int i = 0; i < 128; ++i) acc[i] = 0.f;
-        for (int kb = 0; kb < p.num_kb && ok; ++kb, ++it) {
-          const uint32_t b = it & 1u, sb = g & 1u;
-          if (kb % GROUP_KB == 0 && !wait(&bars->scale_full[sb], (g >> 1) & 1u, 2u)) break;
-          const float* slot = scales + (sb * GROUP_KB + kb % GROUP_KB) * SCALES;
-          const uint32_t col = tmem_base + b * kBN + half * 128 + (static_cast<uint32_t>(q * 32) << 16);
+        for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
+          const uint32_t col = tmem_base + (it & 1u) * kBN + half * 128 + (static_cast<uint32_t>(q * 32) << 16);
+          ok = named_bar_all(BAR_FULL, MEETING, true);
+          if (!ok) break;
+          tc_fence_after_sync();
           auto release = [&]() {  // (the reads are complete)
             tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster_cta(map_to_cta(smem_u32(&bars->tmem_empty[b]), 0u));
+            if (lane == 0) mbar_arrive_cluster_cta(empty_leader + (it & 1u) * 8);
           };
           if constexpr (!kVector) {
-            const float f = scale_product(slot[q * 32 + lane], slot[128 + half]);
-            if (!wait(&bars->tmem_full[b], (it >> 1) & 1u, 0u)) break;
-            tc_fence_after_sync();
-            uint32_t r[2][32];
-            tmem_ld_32x32b_x32(col, r[0]);
+            const float factor = scale_product(f[0], f[1]);
+            uint32_t r[2][16];
+            tmem_ld_32x32b_x16(col, r[0]);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
+            for (int c = 0; c < 8; ++c) {
               tmem_ld_wait();
-              pin_32(r[c & 1]);
-              if (c < 3) {
-                tmem_ld_32x32b_x32(col + (c + 1) * 32, r[(c + 1) & 1]);
+              pin_16(r[c & 1]);
+              if (c < 7) {
+                tmem_ld_32x32b_x16(col + (c + 1) * 16, r[(c + 1) & 1]);
               } else {
                 release();
               }
-              add_scaled<32>(acc + c * 32, r[c & 1], f);
+              add_scaled<16>(acc + c * 16, r[c & 1], factor);
             }
           } else {
-            float f[4];
+            // 16 columns at a time, rows 0-15 and 16-31 of the warp's lanes
+            uint32_t r[2][2][8];
+            float2 s[2][2];
+            auto load = [&](int c) {
+              tmem_ld_16x256b_x2(col + c * 16, r[c & 1][0]);
+              tmem_ld_16x256b_x2(col + c * 16 + (16u << 16), r[c & 1][1]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) f[i] = slot[q * 32 + i * 8 + (lane >> 2)];
-            const float* column = slot + 128 + half * 128 + (lane & 3) * 2;
-            if (!wait(&bars->tmem_full[b], (it >> 1) & 1u, 0u)) break;
-            tc_fence_after_sync();
-            // 32 columns at a time, rows 0-15 and 16-31 of the warp's lanes
-            uint32_t r[2][2][16];
-            tmem_ld_16x256b_x4(col, r[0][0]);
-            tmem_ld_16x256b_x4(col + (16u << 16), r[0][1]);
+              for (int j = 0; j < 2; ++j) s[c & 1][j] = *reinterpret_cast<const float2*>(column_scales + at + c * 16 + j * 8);
+            };
+            load(0);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
+            for (int c = 0; c < 8; ++c) {
               tmem_ld_wait();
-              pin_16(r[c & 1][0]);
-              pin_16(r[c & 1][1]);
-              if (c < 3) {
-                tmem_ld_16x256b_x4(col + (c + 1) * 32, r[(c + 1) & 1][0]);
-                tmem_ld_16x256b_x4(col + (c + 1) * 32 + (16u << 16), r[(c + 1) & 1][1]);
+              pin_8(r[c & 1][0]);
+              pin_8(r[c & 1][1]);
+              if (c < 7) {
+                load(c + 1);
               } else {
                 release();
               }
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const float2 s = *reinterpret_cast<const float2*>(column + c * 32 + j * 8);
+              for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {  // rows i * 8 + lane / 4
                   const uint32_t* part = &r[c & 1][i >> 1][j * 4 + (i & 1) * 2];
-                  float* a = acc + (c * 4 + j) * 8 + i * 2;
-                  const float2 y = __ffma2_rn(__fmul2_rn(make_float2(__uint_as_float(part[0]), __uint_as_float(part[1])), s),
+                  float* a = acc + (c * 2 + j) * 8 + i * 2;
+                  const float2 y = __ffma2_rn(__fmul2_rn(make_float2(__uint_as_float(part[0]), __uint_as_float(part[1])), s[c & 1][j]),
                                               make_float2(f[i], f[i]), make_float2(a[0], a[1]));
                   a[0] = y.x, a[1] = y.y;
                 }
-              }
             }
           }
-          if (kb % GROUP_KB == GROUP_KB - 1 || kb == p.num_kb - 1) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars->scale_empty[sb]);
-            ++g;
-          }
+          // the next block's place: the next of the group, or the first of the other
+          const bool last_of_group = kb % GROUP_KB == GROUP_KB - 1 || kb == p.num_kb - 1;
+          at = last_of_group ? (at >= GROUP_KB * SCALES ? 0u : GROUP_KB * SCALES) : at + SCALES;
+          fetch();
         }
         if (!ok) break;
         int m0, n0;
@@ -783,7 +806,7 @@ struct Fp8Pair {
 };
 
 template <bool kVector, typename T>
-__global__ void __launch_bounds__(384, 1) fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
+__global__ void __launch_bounds__(352, 1) fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
   Fp8Pair<kVector, T>::run(p);
 }
 
@@ -971,6 +994,7 @@ extern "C" int kcg_matmul_fp8(int device, uint64_t stream, const kcg_fp8_product
   }
   p.num_kb = kb;
   p.C = reinterpret_cast<void*>(a->C), p.ldc = ldc, p.bias = reinterpret_cast<const void*>(a->bias);
+  p.fused = a->beta != 0.f || a->bias != 0 || a->relu != 0;
   p.beta = a->beta, p.relu = a->relu, p.splits = plan.splits;
   p.vector_store = a->C % 16 == 0 && ldc * eb % 16 == 0;
   p.vector_sp = reinterpret_cast<uint64_t>(p.sp) % 16 == 0 && p.ldsp % 4 == 0;
