@@ -24,6 +24,19 @@ from codegendemo_b200.kcg.Utils import DeviceInfo
 
 MAX_NORM_WIDTH = 32768
 
+_warm = None  # csrc/kcg_torchcall.cpp once something was launched, False where it was not built for this torch
+
+
+def _launched(status):
+    """The end of a call that went this way: its error, or the next call's shorter way."""
+    global _warm
+    if status:
+        _lib.check(status)
+    if _warm is None:
+        from codegendemo_b200.kcg import matmul_op
+        _warm = matmul_op._warm_calls()
+
+
 
 def _dtype_code(t, what):
     import torch
@@ -93,6 +106,10 @@ def rms_norm(x, weight, residual=None, eps=1e-6, out=None, residual_out=None):
     residual. Sums in fp32, each result rounded once (the norm is taken of the unrounded sum). ``x`` and ``residual`` are
     rows x width, fp16, bf16 or fp32, ``weight`` width values of the same type. ``out`` and ``residual_out`` take the results;
     each may be ``x`` or ``residual`` itself (not both the same one), other overlaps are not allowed."""
+    if _warm and out is None and residual_out is None:
+        results = _warm.rms_norm(x, weight, residual, eps)
+        if results is not None:
+            return results
     dev, code, rows, width, ldx, ldr = _norm_operands(x, weight, residual, eps)
     ldy = 0
     if out is None:
@@ -102,25 +119,29 @@ def rms_norm(x, weight, residual=None, eps=1e-6, out=None, residual_out=None):
     h, ldh = _sum_of(x, residual, residual_out)
     if h is not None and h.data_ptr() == out.data_ptr() and rows > 0:
         raise ValueError("out and residual_out must be different tensors")
-    _lib.check(_lib.get_lib().kcg_rms_norm(dev, DeviceInfo.get_cuda_stream(dev), x.data_ptr(), ldx,
-                                           0 if residual is None else residual.data_ptr(), ldr, weight.data_ptr(), out.data_ptr(), ldy,
-                                           0 if h is None else h.data_ptr(), ldh, rows, width, eps, code))
+    _launched(_lib.get_lib().kcg_rms_norm(dev, DeviceInfo.get_cuda_stream(dev), x.data_ptr(), ldx,
+                                          0 if residual is None else residual.data_ptr(), ldr, weight.data_ptr(), out.data_ptr(), ldy,
+                                          0 if h is None else h.data_ptr(), ldh, rows, width, eps, code))
     return out if h is None else (out, h)
 
 
 def rms_norm_fp8(x, weight, residual=None, eps=1e-6, residual_out=None):
     """``rms_norm`` whose result leaves in 8 bits, as ``quantize_fp8`` would make it of the unrounded norm: returns (values, scales), or
     (values, scales, h) with a residual."""
+    if _warm and residual_out is None:
+        results = _warm.rms_norm_fp8(x, weight, residual, eps)
+        if results is not None:
+            return results
     import torch
     dev, code, rows, width, ldx, ldr = _norm_operands(x, weight, residual, eps)
     q = _rows_of_fp8(x, rows, width, torch.float8_e4m3fn)
     scales = x.new_empty((rows, -(-width // 128)), dtype=torch.float32)
     h, ldh = _sum_of(x, residual, residual_out)
     if rows > 0:
-        _lib.check(_lib.get_lib().kcg_rms_norm_fp8(dev, DeviceInfo.get_cuda_stream(dev), x.data_ptr(), ldx,
-                                                   0 if residual is None else residual.data_ptr(), ldr, weight.data_ptr(), q.data_ptr(),
-                                                   -(-width // 16) * 16, scales.data_ptr(), 0 if h is None else h.data_ptr(), ldh, rows,
-                                                   width, eps, code))
+        _launched(_lib.get_lib().kcg_rms_norm_fp8(dev, DeviceInfo.get_cuda_stream(dev), x.data_ptr(), ldx,
+                                                  0 if residual is None else residual.data_ptr(), ldr, weight.data_ptr(), q.data_ptr(),
+                                                  -(-width // 16) * 16, scales.data_ptr(), 0 if h is None else h.data_ptr(), ldh, rows,
+                                                  width, eps, code))
     return (q, scales) if h is None else (q, scales, h)
 
 
@@ -135,6 +156,10 @@ def rms_norm_backward(dy, h, weight, eps=1e-6, dh=None):
     """Gradients of ``rms_norm`` at ``h`` (x, or x + residual): returns (dx, dweight) for the gradient ``dy`` of its result. ``dh``, the
     gradient that reaches h past the norm, is added to dx, which then is the gradient of both x and the residual. The order of
     dweight's sums is fixed by the shape and the device."""
+    if _warm:
+        results = _warm.rms_norm_backward(dy, h, weight, eps, dh)
+        if results is not None:
+            return results
     dev, code, rows, width, ldh, lddy = _norm_operands(h, weight, dy, eps, ("h", "dy"))
     lddh = 0 if dh is None else _pitch(dh, "dh", h, (rows, width))
     dx = h.new_empty((rows, width))
@@ -145,9 +170,9 @@ def rms_norm_backward(dy, h, weight, eps=1e-6, dh=None):
     lib = _lib.get_lib()
     size = lib.kcg_rms_norm_backward_workspace(dev, rows, width)
     workspace = h.new_empty(max(size, 16), dtype=torch.uint8)
-    _lib.check(lib.kcg_rms_norm_backward(dev, DeviceInfo.get_cuda_stream(dev), dy.data_ptr(), lddy, h.data_ptr(), ldh, weight.data_ptr(),
-                                         0 if dh is None else dh.data_ptr(), lddh, dx.data_ptr(), 0, dw.data_ptr(), workspace.data_ptr(),
-                                         size, rows, width, eps, code))
+    _launched(lib.kcg_rms_norm_backward(dev, DeviceInfo.get_cuda_stream(dev), dy.data_ptr(), lddy, h.data_ptr(), ldh, weight.data_ptr(),
+                                        0 if dh is None else dh.data_ptr(), lddh, dx.data_ptr(), 0, dw.data_ptr(), workspace.data_ptr(),
+                                        size, rows, width, eps, code))
     return dx, dw
 
 
@@ -155,6 +180,10 @@ def quantize_fp8(x, rows=1, transposed=False, dtype=None):
     """(values, scales) of a matrix in blocks of ``rows`` (1 or 128) x 128 values: scale = max(largest magnitude / 448, 2^-126) (e5m2:
     57344), values x / scale rounded to nearest even. ``transposed``: of ``x.t()``, cut into blocks along what were x's rows.
     ``dtype`` is float8_e4m3fn (default) or float8_e5m2. Scales are (row blocks) x ceil(columns / 128), fp32."""
+    if _warm and dtype is None:
+        results = _warm.quantize_fp8(x, rows, transposed)
+        if results is not None:
+            return results
     import torch
     dev = _device(x, "x")
     code = _dtype_code(x, "x")
@@ -168,8 +197,8 @@ def quantize_fp8(x, rows=1, transposed=False, dtype=None):
     q = _rows_of_fp8(x, r, c, dtype)
     scales = x.new_empty((-(-r // rows), -(-c // 128)), dtype=torch.float32)
     if n > 0 and cols > 0:
-        _lib.check(_lib.get_lib().kcg_quantize_fp8(dev, DeviceInfo.get_cuda_stream(dev), x.data_ptr(), ldx, q.data_ptr(), -(-c // 16) * 16,
-                                                   scales.data_ptr(), n, cols, rows, int(bool(transposed)), code, code8))
+        _launched(_lib.get_lib().kcg_quantize_fp8(dev, DeviceInfo.get_cuda_stream(dev), x.data_ptr(), ldx, q.data_ptr(), -(-c // 16) * 16,
+                                                  scales.data_ptr(), n, cols, rows, int(bool(transposed)), code, code8))
     return q, scales
 
 
@@ -179,6 +208,10 @@ def matmul_fp8(a, a_scale, b, b_scale, c=None, beta=0.0, bias=None, relu=False, 
     ceil(N / 128) x ceil(K / 128), or of 1 x 128, ``b_scale`` N x ceil(K / 128). e4m3 or e5m2, each its own. Sums in fp32, one rounding
     to ``out_dtype`` (bf16 by default; fp16, fp32) or c's type. Rows of a and b have to start on 16-byte boundaries, as
     ``quantize_fp8`` and ``rms_norm_fp8`` lay them out. The product of two scales has to be a normal fp32 number."""
+    if _warm and c is None and type(beta) is float and beta == 0.0:
+        c = _warm.matmul_fp8(a, a_scale, b, b_scale, bias, relu, out_dtype)
+        if c is not None:
+            return c
     import torch
     dev = _device(a, "a")
     fa, fb = _fp8_code(a.dtype, "a"), _fp8_code(b.dtype, "b")
@@ -217,7 +250,7 @@ def matmul_fp8(a, a_scale, b, b_scale, c=None, beta=0.0, bias=None, relu=False, 
     p = _lib.Fp8Product(a.data_ptr(), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(), c.data_ptr(),
                         0 if bias is None else bias.data_ptr(), lda, _pitch(a_scale, "a_scale"), ldb, _pitch(b_scale, "b_scale"), ldc,
                         M, N, K, block_b, fa, fb, code, beta, int(bool(relu)))
-    _lib.check(_lib.get_lib().kcg_matmul_fp8(dev, DeviceInfo.get_cuda_stream(dev), ctypes.byref(p)))
+    _launched(_lib.get_lib().kcg_matmul_fp8(dev, DeviceInfo.get_cuda_stream(dev), ctypes.byref(p)))
     return c
 
 
