@@ -46,15 +46,40 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Eight consecutive values from a 16-byte boundary: one 16-byte vector of a 16-bit type, two of fp32.
+// Eight consecutive values from a 16-byte boundary, as they lie in memory: one 16-byte vector of a 16-bit type, two of fp32.
+template <typename T>
+struct Raw8 {
+  uint4 v;
+  __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void zero() { v = make_uint4(0u, 0u, 0u, 0u); }
+  __device__ __forceinline__ void set(const T (&e)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      w[j] = *reinterpret_cast<const uint16_t*>(&e[2 * j]) | static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(&e[2 * j + 1])) << 16;
+    v = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __device__ __forceinline__ void values(float (&f)[8]) const { unpack8(v, f, T()); }
+};
+template <>
+struct Raw8<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  }
+  __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void set(const float (&e)[8]) {
+    a = make_float4(e[0], e[1], e[2], e[3]), b = make_float4(e[4], e[5], e[6], e[7]);
+  }
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  }
+};
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-  } else {
-    unpack8(*reinterpret_cast<const uint4*>(p), v, T());
-  }
+  Raw8<T> raw;
+  raw.load(p);
+  raw.values(v);
 }
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
@@ -70,11 +95,15 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
 // ---- 8-bit blocks. Of a block with largest magnitude top: scale = max(top / largest 8-bit value, 2^-126), values
 // x * (1 / scale) rounded to nearest even. The lower bound keeps 1 / scale finite, also for a block of zeros. Magnitudes are compared
 // as integers, in which a NaN is the largest: it makes the block's scale, and with it every value of the block, a NaN.
+// The larger magnitude of three values, a NaN if one of them is.
+__device__ __forceinline__ float abs_max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)), "f"(fabsf(c)));
+  return r;
+}
 __device__ __forceinline__ uint32_t abs_max(const float (&v)[8]) {
-  uint32_t m = 0u;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
-  return m;
+  const float m = abs_max3(abs_max3(v[0], v[1], v[2]), abs_max3(v[3], v[4], v[5]), abs_max3(v[6], v[7], v[7]));
+  return __float_as_uint(m) & 0x7fffffffu;
 }
 template <bool kE5M2>
 __device__ __forceinline__ float block_scale(uint32_t top) {

@@ -6,11 +6,11 @@
 // y comes from the unrounded sum h, which is rounded only where it is stored.
 //
 // Bound by HBM: a row is read once, into registers, and written once. Widths of whole 16-byte pieces take the kernels below
-// (a warp a row up to 1024 values, a CTA a row beyond), others a kernel that reads single values, twice.
+// (a warp a row up to 1024 values, CTAs that walk rows beyond), others a kernel that reads single values, twice.
 #include <cuda_runtime.h>
 
+#include <cfloat>
 #include <cstdint>
-#include <mutex>
 #include <string>
 
 #include "../../include/kcg_b200.h"
@@ -53,67 +53,131 @@ __device__ __forceinline__ void row_sum(float (&v)[kN], float* scratch) {
   }
 }
 
-// kVPT: pieces of 8 values a thread holds of a row.
-template <typename T, int kVPT, bool kWarpRow, bool kRes, bool kFp8>
-__global__ void __launch_bounds__(kWarpRow ? 256 : 1024) norm_kernel(const NormArgs a) {
-  __shared__ float scratch[32];
+// The end of a forward pass for one piece: h is stored, y (= h * w * r) stored or quantised. kFp8: the 16 neighbouring threads that hold
+// 128 values of the row come together; the factor r goes into the scale and its reciprocal instead of into every value.
+template <typename T, bool kRes, bool kFp8>
+__device__ __forceinline__ void finish_piece(const NormArgs& a, long long row, int v, bool in, int tid, const float (&h)[8], const float (&w)[8],
+                                             float r) {
+  if (kRes && in) store8(static_cast<T*>(a.h) + row * a.ldh + 8 * v, h);
+  float y[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) y[j] = kFp8 ? h[j] * w[j] : h[j] * r * w[j];
+  if constexpr (kFp8) {
+    uint32_t top = in ? abs_max(y) : 0u;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float scale = block_scale<false>(__float_as_uint(__uint_as_float(top) * r));
+    float factor = r / scale;
+    if (factor > FLT_MAX) {  // (the smallest scale, of a block of next to nothing)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] *= r;
+      factor = 1.f / scale;
+    }
+    if (in) {
+      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.y) + row * a.ldy + 8 * v) = quantize8<false>(y, factor);
+      if ((tid & 15) == 0) a.scales[row * a.blocks + (v >> 4)] = scale;
+    }
+  } else if (in) {
+    store8(static_cast<T*>(a.y) + row * a.ldy + 8 * v, y);
+  }
+}
+
+// A warp a row, rows of up to 1024 values. kVPT: pieces of 8 values a thread holds.
+template <typename T, int kVPT, bool kRes, bool kFp8>
+__global__ void __launch_bounds__(256) norm_warp_kernel(const NormArgs a) {
   griddep_launch_dependents();
   griddep_wait();
-  const int tid = kWarpRow ? threadIdx.x & 31 : threadIdx.x, threads = kWarpRow ? 32 : blockDim.x;
-  const long long row = kWarpRow ? static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
-  if (kWarpRow && row >= a.rows) return;
-  const int pieces = a.width / 8;
+  const int tid = threadIdx.x & 31, pieces = a.width / 8;
+  const long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (row >= a.rows) return;
   const T* x = static_cast<const T*>(a.x) + row * a.ldx;
   const T* res = kRes ? static_cast<const T*>(a.residual) + row * a.ldr : nullptr;
-  float h[kVPT][8];
-  float sum[1] = {0.f};
+  float h[kVPT][8], sum[1] = {0.f};
 #pragma unroll
   for (int i = 0; i < kVPT; ++i) {
-    const int v = i * threads + tid;
-    if (v < pieces) {
-      load8(x + 8 * v, h[i]);
-      if constexpr (kRes) {
-        float r[8];
-        load8(res + 8 * v, r);
+    const int v = i * 32 + tid;
+    Raw8<T> p, q;
+    p.zero();
+    if (v < pieces) p.load(x + 8 * v);
+    p.values(h[i]);
+    if constexpr (kRes) {
+      float f[8];
+      q.zero();
+      if (v < pieces) q.load(res + 8 * v);
+      q.values(f);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) h[i][j] += r[j];
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) h[i][j] = 0.f;
+      for (int j = 0; j < 8; ++j) h[i][j] += f[j];
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) sum[0] = fmaf(h[i][j], h[i][j], sum[0]);
   }
-  row_sum<kWarpRow>(sum, scratch);
+  row_sum<true>(sum, nullptr);
   const float r = rsqrtf(sum[0] / static_cast<float>(a.width) + a.eps);
 #pragma unroll
   for (int i = 0; i < kVPT; ++i) {
-    const int v = i * threads + tid;
-    const bool in = v < pieces;
-    if (kRes && in) store8(static_cast<T*>(a.h) + row * a.ldh + 8 * v, h[i]);
-    float y[8];
-    if (in) {
-      float w[8];
-      load8(static_cast<const T*>(a.w) + 8 * v, w);
+    const int v = i * 32 + tid;
+    float w[8] = {};
+    if (v < pieces) load8(static_cast<const T*>(a.w) + 8 * v, w);
+    finish_piece<T, kRes, kFp8>(a, row, v, v < pieces, tid, h[i], w, r);
+  }
+}
+
+// A CTA walks rows blockIdx.x, + gridDim.x, ...; it keeps the weight, and asks for the next row before it reduces the present one (with one
+// row a CTA, 5001 x 5504 fp16 into 8 bits took 37 us: loads, sum and stores of a row by turns).
+template <typename T, int kVPT, bool kRes, bool kFp8, int kThreads, int kCtas>
+__global__ void __launch_bounds__(kThreads, kCtas) norm_kernel(const NormArgs a) {
+  __shared__ float scratch[2][32];
+  constexpr bool kAhead = kThreads <= 512;  // (registers)
+  griddep_launch_dependents();
+  griddep_wait();
+  const int tid = threadIdx.x, threads = blockDim.x, pieces = a.width / 8;
+  Raw8<T> w[kVPT], x[kVPT], res[kRes ? kVPT : 1];
+  auto ask = [&](long long row) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = h[i][j] * r * w[j];
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = 0.f;
-    }
-    if constexpr (kFp8) {
-      // 16 neighbouring threads hold 128 values of the row
-      uint32_t top = abs_max(y);
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float scale = block_scale<false>(top);
-      if (in) {
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.y) + row * a.ldy + 8 * v) = quantize8<false>(y, 1.f / scale);
-        if ((tid & 15) == 0) a.scales[row * a.blocks + v / 16] = scale;
+    for (int i = 0; i < kVPT; ++i) {
+      const int v = i * threads + tid;
+      if (v < pieces) {
+        x[i].load(static_cast<const T*>(a.x) + row * a.ldx + 8 * v);
+        if constexpr (kRes) res[i].load(static_cast<const T*>(a.residual) + row * a.ldr + 8 * v);
       }
-    } else if (in) {
-      store8(static_cast<T*>(a.y) + row * a.ldy + 8 * v, y);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kVPT; ++i) {
+    w[i].zero();
+    x[i].zero();
+    if constexpr (kRes) res[i].zero();
+    if (kAhead && i * threads + tid < pieces) w[i].load(static_cast<const T*>(a.w) + 8 * (i * threads + tid));
+  }
+  long long row = blockIdx.x;
+  if (kAhead && row < a.rows) ask(row);
+  for (int turn = 0; row < a.rows; row += gridDim.x, turn ^= 1) {
+    if constexpr (!kAhead) ask(row);
+    float h[kVPT][8], sum[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < kVPT; ++i) {
+      x[i].values(h[i]);
+      if constexpr (kRes) {
+        float f[8];
+        res[i].values(f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[i][j] += f[j];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum[0] = fmaf(h[i][j], h[i][j], sum[0]);
+    }
+    if (kAhead && row + gridDim.x < a.rows) ask(row + gridDim.x);
+    row_sum<false>(sum, scratch[turn]);  // (two scratches: one barrier a row)
+    const float r = rsqrtf(sum[0] / static_cast<float>(a.width) + a.eps);
+#pragma unroll
+    for (int i = 0; i < kVPT; ++i) {
+      const int v = i * threads + tid;
+      if constexpr (!kAhead) {
+        if (v < pieces) w[i].load(static_cast<const T*>(a.w) + 8 * v);
+      }
+      float f[8];
+      w[i].values(f);
+      finish_piece<T, kRes, kFp8>(a, row, v, v < pieces, tid, h[i], f, r);
     }
   }
 }
@@ -174,58 +238,78 @@ struct GradArgs {
   float eps;
 };
 
-// Each CTA walks rows blockIdx.x, + gridDim.x, ...; a thread keeps its columns' share of dw in registers.
-template <typename T, int kVPT, bool kDh>
-__global__ void __launch_bounds__(1024) norm_grad_kernel(const GradArgs a) {
+// Each CTA walks rows blockIdx.x, + gridDim.x, ...; a thread keeps its columns' share of dw in registers, and asks for the next row
+// before it reduces the present one.
+template <typename T, int kVPT, bool kDh, int kThreads, int kCtas>
+__global__ void __launch_bounds__(kThreads, kCtas) norm_grad_kernel(const GradArgs a) {
   __shared__ float scratch[2][64];
+  constexpr bool kAhead = kVPT <= 2 && kThreads <= 512;  // (registers)
   griddep_launch_dependents();
   griddep_wait();
   const int tid = threadIdx.x, threads = blockDim.x, pieces = a.width / 8;
   float dw[kVPT][8];
-#pragma unroll
-  for (int i = 0; i < kVPT; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) dw[i][j] = 0.f;
-  int turn = 0;
-  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
-    float h[kVPT][8], dy[kVPT][8];
-    float sum[2] = {0.f, 0.f};
+  Raw8<T> w[kVPT], rh[kVPT], rdy[kVPT], rdh[kDh ? kVPT : 1];
+  auto ask = [&](long long row) {
 #pragma unroll
     for (int i = 0; i < kVPT; ++i) {
       const int v = i * threads + tid;
       if (v < pieces) {
-        load8(static_cast<const T*>(a.h) + row * a.ldh + 8 * v, h[i]);
-        load8(static_cast<const T*>(a.dy) + row * a.lddy + 8 * v, dy[i]);
-        float w[8];
-        load8(static_cast<const T*>(a.w) + 8 * v, w);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          sum[0] = fmaf(h[i][j], h[i][j], sum[0]);
-          sum[1] = fmaf(dy[i][j] * w[j], h[i][j], sum[1]);
-        }
+        rh[i].load(static_cast<const T*>(a.h) + row * a.ldh + 8 * v);
+        rdy[i].load(static_cast<const T*>(a.dy) + row * a.lddy + 8 * v);
+        if constexpr (kDh) rdh[i].load(static_cast<const T*>(a.dh) + row * a.lddh + 8 * v);
       }
     }
+  };
+#pragma unroll
+  for (int i = 0; i < kVPT; ++i) {
+    w[i].zero(), rh[i].zero(), rdy[i].zero();
+    if constexpr (kDh) rdh[i].zero();
+    if (kAhead && i * threads + tid < pieces) w[i].load(static_cast<const T*>(a.w) + 8 * (i * threads + tid));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dw[i][j] = 0.f;
+  }
+  const float inv = 1.f / static_cast<float>(a.width);
+  long long row = blockIdx.x;
+  if (kAhead && row < a.rows) ask(row);
+  for (int turn = 0; row < a.rows; row += gridDim.x, turn ^= 1) {
+    if constexpr (!kAhead) {
+      ask(row);
+#pragma unroll
+      for (int i = 0; i < kVPT; ++i)
+        if (i * threads + tid < pieces) w[i].load(static_cast<const T*>(a.w) + 8 * (i * threads + tid));
+    }
+    float h[kVPT][8], dy[kVPT][8], sum[2] = {0.f, 0.f};
+    Raw8<T> dh[kDh ? kVPT : 1];
+#pragma unroll
+    for (int i = 0; i < kVPT; ++i) {
+      float f[8];
+      w[i].values(f);
+      rh[i].values(h[i]);
+      rdy[i].values(dy[i]);
+      if constexpr (kDh) dh[i] = rdh[i];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        sum[0] = fmaf(h[i][j], h[i][j], sum[0]);
+        sum[1] = fmaf(dy[i][j] * f[j], h[i][j], sum[1]);
+      }
+    }
+    if (kAhead && row + gridDim.x < a.rows) ask(row + gridDim.x);
     row_sum<false>(sum, scratch[turn]);  // (two scratches: one barrier a row)
-    const float inv = 1.f / static_cast<float>(a.width);
     const float r = rsqrtf(fmaf(sum[0], inv, a.eps));
     const float back = r * r * (sum[1] * inv);  // dx = r * (g - h * back)
 #pragma unroll
     for (int i = 0; i < kVPT; ++i) {
       const int v = i * threads + tid;
-      if (v < pieces) {
-        float w[8], d[8];
-        load8(static_cast<const T*>(a.w) + 8 * v, w);
-        if constexpr (kDh) {
-          load8(static_cast<const T*>(a.dh) + row * a.lddh + 8 * v, d);
-        }
+      float f[8], d[8];
+      w[i].values(f);
+      if constexpr (kDh) dh[i].values(d);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float dx = r * (dy[i][j] * w[j] - h[i][j] * back);
-          dw[i][j] = fmaf(dy[i][j], h[i][j] * r, dw[i][j]);
-          d[j] = kDh ? d[j] + dx : dx;
-        }
-        store8(static_cast<T*>(a.dx) + row * a.lddx + 8 * v, d);
+      for (int j = 0; j < 8; ++j) {
+        const float dx = r * (dy[i][j] * f[j] - h[i][j] * back);
+        dw[i][j] = fmaf(dy[i][j], h[i][j] * r, dw[i][j]);
+        d[j] = kDh ? d[j] + dx : dx;
       }
+      if (v < pieces) store8(static_cast<T*>(a.dx) + row * a.lddx + 8 * v, d);
     }
   }
   float* mine = a.partial + static_cast<long long>(blockIdx.x) * a.width;
@@ -269,29 +353,50 @@ __global__ void __launch_bounds__(512) norm_grad_any_kernel(const GradArgs a) {
   for (int c = threadIdx.x; c < a.width; c += blockDim.x) mine[c] = dw[c];
 }
 
-// dw = sum of the CTAs' shares, in their order.
+// dw = sum of the CTAs' shares, in their order: 32 threads a column, each a 32nd of the shares.
 template <typename T>
-__global__ void __launch_bounds__(512) norm_grad_sum_kernel(const float* partial, int parts, int width, T* dw) {
-  __shared__ float sums[16][33];
+__global__ void __launch_bounds__(1024) norm_grad_sum_kernel(const float* partial, int parts, int width, T* dw) {
+  __shared__ float sums[32][33];
   griddep_launch_dependents();
   griddep_wait();
   const int lane = threadIdx.x & 31, part = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   float s = 0.f;
-  if (c < width)
-    for (int p = part; p < parts; p += 16) s += partial[static_cast<long long>(p) * width + c];
+  if (c < width) {
+#pragma unroll 8
+    for (int p = part; p < parts; p += 32) s += partial[static_cast<long long>(p) * width + c];
+  }
   sums[part][lane] = s;
   __syncthreads();
-  if (part == 0 && c < width) {
-    s = 0.f;
+  s = sums[lane][part];  // share `lane` of column `part`
 #pragma unroll
-    for (int p = 0; p < 16; ++p) s += sums[p][lane];
-    dw[c] = from_f32<T>(s);
-  }
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane == 0 && blockIdx.x * 32 + part < width) dw[blockIdx.x * 32 + part] = from_f32<T>(s);
 }
 
 // ------------------------------------------------------------------------------------------------ launches
+// CTAs of a kernel that an SM holds at once (asked once per number of threads; one kind of GPU a process).
+template <typename K>
+int ctas_per_sm(K kernel, int threads, int (&known)[33]) {
+  int& n = known[threads / 32];
+  if (n == 0 && (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) != cudaSuccess || n < 1)) {
+    cudaGetLastError();
+    n = 1;
+  }
+  return n;
+}
+
+template <typename T, int kVPT, bool kRes, bool kFp8, int kThreads, int kCtas>
+int launch_norm_rows(Launch& l, const NormArgs& a, int sms) {
+  static int known[33];
+  const auto kernel = norm_kernel<T, kVPT, kRes, kFp8, kThreads, kCtas>;
+  const int threads = ((a.width / 8 + kVPT - 1) / kVPT + 31) / 32 * 32;
+  const long long most = static_cast<long long>(sms) * ctas_per_sm(kernel, threads, known);
+  l.shape(static_cast<unsigned>(a.rows < most ? a.rows : most), threads);
+  return l(kernel, "norm launch", a);
+}
+
 template <typename T, bool kRes, bool kFp8>
-int launch_norm(const NormArgs& a, bool vectors, cudaStream_t st) {
+int launch_norm(const NormArgs& a, bool vectors, int sms, cudaStream_t st) {
   Launch l(st);
   if (!vectors) {
     l.shape(static_cast<unsigned>(a.rows), 256);
@@ -300,27 +405,28 @@ int launch_norm(const NormArgs& a, bool vectors, cudaStream_t st) {
   const int pieces = a.width / 8;
   if (pieces <= 128) {
     l.shape(static_cast<unsigned>((a.rows + 7) / 8), 256);
-    if (pieces <= 32) return l(norm_kernel<T, 1, true, kRes, kFp8>, "norm launch", a);
-    if (pieces <= 64) return l(norm_kernel<T, 2, true, kRes, kFp8>, "norm launch", a);
-    return l(norm_kernel<T, 4, true, kRes, kFp8>, "norm launch", a);
+    if (pieces <= 32) return l(norm_warp_kernel<T, 1, kRes, kFp8>, "norm launch", a);
+    if (pieces <= 64) return l(norm_warp_kernel<T, 2, kRes, kFp8>, "norm launch", a);
+    return l(norm_warp_kernel<T, 4, kRes, kFp8>, "norm launch", a);
   }
-  const int vpt = pieces <= 2048 ? 2 : 4;
-  l.shape(static_cast<unsigned>(a.rows), ((pieces + vpt - 1) / vpt + 31) / 32 * 32);
-  if (vpt == 2) return l(norm_kernel<T, 2, false, kRes, kFp8>, "norm launch", a);
-  return l(norm_kernel<T, 4, false, kRes, kFp8>, "norm launch", a);
+  if (pieces <= 512) return launch_norm_rows<T, 1, kRes, kFp8, 512, 3>(l, a, sms);
+  if (pieces <= 1024) return launch_norm_rows<T, 2, kRes, kFp8, 512, 2>(l, a, sms);
+  if (pieces <= 2048) return launch_norm_rows<T, 4, kRes, kFp8, 512, 1>(l, a, sms);
+  return launch_norm_rows<T, 4, kRes, kFp8, 1024, 1>(l, a, sms);
 }
 
 template <typename T>
-int launch_norm(const NormArgs& a, bool vectors, cudaStream_t st) {
-  if (a.residual) return a.scales ? launch_norm<T, true, true>(a, vectors, st) : launch_norm<T, true, false>(a, vectors, st);
-  return a.scales ? launch_norm<T, false, true>(a, vectors, st) : launch_norm<T, false, false>(a, vectors, st);
+int launch_norm(const NormArgs& a, bool vectors, int sms, cudaStream_t st) {
+  if (a.residual) return a.scales ? launch_norm<T, true, true>(a, vectors, sms, st) : launch_norm<T, true, false>(a, vectors, sms, st);
+  return a.scales ? launch_norm<T, false, true>(a, vectors, sms, st) : launch_norm<T, false, false>(a, vectors, sms, st);
 }
 
 constexpr int kMaxWidth = 32768;  // a row in a CTA's registers, its share of dw in shared memory
 
-// CTAs that walk the rows of the backward pass, each with its own share of dw.
+// CTAs that walk the rows of the backward pass, each with its own share of dw: as many as run at once, with 512 threads or fewer
+// two an SM.
 int grad_ctas(int sms, long long rows, int width) {
-  const long long most = static_cast<long long>(sms) * (width <= 4096 ? 4 : width <= 8192 ? 2 : 1);
+  const long long most = static_cast<long long>(sms) * (width <= 2048 ? 4 : width <= 4096 ? 2 : 1);
   return static_cast<int>(rows < most ? rows : most);
 }
 
@@ -337,18 +443,29 @@ int launch_grad(const GradArgs& a, int ctas, bool vectors, cudaStream_t st) {
     l.shape(ctas, 512, smem);
     return l(norm_grad_any_kernel<T, kDh>, "norm gradient launch", a);
   }
-  const int pieces = a.width / 8, vpt = pieces <= 1024 ? 1 : pieces <= 2048 ? 2 : 4;
-  l.shape(ctas, ((pieces + vpt - 1) / vpt + 31) / 32 * 32);
-  if (vpt == 1) return l(norm_grad_kernel<T, 1, kDh>, "norm gradient launch", a);
-  if (vpt == 2) return l(norm_grad_kernel<T, 2, kDh>, "norm gradient launch", a);
-  return l(norm_grad_kernel<T, 4, kDh>, "norm gradient launch", a);
+  const int pieces = a.width / 8;
+  auto threads = [&](int vpt) { return static_cast<unsigned>(((pieces + vpt - 1) / vpt + 31) / 32 * 32); };
+  if (pieces <= 512) {
+    l.shape(ctas, threads(1));
+    return l(norm_grad_kernel<T, 1, kDh, 512, 2>, "norm gradient launch", a);
+  }
+  if (pieces <= 1024) {
+    l.shape(ctas, threads(2));
+    return l(norm_grad_kernel<T, 2, kDh, 512, 1>, "norm gradient launch", a);
+  }
+  if (pieces <= 2048) {
+    l.shape(ctas, threads(4));
+    return l(norm_grad_kernel<T, 4, kDh, 512, 1>, "norm gradient launch", a);
+  }
+  l.shape(ctas, threads(8));
+  return l(norm_grad_kernel<T, 8, kDh, 512, 1>, "norm gradient launch", a);
 }
 
 template <typename T>
 int launch_grad(const GradArgs& a, int ctas, bool vectors, cudaStream_t st) {
   if (int e = a.dh ? launch_grad<T, true>(a, ctas, vectors, st) : launch_grad<T, false>(a, ctas, vectors, st)) return e;
   Launch l(st);
-  l.shape((a.width + 31) / 32, 512);
+  l.shape((a.width + 31) / 32, 1024);
   return l(norm_grad_sum_kernel<T>, "norm gradient launch", static_cast<const float*>(a.partial), ctas, a.width,
            static_cast<T*>(a.dw));
 }
@@ -381,12 +498,14 @@ int norm_forward(int device, uint64_t stream, NormArgs a, uint64_t X, uint64_t R
                        W % 16 == 0 && (fp8 ? Y % 8 == 0 && a.ldy % 8 == 0 : pieces_of_8(Y, a.ldy, eb));
   a.x = reinterpret_cast<const void*>(X), a.residual = reinterpret_cast<const void*>(R), a.w = reinterpret_cast<const void*>(W);
   a.y = reinterpret_cast<void*>(Y), a.h = reinterpret_cast<void*>(H);
+  int sms = 0;
+  if (int e = sm_count(device, &sms)) return e;
   DeviceGuard guard;
   const cudaError_t e = guard.enter(device);
   if (e != cudaSuccess) return cuda_fail(e, "cudaSetDevice");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == KCG_DTYPE_FLOAT32) return launch_norm<float>(a, vectors, st);
-  return dtype == KCG_DTYPE_FLOAT16 ? launch_norm<__half>(a, vectors, st) : launch_norm<__nv_bfloat16>(a, vectors, st);
+  if (dtype == KCG_DTYPE_FLOAT32) return launch_norm<float>(a, vectors, sms, st);
+  return dtype == KCG_DTYPE_FLOAT16 ? launch_norm<__half>(a, vectors, sms, st) : launch_norm<__nv_bfloat16>(a, vectors, sms, st);
 }
 
 }  // namespace

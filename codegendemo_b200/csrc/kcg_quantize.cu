@@ -27,46 +27,97 @@ struct QuantArgs {
   int cols, blocks;
 };
 
-// Eight values of a row from column c on; those past the row's end as zeros.
+// Eight values of a row from column c on, as they lie in memory; those past the row's end as zeros.
 template <typename T, bool kVec>
-__device__ __forceinline__ void load_piece(const T* row, int c, int cols, float (&v)[8]) {
+__device__ __forceinline__ void load_piece(const T* row, int c, int cols, Raw8<T>& v) {
   if (kVec && c + 8 <= cols) {
-    load8(row + c, v);
+    v.load(row + c);
   } else {
+    T e[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? to_f32(row[c + j]) : 0.f;
+    for (int j = 0; j < 8; ++j) e[j] = c + j < cols ? row[c + j] : T(0.f);
+    v.set(e);
   }
 }
 
-// Blocks of 1 x 128, as the matrix lies: 16 threads a block.
+// Magnitudes, kept in the raw type: its bits without the sign, in whose order a NaN is the largest. Words of two 16-bit values or of
+// one fp32 value; eight values are kWords of them.
+template <typename T>
+struct Tops {
+  static constexpr int kWords = sizeof(T) == 4 ? 8 : 4;
+  __device__ static __forceinline__ uint32_t word(const Raw8<T>& v, int i) { return reinterpret_cast<const uint32_t*>(&v)[i]; }
+  __device__ static __forceinline__ uint32_t magnitude(uint32_t w) { return w & (sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu); }
+  __device__ static __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    if constexpr (sizeof(T) == 4) {
+      return max(a, b);
+    } else {
+      return __vmaxu2(a, b);
+    }
+  }
+  // The larger of a word's values (sizeof(T) == 2: of its two), as the bits of an fp32 number.
+  __device__ static __forceinline__ uint32_t f32(uint32_t w) {
+    if constexpr (sizeof(T) == 4) {
+      return w;
+    } else {
+      return f32_of(max(w >> 16, w & 0xffffu));
+    }
+  }
+  // A 16-bit value's bits as those of an fp32 number.
+  __device__ static __forceinline__ uint32_t f32_of(uint32_t bits) {
+    const uint16_t h = static_cast<uint16_t>(bits);
+    return __float_as_uint(to_f32(*reinterpret_cast<const T*>(&h)));
+  }
+  __device__ static __forceinline__ uint32_t of(const Raw8<T>& v) {
+    uint32_t m = magnitude(word(v, 0));
+#pragma unroll
+    for (int i = 1; i < kWords; ++i) m = larger(m, magnitude(word(v, i)));
+    return m;
+  }
+};
+
+// Blocks of 1 x 128, as the matrix lies: 16 threads a block, kBlocks of them at once.
 template <typename T, bool kVec, bool kE5M2>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantArgs a) {
+  constexpr int kBlocks = 4;
   griddep_launch_dependents();
   griddep_wait();
-  const long long total = a.rows * a.blocks;
   const int part = threadIdx.x & 15;
-  for (long long b = static_cast<long long>(blockIdx.x) * 16 + (threadIdx.x >> 4); b - (threadIdx.x >> 4 & 1) < total;
-       b += static_cast<long long>(gridDim.x) * 16) {  // (both halves of a warp stay for the exchange)
-    const bool in = b < total;
-    const long long row = in ? b / a.blocks : 0;
-    const int block = in ? static_cast<int>(b - row * a.blocks) : 0, c = block * 128 + part * 8;
-    float v[8];
-    load_piece<T, kVec>(static_cast<const T*>(a.x) + row * a.ldx, c, in ? a.cols : 0, v);
-    uint32_t top = abs_max(v);
+  // A CTA takes the 16 kBlocks blocks from blockIdx.x on, in the order of the rows.
+  const long long first = static_cast<long long>(blockIdx.x) * (16 * kBlocks) + (threadIdx.x >> 4);
+  const long long total = a.rows * a.blocks;
+  Raw8<T> v[kBlocks];
+  long long row[kBlocks];
+  int c[kBlocks];
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float scale = block_scale<kE5M2>(top);
-    if (in && c < a.cols) {  // (rows of q are padded to whole pieces)
-      *reinterpret_cast<uint2*>(a.q + row * a.ldq + c) = quantize8<kE5M2>(v, 1.f / scale);
-      if (part == 0) a.scales[b] = scale;
+  for (int i = 0; i < kBlocks; ++i) {
+    const long long b = first + i * 16;
+    const bool in = b < total;
+    row[i] = !in ? 0 : b <= 0x7fffffffLL ? static_cast<long long>(static_cast<uint32_t>(b) / static_cast<uint32_t>(a.blocks)) : b / a.blocks;
+    c[i] = in ? static_cast<int>(b - row[i] * a.blocks) * 128 + part * 8 : a.cols;
+    load_piece<T, kVec>(static_cast<const T*>(a.x) + row[i] * a.ldx, c[i], a.cols, v[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kBlocks; ++i) {
+    uint32_t top = Tops<T>::of(v[i]);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = Tops<T>::larger(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float scale = block_scale<kE5M2>(Tops<T>::f32(top));
+    if (c[i] < a.cols) {  // (rows of q are padded to whole pieces)
+      float f[8];
+      v[i].values(f);
+      *reinterpret_cast<uint2*>(a.q + row[i] * a.ldq + c[i]) = quantize8<kE5M2>(f, 1.f / scale);
+      if (part == 0) a.scales[first + i * 16] = scale;
     }
   }
 }
 
-// A CTA quantises 128 x 128 values of x; thread (g, l) rows 8 g .. 8 g + 7, columns 8 l .. 8 l + 7 of them.
+// A CTA quantises 128 x 128 values of x; thread (g, l) rows 8 g .. 8 g + 7, columns 8 l .. 8 l + 7 of them, which it keeps as they lie in
+// memory (as fp32 numbers they took 93 registers, two CTAs an SM: 11008 x 4096 bf16 in 128 x 128 40 us).
 template <typename T, bool kVec, bool kE5M2, bool kSquare, bool kTransposed>
 __global__ void __launch_bounds__(256) quantize_tile_kernel(const QuantArgs a) {
-  __shared__ uint32_t tops[kSquare ? 8 : 8 * 128];
+  using Top = Tops<T>;
+  constexpr int kWords = Top::kWords;
+  __shared__ uint32_t tops[kSquare ? 8 : 8 * 16 * kWords];
   __shared__ uint2 bytes[kTransposed ? 128 * 16 : 1];  // [column of x][8 rows of x], the latter XORed with l
   griddep_launch_dependents();
   griddep_wait();
@@ -76,53 +127,66 @@ __global__ void __launch_bounds__(256) quantize_tile_kernel(const QuantArgs a) {
   const int tile_c = static_cast<int>(blockIdx.x - tile_r * tiles_c);
   const long long r0 = tile_r * 128 + g * 8;
   const int c0 = tile_c * 128 + l * 8;
-  float v[8][8];
+  Raw8<T> v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i)
     load_piece<T, kVec>(static_cast<const T*>(a.x) + (r0 + i < a.rows ? r0 + i : 0) * a.ldx, c0, r0 + i < a.rows ? a.cols : 0, v[i]);
-  float inv[8];  // of each column (kSquare: all alike)
+  float inv[kSquare ? 1 : 8];  // of each column, or of all
   if constexpr (kSquare) {
-    uint32_t top = 0u;
+    uint32_t top = Top::of(v[0]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, abs_max(v[i]));
-    top = __reduce_max_sync(0xffffffffu, top);
+    for (int i = 1; i < 8; ++i) top = Top::larger(top, Top::of(v[i]));
+    top = __reduce_max_sync(0xffffffffu, Top::f32(top));
     if (lane == 0) tops[warp] = top;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = max(top, tops[i]);
     const float scale = block_scale<kE5M2>(top);
     if (threadIdx.x == 0) a.scales[kTransposed ? static_cast<long long>(tile_c) * a.blocks + tile_r : tile_r * a.blocks + tile_c] = scale;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) inv[j] = 1.f / scale;
+    inv[0] = 1.f / scale;
   } else {
+    // columns' magnitudes: a word's over the thread's rows, the warp's two groups of rows, the CTA's warps
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      uint32_t top = 0u;
+    for (int k = 0; k < kWords; ++k) {
+      uint32_t top = Top::magnitude(Top::word(v[0], k));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i][j]) & 0x7fffffffu);
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 16));
-      if (lane < 16) tops[warp * 128 + l * 8 + j] = top;
+      for (int i = 1; i < 8; ++i) top = Top::larger(top, Top::magnitude(Top::word(v[i], k)));
+      top = Top::larger(top, __shfl_xor_sync(0xffffffffu, top, 16));
+      if (lane < 16) tops[(warp * kWords + k) * 16 + l] = top;
     }
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int k = 0; k < kWords; ++k) {
       uint32_t top = 0u;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, tops[i * 128 + l * 8 + j]);
-      const float scale = block_scale<kE5M2>(top);
-      inv[j] = 1.f / scale;
-      if (g == 0 && c0 + j < a.cols) a.scales[static_cast<long long>(c0 + j) * a.blocks + tile_r] = scale;
+      for (int i = 0; i < 8; ++i) top = Top::larger(top, tops[(i * kWords + k) * 16 + l]);
+#pragma unroll
+      for (int h = 0; h < 8 / kWords; ++h) {
+        const int j = k * (8 / kWords) + h;
+        const float scale = block_scale<kE5M2>(sizeof(T) == 4 ? top : Top::f32_of(top >> 16 * h & 0xffffu));
+        inv[j] = 1.f / scale;
+        if (g == 0 && c0 + j < a.cols) a.scales[static_cast<long long>(c0 + j) * a.blocks + tile_r] = scale;
+      }
     }
   }
   if constexpr (!kTransposed) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (r0 + i < a.rows && c0 < a.cols) *reinterpret_cast<uint2*>(a.q + (r0 + i) * a.ldq + c0) = quantize8<kE5M2>(v[i], inv[0]);
+    for (int i = 0; i < 8; ++i) {
+      float f[8];
+      v[i].values(f);
+      if (r0 + i < a.rows && c0 < a.cols) *reinterpret_cast<uint2*>(a.q + (r0 + i) * a.ldq + c0) = quantize8<kE5M2>(f, inv[0]);
+    }
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float column[8] = {v[0][j], v[1][j], v[2][j], v[3][j], v[4][j], v[5][j], v[6][j], v[7][j]};
-      bytes[(l * 8 + j) * 16 + (g ^ l)] = quantize8<kE5M2>(column, inv[j]);
+      float column[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float f[8];
+        v[i].values(f);
+        column[i] = f[j];
+      }
+      bytes[(l * 8 + j) * 16 + (g ^ l)] = quantize8<kE5M2>(column, inv[kSquare ? 0 : j]);
     }
     __syncthreads();
     // a row of q: 128 bytes from 8 threads
@@ -138,11 +202,12 @@ __global__ void __launch_bounds__(256) quantize_tile_kernel(const QuantArgs a) {
 }
 
 template <typename T, bool kVec, bool kE5M2>
-int launch_quantize(const QuantArgs& a, int block_rows, bool transposed, int sms, cudaStream_t st) {
+int launch_quantize(const QuantArgs& a, int block_rows, bool transposed, cudaStream_t st) {
   Launch l(st);
   if (block_rows == 1 && !transposed) {
-    const long long ctas = (a.rows * a.blocks + 15) / 16, most = static_cast<long long>(sms) * 64;
-    l.shape(static_cast<unsigned>(ctas < most ? ctas : most), 256);
+    const long long ctas = (a.rows * a.blocks + 63) / 64;
+    if (ctas > 0x7fffffffLL) return fail(KCG_E_TOO_LARGE, "too many blocks for one launch");
+    l.shape(static_cast<unsigned>(ctas), 256);
     return l(quantize_rows_kernel<T, kVec, kE5M2>, "quantize launch", a);
   }
   const long long tiles = ((a.rows + 127) / 128) * ((a.cols + 127) / 128);
@@ -154,13 +219,13 @@ int launch_quantize(const QuantArgs& a, int block_rows, bool transposed, int sms
 }
 
 template <typename T>
-int launch_quantize(const QuantArgs& a, int block_rows, bool transposed, bool e5m2, int sms, cudaStream_t st) {
+int launch_quantize(const QuantArgs& a, int block_rows, bool transposed, bool e5m2, cudaStream_t st) {
   const bool vec = reinterpret_cast<uint64_t>(a.x) % 16 == 0 && a.ldx * static_cast<long long>(sizeof(T)) % 16 == 0;
   if (vec)
-    return e5m2 ? launch_quantize<T, true, true>(a, block_rows, transposed, sms, st)
-                : launch_quantize<T, true, false>(a, block_rows, transposed, sms, st);
-  return e5m2 ? launch_quantize<T, false, true>(a, block_rows, transposed, sms, st)
-              : launch_quantize<T, false, false>(a, block_rows, transposed, sms, st);
+    return e5m2 ? launch_quantize<T, true, true>(a, block_rows, transposed, st)
+                : launch_quantize<T, true, false>(a, block_rows, transposed, st);
+  return e5m2 ? launch_quantize<T, false, true>(a, block_rows, transposed, st)
+              : launch_quantize<T, false, false>(a, block_rows, transposed, st);
 }
 
 }  // namespace
@@ -180,8 +245,6 @@ extern "C" int kcg_quantize_fp8(int device, uint64_t stream, uint64_t X, int64_t
   if (Q % 16 || ldq % 16) return fail(KCG_E_BAD_ARG, "rows of 8-bit values must start on 16-byte boundaries");
   const int eb = dtype == KCG_DTYPE_FLOAT32 ? 4 : 2;
   if (X % eb || S % 4) return fail(KCG_E_BAD_ARG, "operands must be aligned to their values");
-  int sms = 0;
-  if (int e = sm_count(device, &sms)) return e;
   QuantArgs a{};
   a.x = reinterpret_cast<const void*>(X), a.q = reinterpret_cast<uint8_t*>(Q), a.scales = reinterpret_cast<float*>(S);
   a.ldx = ldx, a.ldq = ldq, a.rows = rows, a.cols = cols, a.blocks = static_cast<int>((out_cols + 127) / 128);
@@ -190,7 +253,7 @@ extern "C" int kcg_quantize_fp8(int device, uint64_t stream, uint64_t X, int64_t
   if (e != cudaSuccess) return cuda_fail(e, "cudaSetDevice");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool e5m2 = dtype8 == KCG_FP8_E5M2, t = transposed != 0;
-  if (dtype == KCG_DTYPE_FLOAT32) return launch_quantize<float>(a, block_rows, t, e5m2, sms, st);
-  return dtype == KCG_DTYPE_FLOAT16 ? launch_quantize<__half>(a, block_rows, t, e5m2, sms, st)
-                                    : launch_quantize<__nv_bfloat16>(a, block_rows, t, e5m2, sms, st);
+  if (dtype == KCG_DTYPE_FLOAT32) return launch_quantize<float>(a, block_rows, t, e5m2, st);
+  return dtype == KCG_DTYPE_FLOAT16 ? launch_quantize<__half>(a, block_rows, t, e5m2, st)
+                                    : launch_quantize<__nv_bfloat16>(a, block_rows, t, e5m2, st);
 }
