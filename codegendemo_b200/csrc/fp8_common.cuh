@@ -75,6 +75,24 @@ struct Raw8<float> {
     v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
   }
 };
+// The same as pairs, for instructions that take two numbers at once.
+template <typename T>
+__device__ __forceinline__ void pairs_of(const Raw8<T>& raw, float2 (&f)[4]) {
+  float v[8];
+  raw.values(v);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f[j] = make_float2(v[2 * j], v[2 * j + 1]);
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float2 (&v)[4]) {
+  if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+  } else {
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack2(v[0].x, v[0].y, T()), pack2(v[1].x, v[1].y, T()), pack2(v[2].x, v[2].y, T()),
+                                              pack2(v[3].x, v[3].y, T()));
+  }
+}
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
   Raw8<T> raw;
@@ -101,8 +119,8 @@ __device__ __forceinline__ float abs_max3(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)), "f"(fabsf(c)));
   return r;
 }
-__device__ __forceinline__ uint32_t abs_max(const float (&v)[8]) {
-  const float m = abs_max3(abs_max3(v[0], v[1], v[2]), abs_max3(v[3], v[4], v[5]), abs_max3(v[6], v[7], v[7]));
+__device__ __forceinline__ uint32_t abs_max(const float2 (&v)[4]) {
+  const float m = abs_max3(abs_max3(v[0].x, v[0].y, v[1].x), abs_max3(v[1].y, v[2].x, v[2].y), abs_max3(v[3].x, v[3].y, v[3].y));
   return __float_as_uint(m) & 0x7fffffffu;
 }
 template <bool kE5M2>
@@ -126,6 +144,16 @@ __device__ __forceinline__ uint2 quantize8(const float (&v)[8], float inv) {
   uint2 q;
   q.x = pack_fp8<kE5M2>(v[0] * inv, v[1] * inv) | pack_fp8<kE5M2>(v[2] * inv, v[3] * inv) << 16;
   q.y = pack_fp8<kE5M2>(v[4] * inv, v[5] * inv) | pack_fp8<kE5M2>(v[6] * inv, v[7] * inv) << 16;
+  return q;
+}
+template <bool kE5M2>
+__device__ __forceinline__ uint2 quantize8(const float2 (&v)[4], float inv) {
+  float2 y[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) y[j] = __fmul2_rn(v[j], make_float2(inv, inv));
+  uint2 q;
+  q.x = pack_fp8<kE5M2>(y[0].x, y[0].y) | pack_fp8<kE5M2>(y[1].x, y[1].y) << 16;
+  q.y = pack_fp8<kE5M2>(y[2].x, y[2].y) | pack_fp8<kE5M2>(y[3].x, y[3].y) << 16;
   return q;
 }
 template <bool kE5M2>

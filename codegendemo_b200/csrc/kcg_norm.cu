@@ -31,46 +31,56 @@ struct NormArgs {
   float eps;
 };
 
-// Sum over the threads of a row: a warp's, or the CTA's.
-template <bool kWarpRow, int kN>
+// Sums over the threads of a row: a warp's (kWarps = 1), or those of a CTA of kWarps warps at most (a power of two).
+template <int kWarps, int kN>
 __device__ __forceinline__ void row_sum(float (&v)[kN], float* scratch) {
 #pragma unroll
   for (int n = 0; n < kN; ++n)
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
-  if constexpr (!kWarpRow) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  if constexpr (kWarps > 1) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5, from = lane & (kWarps - 1);
     if (lane == 0)
 #pragma unroll
-      for (int n = 0; n < kN; ++n) scratch[n * 32 + warp] = v[n];
+      for (int n = 0; n < kN; ++n) scratch[n * kWarps + warp] = v[n];
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
-      v[n] = lane < warps ? scratch[n * 32 + lane] : 0.f;
+      v[n] = from < warps ? scratch[n * kWarps + from] : 0.f;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+      for (int o = kWarps / 2; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
     }
   }
+}
+
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float rcp_ftz(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // The end of a forward pass for one piece: h is stored, y (= h * w * r) stored or quantised. kFp8: the 16 neighbouring threads that hold
 // 128 values of the row come together; the factor r goes into the scale and its reciprocal instead of into every value.
 template <typename T, bool kRes, bool kFp8>
-__device__ __forceinline__ void finish_piece(const NormArgs& a, long long row, int v, bool in, int tid, const float (&h)[8], const float (&w)[8],
-                                             float r) {
+__device__ __forceinline__ void finish_piece(const NormArgs& a, long long row, int v, bool in, int tid, const float2 (&h)[4],
+                                             const float2 (&w)[4], float r) {
   if (kRes && in) store8(static_cast<T*>(a.h) + row * a.ldh + 8 * v, h);
-  float y[8];
+  float2 y[4];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) y[j] = kFp8 ? h[j] * w[j] : h[j] * r * w[j];
+  for (int j = 0; j < 4; ++j) y[j] = kFp8 ? __fmul2_rn(h[j], w[j]) : __fmul2_rn(__fmul2_rn(h[j], both(r)), w[j]);
   if constexpr (kFp8) {
-    uint32_t top = in ? abs_max(y) : 0u;
+    uint32_t bits = in ? abs_max(y) : 0u;  // (__reduce_max_sync of a warp's halves runs them one after the other, all that follows too)
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float scale = block_scale<false>(__float_as_uint(__uint_as_float(top) * r));
-    float factor = r / scale;
-    if (factor > FLT_MAX) {  // (the smallest scale, of a block of next to nothing)
+    for (int o = 8; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+    const float top = __uint_as_float(bits);
+    // scale = top * r / 448 and, for r / scale, 448 / top, off by an ulp or two. Where one of them is no normal number (a block of next to
+    // nothing, an infinity or a NaN in the row) by the definition, from the values themselves.
+    float scale = top * r * (1.f / 448.f), factor = 448.f * rcp_ftz(top);
+    if (!(scale >= FLT_MIN && factor >= FLT_MIN && factor <= FLT_MAX)) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] *= r;
+      for (int j = 0; j < 4; ++j) y[j] = __fmul2_rn(y[j], both(r));
+      if (scale < FLT_MIN) scale = FLT_MIN;
       factor = 1.f / scale;
     }
     if (in) {
@@ -80,6 +90,20 @@ __device__ __forceinline__ void finish_piece(const NormArgs& a, long long row, i
   } else if (in) {
     store8(static_cast<T*>(a.y) + row * a.ldy + 8 * v, y);
   }
+}
+
+// h = x + residual of a piece, and its squares on top of `sum`.
+template <typename T, bool kRes>
+__device__ __forceinline__ void sum_piece(const Raw8<T>& x, const Raw8<T>& res, float2 (&h)[4], float2& sum) {
+  pairs_of(x, h);
+  if constexpr (kRes) {
+    float2 f[4];
+    pairs_of(res, f);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[j] = __fadd2_rn(h[j], f[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) sum = __ffma2_rn(h[j], h[j], sum);
 }
 
 // A warp a row, rows of up to 1024 values. kVPT: pieces of 8 values a thread holds.
@@ -92,32 +116,29 @@ __global__ void __launch_bounds__(256) norm_warp_kernel(const NormArgs a) {
   if (row >= a.rows) return;
   const T* x = static_cast<const T*>(a.x) + row * a.ldx;
   const T* res = kRes ? static_cast<const T*>(a.residual) + row * a.ldr : nullptr;
-  float h[kVPT][8], sum[1] = {0.f};
+  float2 h[kVPT][4], squares = both(0.f);
 #pragma unroll
   for (int i = 0; i < kVPT; ++i) {
     const int v = i * 32 + tid;
     Raw8<T> p, q;
-    p.zero();
-    if (v < pieces) p.load(x + 8 * v);
-    p.values(h[i]);
-    if constexpr (kRes) {
-      float f[8];
-      q.zero();
-      if (v < pieces) q.load(res + 8 * v);
-      q.values(f);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) h[i][j] += f[j];
+    p.zero(), q.zero();
+    if (v < pieces) {
+      p.load(x + 8 * v);
+      if constexpr (kRes) q.load(res + 8 * v);
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) sum[0] = fmaf(h[i][j], h[i][j], sum[0]);
+    sum_piece<T, kRes>(p, q, h[i], squares);
   }
-  row_sum<true>(sum, nullptr);
+  float sum[1] = {squares.x + squares.y};
+  row_sum<1>(sum, nullptr);
   const float r = rsqrtf(sum[0] / static_cast<float>(a.width) + a.eps);
 #pragma unroll
   for (int i = 0; i < kVPT; ++i) {
     const int v = i * 32 + tid;
-    float w[8] = {};
-    if (v < pieces) load8(static_cast<const T*>(a.w) + 8 * v, w);
+    Raw8<T> raw;
+    raw.zero();
+    if (v < pieces) raw.load(static_cast<const T*>(a.w) + 8 * v);
+    float2 w[4];
+    pairs_of(raw, w);
     finish_piece<T, kRes, kFp8>(a, row, v, v < pieces, tid, h[i], w, r);
   }
 }
@@ -127,10 +148,12 @@ __global__ void __launch_bounds__(256) norm_warp_kernel(const NormArgs a) {
 template <typename T, int kVPT, bool kRes, bool kFp8, int kThreads, int kCtas>
 __global__ void __launch_bounds__(kThreads, kCtas) norm_kernel(const NormArgs a) {
   __shared__ float scratch[2][32];
-  constexpr bool kAhead = kThreads <= 512;  // (registers)
+  constexpr bool kAhead = kThreads <= 512;                    // (registers)
+  constexpr bool kWide = kAhead && !kRes && kVPT <= 2;        // the weight as fp32 numbers
   griddep_launch_dependents();
   griddep_wait();
   const int tid = threadIdx.x, threads = blockDim.x, pieces = a.width / 8;
+  float2 wide[kWide ? kVPT : 1][4];
   Raw8<T> w[kVPT], x[kVPT], res[kRes ? kVPT : 1];
   auto ask = [&](long long row) {
 #pragma unroll
@@ -148,26 +171,18 @@ __global__ void __launch_bounds__(kThreads, kCtas) norm_kernel(const NormArgs a)
     x[i].zero();
     if constexpr (kRes) res[i].zero();
     if (kAhead && i * threads + tid < pieces) w[i].load(static_cast<const T*>(a.w) + 8 * (i * threads + tid));
+    if constexpr (kWide) pairs_of(w[i], wide[i]);
   }
   long long row = blockIdx.x;
   if (kAhead && row < a.rows) ask(row);
   for (int turn = 0; row < a.rows; row += gridDim.x, turn ^= 1) {
     if constexpr (!kAhead) ask(row);
-    float h[kVPT][8], sum[1] = {0.f};
+    float2 h[kVPT][4], squares = both(0.f);
 #pragma unroll
-    for (int i = 0; i < kVPT; ++i) {
-      x[i].values(h[i]);
-      if constexpr (kRes) {
-        float f[8];
-        res[i].values(f);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) h[i][j] += f[j];
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) sum[0] = fmaf(h[i][j], h[i][j], sum[0]);
-    }
+    for (int i = 0; i < kVPT; ++i) sum_piece<T, kRes>(x[i], res[kRes ? i : 0], h[i], squares);
+    float sum[1] = {squares.x + squares.y};
     if (kAhead && row + gridDim.x < a.rows) ask(row + gridDim.x);
-    row_sum<false>(sum, scratch[turn]);  // (two scratches: one barrier a row)
+    row_sum<kThreads / 32>(sum, scratch[turn]);  // (two scratches: one barrier a row)
     const float r = rsqrtf(sum[0] / static_cast<float>(a.width) + a.eps);
 #pragma unroll
     for (int i = 0; i < kVPT; ++i) {
@@ -175,9 +190,13 @@ __global__ void __launch_bounds__(kThreads, kCtas) norm_kernel(const NormArgs a)
       if constexpr (!kAhead) {
         if (v < pieces) w[i].load(static_cast<const T*>(a.w) + 8 * v);
       }
-      float f[8];
-      w[i].values(f);
-      finish_piece<T, kRes, kFp8>(a, row, v, v < pieces, tid, h[i], f, r);
+      if constexpr (kWide) {
+        finish_piece<T, kRes, kFp8>(a, row, v, v < pieces, tid, h[i], wide[i], r);
+      } else {
+        float2 f[4];
+        pairs_of(w[i], f);
+        finish_piece<T, kRes, kFp8>(a, row, v, v < pieces, tid, h[i], f, r);
+      }
     }
   }
 }
@@ -199,7 +218,7 @@ __global__ void __launch_bounds__(256) norm_any_kernel(const NormArgs a) {
     const float v = value(c);
     sum[0] = fmaf(v, v, sum[0]);
   }
-  row_sum<false>(sum, scratch);
+  row_sum<8>(sum, scratch);
   const float r = rsqrtf(sum[0] / static_cast<float>(a.width) + a.eps);
   for (int b = warp; b * 128 < a.width; b += blockDim.x >> 5) {
     float y[4];
@@ -294,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) norm_grad_kernel(const GradAr
       }
     }
     if (kAhead && row + gridDim.x < a.rows) ask(row + gridDim.x);
-    row_sum<false>(sum, scratch[turn]);  // (two scratches: one barrier a row)
+    row_sum<kThreads / 32>(sum, scratch[turn]);  // (two scratches: one barrier a row)
     const float r = rsqrtf(fmaf(sum[0], inv, a.eps));
     const float back = r * r * (sum[1] * inv);  // dx = r * (g - h * back)
 #pragma unroll
@@ -338,7 +357,7 @@ __global__ void __launch_bounds__(512) norm_grad_any_kernel(const GradArgs a) {
       sum[0] = fmaf(v, v, sum[0]);
       sum[1] = fmaf(to_f32(dy[c]) * to_f32(w[c]), v, sum[1]);
     }
-    row_sum<false>(sum, scratch[turn]);
+    row_sum<16>(sum, scratch[turn]);
     const float inv = 1.f / static_cast<float>(a.width);
     const float r = rsqrtf(fmaf(sum[0], inv, a.eps)), back = r * r * (sum[1] * inv);
     for (int c = threadIdx.x; c < a.width; c += blockDim.x) {
@@ -409,7 +428,8 @@ int launch_norm(const NormArgs& a, bool vectors, int sms, cudaStream_t st) {
     if (pieces <= 64) return l(norm_warp_kernel<T, 2, kRes, kFp8>, "norm launch", a);
     return l(norm_warp_kernel<T, 4, kRes, kFp8>, "norm launch", a);
   }
-  if (pieces <= 512) return launch_norm_rows<T, 1, kRes, kFp8, 512, 3>(l, a, sms);
+  if (pieces <= 256) return launch_norm_rows<T, 1, kRes, kFp8, 256, 6>(l, a, sms);
+  if (pieces <= 512) return launch_norm_rows<T, 2, kRes, kFp8, 256, 4>(l, a, sms);
   if (pieces <= 1024) return launch_norm_rows<T, 2, kRes, kFp8, 512, 2>(l, a, sms);
   if (pieces <= 2048) return launch_norm_rows<T, 4, kRes, kFp8, 512, 1>(l, a, sms);
   return launch_norm_rows<T, 4, kRes, kFp8, 1024, 1>(l, a, sms);
@@ -426,7 +446,7 @@ constexpr int kMaxWidth = 32768;  // a row in a CTA's registers, its share of dw
 // CTAs that walk the rows of the backward pass, each with its own share of dw: as many as run at once, with 512 threads or fewer
 // two an SM.
 int grad_ctas(int sms, long long rows, int width) {
-  const long long most = static_cast<long long>(sms) * (width <= 2048 ? 4 : width <= 4096 ? 2 : 1);
+  const long long most = static_cast<long long>(sms) * (width <= 2048 ? 3 : width <= 4096 ? 2 : 1);
   return static_cast<int>(rows < most ? rows : most);
 }
 
@@ -445,9 +465,13 @@ int launch_grad(const GradArgs& a, int ctas, bool vectors, cudaStream_t st) {
   }
   const int pieces = a.width / 8;
   auto threads = [&](int vpt) { return static_cast<unsigned>(((pieces + vpt - 1) / vpt + 31) / 32 * 32); };
-  if (pieces <= 512) {
+  if (pieces <= 256) {
     l.shape(ctas, threads(1));
-    return l(norm_grad_kernel<T, 1, kDh, 512, 2>, "norm gradient launch", a);
+    return l(norm_grad_kernel<T, 1, kDh, 256, 3>, "norm gradient launch", a);
+  }
+  if (pieces <= 512) {
+    l.shape(ctas, threads(2));
+    return l(norm_grad_kernel<T, 2, kDh, 256, 2>, "norm gradient launch", a);
   }
   if (pieces <= 1024) {
     l.shape(ctas, threads(2));
