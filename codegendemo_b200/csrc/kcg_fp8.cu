@@ -72,17 +72,10 @@ __device__ __forceinline__ void tmem_ld_16x256b_x2(uint32_t taddr, uint32_t (&r)
                : "memory");
 }
 // Ties the registers of an earlier load to the wait before it: no use of them may be scheduled ahead of this.
-__device__ __forceinline__ void pin_32(uint32_t (&r)[32]) {
+template <int kN>
+__device__ __forceinline__ void pin(uint32_t (&r)[kN]) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i]));
-}
-__device__ __forceinline__ void pin_16(uint32_t (&r)[16]) {
-#pragma unroll
-  for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(r[i]));
-}
-__device__ __forceinline__ void pin_8(uint32_t (&r)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) asm volatile("" : "+r"(r[i]));
+  for (int i = 0; i < kN; ++i) asm volatile("" : "+r"(r[i]));
 }
 
 // Completion of the pair's products issued so far -> one arrival on this barrier of both CTAs.
@@ -112,7 +105,7 @@ struct Fp8Params {
   float beta;
   int relu;
   int fused;  // any of the three
-  int vector_store;  // rows of C start on 16-byte boundaries
+  int vector_store, word_store;  // rows of C start on 16-byte boundaries, on 4-byte ones
   int vector_sp, vector_sq;  // so do those of the scales
   int splits;        // Fp8Tile: CTAs that share a tile's K
 };
@@ -159,28 +152,67 @@ __device__ __forceinline__ float bias_at(const Fp8Params& p, int n) {
   return p.bias ? to_f32(static_cast<const T*>(p.bias)[n]) : 0.f;
 }
 
-// Eight columns of one row of C from column n on.
+// Unit u of 16 bytes of values of C.
 template <typename T>
-__device__ __forceinline__ void store_span8(const Fp8Params& p, const float* v, long long m, int n, int cols) {
-  T* c = static_cast<T*>(p.C) + m * p.ldc + n;
-  if (p.vector_store && n + 8 <= cols) {
-    float out[8];
-    float old[8];
-    if (p.beta != 0.f) load8(c, old);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      out[j] = v[j];
-      if (p.beta != 0.f) out[j] = fmaf(p.beta, old[j], out[j]);
-      out[j] += bias_at<T>(p, n + j);
-      if (p.relu) out[j] = fmaxf(out[j], 0.f);
-    }
-    store8(c, out);
+__device__ __forceinline__ uint4 unit16(const float* v, int u) {
+  if constexpr (sizeof(T) == 4) {
+    return make_uint4(__float_as_uint(v[4 * u]), __float_as_uint(v[4 * u + 1]), __float_as_uint(v[4 * u + 2]), __float_as_uint(v[4 * u + 3]));
   } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (n + j < cols) c[j] = from_f32<T>(finish<T>(p, v[j], c + j, bias_at<T>(p, n + j)));
+    return make_uint4(pack2(v[8 * u], v[8 * u + 1], T()), pack2(v[8 * u + 2], v[8 * u + 3], T()), pack2(v[8 * u + 4], v[8 * u + 5], T()),
+                      pack2(v[8 * u + 6], v[8 * u + 7], T()));
   }
 }
+
+// bias, beta and ReLU of kN values of row m from column n on.
+template <typename T, int kN>
+__device__ __forceinline__ void finish_row(const Fp8Params& p, float (&v)[kN], int m, int n) {
+  if (m >= p.rows_p) return;
+  const T* c = static_cast<const T*>(p.C) + static_cast<long long>(m) * p.ldc + n;
+#pragma unroll
+  for (int i = 0; i < kN; ++i)
+    if (n + i < p.rows_q) v[i] = finish<T>(p, v[i], c + i, bias_at<T>(p, n + i));
+}
+
+// 32 rows of kN values of C wait in a warp's shared memory, kPitch bytes a row (16-byte units of the rows then lie in different banks), and
+// go to C row by row. (Written from the registers of a thread a row, single values of an odd N took 60 us instead of 10 at 2049 x 2305 x 304.)
+template <typename T, int kN>
+struct RowStore {
+  static constexpr int kPitch = kN * static_cast<int>(sizeof(T)) + 16, kBytes = 32 * kPitch;
+  __device__ static __forceinline__ void put_row(uint8_t* stage, const float* v) {
+    uint8_t* to = stage + (threadIdx.x & 31) * kPitch;
+#pragma unroll
+    for (int u = 0; u < kN * static_cast<int>(sizeof(T)) / 16; ++u) *reinterpret_cast<uint4*>(to + 16 * u) = unit16<T>(v, u);
+  }
+  // Called by a whole warp; the rows have been put (__syncwarp) and may be overwritten afterwards.
+  __device__ static __forceinline__ void copy(const Fp8Params& p, const uint8_t* stage, int row0, int col0) {
+    const int lane = threadIdx.x & 31, rows = min(32, p.rows_p - row0), cols = min(kN, p.rows_q - col0);
+    T* c = static_cast<T*>(p.C) + static_cast<long long>(row0) * p.ldc + col0;
+    __syncwarp();
+    constexpr int kEach = 16 / static_cast<int>(sizeof(T)), kUnits = kN / kEach;
+    if (p.vector_store && cols % kEach == 0) {
+      const int units = cols / kEach;
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        const int r = (i * 32 + lane) / kUnits, u = (i * 32 + lane) % kUnits;
+        if (r < rows && u < units) reinterpret_cast<uint4*>(c + r * p.ldc)[u] = *reinterpret_cast<const uint4*>(stage + r * kPitch + u * 16);
+      }
+    } else if (sizeof(T) == 2 && p.word_store) {
+      const int words = cols / 2;
+#pragma unroll 8
+      for (int r = 0; r < rows; ++r) {
+        const uint32_t* from = reinterpret_cast<const uint32_t*>(stage + r * kPitch);
+        uint32_t* to = reinterpret_cast<uint32_t*>(c + r * p.ldc);
+        for (int i = lane; i < words; i += 32) to[i] = from[i];
+        if ((cols & 1) && lane == 0) c[r * p.ldc + cols - 1] = reinterpret_cast<const T*>(from)[cols - 1];
+      }
+    } else {
+#pragma unroll 8
+      for (int r = 0; r < rows; ++r)
+        for (int i = lane; i < cols; i += 32) c[r * p.ldc + i] = reinterpret_cast<const T*>(stage + r * kPitch)[i];
+    }
+    __syncwarp();
+  }
+};
 
 template <typename Bars>
 __device__ __forceinline__ void report(Bars* bars, uint32_t code, uint32_t d0, uint32_t d1) {
@@ -194,26 +226,86 @@ __device__ __forceinline__ void report(Bars* bars, uint32_t code, uint32_t d0, u
 
 // kBN: columns of a tile. kVector: each column has a scale of its own, else the tile's columns share one (kBN <= 128).
 // kSwap: the tile's rows are columns of C (weights), its columns rows of C (tokens).
+// Four accumulators in tensor memory: products, signals and additions of a block take about three times as long as the products alone, with
+// two accumulators 128 x 128 tiles took 800 cycles a block.
 template <int kBN, bool kVector, bool kSwap, typename T>
 struct Fp8Tile {
-  static constexpr int NUM_THREADS = 192;  // producer, issuer, four accumulating warps
+  // producer, issuer, four accumulating warps, or eight that share the columns: four are busy 800 cycles with 128 of them
+  static constexpr int GROUPS = kBN == 128 ? 2 : 1, COLS = kBN / GROUPS;
+  static constexpr int NUM_THREADS = 64 + 128 * GROUPS;
   static constexpr int P_BYTES = 128 * 128, STAGE_BYTES = P_BYTES + kBN * 128;
   static constexpr int STAGES = kBN == 16 ? 6 : kBN == 32 ? 5 : kBN == 64 ? 4 : 6;
   static constexpr int CTAS_PER_SM = kBN <= 64 ? 2 : 1;
   static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
-  static constexpr int PIECE = kBN < 32 ? 16 : 32;
-  static constexpr uint32_t TMEM_COLS = 2 * kBN;  // (32 at least, a power of two)
+  static constexpr int BUFS = 4, PIECE = kBN < 32 ? 16 : 32;
+  static constexpr uint32_t TMEM_COLS = BUFS * kBN;  // (a power of two; two CTAs an SM: 512 together at most)
   static constexpr int SMEM_BYTES = RING_BYTES + 1024 + 2048;
-  static_assert(kBN * 128 * 4 <= RING_BYTES, "the joining lays a tile over the ring");
+  static constexpr int PART_BYTES = kBN * 128 * 4;  // a tile in fp32
+  static_assert(PART_BYTES + (kSwap ? 0 : 4 * GROUPS * RowStore<T, COLS>::kBytes) <= RING_BYTES, "a tile, and rows to store, are laid over the ring");
 
   struct Barriers {
     uint64_t full[STAGES], empty[STAGES];
-    uint64_t tmem_full[2], tmem_empty[2];
+    uint64_t tmem_full[BUFS], tmem_empty[BUFS];
     uint32_t tmem_base;
     volatile uint32_t abort_flag;
     alignas(16) float scale[2][kVector ? kBN : 4];
   };
   static_assert(sizeof(Barriers) <= 2048, "barrier block exceeds its shared-memory slot");
+
+  __device__ static __forceinline__ void load(uint32_t taddr, uint32_t (&r)[PIECE]) {
+    if constexpr (PIECE == 16) {
+      tmem_ld_32x32b_x16(taddr, r);
+    } else {
+      tmem_ld_32x32b_x32(taddr, r);
+    }
+  }
+
+  // kN columns of this thread's row of the tile to C. `stage`: this warp's shared memory.
+  template <int kN>
+  __device__ static __forceinline__ void store(const Fp8Params& p, float (&v)[kN], int gp, int gq, uint8_t* stage) {
+    if constexpr (kSwap) {
+      if (gp >= p.rows_p) return;
+      const float bias = bias_at<T>(p, gp);
+      T* out = static_cast<T*>(p.C) + static_cast<long long>(gq) * p.ldc + gp;
+#pragma unroll
+      for (int c = 0; c < kN; ++c, out += p.ldc)
+        if (gq + c < p.rows_q) *out = from_f32<T>(finish<T>(p, v[c], out, bias));
+    } else {
+      const int row0 = gp - static_cast<int>(threadIdx.x & 31);
+      if (row0 >= p.rows_p || gq >= p.rows_q) return;
+      if (p.fused) finish_row<T, kN>(p, v, gp, gq);
+      RowStore<T, kN>::put_row(stage, v);
+      RowStore<T, kN>::copy(p, stage, row0, gq);
+    }
+  }
+
+  // The tile from the parts of kS CTAs, in the order of their ranks; this one's share of the columns, this group's share of that.
+  template <int kS>
+  __device__ static __forceinline__ void join(const Fp8Params& p, const float* part, int rank, int group, int row, int p0, int q0,
+                                              uint8_t* stage) {
+    constexpr int kPer = kBN / kS / GROUPS, kAtOnce = kPer < 8 ? kPer : 8;
+    const int first = (rank * GROUPS + group) * kPer;
+    const uint32_t mine = smem_u32(part + first * 128 + row);
+    uint32_t from[kS];
+#pragma unroll
+    for (int r = 0; r < kS; ++r) from[r] = map_to_cta(mine, r);
+    float v[kPer];
+#pragma unroll
+    for (int c0 = 0; c0 < kPer; c0 += kAtOnce) {
+      float x[kS][kAtOnce];
+#pragma unroll
+      for (int r = 0; r < kS; ++r)
+#pragma unroll
+        for (int c = 0; c < kAtOnce; ++c) x[r][c] = ld_cluster_f32(from[r] + (c0 + c) * 512);
+#pragma unroll
+      for (int c = 0; c < kAtOnce; ++c) {
+        v[c0 + c] = x[0][c];
+#pragma unroll
+        for (int r = 1; r < kS; ++r) v[c0 + c] += x[r][c];
+      }
+    }
+    store<kPer>(p, v, p0 + row, q0 + first, stage);
+  }
 
   __device__ static void run(const Fp8Params& p) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -235,9 +327,9 @@ struct Fp8Tile {
         mbar_init(&bars->full[s], 1);
         mbar_init(&bars->empty[s], 1);
       }
-      for (int b = 0; b < 2; ++b) {
+      for (int b = 0; b < BUFS; ++b) {
         mbar_init(&bars->tmem_full[b], 1);
-        mbar_init(&bars->tmem_empty[b], 4);
+        mbar_init(&bars->tmem_empty[b], 4 * GROUPS);
       }
       bars->abort_flag = 0u;
       fence_mbar_init();
@@ -253,8 +345,9 @@ struct Fp8Tile {
     const uint32_t tmem_base = bars->tmem_base;
     griddep_wait();
 
-    float acc[kBN];
-    const int q = warp & 3, row = q * 32 + lane;  // (accumulating warps) TMEM lane quarter, row of the tile
+    float acc[COLS];
+    // (accumulating warps) TMEM lane quarter, row of the tile, which columns
+    const int q = warp & 3, row = q * 32 + lane, group = (warp - 2) >> 2;
     bool ok = true;
     if (warp == 0) {
       if (lane == 0) {
@@ -277,9 +370,9 @@ struct Fp8Tile {
       const uint64_t qdesc = make_smem_desc(smem_u32(smem) + P_BYTES, 16, 1024, SWZ_128B);
       const uint32_t idesc = make_instr_desc(0u, 0u, 0u, 128u, kBN) | p.fmt_p << 7 | p.fmt_q << 10;
       for (int i = 0; i < n; ++i) {
-        const uint32_t s = i % STAGES, b = i & 1u;
-        if (!mbar_wait_warp(&bars->tmem_empty[b], ((i >> 1) & 1u) ^ 1u, &bars->abort_flag) ||
-            !mbar_wait_warp(&bars->full[s], (i / STAGES) & 1u, &bars->abort_flag)) {
+        const uint32_t s = i % STAGES, b = i % BUFS;
+        if (!mbar_wait_warp(&bars->full[s], (i / STAGES) & 1u, &bars->abort_flag) ||
+            !mbar_wait_warp(&bars->tmem_empty[b], ((i / BUFS) & 1u) ^ 1u, &bars->abort_flag)) {
           if (lane == 0) report(bars, FP8_TIMEOUT_MMA, i, s);
           break;
         }
@@ -289,99 +382,101 @@ struct Fp8Tile {
           for (int ks = 0; ks < 4; ++ks)  // 32 values = 32 bytes of a row
             umma_fp8<1>(tmem + b * kBN, pdesc + s * (STAGE_BYTES >> 4) + ks * 2, qdesc + s * (STAGE_BYTES >> 4) + ks * 2, idesc,
                         ks > 0 ? 1u : 0u);
-          umma_commit(&bars->empty[s]);
           umma_commit(&bars->tmem_full[b]);
+          umma_commit(&bars->empty[s]);
         }
         __syncwarp();
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < kBN; ++i) acc[i] = 0.f;
-      const int t = threadIdx.x - 64;  // also: column whose scale this thread fetches
+      for (int i = 0; i < COLS; ++i) acc[i] = 0.f;
+      const int t = group * COLS + (threadIdx.x - 64) % 128;  // column whose scale this thread fetches
       const float* sp = p.sp + (static_cast<long long>(min(p0 + row, p.rows_p - 1)) >> p.sp_shift) * p.ldsp + kb0;
       const float* sq = p.sq + (static_cast<long long>(min(q0 + (kVector ? t : 0), p.rows_q - 1)) >> p.sq_shift) * p.ldsq + kb0;
-      const bool fetches = !kVector || t < kBN;
-      float next_p = __ldg(sp), next_q = fetches ? __ldg(sq) : 0.f;
-      for (int i = 0; i < n; ++i) {
-        const uint32_t b = i & 1u;
-        const float f = kVector ? next_p : scale_product(next_p, next_q);
-        if constexpr (kVector) {
-          // (two buffers: a thread that writes one again has passed the meeting behind which all have read it)
-          if (fetches) bars->scale[b][t] = next_q;
-          named_bar_sync(1, 128);
-        }
-        if (i + 1 < n) {
-          next_p = __ldg(sp + i + 1);
-          if (fetches) next_q = __ldg(sq + i + 1);
-        }
-        if (ok) {
-          const bool got = mbar_wait(&bars->tmem_full[b], (i >> 1) & 1u, &bars->abort_flag);
-          if (!__all_sync(0xffffffffu, got)) {
-            if (lane == 0) report(bars, FP8_TIMEOUT_ACCUMULATE, i, b);
-            ok = false;
-          }
-        }
-        if (!ok) continue;  // (the meetings go on)
-        tc_fence_after_sync();
-        const uint32_t col = tmem_base + b * kBN + (static_cast<uint32_t>(q * 32) << 16);
+      const bool fetches = !kVector || (threadIdx.x - 64) % 128 < COLS;
+      // the scales of four blocks at a time, four blocks ahead
+      float next_p[4], next_q[4];
+      auto fetch = [&](int i) {
 #pragma unroll
-        for (int c = 0; c < kBN; c += PIECE) {
-          uint32_t r[PIECE];
-          if constexpr (PIECE == 16) {
-            tmem_ld_32x32b_x16(col + c, r);
-          } else {
-            tmem_ld_32x32b_x32(col + c, r);
-          }
-          tmem_ld_wait();
+        for (int j = 0; j < 4; ++j) {
+          next_p[j] = i + j < n ? __ldg(sp + i + j) : 0.f;
+          next_q[j] = fetches && i + j < n ? __ldg(sq + i + j) : 0.f;
+        }
+      };
+      fetch(0);
+      for (int i0 = 0; i0 < n; i0 += 4) {
+        float f[4], g[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = next_p[j], g[j] = next_q[j];
+        if (i0 + 4 < n) fetch(i0 + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = i0 + j;
+          if (i >= n) break;
           if constexpr (kVector) {
-            add_scaled<PIECE>(acc + c, r, &bars->scale[b][c], f);
-          } else {
-            add_scaled<PIECE>(acc + c, r, f);
+            // (two buffers: a thread that writes one again has passed the meeting behind which all have read it)
+            if (fetches) bars->scale[j & 1][t] = g[j];
+            named_bar_sync(1 + group, 128);
+          }
+          if (ok) {
+            const bool got = mbar_wait(&bars->tmem_full[j], (i0 / 4) & 1u, &bars->abort_flag);
+            if (!__all_sync(0xffffffffu, got)) {
+              if (lane == 0) report(bars, FP8_TIMEOUT_ACCUMULATE, i, j);
+              ok = false;
+            }
+          }
+          if (!ok) continue;  // (the meetings go on)
+          tc_fence_after_sync();
+          const uint32_t col = tmem_base + j * kBN + group * COLS + (static_cast<uint32_t>(q * 32) << 16);
+          const float* scale = &bars->scale[j & 1][kVector ? group * COLS : 0];
+          const float factor = kVector ? f[j] : scale_product(f[j], g[j]);
+          uint32_t r[2][PIECE];
+          load(col, r[0]);
+#pragma unroll
+          for (int c = 0; c < COLS / PIECE; ++c) {
+            tmem_ld_wait();
+            pin(r[c & 1]);
+            if (c + 1 < COLS / PIECE) {
+              load(col + (c + 1) * PIECE, r[(c + 1) & 1]);
+            } else {
+              tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&bars->tmem_empty[j]);
+            }
+            if constexpr (kVector) {
+              add_scaled<PIECE>(acc + c * PIECE, r[c & 1], scale + c * PIECE, factor);
+            } else {
+              add_scaled<PIECE>(acc + c * PIECE, r[c & 1], factor);
+            }
           }
         }
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->tmem_empty[b]);
       }
     }
 
+    // Every product has been read, so the ring is idle (the accumulating warps' shared memory lies behind a tile's).
+    uint8_t* stage = smem + (kSwap ? 0 : PART_BYTES + (warp >= 2 ? warp - 2 : 0) * RowStore<T, COLS>::kBytes);
     if (p.splits > 1) {
-      // Every product has been read, so the ring is idle: the CTA's tile goes there, column after column of 128 rows.
+      // the CTA's tile, column after column of 128 rows
       float* part = reinterpret_cast<float*>(smem);
       if (warp >= 2 && ok) {
 #pragma unroll
-        for (int c = 0; c < kBN; ++c) part[c * 128 + row] = acc[c];
+        for (int c = 0; c < COLS; ++c) part[(group * COLS + c) * 128 + row] = acc[c];
       }
       __syncwarp();
       cluster_sync_all();
       if (warp >= 2 && ok) {
-        const int per = kBN / p.splits, c0 = rank * per;  // (splits: a power of two, at most 8)
-        const uint32_t mine = smem_u32(part + row);
-        for (int c = c0; c < c0 + per; ++c) {
-          float v = 0.f;
-          for (int r = 0; r < p.splits; ++r) v += ld_cluster_f32(map_to_cta(mine + c * 512, r));
-          const int gp = p0 + row, gq = q0 + c;
-          if (gp < p.rows_p && gq < p.rows_q) {
-            T* out = static_cast<T*>(p.C) + (kSwap ? gq * p.ldc + gp : gp * p.ldc + gq);
-            *out = from_f32<T>(finish<T>(p, v, out, bias_at<T>(p, kSwap ? gp : gq)));
-          }
+        if (p.splits == 2) {
+          join<2>(p, part, rank, group, row, p0, q0, stage);
+        } else if (p.splits == 4) {
+          join<4>(p, part, rank, group, row, p0, q0, stage);
+        } else if constexpr (kSwap) {
+          join<8>(p, part, rank, group, row, p0, q0, stage);
         }
       }
       __syncwarp();
       cluster_sync_all();  // shared memory stays until the others have read it
-    } else if (warp >= 2 && ok && p0 + row < p.rows_p) {
-      if constexpr (kSwap) {
-        const float bias = bias_at<T>(p, p0 + row);
-#pragma unroll
-        for (int c = 0; c < kBN; ++c)
-          if (q0 + c < p.rows_q) {
-            T* out = static_cast<T*>(p.C) + static_cast<long long>(q0 + c) * p.ldc + p0 + row;
-            *out = from_f32<T>(finish<T>(p, acc[c], out, bias));
-          }
-      } else {
-#pragma unroll
-        for (int c = 0; c < kBN; c += 8) store_span8<T>(p, acc + c, p0 + row, q0 + c, p.rows_q);
-      }
+    } else if (warp >= 2 && ok) {
+      store<COLS>(p, acc, p0 + row, q0 + group * COLS, stage);
     }
 
     // ---------------------------------------------------------------- common exit
@@ -401,7 +496,8 @@ struct Fp8Tile {
 };
 
 template <int kBN, bool kVector, bool kSwap, typename T>
-__global__ void __launch_bounds__(192, Fp8Tile<kBN, kVector, kSwap, T>::CTAS_PER_SM) fp8_tile_kernel(const __grid_constant__ Fp8Params p) {
+__global__ void __launch_bounds__(Fp8Tile<kBN, kVector, kSwap, T>::NUM_THREADS, Fp8Tile<kBN, kVector, kSwap, T>::CTAS_PER_SM)
+fp8_tile_kernel(const __grid_constant__ Fp8Params p) {
   Fp8Tile<kBN, kVector, kSwap, T>::run(p);
 }
 
@@ -427,7 +523,10 @@ struct Fp8Pair {
   static constexpr int STORE_BYTES = 8 * 2 * 32 * 128;  // two blocks of 32 rows of 128 bytes for each accumulating warp
   static constexpr int SCALES = 128 + (kVector ? 256 : 4);  // of a block of K: the CTA's rows, the tile's columns (or halves)
   static constexpr int GROUP_KB = 4;                        // blocks of K whose scales come together
-  static constexpr int SCALE_BYTES = 2 * GROUP_KB * SCALES * 4;
+  // Groups in shared memory: the one that may still be read until all have met at the next one's first block, that one, and the one after
+  // it, which has to be there before its last block (that may be its first).
+  static constexpr int GROUPS = 3;
+  static constexpr int SCALE_BYTES = GROUPS * GROUP_KB * SCALES * 4;
   static constexpr int SMEM_BYTES = RING_BYTES + STORE_BYTES + SCALE_BYTES + 1024 + 512;
   static constexpr int GROUP = 8;  // tile rows that are walked together, column after column
   static constexpr uint32_t TMEM_COLS = 512;
@@ -436,7 +535,7 @@ struct Fp8Pair {
   struct Barriers {
     uint64_t full[STAGES], empty[STAGES];
     uint64_t tmem_full[2], tmem_empty[2];
-    uint64_t scale_full[2], scale_empty[2];
+    uint64_t scale_full[GROUPS], scale_empty[GROUPS];
     uint32_t tmem_base;
     volatile uint32_t abort_flag;
   };
@@ -491,56 +590,47 @@ struct Fp8Pair {
     }
   };
 
-  // This warp's accumulators to C: 32 rows of 128 columns, through blocks of shared memory (16-byte units XORed with the row, the
-  // swizzle of the tensor map) and TMA stores, two under way.
+  // This warp's accumulators to C: 32 rows of 128 columns, through blocks of shared memory: 16-byte units XORed with the row, the
+  // swizzle of the tensor map, and TMA stores, two under way; or rows by RowStore where TMA cannot address them.
   __device__ static __forceinline__ void store(const Fp8Params& p, float (&acc)[128], int row0, int col0, uint8_t* blocks) {
+    using Rows = RowStore<T, COLS_BLOCK>;
+    static_assert(Rows::kBytes <= 8192, "a block of rows exceeds a warp's shared memory");
     const int lane = threadIdx.x & 31;
-    // Row and column of accumulator i: kVector as tcgen05.ld.16x256b lays them out, else a row a thread.
-    auto row_of = [&](int i) { return kVector ? (i >> 1 & 3) * 8 + (lane >> 2) : lane; };
-    auto col_of = [&](int i) { return kVector ? (i >> 3) * 8 + (lane & 3) * 2 + (i & 1) : i; };
-    if (p.fused || !p.vector_store) {
+    if (p.fused) {
+      // Row and column of accumulator i: kVector as tcgen05.ld.16x256b lays them out, else a row a thread.
 #pragma unroll
       for (int i = 0; i < 128; ++i) {
-        const int m = row0 + row_of(i), n = col0 + col_of(i);
-        if (m < p.rows_p && n < p.rows_q) {
-          T* c = static_cast<T*>(p.C) + static_cast<long long>(m) * p.ldc + n;
-          acc[i] = finish<T>(p, acc[i], c, bias_at<T>(p, n));
-          if (!p.vector_store) *c = from_f32<T>(acc[i]);
-        }
+        const int m = row0 + (kVector ? (i >> 1 & 3) * 8 + (lane >> 2) : lane), n = col0 + (kVector ? (i >> 3) * 8 + (lane & 3) * 2 + (i & 1) : i);
+        if (m < p.rows_p && n < p.rows_q)
+          acc[i] = finish<T>(p, acc[i], static_cast<const T*>(p.C) + static_cast<long long>(m) * p.ldc + n, bias_at<T>(p, n));
       }
-      if (!p.vector_store) return;
     }
 #pragma unroll
     for (int b = 0; b < 128 / COLS_BLOCK; ++b) {
       if (row0 >= p.rows_p || col0 + b * COLS_BLOCK >= p.rows_q) break;
-      uint8_t* block = blocks + (b & 1) * 4096;
-      if (lane == 0) tma_store_wait_read<1>();  // the store before the last has read its block
-      __syncwarp();
+      uint8_t* block = blocks + (p.vector_store ? (b & 1) * 4096 : 0);
+      if (p.vector_store) {
+        if (lane == 0) tma_store_wait_read<1>();  // the store before the last has read its block
+        __syncwarp();
+      }
       if constexpr (!kVector) {
-        uint8_t* to = block + lane * 128;
         const float* v = acc + b * COLS_BLOCK;
+        if (p.vector_store) {
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          uint4 raw;
-          if constexpr (sizeof(T) == 4) {
-            raw = make_uint4(__float_as_uint(v[4 * u]), __float_as_uint(v[4 * u + 1]), __float_as_uint(v[4 * u + 2]),
-                             __float_as_uint(v[4 * u + 3]));
-          } else {
-            raw = make_uint4(pack2(v[8 * u], v[8 * u + 1], T()), pack2(v[8 * u + 2], v[8 * u + 3], T()),
-                             pack2(v[8 * u + 4], v[8 * u + 5], T()), pack2(v[8 * u + 6], v[8 * u + 7], T()));
-          }
-          *reinterpret_cast<uint4*>(to + ((u ^ (lane & 7)) << 4)) = raw;
+          for (int u = 0; u < 8; ++u) *reinterpret_cast<uint4*>(block + lane * 128 + ((u ^ (lane & 7)) << 4)) = unit16<T>(v, u);
+        } else {
+          Rows::put_row(block, v);
         }
       } else {
         const uint32_t x = lane >> 2, t = lane & 3;  // (row within eight, pair of columns within eight)
-        uint8_t* to = block + x * 128 + (sizeof(T) == 4 ? (t & 1) * 8 : t * 4);
-        const uint32_t swizzle = (sizeof(T) == 4 ? x ^ (t >> 1) : x) << 4;
+        const uint32_t swizzle = !p.vector_store ? 0u : (sizeof(T) == 4 ? x ^ (t >> 1) : x) << 4, pitch = p.vector_store ? 128 : Rows::kPitch;
+        uint8_t* to = block + x * pitch + (sizeof(T) == 4 ? (t & 1) * 8 + (p.vector_store ? 0 : (t >> 1) * 16) : t * 4);
 #pragma unroll
-        for (int j = 0; j < COLS_BLOCK / 8; ++j)
+        for (int r = 0; r < 4; ++r, to += 8 * pitch)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
+          for (int j = 0; j < COLS_BLOCK / 8; ++j) {
             const float* v = acc + (b * (COLS_BLOCK / 8) + j) * 8 + r * 2;
-            uint8_t* at = to + r * 1024 + ((j * (sizeof(T) == 4 ? 32 : 16)) ^ swizzle);
+            uint8_t* at = to + ((j * (sizeof(T) == 4 ? 32 : 16)) ^ swizzle);
             if constexpr (sizeof(T) == 4) {
               *reinterpret_cast<float2*>(at) = make_float2(v[0], v[1]);
             } else {
@@ -548,7 +638,11 @@ struct Fp8Pair {
             }
           }
       }
-      send(p, block, row0, col0 + b * COLS_BLOCK);
+      if (p.vector_store) {
+        send(p, block, row0, col0 + b * COLS_BLOCK);
+      } else {
+        Rows::copy(p, block, row0, col0 + b * COLS_BLOCK);
+      }
     }
   }
   __device__ static __forceinline__ void send(const Fp8Params& p, uint8_t* block, int row, int col) {
@@ -580,8 +674,10 @@ struct Fp8Pair {
       for (int b = 0; b < 2; ++b) {
         mbar_init(&bars->tmem_full[b], 1);
         mbar_init(&bars->tmem_empty[b], 16);  // one arrival for each accumulating warp of both CTAs
-        mbar_init(&bars->scale_full[b], 32);
-        mbar_init(&bars->scale_empty[b], 1);
+      }
+      for (int g = 0; g < GROUPS; ++g) {
+        mbar_init(&bars->scale_full[g], 32);
+        mbar_init(&bars->scale_empty[g], 1);
       }
       bars->abort_flag = 0u;
       fence_mbar_init();
@@ -610,16 +706,15 @@ struct Fp8Pair {
       ok = named_bar_all(BAR_FULL, MEETING, ok);  // the first block's scales
       for (int tile = tile0; tile < tiles && ok; tile += stride) {
         for (int kb = 0; kb < p.num_kb && ok; ++kb, ++it) {
+          const bool begins = kb % GROUP_KB == 0 && it > 0;  // a group after the first
+          if (begins) ++g;
           if ((kb % GROUP_KB == GROUP_KB - 1 || kb == p.num_kb - 1) && (kb < p.num_kb - 1 || tile + stride < tiles))
-            wait(&bars->scale_full[(g + 1) & 1u], ((g + 1) >> 1) & 1u, 2u);
+            wait(&bars->scale_full[(g + 1) % GROUPS], ((g + 1) / GROUPS) & 1u, 2u);
           wait(&bars->tmem_full[it & 1u], (it >> 1) & 1u, 0u);
           tc_fence_after_sync();
           tc_fence_before_sync();
           ok = named_bar_all(BAR_FULL, MEETING, ok);
-          if (kb % GROUP_KB == 0 && it > 0) {  // nobody reads the group before any more
-            if (lane == 0) mbar_arrive(&bars->scale_empty[g & 1u]);
-            ++g;
-          }
+          if (begins && lane == 0) mbar_arrive(&bars->scale_empty[(g - 1) % GROUPS]);  // nobody reads the group before any more
         }
       }
     } else if (warp == 1) {
@@ -680,9 +775,9 @@ struct Fp8Pair {
           }
           __syncwarp();
           if (kb % GROUP_KB == 0) {
-            if (!wait(&bars->scale_empty[g & 1u], ((g >> 1) & 1u) ^ 1u, 100u)) break;
-            held.store(scales + (g & 1u) * GROUP_KB * SCALES);
-            mbar_arrive(&bars->scale_full[g & 1u]);
+            if (!wait(&bars->scale_empty[g % GROUPS], ((g / GROUPS) & 1u) ^ 1u, 100u)) break;
+            held.store(scales + g % GROUPS * GROUP_KB * SCALES);
+            mbar_arrive(&bars->scale_full[g % GROUPS]);
             ++g;
             if (kb + GROUP_KB < p.num_kb) held.load(p, m0, n0, kb + GROUP_KB);
           }
@@ -699,7 +794,7 @@ struct Fp8Pair {
       const uint32_t empty_leader = map_to_cta(smem_u32(&bars->tmem_empty[0]), 0u);
       constexpr int kF = kVector ? 4 : 2;
       float f[kF];
-      uint32_t at = 0, it = 0;  // where the block's scales lie
+      uint32_t at = 0, group_at = 0, it = 0;  // where the block's scales lie, and its group's
       auto fetch = [&]() {
         if constexpr (kVector) {
 #pragma unroll
@@ -732,7 +827,7 @@ struct Fp8Pair {
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
               tmem_ld_wait();
-              pin_16(r[c & 1]);
+              pin(r[c & 1]);
               if (c < 7) {
                 tmem_ld_32x32b_x16(col + (c + 1) * 16, r[(c + 1) & 1]);
               } else {
@@ -754,8 +849,8 @@ struct Fp8Pair {
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
               tmem_ld_wait();
-              pin_8(r[c & 1][0]);
-              pin_8(r[c & 1][1]);
+              pin(r[c & 1][0]);
+              pin(r[c & 1][1]);
               if (c < 7) {
                 load(c + 1);
               } else {
@@ -773,9 +868,13 @@ struct Fp8Pair {
                 }
             }
           }
-          // the next block's place: the next of the group, or the first of the other
-          const bool last_of_group = kb % GROUP_KB == GROUP_KB - 1 || kb == p.num_kb - 1;
-          at = last_of_group ? (at >= GROUP_KB * SCALES ? 0u : GROUP_KB * SCALES) : at + SCALES;
+          // the next block's place: the next of the group, or the first of the next group
+          if (kb % GROUP_KB == GROUP_KB - 1 || kb == p.num_kb - 1) {
+            group_at = group_at == (GROUPS - 1) * GROUP_KB * SCALES ? 0u : group_at + GROUP_KB * SCALES;
+            at = group_at;
+          } else {
+            at += SCALES;
+          }
           fetch();
         }
         if (!ok) break;
@@ -875,28 +974,39 @@ struct Plan {
   int splits;  // CTAs that share a tile's K
 };
 
-// Which kernel takes a product.
-Plan plan_of(int m, int n, int k, int sms) {
-  const int num_kb = (k + 127) / 128;
+// Which kernel takes a product. `vector`: each row of B has scales of its own.
+// Up to 32 tokens (64 with `vector`, where 128 weights would be 128 columns with a scale each: 64 x 4096 x 4096 9.8 us against 11.4) the
+// weight's rows are the tile's rows, and K is split until a quarter more CTAs run than there are SMs (two fit one): 1 x 4096 x 4096 in 1, 2,
+// 4, 8 parts 10.9, 7.6, 5.8, 6.2 us, 1 x 14336 x 4096 13.0, 13.6, 16.5, 22.3.
+// More tokens: 128 x 128 tiles, K in up to four parts while all run at once (eight: 200 x 1024 x 8192 17.4 us against 10.9), or pairs, whichever
+// takes less time by {fixed, per wave and block of K, per wave, joining 2 and 4 parts}, fitted to 35 shapes of 33 to 3700 tokens x 264 to 9600 x
+// 128 to 11008, 5 to 8 % rms, of which it picks the faster every time. Tiles of 128 against pairs: 128 x 4096 x 4096 in four parts 10.2 / 19.3
+// us, 512 x 4096 x 11008 30 / 47, 1444 x 1040 x 1760 7.9 / 12.1; 777 x 2752 x 1488 13.2 / 11.0, 512 x 11008 x 4096 40 / 36, 1204 x 6600 x 128 13.7 / 8.9.
+Plan plan_of(int m, int n, int k, bool vector, int sms) {
+  const int num_kb = (k - 1) / 128 + 1;
   Plan plan{0, 0, 128, 1};
-  long long tiles;
-  int at_once;
-  if (m <= 64) {
+  if (m <= (vector ? 64 : 32)) {
     plan.swap = 1;
     plan.bn = m <= 16 ? 16 : m <= 32 ? 32 : 64;
-    tiles = (n + 127) / 128;
-    at_once = 2 * sms;
-  } else {
-    const long long large = static_cast<long long>((m + 255) / 256) * ((n + 255) / 256);
-    if (large >= sms / 2) {
-      plan.pair = 1;
-      plan.bn = 256;
-      return plan;
-    }
-    tiles = static_cast<long long>((m + 127) / 128) * ((n + 127) / 128);
-    at_once = sms;
+    const long long tiles = (n - 1) / 128 + 1;
+    while (plan.splits < 8 && 4 * tiles * 2 * plan.splits <= 5LL * sms && num_kb >= 4 * plan.splits) plan.splits *= 2;
+    return plan;
   }
-  while (plan.splits < 8 && tiles * plan.splits * 2 <= at_once && num_kb >= plan.splits * 4) plan.splits *= 2;
+  const double pair_us[3] = {vector ? 3.6 : 3.2, vector ? 0.71 : 0.5, 1.8};
+  const double tile_us[3] = {vector ? -0.5 : -0.8, vector ? 0.563 : 0.335, vector ? 3.3 : 3.7};
+  const long long tiles = (static_cast<long long>(m - 1) / 128 + 1) * ((n - 1) / 128 + 1);
+  const long long large = (static_cast<long long>(m - 1) / 256 + 1) * ((n - 1) / 256 + 1), pairs = sms >= 2 ? sms / 2 : 1;
+  double best = pair_us[0] + static_cast<double>((large - 1) / pairs + 1) * (num_kb * pair_us[1] + pair_us[2]);
+  plan.pair = 1, plan.bn = 256;
+  for (int s = 1; s <= 4; s *= 2) {
+    if (s > 1 && (tiles * s > sms || num_kb < 2 * s)) break;
+    const double us = tile_us[0] + static_cast<double>((tiles * s - 1) / sms + 1) * (((num_kb - 1) / s + 1) * tile_us[1] + tile_us[2]) +
+                      (s == 2 ? 2.2 : s == 4 ? 3.2 : 0.0);
+    if (us < best) {
+      best = us;
+      plan = Plan{0, 0, 128, s};
+    }
+  }
   return plan;
 }
 
@@ -941,8 +1051,8 @@ int launch(const Plan& plan, int device, int sms, cudaStream_t st, const Fp8Para
 }  // namespace
 
 // For tests of the host logic: the plan of a product as {pair, swap, columns of a tile, splits}.
-extern "C" int kcg_internal_fp8_plan(int m, int n, int k, int sms, int out[4]) {
-  const Plan plan = plan_of(m, n, k, sms);
+extern "C" int kcg_internal_fp8_plan(int m, int n, int k, int block_b, int sms, int out[4]) {
+  const Plan plan = plan_of(m, n, k, block_b == 1, sms);
   out[0] = plan.pair, out[1] = plan.swap, out[2] = plan.bn, out[3] = plan.splits;
   return 0;
 }
@@ -975,7 +1085,7 @@ extern "C" int kcg_matmul_fp8(int device, uint64_t stream, const kcg_fp8_product
   if (e != cudaSuccess) return cuda_fail(e, "cudaSetDevice");
   EncodeFn enc = nullptr;
   if (int r = encoder(&enc)) return r;
-  const Plan plan = plan_of(a->m, a->n, a->k, sms);
+  const Plan plan = plan_of(a->m, a->n, a->k, a->block_b == 1, sms);
   Fp8Params p{};
   const int rows_box = plan.pair ? 128 : plan.bn;
   const uint32_t fa = a->dtype_a == KCG_FP8_E5M2, fb = a->dtype_b == KCG_FP8_E5M2;
@@ -997,6 +1107,7 @@ extern "C" int kcg_matmul_fp8(int device, uint64_t stream, const kcg_fp8_product
   p.fused = a->beta != 0.f || a->bias != 0 || a->relu != 0;
   p.beta = a->beta, p.relu = a->relu, p.splits = plan.splits;
   p.vector_store = a->C % 16 == 0 && ldc * eb % 16 == 0;
+  p.word_store = a->C % 4 == 0 && ldc * eb % 4 == 0;
   p.vector_sp = reinterpret_cast<uint64_t>(p.sp) % 16 == 0 && p.ldsp % 4 == 0;
   p.vector_sq = reinterpret_cast<uint64_t>(p.sq) % 16 == 0 && p.ldsq % 4 == 0;
   if (plan.pair && p.vector_store)

@@ -31,6 +31,9 @@ struct NormArgs {
   float eps;
 };
 
+// Warps of a CTA of so many threads, up to the next power of two.
+__host__ __device__ constexpr int warps_of(int threads) { return threads <= 256 ? 8 : threads <= 512 ? 16 : 32; }
+
 // Sums over the threads of a row: a warp's (kWarps = 1), or those of a CTA of kWarps warps at most (a power of two).
 template <int kWarps, int kN>
 __device__ __forceinline__ void row_sum(float (&v)[kN], float* scratch) {
@@ -38,6 +41,7 @@ __device__ __forceinline__ void row_sum(float (&v)[kN], float* scratch) {
   for (int n = 0; n < kN; ++n)
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+  static_assert((kWarps & (kWarps - 1)) == 0, "lanes stand for warps");
   if constexpr (kWarps > 1) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5, from = lane & (kWarps - 1);
     if (lane == 0)
@@ -148,12 +152,10 @@ __global__ void __launch_bounds__(256) norm_warp_kernel(const NormArgs a) {
 template <typename T, int kVPT, bool kRes, bool kFp8, int kThreads, int kCtas>
 __global__ void __launch_bounds__(kThreads, kCtas) norm_kernel(const NormArgs a) {
   __shared__ float scratch[2][32];
-  constexpr bool kAhead = kThreads <= 512;                    // (registers)
-  constexpr bool kWide = kAhead && !kRes && kVPT <= 2;        // the weight as fp32 numbers
+  constexpr bool kAhead = kThreads <= 512;  // (registers)
   griddep_launch_dependents();
   griddep_wait();
   const int tid = threadIdx.x, threads = blockDim.x, pieces = a.width / 8;
-  float2 wide[kWide ? kVPT : 1][4];
   Raw8<T> w[kVPT], x[kVPT], res[kRes ? kVPT : 1];
   auto ask = [&](long long row) {
 #pragma unroll
@@ -171,7 +173,6 @@ __global__ void __launch_bounds__(kThreads, kCtas) norm_kernel(const NormArgs a)
     x[i].zero();
     if constexpr (kRes) res[i].zero();
     if (kAhead && i * threads + tid < pieces) w[i].load(static_cast<const T*>(a.w) + 8 * (i * threads + tid));
-    if constexpr (kWide) pairs_of(w[i], wide[i]);
   }
   long long row = blockIdx.x;
   if (kAhead && row < a.rows) ask(row);
@@ -182,7 +183,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) norm_kernel(const NormArgs a)
     for (int i = 0; i < kVPT; ++i) sum_piece<T, kRes>(x[i], res[kRes ? i : 0], h[i], squares);
     float sum[1] = {squares.x + squares.y};
     if (kAhead && row + gridDim.x < a.rows) ask(row + gridDim.x);
-    row_sum<kThreads / 32>(sum, scratch[turn]);  // (two scratches: one barrier a row)
+    row_sum<warps_of(kThreads)>(sum, scratch[turn]);  // (two scratches: one barrier a row)
     const float r = rsqrtf(sum[0] / static_cast<float>(a.width) + a.eps);
 #pragma unroll
     for (int i = 0; i < kVPT; ++i) {
@@ -190,13 +191,9 @@ __global__ void __launch_bounds__(kThreads, kCtas) norm_kernel(const NormArgs a)
       if constexpr (!kAhead) {
         if (v < pieces) w[i].load(static_cast<const T*>(a.w) + 8 * v);
       }
-      if constexpr (kWide) {
-        finish_piece<T, kRes, kFp8>(a, row, v, v < pieces, tid, h[i], wide[i], r);
-      } else {
-        float2 f[4];
-        pairs_of(w[i], f);
-        finish_piece<T, kRes, kFp8>(a, row, v, v < pieces, tid, h[i], f, r);
-      }
+      float2 f[4];
+      pairs_of(w[i], f);
+      finish_piece<T, kRes, kFp8>(a, row, v, v < pieces, tid, h[i], f, r);
     }
   }
 }
@@ -313,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) norm_grad_kernel(const GradAr
       }
     }
     if (kAhead && row + gridDim.x < a.rows) ask(row + gridDim.x);
-    row_sum<kThreads / 32>(sum, scratch[turn]);  // (two scratches: one barrier a row)
+    row_sum<warps_of(kThreads)>(sum, scratch[turn]);  // (two scratches: one barrier a row)
     const float r = rsqrtf(fmaf(sum[0], inv, a.eps));
     const float back = r * r * (sum[1] * inv);  // dx = r * (g - h * back)
 #pragma unroll
@@ -429,7 +426,8 @@ int launch_norm(const NormArgs& a, bool vectors, int sms, cudaStream_t st) {
     return l(norm_warp_kernel<T, 4, kRes, kFp8>, "norm launch", a);
   }
   if (pieces <= 256) return launch_norm_rows<T, 1, kRes, kFp8, 256, 6>(l, a, sms);
-  if (pieces <= 512) return launch_norm_rows<T, 2, kRes, kFp8, 256, 4>(l, a, sms);
+  if (pieces <= 512) return launch_norm_rows<T, 2, kRes, kFp8, 256, kRes || kFp8 ? 4 : 5>(l, a, sms);
+  if (!kRes && pieces <= 768) return launch_norm_rows<T, 2, kRes, kFp8, 384, 3>(l, a, sms);
   if (pieces <= 1024) return launch_norm_rows<T, 2, kRes, kFp8, 512, 2>(l, a, sms);
   if (pieces <= 2048) return launch_norm_rows<T, 4, kRes, kFp8, 512, 1>(l, a, sms);
   return launch_norm_rows<T, 4, kRes, kFp8, 1024, 1>(l, a, sms);

@@ -111,41 +111,48 @@ def test_the_c_entry_refuses_what_it_cannot_take():
     assert lib.kcg_matmul_fp8(0, 0, None) == _lib.E_BAD_ARG
 
 
-def _plan(m, n, k, sms=148):
+def _plan(m, n, k, block_b=128, sms=148):
     out = (ctypes.c_int * 4)()
-    _lib.get_lib().kcg_internal_fp8_plan(m, n, k, sms, out)
+    _lib.get_lib().kcg_internal_fp8_plan(m, n, k, block_b, sms, out)
     return list(out)
 
 
 def test_every_plan_gives_every_part_work():
-    """Splits are a power of two, at most 8 and at most the blocks of K, for any GPU; few tokens are columns of a tile."""
-    for m in (1, 16, 17, 64, 65, 128, 500, 2048, 30000):
+    """Splits are a power of two, at most 8 (tiles of 128 columns: 4) and at most half the blocks of K, for any GPU; few tokens are columns
+    of a tile."""
+    for m in (1, 16, 17, 32, 33, 64, 65, 128, 500, 2048, 30000):
         for n in (1, 100, 128, 1000, 4096, 11008):
             for k in (1, 128, 129, 512, 4096, 11008):
                 for sms in (148, 132, 20, 1):
-                    pair, swap, bn, splits = _plan(m, n, k, sms)
-                    assert splits in (1, 2, 4, 8) and splits <= -(-k // 128) and (splits == 1 or not pair)
-                    assert bn == 256 if pair else bn in (16, 32, 64, 128)
-                    assert not swap or bn >= m
+                    for block_b in (1, 128):
+                        pair, swap, bn, splits = _plan(m, n, k, block_b, sms)
+                        assert splits in (1, 2, 4, 8) and (splits == 1 or 2 * splits <= -(-k // 128) and not pair)
+                        assert bn == 256 if pair else bn in (16, 32, 64, 128) and (swap or bn == 128)
+                        assert splits < 8 or swap
+                        assert not swap or bn >= m
 
 
 # (m, n, k): tokens at each width of a tile, full and one past it; widths and sums that end inside a tile or a block, one of one
-# column and one value; K shared by 2, 4, 8 CTAs; tiles of 128 x 128, alone and shared; CTA pairs
-FEW = [(1, 4096, 11008), (1, 1, 1), (1, 128, 128), (2, 130, 144), (16, 256, 1024), (17, 1000, 528), (32, 100, 2048), (33, 2752, 1376), (64, 4096, 512),
-       (64, 11008, 4096), (5, 257, 16384), (48, 64, 100)]
-MIDDLING = [(65, 64, 100), (127, 4096, 4096), (128, 257, 1040), (129, 1000, 127), (777, 2752, 1488), (300, 128, 8192)]
-MANY = [(2049, 2305, 300), (2304, 2304, 128), (5000, 1024, 1000), (256, 18944, 257)]
+# column and one value; K shared by 2, 4, 8 CTAs; tiles of 128 x 128, alone and shared; CTA pairs, one tile each and several
+FEW = [(1, 4096, 11008), (1, 1, 1), (1, 128, 128), (2, 130, 144), (16, 256, 1024), (17, 1000, 528), (32, 100, 2048), (31, 2752, 1376), (32, 4096, 512),
+       (25, 11008, 4096), (5, 257, 16384), (9, 64, 100), (3, 10240, 640)]
+SOME = [(33, 2752, 1376), (64, 4096, 512), (48, 64, 100), (64, 300, 8192), (50, 10240, 700)]
+MIDDLING = [(65, 64, 100), (127, 4096, 4096), (128, 257, 1040), (129, 1000, 127), (300, 128, 8192), (256, 4096, 2000), (100, 14336, 300)]
+MANY = [(2049, 2305, 300), (2304, 2304, 128), (5000, 1024, 1000), (256, 18944, 257), (777, 2752, 1488), (4000, 4000, 520)]
 
 
 def test_the_shapes_reach_every_kernel():
-    assert {_plan(*s)[1] for s in FEW} == {1} and {_plan(*s)[2] for s in FEW} == {16, 32, 64}
+    assert {_plan(*s, b)[1] for s in FEW for b in (1, 128)} == {1} and {_plan(*s)[2] for s in FEW} == {16, 32}
     assert {_plan(*s)[3] for s in FEW} == {1, 2, 4, 8}
-    assert {tuple(_plan(*s)[:2]) for s in MIDDLING} == {(0, 0)} and {tuple(_plan(*s)[:2]) for s in MANY} == {(1, 0)}
+    assert {_plan(*s, 1)[2] for s in SOME} == {64} and {_plan(*s, 1)[3] for s in SOME} == {1, 2, 4, 8}
+    for b in (1, 128):
+        assert {tuple(_plan(*s, b)[:2]) for s in MIDDLING} == {(0, 0)} and {_plan(*s, b)[3] for s in MIDDLING} == {1, 2, 4}
+        assert {tuple(_plan(*s, b)[:2]) for s in MANY} == {(1, 0)}
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("block_b", [128, 1])
-@pytest.mark.parametrize("m,n,k", FEW + MIDDLING + MANY)
+@pytest.mark.parametrize("m,n,k", FEW + SOME + MIDDLING + MANY)
 def test_shapes(m, n, k, block_b):
     for out in (torch.bfloat16, torch.float32, torch.float16):
         check(m, n, k, block_b, out)
@@ -234,6 +241,22 @@ def test_no_tokens():
     b, sb = operand(300, 256, 128, 1)
     y = matmul_op.matmul_fp8(torch.empty((0, 256), device="cuda").to(E4), torch.empty((0, 2), device="cuda"), b, sb)
     assert y.shape == (0, 300)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("block_b", [128, 1])
+@pytest.mark.parametrize("k", [128, 640, 200, 1100])
+def test_many_tiles_a_pair_and_groups_of_few_blocks(k, block_b):
+    """Scales of one to four blocks come together, those of the next group while a group is used; a pair walks about six tiles."""
+    a, sa = operand(6144, k, 1, 2)
+    b, sb = operand(5120, k, block_b, 3)
+    assert _plan(6144, 5120, k, block_b)[0] == 1
+    want = wide64(a, sa, 1) @ wide64(b, sb, block_b).t()
+    size = wide64(a, sa, 1).abs() @ wide64(b, sb, block_b).abs().t()
+    first = matmul_op.matmul_fp8(a, sa, b, sb, out_dtype=torch.float32)
+    assert bool(((first.double() - want).abs() <= (2.0 ** -16 + 2.0 ** -20) * size).all())
+    for _ in range(5):
+        assert torch.equal(matmul_op.matmul_fp8(a, sa, b, sb, out_dtype=torch.float32), first)
 
 
 @pytest.mark.gpu
