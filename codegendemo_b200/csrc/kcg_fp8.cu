@@ -163,14 +163,38 @@ __device__ __forceinline__ uint4 unit16(const float* v, int u) {
   }
 }
 
-// bias, beta and ReLU of kN values of row m from column n on.
+// beta * C, bias and ReLU of kN values of row m from column n on, a row a thread, the warp's rows together (a column's bias is in
+// one lane: loaded by every thread for every column it took as long as the rest of 777 x 2752 x 1488).
 template <typename T, int kN>
 __device__ __forceinline__ void finish_row(const Fp8Params& p, float (&v)[kN], int m, int n) {
-  if (m >= p.rows_p) return;
-  const T* c = static_cast<const T*>(p.C) + static_cast<long long>(m) * p.ldc + n;
+  if (p.beta != 0.f && m < p.rows_p) {
+    const T* c = static_cast<const T*>(p.C) + static_cast<long long>(m) * p.ldc + n;
 #pragma unroll
-  for (int i = 0; i < kN; ++i)
-    if (n + i < p.rows_q) v[i] = finish<T>(p, v[i], c + i, bias_at<T>(p, n + i));
+    for (int i = 0; i < kN; i += 8) {
+      if (p.vector_store && n + i + 8 <= p.rows_q) {
+        float old[8];
+        load8(c + i, old);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i + j] = fmaf(p.beta, old[j], v[i + j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (n + i + j < p.rows_q) v[i + j] = fmaf(p.beta, to_f32(c[i + j]), v[i + j]);
+      }
+    }
+  }
+  if (p.bias) {
+    const int lane = threadIdx.x & 31;
+    float b[(kN + 31) / 32];
+#pragma unroll
+    for (int i = 0; i < (kN + 31) / 32; ++i) b[i] = n + i * 32 + lane < p.rows_q ? bias_at<T>(p, n + i * 32 + lane) : 0.f;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) v[i] += __shfl_sync(0xffffffffu, b[i / 32], i % 32);
+  }
+  if (p.relu) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) v[i] = fmaxf(v[i], 0.f);
+  }
 }
 
 // 32 rows of kN values of C wait in a warp's shared memory, kPitch bytes a row (16-byte units of the rows then lie in different banks), and
@@ -597,12 +621,25 @@ struct Fp8Pair {
     static_assert(Rows::kBytes <= 8192, "a block of rows exceeds a warp's shared memory");
     const int lane = threadIdx.x & 31;
     if (p.fused) {
-      // Row and column of accumulator i: kVector as tcgen05.ld.16x256b lays them out, else a row a thread.
+      if constexpr (!kVector) {
+        finish_row<T, 128>(p, acc, row0 + lane, col0);
+      } else {
+        // tcgen05.ld.16x256b's layout: pairs of columns, four rows
 #pragma unroll
-      for (int i = 0; i < 128; ++i) {
-        const int m = row0 + (kVector ? (i >> 1 & 3) * 8 + (lane >> 2) : lane), n = col0 + (kVector ? (i >> 3) * 8 + (lane & 3) * 2 + (i & 1) : i);
-        if (m < p.rows_p && n < p.rows_q)
-          acc[i] = finish<T>(p, acc[i], static_cast<const T*>(p.C) + static_cast<long long>(m) * p.ldc + n, bias_at<T>(p, n));
+        for (int j = 0; j < 16; ++j) {
+          const int n = col0 + j * 8 + (lane & 3) * 2;
+          float bias[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) bias[e] = n + e < p.rows_q ? bias_at<T>(p, n + e) : 0.f;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int m = row0 + r * 8 + (lane >> 2);
+            const T* c = static_cast<const T*>(p.C) + static_cast<long long>(m) * p.ldc + n;
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (m < p.rows_p && n + e < p.rows_q) acc[j * 8 + r * 2 + e] = finish<T>(p, acc[j * 8 + r * 2 + e], c + e, bias[e]);
+          }
+        }
       }
     }
 #pragma unroll
