@@ -5,8 +5,10 @@
 // rounding to bf16, fp16 or fp32.
 //
 // The scales change with every 128 values of K, so the tensor core sums 128 values only (kind::f8f6f4, four instructions of 32),
-// into one of two accumulators in tensor memory; while it fills the other, warps read the first, one row of the tile a thread, and add
-// it to fp32 registers, times its scales.
+// into one of several accumulators in tensor memory; while it fills the next, warps read that one and add it to fp32 registers, times
+// its scales.
+//
+// Error against the same sums in 64 bits, fp32 results, 4096 x 4096 x 8192: 1.5e-7 of the norm.
 //
 // Two kernels. Fp8Tile: one CTA a tile of 128 rows by kBN columns, K split over the CTAs of a cluster, which add their tiles through
 // distributed shared memory (in the order of their ranks). With few tokens the weight's rows are the tile's rows and the tokens its
@@ -859,18 +861,15 @@ struct Fp8Pair {
           };
           if constexpr (!kVector) {
             const float factor = scale_product(f[0], f[1]);
-            uint32_t r[2][16];
-            tmem_ld_32x32b_x16(col, r[0]);
+            // (the next 32 columns asked for beside these, or 16 at a time, are no faster)
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
+            for (int c = 0; c < 128; c += 32) {
+              uint32_t r[32];
+              tmem_ld_32x32b_x32(col + c, r);
               tmem_ld_wait();
-              pin(r[c & 1]);
-              if (c < 7) {
-                tmem_ld_32x32b_x16(col + (c + 1) * 16, r[(c + 1) & 1]);
-              } else {
-                release();
-              }
-              add_scaled<16>(acc + c * 16, r[c & 1], factor);
+              pin(r);
+              if (c == 96) release();
+              add_scaled<32>(acc + c, r, factor);
             }
           } else {
             // 16 columns at a time, rows 0-15 and 16-31 of the warp's lanes

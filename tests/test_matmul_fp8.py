@@ -328,3 +328,11 @@ def test_a_training_step_of_a_layer():
     # the same step adds to a gradient that is there
     twice = matmul_op.matmul_fp8(*matmul_op.quantize_fp8(dy, transposed=True), *matmul_op.quantize_fp8(u, transposed=True), c=dw.clone(), beta=1.0)
     assert (twice - 2 * dw).norm() <= 1e-6 * dw.norm()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("args", [[], ["--backward", "--dtype", "fp32"]])
+def test_the_command_runs_and_checks(args, capsys):
+    from codegendemo_b200.kcg.run_linear_fp8 import main
+    assert main(["--m", "300", "--n", "520", "--k", "768", "--launches", "2", "--warmup", "1"] + args) == 0
+    assert "OK" in capsys.readouterr().out
