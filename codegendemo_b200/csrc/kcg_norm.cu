@@ -254,76 +254,80 @@ struct GradArgs {
   float eps;
 };
 
-// Each CTA walks rows blockIdx.x, + gridDim.x, ...; a thread keeps its columns' share of dw in registers, and asks for the next row
-// before it reduces the present one.
-template <typename T, int kVPT, bool kDh, int kThreads, int kCtas>
+// Each CTA walks rows blockIdx.x, + gridDim.x, ...; a thread keeps its columns' share of dw in registers, the row as it lies in
+// memory, and (kAhead: rows of up to 8192 values) asks for the next row before it reduces the present one.
+template <typename T, int kVPT, bool kDh, int kThreads, int kCtas, bool kAhead>
 __global__ void __launch_bounds__(kThreads, kCtas) norm_grad_kernel(const GradArgs a) {
-  __shared__ float scratch[2][64];
-  constexpr bool kAhead = kVPT <= 2 && kThreads <= 512;  // (registers)
+  constexpr int kWarps = warps_of(kThreads);
+  __shared__ float scratch[2][2 * kWarps];
   griddep_launch_dependents();
   griddep_wait();
   const int tid = threadIdx.x, threads = blockDim.x, pieces = a.width / 8;
-  float dw[kVPT][8];
-  Raw8<T> w[kVPT], rh[kVPT], rdy[kVPT], rdh[kDh ? kVPT : 1];
-  auto ask = [&](long long row) {
+  struct Row {
+    Raw8<T> h[kVPT], dy[kVPT], dh[kDh ? kVPT : 1];
+  };
+  float2 dw[kVPT][4];
+  Raw8<T> w[kVPT];
+  Row at, next;
+  auto ask = [&](Row& to, long long row) {
 #pragma unroll
     for (int i = 0; i < kVPT; ++i) {
       const int v = i * threads + tid;
       if (v < pieces) {
-        rh[i].load(static_cast<const T*>(a.h) + row * a.ldh + 8 * v);
-        rdy[i].load(static_cast<const T*>(a.dy) + row * a.lddy + 8 * v);
-        if constexpr (kDh) rdh[i].load(static_cast<const T*>(a.dh) + row * a.lddh + 8 * v);
+        to.h[i].load(static_cast<const T*>(a.h) + row * a.ldh + 8 * v);
+        to.dy[i].load(static_cast<const T*>(a.dy) + row * a.lddy + 8 * v);
+        if constexpr (kDh) to.dh[i].load(static_cast<const T*>(a.dh) + row * a.lddh + 8 * v);
       }
     }
   };
 #pragma unroll
   for (int i = 0; i < kVPT; ++i) {
-    w[i].zero(), rh[i].zero(), rdy[i].zero();
-    if constexpr (kDh) rdh[i].zero();
-    if (kAhead && i * threads + tid < pieces) w[i].load(static_cast<const T*>(a.w) + 8 * (i * threads + tid));
+    w[i].zero(), at.h[i].zero(), at.dy[i].zero(), next.h[i].zero(), next.dy[i].zero();
+    if constexpr (kDh) at.dh[i].zero(), next.dh[i].zero();
+    if (i * threads + tid < pieces) w[i].load(static_cast<const T*>(a.w) + 8 * (i * threads + tid));
 #pragma unroll
-    for (int j = 0; j < 8; ++j) dw[i][j] = 0.f;
+    for (int j = 0; j < 4; ++j) dw[i][j] = both(0.f);
   }
   const float inv = 1.f / static_cast<float>(a.width);
   long long row = blockIdx.x;
-  if (kAhead && row < a.rows) ask(row);
+  if (kAhead && row < a.rows) ask(next, row);
   for (int turn = 0; row < a.rows; row += gridDim.x, turn ^= 1) {
-    if constexpr (!kAhead) {
-      ask(row);
-#pragma unroll
-      for (int i = 0; i < kVPT; ++i)
-        if (i * threads + tid < pieces) w[i].load(static_cast<const T*>(a.w) + 8 * (i * threads + tid));
+    if constexpr (kAhead) {
+      at = next;
+      if (row + gridDim.x < a.rows) ask(next, row + gridDim.x);
+    } else {
+      ask(at, row);
     }
-    float h[kVPT][8], dy[kVPT][8], sum[2] = {0.f, 0.f};
-    Raw8<T> dh[kDh ? kVPT : 1];
+    float2 squares = both(0.f), products = both(0.f);
 #pragma unroll
     for (int i = 0; i < kVPT; ++i) {
-      float f[8];
-      w[i].values(f);
-      rh[i].values(h[i]);
-      rdy[i].values(dy[i]);
-      if constexpr (kDh) dh[i] = rdh[i];
+      float2 h[4], dy[4], f[4];
+      pairs_of(at.h[i], h);
+      pairs_of(at.dy[i], dy);
+      pairs_of(w[i], f);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        sum[0] = fmaf(h[i][j], h[i][j], sum[0]);
-        sum[1] = fmaf(dy[i][j] * f[j], h[i][j], sum[1]);
+      for (int j = 0; j < 4; ++j) {
+        squares = __ffma2_rn(h[j], h[j], squares);
+        products = __ffma2_rn(__fmul2_rn(dy[j], f[j]), h[j], products);
       }
     }
-    if (kAhead && row + gridDim.x < a.rows) ask(row + gridDim.x);
-    row_sum<warps_of(kThreads)>(sum, scratch[turn]);  // (two scratches: one barrier a row)
+    float sum[2] = {squares.x + squares.y, products.x + products.y};
+    row_sum<kWarps>(sum, scratch[turn]);  // (two scratches: one barrier a row)
     const float r = rsqrtf(fmaf(sum[0], inv, a.eps));
-    const float back = r * r * (sum[1] * inv);  // dx = r * (g - h * back)
+    const float back = -r * r * (sum[1] * inv);  // dx = r * (g + h * back)
 #pragma unroll
     for (int i = 0; i < kVPT; ++i) {
       const int v = i * threads + tid;
-      float f[8], d[8];
-      w[i].values(f);
-      if constexpr (kDh) dh[i].values(d);
+      float2 h[4], dy[4], f[4], d[4];
+      pairs_of(at.h[i], h);
+      pairs_of(at.dy[i], dy);
+      pairs_of(w[i], f);
+      if constexpr (kDh) pairs_of(at.dh[i], d);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float dx = r * (dy[i][j] * f[j] - h[i][j] * back);
-        dw[i][j] = fmaf(dy[i][j], h[i][j] * r, dw[i][j]);
-        d[j] = kDh ? d[j] + dx : dx;
+      for (int j = 0; j < 4; ++j) {
+        const float2 g = __ffma2_rn(h[j], both(back), __fmul2_rn(dy[j], f[j]));
+        dw[i][j] = __ffma2_rn(dy[j], __fmul2_rn(h[j], both(r)), dw[i][j]);
+        d[j] = kDh ? __ffma2_rn(g, both(r), d[j]) : __fmul2_rn(g, both(r));
       }
       if (v < pieces) store8(static_cast<T*>(a.dx) + row * a.lddx + 8 * v, d);
     }
@@ -441,17 +445,23 @@ int launch_norm(const NormArgs& a, bool vectors, int sms, cudaStream_t st) {
 
 constexpr int kMaxWidth = 32768;  // a row in a CTA's registers, its share of dw in shared memory
 
-// CTAs that walk the rows of the backward pass, each with its own share of dw: as many as run at once, with 512 threads or fewer
-// two an SM.
+// Threads of a CTA of the backward pass: two pieces each up to 8192 values a row, then four.
+int grad_threads(int width) {
+  const int pieces = (width + 7) / 8, each = pieces <= 1024 ? 2 : 4;
+  return ((pieces + each - 1) / each + 31) / 32 * 32;
+}
+// CTAs that walk its rows, each with its own share of dw: as many as run at once (512 threads an SM, by their registers), with two rows
+// each or more (513 x 1376 bf16 with one, two, four 5.3, 4.6, 6.1 us).
 int grad_ctas(int sms, long long rows, int width) {
-  const long long most = static_cast<long long>(sms) * (width <= 2048 ? 3 : width <= 4096 ? 2 : 1);
-  return static_cast<int>(rows < most ? rows : most);
+  const int per_sm = 512 / grad_threads(width);
+  const long long most = static_cast<long long>(sms) * (per_sm < 1 ? 1 : per_sm), few = (rows + 1) / 2;
+  return static_cast<int>(few < most ? few : most);
 }
 
 template <typename T, bool kDh>
 int launch_grad(const GradArgs& a, int ctas, bool vectors, cudaStream_t st) {
   Launch l(st);
-  if (!vectors) {
+  if (!vectors || a.width > 16384) {  // a row of fp32 sums in shared memory
     const size_t smem = static_cast<size_t>(a.width) * sizeof(float);
     if (smem > 40 * 1024) {
       const cudaError_t e = cudaFuncSetAttribute(norm_grad_any_kernel<T, kDh>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -461,26 +471,11 @@ int launch_grad(const GradArgs& a, int ctas, bool vectors, cudaStream_t st) {
     l.shape(ctas, 512, smem);
     return l(norm_grad_any_kernel<T, kDh>, "norm gradient launch", a);
   }
-  const int pieces = a.width / 8;
-  auto threads = [&](int vpt) { return static_cast<unsigned>(((pieces + vpt - 1) / vpt + 31) / 32 * 32); };
-  if (pieces <= 256) {
-    l.shape(ctas, threads(1));
-    return l(norm_grad_kernel<T, 1, kDh, 256, 3>, "norm gradient launch", a);
-  }
-  if (pieces <= 512) {
-    l.shape(ctas, threads(2));
-    return l(norm_grad_kernel<T, 2, kDh, 256, 2>, "norm gradient launch", a);
-  }
-  if (pieces <= 1024) {
-    l.shape(ctas, threads(2));
-    return l(norm_grad_kernel<T, 2, kDh, 512, 1>, "norm gradient launch", a);
-  }
-  if (pieces <= 2048) {
-    l.shape(ctas, threads(4));
-    return l(norm_grad_kernel<T, 4, kDh, 512, 1>, "norm gradient launch", a);
-  }
-  l.shape(ctas, threads(8));
-  return l(norm_grad_kernel<T, 8, kDh, 512, 1>, "norm gradient launch", a);
+  const int threads = grad_threads(a.width);
+  l.shape(ctas, threads);
+  if (a.width > 8192) return l(norm_grad_kernel<T, 4, kDh, 512, 1, false>, "norm gradient launch", a);
+  if (threads > 256) return l(norm_grad_kernel<T, 2, kDh, 512, 1, true>, "norm gradient launch", a);
+  return l(norm_grad_kernel<T, 2, kDh, 256, 2, true>, "norm gradient launch", a);
 }
 
 template <typename T>
