@@ -110,6 +110,32 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
   }
 }
 
+// Eight values of a row from column c on, as they lie in memory; those past the row's end as zeros. kVec: rows start on 16-byte
+// boundaries.
+template <typename T, bool kVec>
+__device__ __forceinline__ void load_piece(const T* row, int c, int cols, Raw8<T>& v) {
+  if (kVec && c + 8 <= cols) {
+    v.load(row + c);
+  } else {
+    T e[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) e[j] = c + j < cols ? row[c + j] : T(0.f);
+    v.set(e);
+  }
+}
+
+// Eight values to a row from column c on, as far as the row goes. kWhole: rows of whole pieces on 16-byte boundaries.
+template <typename T, bool kWhole>
+__device__ __forceinline__ void store_piece(T* row, int c, int cols, const float2 (&v)[4]) {
+  if constexpr (kWhole) {
+    store8(row + c, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (c + j < cols) row[c + j] = from_f32<T>(j & 1 ? v[j / 2].y : v[j / 2].x);
+  }
+}
+
 // ---- 8-bit blocks. Of a block with largest magnitude top: scale = max(top / largest 8-bit value, 2^-126), values
 // x * (1 / scale) rounded to nearest even. The lower bound keeps 1 / scale finite, also for a block of zeros. Magnitudes are compared
 // as integers, in which a NaN is the largest: it makes the block's scale, and with it every value of the block, a NaN.

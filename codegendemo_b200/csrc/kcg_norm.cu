@@ -5,8 +5,8 @@
 // (dh: the gradient that reaches h past the norm, along the residual stream.) Sums and products in fp32, one rounding at the end:
 // y comes from the unrounded sum h, which is rounded only where it is stored.
 //
-// Bound by HBM: a row is read once, into registers, and written once. Widths of whole 16-byte pieces take the kernels below
-// (a warp a row up to 1024 values, CTAs that walk rows beyond), others a kernel that reads single values, twice.
+// Bound by HBM: a row is read once, into registers, and written once, by a warp (forward, up to 1024 values) or by CTAs that walk rows. Rows
+// that are no whole 16-byte pieces are read value by value, forward by a kernel of their own that reads them twice.
 #include <cuda_runtime.h>
 
 #include <cfloat>
@@ -255,28 +255,36 @@ struct GradArgs {
 };
 
 // Each CTA walks rows blockIdx.x, + gridDim.x, ...; a thread keeps its columns' share of dw in registers, the row as it lies in
-// memory, and (kAhead: rows of up to 8192 values) asks for the next row before it reduces the present one.
-template <typename T, int kVPT, bool kDh, int kThreads, int kCtas, bool kAhead>
+// memory, and (kAhead: rows of up to 8192 values) asks for the next row before it reduces the present one. !kWhole: rows that
+// are no whole 16-byte pieces, value by value (8192 x 4095 bf16 157 us; by threads that each own every 512th value, dw in shared memory, 300).
+template <typename T, int kVPT, bool kDh, bool kWhole, int kThreads, int kCtas, bool kAhead>
 __global__ void __launch_bounds__(kThreads, kCtas) norm_grad_kernel(const GradArgs a) {
   constexpr int kWarps = warps_of(kThreads);
   __shared__ float scratch[2][2 * kWarps];
   griddep_launch_dependents();
   griddep_wait();
-  const int tid = threadIdx.x, threads = blockDim.x, pieces = a.width / 8;
+  const int tid = threadIdx.x, threads = blockDim.x, pieces = (a.width + 7) / 8;
   struct Row {
     Raw8<T> h[kVPT], dy[kVPT], dh[kDh ? kVPT : 1];
   };
   float2 dw[kVPT][4];
   Raw8<T> w[kVPT];
   Row at, next;
+  auto read = [&](Raw8<T>& to, const T* from, int v) {
+    if constexpr (kWhole) {
+      to.load(from + 8 * v);
+    } else {
+      load_piece<T, false>(from, 8 * v, a.width, to);
+    }
+  };
   auto ask = [&](Row& to, long long row) {
 #pragma unroll
     for (int i = 0; i < kVPT; ++i) {
       const int v = i * threads + tid;
       if (v < pieces) {
-        to.h[i].load(static_cast<const T*>(a.h) + row * a.ldh + 8 * v);
-        to.dy[i].load(static_cast<const T*>(a.dy) + row * a.lddy + 8 * v);
-        if constexpr (kDh) to.dh[i].load(static_cast<const T*>(a.dh) + row * a.lddh + 8 * v);
+        read(to.h[i], static_cast<const T*>(a.h) + row * a.ldh, v);
+        read(to.dy[i], static_cast<const T*>(a.dy) + row * a.lddy, v);
+        if constexpr (kDh) read(to.dh[i], static_cast<const T*>(a.dh) + row * a.lddh, v);
       }
     }
   };
@@ -284,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) norm_grad_kernel(const GradAr
   for (int i = 0; i < kVPT; ++i) {
     w[i].zero(), at.h[i].zero(), at.dy[i].zero(), next.h[i].zero(), next.dy[i].zero();
     if constexpr (kDh) at.dh[i].zero(), next.dh[i].zero();
-    if (i * threads + tid < pieces) w[i].load(static_cast<const T*>(a.w) + 8 * (i * threads + tid));
+    if (i * threads + tid < pieces) read(w[i], static_cast<const T*>(a.w), i * threads + tid);
 #pragma unroll
     for (int j = 0; j < 4; ++j) dw[i][j] = both(0.f);
   }
@@ -329,18 +337,18 @@ __global__ void __launch_bounds__(kThreads, kCtas) norm_grad_kernel(const GradAr
         dw[i][j] = __ffma2_rn(dy[j], __fmul2_rn(h[j], both(r)), dw[i][j]);
         d[j] = kDh ? __ffma2_rn(g, both(r), d[j]) : __fmul2_rn(g, both(r));
       }
-      if (v < pieces) store8(static_cast<T*>(a.dx) + row * a.lddx + 8 * v, d);
+      if (v < pieces) store_piece<T, kWhole>(static_cast<T*>(a.dx) + row * a.lddx, 8 * v, a.width, d);
     }
   }
   float* mine = a.partial + static_cast<long long>(blockIdx.x) * a.width;
 #pragma unroll
   for (int i = 0; i < kVPT; ++i) {
     const int v = i * threads + tid;
-    if (v < pieces) store8(mine + 8 * v, dw[i]);
+    if (v < pieces) store_piece<float, kWhole>(mine, 8 * v, a.width, dw[i]);
   }
 }
 
-// Any width, pitch and alignment: the CTA's share of dw in shared memory, each value owned by one thread.
+// Rows of more than 16384 values, any pitch and alignment: the CTA's share of dw in shared memory, each value owned by one thread.
 template <typename T, bool kDh>
 __global__ void __launch_bounds__(512) norm_grad_any_kernel(const GradArgs a) {
   extern __shared__ float dw[];
@@ -458,24 +466,24 @@ int grad_ctas(int sms, long long rows, int width) {
   return static_cast<int>(few < most ? few : most);
 }
 
-template <typename T, bool kDh>
-int launch_grad(const GradArgs& a, int ctas, bool vectors, cudaStream_t st) {
+template <typename T, bool kDh, bool kWhole>
+int launch_grad(const GradArgs& a, int ctas, cudaStream_t st) {
   Launch l(st);
-  if (!vectors || a.width > 16384) {  // a row of fp32 sums in shared memory
-    const size_t smem = static_cast<size_t>(a.width) * sizeof(float);
-    if (smem > 40 * 1024) {
-      const cudaError_t e = cudaFuncSetAttribute(norm_grad_any_kernel<T, kDh>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 kMaxWidth * static_cast<int>(sizeof(float)));
-      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(MaxDynamicSharedMemorySize)");
-    }
-    l.shape(ctas, 512, smem);
-    return l(norm_grad_any_kernel<T, kDh>, "norm gradient launch", a);
-  }
   const int threads = grad_threads(a.width);
   l.shape(ctas, threads);
-  if (a.width > 8192) return l(norm_grad_kernel<T, 4, kDh, 512, 1, false>, "norm gradient launch", a);
-  if (threads > 256) return l(norm_grad_kernel<T, 2, kDh, 512, 1, true>, "norm gradient launch", a);
-  return l(norm_grad_kernel<T, 2, kDh, 256, 2, true>, "norm gradient launch", a);
+  if (a.width > 8192) return l(norm_grad_kernel<T, 4, kDh, kWhole, 512, 1, false>, "norm gradient launch", a);
+  if (threads > 256) return l(norm_grad_kernel<T, 2, kDh, kWhole, 512, 1, true>, "norm gradient launch", a);
+  return l(norm_grad_kernel<T, 2, kDh, kWhole, 256, 2, true>, "norm gradient launch", a);
+}
+template <typename T, bool kDh>
+int launch_grad(const GradArgs& a, int ctas, bool whole, cudaStream_t st) {
+  if (a.width <= 16384) return whole ? launch_grad<T, kDh, true>(a, ctas, st) : launch_grad<T, kDh, false>(a, ctas, st);
+  Launch l(st);
+  const cudaError_t e = cudaFuncSetAttribute(norm_grad_any_kernel<T, kDh>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             kMaxWidth * static_cast<int>(sizeof(float)));
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(MaxDynamicSharedMemorySize)");
+  l.shape(ctas, 512, static_cast<size_t>(a.width) * sizeof(float));
+  return l(norm_grad_any_kernel<T, kDh>, "norm gradient launch", a);
 }
 
 template <typename T>

@@ -27,19 +27,6 @@ struct QuantArgs {
   int cols, blocks;
 };
 
-// Eight values of a row from column c on, as they lie in memory; those past the row's end as zeros.
-template <typename T, bool kVec>
-__device__ __forceinline__ void load_piece(const T* row, int c, int cols, Raw8<T>& v) {
-  if (kVec && c + 8 <= cols) {
-    v.load(row + c);
-  } else {
-    T e[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) e[j] = c + j < cols ? row[c + j] : T(0.f);
-    v.set(e);
-  }
-}
-
 // Magnitudes, kept in the raw type: its bits without the sign, in whose order a NaN is the largest. Words of two 16-bit values or of
 // one fp32 value; eight values are kWords of them.
 template <typename T>
