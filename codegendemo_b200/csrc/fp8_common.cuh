@@ -166,13 +166,6 @@ __device__ __forceinline__ uint32_t pack_fp8(float lo, float hi) {
   return r;
 }
 template <bool kE5M2>
-__device__ __forceinline__ uint2 quantize8(const float (&v)[8], float inv) {
-  uint2 q;
-  q.x = pack_fp8<kE5M2>(v[0] * inv, v[1] * inv) | pack_fp8<kE5M2>(v[2] * inv, v[3] * inv) << 16;
-  q.y = pack_fp8<kE5M2>(v[4] * inv, v[5] * inv) | pack_fp8<kE5M2>(v[6] * inv, v[7] * inv) << 16;
-  return q;
-}
-template <bool kE5M2>
 __device__ __forceinline__ uint2 quantize8(const float2 (&v)[4], float inv) {
   float2 y[4];
 #pragma unroll
