@@ -5,6 +5,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <cstdlib>
 #include <string>
@@ -213,15 +214,15 @@ inline bool pdl_on() {
 }
 
 inline int sm_count(int device, int* out) {
-  static int known[64];  // (written with the same value by whoever asks first)
+  static std::atomic<int> known[64];
   if (device < 0 || device >= 64) return fail(KCG_E_BAD_ARG, "device index out of range");
-  if (!known[device]) {
-    int n = 0;
+  int n = known[device].load();
+  if (n == 0) {
     const cudaError_t e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device);
     if (e != cudaSuccess) return cuda_fail(e, "cudaDeviceGetAttribute(MultiProcessorCount)");
-    known[device] = n;
+    known[device].store(n);
   }
-  *out = known[device];
+  *out = n;
   return 0;
 }
 

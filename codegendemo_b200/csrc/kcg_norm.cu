@@ -404,18 +404,21 @@ __global__ void __launch_bounds__(1024) norm_grad_sum_kernel(const float* partia
 // ------------------------------------------------------------------------------------------------ launches
 // CTAs of a kernel that an SM holds at once (asked once per number of threads; one kind of GPU a process).
 template <typename K>
-int ctas_per_sm(K kernel, int threads, int (&known)[33]) {
-  int& n = known[threads / 32];
-  if (n == 0 && (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) != cudaSuccess || n < 1)) {
-    cudaGetLastError();
-    n = 1;
+int ctas_per_sm(K kernel, int threads, std::atomic<int> (&known)[33]) {
+  int n = known[threads / 32].load();
+  if (n == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = 1;
+    }
+    known[threads / 32].store(n);
   }
   return n;
 }
 
 template <typename T, int kVPT, bool kRes, bool kFp8, int kThreads, int kCtas>
 int launch_norm_rows(Launch& l, const NormArgs& a, int sms) {
-  static int known[33];
+  static std::atomic<int> known[33];
   const auto kernel = norm_kernel<T, kVPT, kRes, kFp8, kThreads, kCtas>;
   const int threads = ((a.width / 8 + kVPT - 1) / kVPT + 31) / 32 * 32;
   const long long most = static_cast<long long>(sms) * ctas_per_sm(kernel, threads, known);

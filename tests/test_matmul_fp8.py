@@ -336,3 +336,74 @@ def test_the_command_runs_and_checks(args, capsys):
     from codegendemo_b200.kcg.run_linear_fp8 import main
     assert main(["--m", "300", "--n", "520", "--k", "768", "--launches", "2", "--warmup", "1"] + args) == 0
     assert "OK" in capsys.readouterr().out
+
+
+_FIRST_CALL_CAPTURED = """
+import torch
+from codegendemo_b200.kcg import matmul_op
+x = torch.randn(200, 1024, device="cuda").bfloat16()
+w = torch.randn(300, 1024, device="cuda").bfloat16()
+nw = torch.ones(1024, device="cuda").bfloat16()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    for m in (200, 3):
+        h = x[:m]
+        q, s, _ = matmul_op.rms_norm_fp8(h, nw, h)
+        y = matmul_op.matmul_fp8(q, s, *matmul_op.quantize_fp8(w, rows=128))
+        z = matmul_op.rms_norm(h, nw)
+        dx, dw = matmul_op.rms_norm_backward(h, h, nw)
+        t = matmul_op.quantize_fp8(h, transposed=True)
+for _ in range(2):
+    graph.replay()
+torch.cuda.synchronize()
+q, s, _ = matmul_op.rms_norm_fp8(x[:3], nw, x[:3])
+assert torch.equal(y, matmul_op.matmul_fp8(q, s, *matmul_op.quantize_fp8(w, rows=128)))
+assert torch.equal(z, matmul_op.rms_norm(x[:3], nw)) and torch.equal(dx, matmul_op.rms_norm_backward(x[:3], x[:3], nw)[0])
+matmul_op.matmul_fp8_status()
+print("replayed")
+"""
+
+
+@pytest.mark.gpu
+def test_the_first_calls_of_a_process_may_be_captured():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", _FIRST_CALL_CAPTURED], cwd=root, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "replayed" in run.stdout, run.stderr[-2000:]
+
+
+@pytest.mark.gpu
+def test_threads_with_streams_of_their_own():
+    """Four host threads, each with its stream and inputs, through the whole layer at once: the bits of calls one after another."""
+    import threading
+    d, n = 768, 1000
+    w8, ws = operand(n, d, 128, 9)
+    nw = torch.rand(d, device="cuda").to(torch.bfloat16)
+    inputs = [(torch.randn(m, d, device="cuda").to(torch.bfloat16), torch.randn(m, d, device="cuda").to(torch.bfloat16)) for m in (1, 40, 300, 2500)]
+
+    def work(x, r):
+        y, h = layer(x, r, nw, w8, ws)
+        return y, h, *matmul_op.rms_norm_backward(r, h, nw, dh=x), *matmul_op.quantize_fp8(x, transposed=True)
+    want = [work(*i) for i in inputs]
+    torch.cuda.synchronize()
+    got, failed = [None] * 4, []
+
+    def run(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    got[i] = work(*inputs[i])
+            stream.synchronize()
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not failed, failed
+    for p, q in zip(got, want):
+        assert all(torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8)) for a, b in zip(p, q))
+    matmul_op.matmul_fp8_status()
