@@ -188,6 +188,9 @@ inline int cuda_fail(cudaError_t e, const char* what) {
 }
 inline bool known_dtype(int dt) { return dt == KCG_DTYPE_FLOAT32 || dt == KCG_DTYPE_FLOAT16 || dt == KCG_DTYPE_BFLOAT16; }
 
+// Rows or columns of an 8-bit matrix: rounding them up to tiles stays within 32 bits.
+constexpr int kMaxSize = 0x7fffff00;
+
 // Makes a device current, and the caller's again when it goes.
 struct DeviceGuard {
   int prev = -1;

@@ -243,7 +243,8 @@ extern "C" int kcg_quantize_fp8(int device, uint64_t stream, uint64_t X, int64_t
   if (!known_dtype(dtype)) return fail(KCG_E_BAD_ARG, "quantisation takes float16, bfloat16 or float32 data");
   if (dtype8 != KCG_FP8_E4M3 && dtype8 != KCG_FP8_E5M2) return fail(KCG_E_BAD_ARG, "quantisation gives e4m3 or e5m2 values");
   if (block_rows != 1 && block_rows != 128) return fail(KCG_E_BAD_ARG, "blocks have 1 or 128 rows");
-  if (rows < 0 || rows > 0x7fffffffLL || cols <= 0) return fail(KCG_E_BAD_ARG, "shape out of range");
+  if (rows < 0 || cols <= 0) return fail(KCG_E_BAD_ARG, "shape out of range");
+  if (rows > kMaxSize || cols > kMaxSize) return fail(KCG_E_TOO_LARGE, "a size of an 8-bit matrix is above 2^31 - 256");
   if (rows == 0) return 0;
   if (!X || !Q || !S) return fail(KCG_E_BAD_ARG, "null matrix");
   const int64_t out_cols = transposed ? rows : cols;

@@ -23,6 +23,7 @@ from codegendemo_b200 import _lib
 from codegendemo_b200.kcg.Utils import DeviceInfo
 
 MAX_NORM_WIDTH = 32768
+MAX_SIZE = 2 ** 31 - 256  # rows or columns of an 8-bit matrix
 
 _warm = None  # csrc/kcg_torchcall.cpp once something was launched, False where it was not built for this torch
 
@@ -35,7 +36,6 @@ def _launched(status):
     if _warm is None:
         from codegendemo_b200.kcg import matmul_op
         _warm = matmul_op._warm_calls()
-
 
 
 def _dtype_code(t, what):
@@ -193,6 +193,8 @@ def quantize_fp8(x, rows=1, transposed=False, dtype=None):
     dtype = torch.float8_e4m3fn if dtype is None else dtype
     code8 = _fp8_code(dtype, "dtype")
     n, cols = x.shape
+    if max(n, cols) > MAX_SIZE:
+        raise ValueError(f"x has more than {MAX_SIZE} rows or columns")
     r, c = (cols, n) if transposed else (n, cols)
     q = _rows_of_fp8(x, r, c, dtype)
     scales = x.new_empty((-(-r // rows), -(-c // 128)), dtype=torch.float32)
@@ -207,7 +209,8 @@ def matmul_fp8(a, a_scale, b, b_scale, c=None, beta=0.0, bias=None, relu=False, 
     ``a_scale`` M x ceil(K / 128); ``b`` is N x K (a weight as linear layers keep it) in blocks of 128 x 128, ``b_scale``
     ceil(N / 128) x ceil(K / 128), or of 1 x 128, ``b_scale`` N x ceil(K / 128). e4m3 or e5m2, each its own. Sums in fp32, one rounding
     to ``out_dtype`` (bf16 by default; fp16, fp32) or c's type. Rows of a and b have to start on 16-byte boundaries, as
-    ``quantize_fp8`` and ``rms_norm_fp8`` lay them out. The product of two scales has to be a normal fp32 number."""
+    ``quantize_fp8`` and ``rms_norm_fp8`` lay them out. Scales may reach 2^88 (values of 1e29), and the product
+    of two, but for blocks of zeros, has to be a normal fp32 number."""
     if _warm and c is None and type(beta) is float and beta == 0.0:
         c = _warm.matmul_fp8(a, a_scale, b, b_scale, bias, relu, out_dtype)
         if c is not None:
@@ -220,6 +223,8 @@ def matmul_fp8(a, a_scale, b, b_scale, c=None, beta=0.0, bias=None, relu=False, 
     N, K2 = b.shape
     if K != K2:
         raise ValueError(f"a has rows of {K} values, b of {K2}")
+    if max(M, N, K) > MAX_SIZE:
+        raise ValueError(f"an operand has more than {MAX_SIZE} rows or columns")
     if N < 1 or K < 1:
         raise ValueError("a product of no columns, or of rows without values")
     kb = -(-K // 128)

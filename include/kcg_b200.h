@@ -257,8 +257,9 @@ int kcg_rms_norm_backward(int device, uint64_t stream, uint64_t DY, int64_t lddy
 int kcg_quantize_fp8(int device, uint64_t stream, uint64_t X, int64_t ldx, uint64_t Q, int64_t ldq, uint64_t S, int64_t rows,
                      int cols, int block_rows, int transposed, int dtype, int dtype8);
 /* C = act(sum over blocks of scale_a * scale_b * (A * B^T of the block) + beta * C + bias[col]): A is M x K in blocks of 1 x 128,
- * B is N x K (a weight as linear layers keep it) in blocks of block_b (1 or 128) x 128. The scales' products have to
- * be normal fp32 numbers. Rows of A and B start on 16-byte boundaries; C and bias are of dtype_c. beta * C is skipped when beta
+ * B is N x K (a weight as linear layers keep it) in blocks of block_b (1 or 128) x 128. Scales may
+ * reach 2^88, and the product of two, but for blocks of zeros, has to be a normal fp32 number. M, N and K up to
+ * 2^31 - 256. Rows of A and B start on 16-byte boundaries; C and bias are of dtype_c. beta * C is skipped when beta
  * == 0. C must not overlap the operands. */
 typedef struct kcg_fp8_product {
   uint64_t A, scale_a, B, scale_b, C, bias;

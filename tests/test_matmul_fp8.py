@@ -111,6 +111,16 @@ def test_the_c_entry_refuses_what_it_cannot_take():
     assert lib.kcg_matmul_fp8(0, 0, None) == _lib.E_BAD_ARG
 
 
+def test_sizes_that_no_32_bits_hold_are_refused():
+    lib = _lib.get_lib()
+    ok = dict(A=256, scale_a=256, B=256, scale_b=256, C=256, m=8, n=8, k=128, block_b=128, dtype_a=1, dtype_b=1, dtype_c=62)
+    for bad in (dict(m=2 ** 31 - 1), dict(n=2 ** 31 - 255), dict(k=2 ** 31 - 1)):
+        assert lib.kcg_matmul_fp8(0, 0, ctypes.byref(_lib.Fp8Product(**{**ok, **bad}))) == _lib.E_TOO_LARGE, bad
+    for rows, cols in ((2 ** 31 - 255, 8), (8, 2 ** 31 - 1)):
+        for block, transposed in ((1, 0), (1, 1), (128, 0), (128, 1)):
+            assert lib.kcg_quantize_fp8(0, 0, 256, 0, 256, 2 ** 31, 256, rows, cols, block, transposed, 62, 1) == _lib.E_TOO_LARGE
+
+
 def _plan(m, n, k, block_b=128, sms=148):
     out = (ctypes.c_int * 4)()
     _lib.get_lib().kcg_internal_fp8_plan(m, n, k, block_b, sms, out)
@@ -222,6 +232,20 @@ def test_scales_whose_product_leaves_the_range_of_fp32():
     for m in (4, 200):
         y = matmul_op.matmul_fp8(a[:1].repeat(m, 1), big[:1].repeat(m, 1), b, torch.full((3, 1), 2.0 ** 100, device="cuda"))
         assert torch.all(y == 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("block_b", [128, 1])
+@pytest.mark.parametrize("m", [4, 40, 200, 2304])
+def test_a_large_scale_meets_a_small_one(m, block_b):
+    """The largest parts, and the largest scale on either side: exact."""
+    n, k = 2304, 256
+    a, b = torch.full((m, k), 57344.0, device="cuda").to(E5), torch.full((n, k), 57344.0, device="cuda").to(E5)
+    for ea, eb in ((88, -60), (-60, 88)):
+        sa = torch.full((m, 2), 2.0 ** ea, device="cuda")
+        sb = torch.full((n if block_b == 1 else n // 128, 2), 2.0 ** eb, device="cuda")
+        y = matmul_op.matmul_fp8(a, sa, b, sb, out_dtype=torch.float32)
+        assert bool((y == 49 * 2.0 ** (26 + 8 + 28)).all())
 
 
 @pytest.mark.gpu
