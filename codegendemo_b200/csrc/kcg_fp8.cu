@@ -73,6 +73,15 @@ __device__ __forceinline__ void tmem_ld_16x256b_x2(uint32_t taddr, uint32_t (&r)
                : "r"(taddr)
                : "memory");
 }
+// The registers of the warps of a warpgroup, all of which come here.
+template <int kRegs>
+__device__ __forceinline__ void set_max_registers_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+template <int kRegs>
+__device__ __forceinline__ void set_max_registers_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
 // Ties the registers of an earlier load to the wait before it: no use of them may be scheduled ahead of this.
 template <int kN>
 __device__ __forceinline__ void pin(uint32_t (&r)[kN]) {
@@ -529,14 +538,18 @@ fp8_tile_kernel(const __grid_constant__ Fp8Params p) {
   Fp8Tile<kBN, kVector, kSwap, T>::run(p);
 }
 
-// CTA pairs, tiles of 256 x 256, one after another. Each CTA holds 128 rows of A and 128 of B a stage. Eleven warps of up to 184
-// registers: warp 0 waits in the accumulating warps' place, warp 1 of the leader issues the products, warp 2 loads the operands and brings
-// the scales of four blocks of K at a time into shared memory, warps 3-6 accumulate the first 128 columns and warps 7-10 the others.
+// CTA pairs, tiles of 256 x 256, one after another. Each CTA holds 128 rows of A and 128 of B a stage. Twelve warps: warp 0 waits in the
+// accumulating warps' place, warp 1 of the leader issues the products, warp 2 loads the operands, warp 3 brings the scales of four
+// blocks of K at a time into shared memory, warps 4-7 accumulate the first 128 columns and warps 8-11 the others.
 //
 // A block of K takes 512 cycles of the tensor pipe, and its accumulator has to be read, and the leader's issuer to hear of it from both
 // CTAs, while the other fills. The products' operands and TMA fill the shared-memory port, where an access then takes
-// hundreds of cycles, so the accumulating warps look at no mbarrier and spill nothing: warp 0 looks, and meets them on two named barriers
-// a block. (With mbarriers of their own a block took 1070 cycles, with a few spilled registers 1300.)
+// hundreds of cycles, so the accumulating warps look at no mbarrier and have registers enough: warp 0 looks, and tells each half's four
+// warps on a named barrier. (With mbarriers of their own a block took 1070 cycles, with a few spilled registers 1300.) The halves do not
+// meet: one adds while the other waits for tensor memory, and the next 32 columns are asked for while these are added, for which the
+// first four warps give up registers. 4096 x 4096 x 4096, all warps on one barrier and 32 columns at a time in 168 registers 71.2 us, the next 32 columns
+// ahead in 224 65.8, a barrier a half 65.6; kVector, with its own 16 columns ahead in both, 99.8, 100.4, 94.9. (Barriers of two warps each
+// are no faster.)
 //
 // Where the columns of a half share a scale, a thread accumulates one row of 128 columns, times one factor. Where each has its own
 // (kVector), a thread takes two neighbouring columns of each eight of four rows, as tcgen05.ld.16x256b gives them: 32 scales
@@ -544,15 +557,17 @@ fp8_tile_kernel(const __grid_constant__ Fp8Params p) {
 // cycles of its port a block of K against 512 of the tensor pipe.
 template <bool kVector, typename T>
 struct Fp8Pair {
-  static constexpr int NUM_THREADS = 352, kBM = 256, kBN = 256;
+  static constexpr int NUM_THREADS = 384, kBM = 256, kBN = 256;
+  // Registers: 168 a thread at launch, of which the first four warps give up what the accumulating ones take.
+  static constexpr int LAUNCH_REGS = 168, FEW_REGS = 56, MANY_REGS = 224;
+  static_assert(128 * FEW_REGS + 256 * MANY_REGS <= NUM_THREADS * LAUNCH_REGS, "the shares exceed what the CTA was launched with");
   static constexpr int HALF_BYTES = 128 * 128, STAGE_BYTES = 2 * HALF_BYTES;
   static constexpr int STAGES = 4;  // (three are as fast)
   static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
   static constexpr int STORE_BYTES = 8 * 2 * 32 * 128;  // two blocks of 32 rows of 128 bytes for each accumulating warp
   static constexpr int SCALES = 128 + (kVector ? 256 : 4);  // of a block of K: the CTA's rows, the tile's columns (or halves)
   static constexpr int GROUP_KB = 4;                        // blocks of K whose scales come together
-  // Groups in shared memory: the one that may still be read until all have met at the next one's first block, that one, and the one after
-  // it, which has to be there before its last block (that may be its first).
+  // Groups in shared memory: one that the later half may still read, the next, and the one after it on its way.
   static constexpr int GROUPS = 3;
   static constexpr int SCALE_BYTES = GROUPS * GROUP_KB * SCALES * 4;
   static constexpr int SMEM_BYTES = RING_BYTES + STORE_BYTES + SCALE_BYTES + 1024 + 512;
@@ -569,9 +584,11 @@ struct Fp8Pair {
   };
   static_assert(sizeof(Barriers) <= 512, "barrier block exceeds its shared-memory slot");
 
-  // Named barrier on which warp 0 and the accumulating warps meet in every block of K: the block's accumulator is complete, its scales
-  // and the next block's are in shared memory. All leave together where a wait of warp 0 ran out.
-  static constexpr uint32_t BAR_FULL = 1, MEETING = 32 + 256;
+  // Named barriers. At BAR_FULL warp 0 and the accumulating warps meet once: the first scales are there. At BAR_HALF + 2 half + (block & 1)
+  // warp 0 arrives, without waiting, and the half's warps wait: the block's accumulator is complete, its scales and the next block's
+  // are in shared memory. Warp 0 comes back to a barrier only when the accumulator of two blocks later is complete, for which all have left
+  // it. Where a wait of warp 0 ran out, it does meet the halves in every block left, so that all of them end; they store nothing.
+  static constexpr uint32_t BAR_HALF = 2, BAR_FULL = 1, MEETING = 32 + 256;
 
   // Rows and columns of C at which tile i starts.
   __device__ static __forceinline__ void tile_at(int i, int tiles_m, int tiles_n, int& m0, int& n0) {
@@ -581,42 +598,25 @@ struct Fp8Pair {
     n0 = in / rows * kBN;
   }
 
-  // The scales of GROUP_KB blocks of K, on their way through the registers of warp 2: four rows of the tile a lane (kVector: and
-  // eight columns).
-  struct Scales {
-    float4 p[4], q[kVector ? 8 : 1];
-    __device__ static __forceinline__ float4 four(const float* s, long long ld, int shift, int row, int rows, int kb, int num_kb, bool vec) {
-      const float* at = s + (static_cast<long long>(min(row, rows - 1)) >> shift) * ld + kb;
-      if (vec && kb + 4 <= num_kb) return __ldg(reinterpret_cast<const float4*>(at));
-      const int left = num_kb - kb;  // (those past the last block are not used)
-      return make_float4(__ldg(at), left > 1 ? __ldg(at + 1) : 0.f, left > 2 ? __ldg(at + 2) : 0.f, left > 3 ? __ldg(at + 3) : 0.f);
-    }
-    __device__ __forceinline__ void load(const Fp8Params& a, int m0, int n0, int kb) {
-      const int lane = threadIdx.x & 31;
+  // The scales of GROUP_KB blocks of K from block kb on, those of 32 kRows rows from `row` on: four of a row a lane, all rows under way at
+  // once, to slot[i] of each block's place.
+  template <int kRows>
+  __device__ static __forceinline__ void bring(const float* s, long long ld, int shift, int row, int rows, int kb, int num_kb, bool vec,
+                                               float* slot) {
+    const int lane = threadIdx.x & 31, left = num_kb - kb;  // (those past the last block are not used)
+    float4 v[kRows];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = four(a.sp, a.ldsp, a.sp_shift, m0 + i * 32 + lane, a.rows_p, kb, a.num_kb, a.vector_sp);
-      if constexpr (kVector) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = four(a.sq, a.ldsq, a.sq_shift, n0 + i * 32 + lane, a.rows_q, kb, a.num_kb, a.vector_sq);
-      } else {
-        q[0] = four(a.sq, a.ldsq, a.sq_shift, n0 + (lane & 1) * 128, a.rows_q, kb, a.num_kb, a.vector_sq);
-      }
+    for (int i = 0; i < kRows; ++i) {
+      const float* at = s + (static_cast<long long>(min(row + i * 32 + lane, rows - 1)) >> shift) * ld + kb;
+      v[i] = vec && left >= 4 ? __ldg(reinterpret_cast<const float4*>(at))
+                              : make_float4(__ldg(at), left > 1 ? __ldg(at + 1) : 0.f, left > 2 ? __ldg(at + 2) : 0.f, left > 3 ? __ldg(at + 3) : 0.f);
     }
-    __device__ static __forceinline__ void put4(float* slot, int i, const float4& v) {
-      slot[i] = v.x, slot[SCALES + i] = v.y, slot[2 * SCALES + i] = v.z, slot[3 * SCALES + i] = v.w;
-    }
-    __device__ __forceinline__ void store(float* slot) const {
-      const int lane = threadIdx.x & 31;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) put4(slot, i * 32 + lane, p[i]);
-      if constexpr (kVector) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) put4(slot, 128 + i * 32 + lane, q[i]);
-      } else if (lane < 2) {
-        put4(slot, 128 + lane, q[0]);
-      }
+    for (int i = 0; i < kRows; ++i) {
+      float* to = slot + i * 32 + lane;
+      to[0] = v[i].x, to[SCALES] = v[i].y, to[2 * SCALES] = v[i].z, to[3 * SCALES] = v[i].w;
     }
-  };
+  }
 
   // This warp's accumulators to C: 32 rows of 128 columns, through blocks of shared memory: 16-byte units XORed with the row, the
   // swizzle of the tensor map, and TMA stores, two under way; or rows by RowStore where TMA cannot address them.
@@ -718,7 +718,7 @@ struct Fp8Pair {
       }
       for (int g = 0; g < GROUPS; ++g) {
         mbar_init(&bars->scale_full[g], 32);
-        mbar_init(&bars->scale_empty[g], 1);
+        mbar_init(&bars->scale_empty[g], 8);
       }
       bars->abort_flag = 0u;
       fence_mbar_init();
@@ -735,99 +735,10 @@ struct Fp8Pair {
     const uint32_t tmem_base = bars->tmem_base;
     griddep_wait();
 
-    if (warp == 0) {
-      // ------------------------------------------------ waits in the accumulating warps' place
-      uint32_t it = 0, g = 0;
-      bool ok = true;
-      auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t what) {
-        if (ok) ok = mbar_wait_warp(bar, parity, &bars->abort_flag);
-        if (!ok && lane == 0) report(bars, FP8_TIMEOUT_ACCUMULATE, it, what);
-      };
-      wait(&bars->scale_full[0], 0u, 2u);
-      ok = named_bar_all(BAR_FULL, MEETING, ok);  // the first block's scales
-      for (int tile = tile0; tile < tiles && ok; tile += stride) {
-        for (int kb = 0; kb < p.num_kb && ok; ++kb, ++it) {
-          const bool begins = kb % GROUP_KB == 0 && it > 0;  // a group after the first
-          if (begins) ++g;
-          if ((kb % GROUP_KB == GROUP_KB - 1 || kb == p.num_kb - 1) && (kb < p.num_kb - 1 || tile + stride < tiles))
-            wait(&bars->scale_full[(g + 1) % GROUPS], ((g + 1) / GROUPS) & 1u, 2u);
-          wait(&bars->tmem_full[it & 1u], (it >> 1) & 1u, 0u);
-          tc_fence_after_sync();
-          tc_fence_before_sync();
-          ok = named_bar_all(BAR_FULL, MEETING, ok);
-          if (begins && lane == 0) mbar_arrive(&bars->scale_empty[(g - 1) % GROUPS]);  // nobody reads the group before any more
-        }
-      }
-    } else if (warp == 1) {
-      if (rank == 0u) {
-        const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
-        const uint64_t adesc = make_smem_desc(smem_u32(smem), 16, 1024, SWZ_128B);
-        const uint64_t bdesc = make_smem_desc(smem_u32(smem) + HALF_BYTES, 16, 1024, SWZ_128B);
-        const uint32_t idesc = make_instr_desc(0u, 0u, 0u, 256u, kBN) | p.fmt_p << 7 | p.fmt_q << 10;
-        uint32_t it = 0;
-        bool ok = true;
-        for (int tile = tile0; tile < tiles && ok; tile += stride) {
-          for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
-            const uint32_t s = it % STAGES, b = it & 1u;
-            // (the operands have mostly been there for long: what is waited for is the accumulator)
-            if (!mbar_wait_warp(&bars->full[s], (it / STAGES) & 1u, &bars->abort_flag) ||
-                !mbar_wait_warp(&bars->tmem_empty[b], ((it >> 1) & 1u) ^ 1u, &bars->abort_flag)) {
-              if (lane == 0) report(bars, FP8_TIMEOUT_MMA, it, s);
-              ok = false;
-              break;
-            }
-            tc_fence_after_sync();
-            if (elect_one()) {
-#pragma unroll
-              for (int ks = 0; ks < 4; ++ks)
-                umma_fp8<2>(tmem + b * kBN, adesc + s * (STAGE_BYTES >> 4) + ks * 2, bdesc + s * (STAGE_BYTES >> 4) + ks * 2, idesc,
-                            ks > 0 ? 1u : 0u);
-              umma_commit_both(&bars->tmem_full[b]);
-              umma_commit_both(&bars->empty[s]);
-            }
-            __syncwarp();
-          }
-        }
-      }
-    } else if (warp == 2) {
-      // ------------------------------------------------ operands, and scales GROUP_KB blocks at a time
-      uint32_t it = 0, g = 0;
-      bool ok = true;
-      auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t what) {
-        ok = mbar_wait_warp(bar, parity, &bars->abort_flag);
-        if (!ok && lane == 0) report(bars, FP8_TIMEOUT_PRODUCER, it, what);
-        return ok;
-      };
-      for (int tile = tile0; tile < tiles && ok; tile += stride) {
-        int m0, n0;
-        tile_at(tile, tiles_m, tiles_n, m0, n0);
-        m0 += static_cast<int>(rank) * 128;
-        Scales held;
-        held.load(p, m0, n0, 0);
-        for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
-          const uint32_t s = it % STAGES;
-          if (!wait(&bars->empty[s], ((it / STAGES) & 1u) ^ 1u, s)) break;
-          if (lane == 0) {
-            // completion bytes of both CTAs land on the leader's barrier
-            const uint32_t full_leader = map_to_cta(smem_u32(&bars->full[s]), 0u);
-            if (rank == 0u) mbar_expect_tx(&bars->full[s], 2 * STAGE_BYTES);
-            tma_load_2d_pair(smem + s * STAGE_BYTES, &p.tmP, full_leader, kb * 128, m0);
-            tma_load_2d_pair(smem + s * STAGE_BYTES + HALF_BYTES, &p.tmQ, full_leader, kb * 128, n0 + static_cast<int>(rank) * 128);
-          }
-          __syncwarp();
-          if (kb % GROUP_KB == 0) {
-            if (!wait(&bars->scale_empty[g % GROUPS], ((g / GROUPS) & 1u) ^ 1u, 100u)) break;
-            held.store(scales + g % GROUPS * GROUP_KB * SCALES);
-            mbar_arrive(&bars->scale_full[g % GROUPS]);
-            ++g;
-            if (kb + GROUP_KB < p.num_kb) held.load(p, m0, n0, kb + GROUP_KB);
-          }
-        }
-      }
-      griddep_launch_dependents();
-    } else {
-      const int q = warp & 3, half = (warp - 3) >> 2;  // TMEM lane quarter of this warp, half of the tile's columns
-      uint8_t* block = smem + RING_BYTES + (warp - 3) * 8192;
+    if (warp >= 4) {
+      set_max_registers_up<MANY_REGS>();
+      const int q = warp & 3, half = (warp - 4) >> 2;  // TMEM lane quarter of this warp, half of the tile's columns
+      uint8_t* block = smem + RING_BYTES + (warp - 4) * 8192;
       // The scales of a block's rows (and of its half's columns, where they share one) are read when the block before has been added:
       // read before its additions they cost a third of the speed.
       const float* row_scales = scales + q * 32 + (kVector ? lane >> 2 : lane);
@@ -845,16 +756,15 @@ struct Fp8Pair {
           f[1] = column_scales[at];
         }
       };
-      bool ok = named_bar_all(BAR_FULL, MEETING, true);
+      named_bar_sync(BAR_FULL, MEETING);
       fetch();
-      for (int tile = tile0; tile < tiles && ok; tile += stride) {
+      for (int tile = tile0; tile < tiles; tile += stride) {
         float acc[128];
 #pragma unroll
         for (int i = 0; i < 128; ++i) acc[i] = 0.f;
         for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
           const uint32_t col = tmem_base + (it & 1u) * kBN + half * 128 + (static_cast<uint32_t>(q * 32) << 16);
-          ok = named_bar_all(BAR_FULL, MEETING, true);
-          if (!ok) break;
+          named_bar_sync(BAR_HALF + half * 2 + (it & 1u), 160);
           tc_fence_after_sync();
           auto release = [&]() {  // (the reads are complete)
             tc_fence_before_sync();
@@ -863,18 +773,20 @@ struct Fp8Pair {
           };
           if constexpr (!kVector) {
             const float factor = scale_product(f[0], f[1]);
-            // (the next 32 columns asked for beside these, or 16 at a time, are no faster)
+            uint32_t r[2][32];
+            tmem_ld_32x32b_x32(col, r[0]);
 #pragma unroll
-            for (int c = 0; c < 128; c += 32) {
-              uint32_t r[32];
-              tmem_ld_32x32b_x32(col + c, r);
+            for (int c = 0; c < 4; ++c) {
               tmem_ld_wait();
-              pin(r);
-              if (c == 96) release();
-              add_scaled<32>(acc + c, r, factor);
+              pin(r[c & 1]);
+              if (c < 3) {
+                tmem_ld_32x32b_x32(col + (c + 1) * 32, r[(c + 1) & 1]);
+              } else {
+                release();
+              }
+              add_scaled<32>(acc + c * 32, r[c & 1], factor);
             }
           } else {
-            // 16 columns at a time, rows 0-15 and 16-31 of the warp's lanes
             uint32_t r[2][2][8];
             float2 s[2][2];
             auto load = [&](int c) {
@@ -908,6 +820,8 @@ struct Fp8Pair {
           }
           // the next block's place: the next of the group, or the first of the next group
           if (kb % GROUP_KB == GROUP_KB - 1 || kb == p.num_kb - 1) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->scale_empty[group_at / (GROUP_KB * SCALES)]);
             group_at = group_at == (GROUPS - 1) * GROUP_KB * SCALES ? 0u : group_at + GROUP_KB * SCALES;
             at = group_at;
           } else {
@@ -915,13 +829,128 @@ struct Fp8Pair {
           }
           fetch();
         }
-        if (!ok) break;
+        if (bars->abort_flag != 0u) continue;
         int m0, n0;
         tile_at(tile, tiles_m, tiles_n, m0, n0);
         store(p, acc, m0 + static_cast<int>(rank) * 128 + q * 32, n0 + half * 128, block);
       }
       if (lane == 0) tma_store_wait_read<0>();  // shared memory outlives the stores' reads
       __syncwarp();
+    } else {
+      set_max_registers_down<FEW_REGS>();
+      if (warp == 0) {
+        // ------------------------------------------------ waits in the accumulating warps' place
+        uint32_t it = 0, g = 0;
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t what) {
+          if (ok) ok = mbar_wait_warp(bar, parity, &bars->abort_flag);
+          if (!ok && lane == 0) report(bars, FP8_TIMEOUT_ACCUMULATE, it, what);
+        };
+        wait(&bars->scale_full[0], 0u, 2u);
+        named_bar_sync(BAR_FULL, MEETING);  // the first block's scales
+        for (int tile = tile0; tile < tiles; tile += stride) {
+          for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
+            if (kb == p.num_kb - 1 ? tile + stride < tiles : kb % GROUP_KB == GROUP_KB - 1) {
+              ++g;
+              wait(&bars->scale_full[g % GROUPS], (g / GROUPS) & 1u, 2u);
+            }
+            wait(&bars->tmem_full[it & 1u], (it >> 1) & 1u, 0u);
+            tc_fence_after_sync();
+            tc_fence_before_sync();
+            if (ok) {
+              named_bar_arrive(BAR_HALF + (it & 1u), 160);
+              named_bar_arrive(BAR_HALF + 2 + (it & 1u), 160);
+            } else {
+              named_bar_sync(BAR_HALF + (it & 1u), 160);
+              named_bar_sync(BAR_HALF + 2 + (it & 1u), 160);
+            }
+          }
+        }
+      } else if (warp == 1) {
+        if (rank == 0u) {
+          const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+          const uint64_t adesc = make_smem_desc(smem_u32(smem), 16, 1024, SWZ_128B);
+          const uint64_t bdesc = make_smem_desc(smem_u32(smem) + HALF_BYTES, 16, 1024, SWZ_128B);
+          const uint32_t idesc = make_instr_desc(0u, 0u, 0u, 256u, kBN) | p.fmt_p << 7 | p.fmt_q << 10;
+          uint32_t it = 0;
+          bool ok = true;
+          for (int tile = tile0; tile < tiles && ok; tile += stride) {
+            for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
+              const uint32_t s = it % STAGES, b = it & 1u;
+              // (the operands have mostly been there for long: what is waited for is the accumulator)
+              if (!mbar_wait_warp(&bars->full[s], (it / STAGES) & 1u, &bars->abort_flag) ||
+                  !mbar_wait_warp(&bars->tmem_empty[b], ((it >> 1) & 1u) ^ 1u, &bars->abort_flag)) {
+                if (lane == 0) report(bars, FP8_TIMEOUT_MMA, it, s);
+                ok = false;
+                break;
+              }
+              tc_fence_after_sync();
+              if (elect_one()) {
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks)
+                  umma_fp8<2>(tmem + b * kBN, adesc + s * (STAGE_BYTES >> 4) + ks * 2, bdesc + s * (STAGE_BYTES >> 4) + ks * 2, idesc,
+                              ks > 0 ? 1u : 0u);
+                umma_commit_both(&bars->tmem_full[b]);
+                umma_commit_both(&bars->empty[s]);
+              }
+              __syncwarp();
+            }
+          }
+        }
+      } else if (warp == 2) {
+        // ------------------------------------------------ operands
+        uint32_t it = 0;
+        bool ok = true;
+        for (int tile = tile0; tile < tiles && ok; tile += stride) {
+          int m0, n0;
+          tile_at(tile, tiles_m, tiles_n, m0, n0);
+          m0 += static_cast<int>(rank) * 128, n0 += static_cast<int>(rank) * 128;
+          for (int kb = 0; kb < p.num_kb; ++kb, ++it) {
+            const uint32_t s = it % STAGES;
+            ok = mbar_wait_warp(&bars->empty[s], ((it / STAGES) & 1u) ^ 1u, &bars->abort_flag);
+            if (!ok) {
+              if (lane == 0) report(bars, FP8_TIMEOUT_PRODUCER, it, s);
+              break;
+            }
+            if (lane == 0) {
+              // completion bytes of both CTAs land on the leader's barrier
+              const uint32_t full_leader = map_to_cta(smem_u32(&bars->full[s]), 0u);
+              if (rank == 0u) mbar_expect_tx(&bars->full[s], 2 * STAGE_BYTES);
+              tma_load_2d_pair(smem + s * STAGE_BYTES, &p.tmP, full_leader, kb * 128, m0);
+              tma_load_2d_pair(smem + s * STAGE_BYTES + HALF_BYTES, &p.tmQ, full_leader, kb * 128, n0);
+            }
+            __syncwarp();
+          }
+        }
+        griddep_launch_dependents();
+      } else {
+        // ------------------------------------------------ scales, GROUP_KB blocks at a time, as soon as a group's place is free
+        uint32_t g = 0;
+        bool ok = true;
+        for (int tile = tile0; tile < tiles && ok; tile += stride) {
+          int m0, n0;
+          tile_at(tile, tiles_m, tiles_n, m0, n0);
+          m0 += static_cast<int>(rank) * 128;
+          for (int kb = 0; kb < p.num_kb; kb += GROUP_KB, ++g) {
+            ok = mbar_wait_warp(&bars->scale_empty[g % GROUPS], ((g / GROUPS) & 1u) ^ 1u, &bars->abort_flag);
+            if (!ok) {
+              if (lane == 0) report(bars, FP8_TIMEOUT_PRODUCER, g, 100u);
+              break;
+            }
+            float* slot = scales + g % GROUPS * GROUP_KB * SCALES;
+            bring<4>(p.sp, p.ldsp, p.sp_shift, m0, p.rows_p, kb, p.num_kb, p.vector_sp, slot);
+            if constexpr (kVector) {
+#pragma unroll 1
+              for (int half = 0; half < 256; half += 128)  // (one after the other: 16 registers)
+                bring<4>(p.sq, p.ldsq, p.sq_shift, n0 + half, p.rows_q, kb, p.num_kb, p.vector_sq, slot + 128 + half);
+            } else if (lane < 2) {  // (lanes 0 and 1: the tile's two halves)
+              bring<1>(p.sq, p.ldsq, 0, n0 >> 7, (p.rows_q + 127) / 128, kb, p.num_kb, p.vector_sq, slot + 128);
+            }
+            mbar_arrive(&bars->scale_full[g % GROUPS]);
+            __syncwarp();
+          }
+        }
+      }
     }
 
     // ------------------------------------------------------------ common exit
@@ -943,7 +972,7 @@ struct Fp8Pair {
 };
 
 template <bool kVector, typename T>
-__global__ void __launch_bounds__(352, 1) fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
+__global__ void __launch_bounds__(384, 1) fp8_pair_kernel(const __grid_constant__ Fp8Params p) {
   Fp8Pair<kVector, T>::run(p);
 }
 
@@ -1017,9 +1046,10 @@ struct Plan {
 // weight's rows are the tile's rows, and K is split until a quarter more CTAs run than there are SMs (two fit one): 1 x 4096 x 4096 in 1, 2,
 // 4, 8 parts 10.9, 7.6, 5.8, 6.2 us, 1 x 14336 x 4096 13.0, 13.6, 16.5, 22.3.
 // More tokens: 128 x 128 tiles, K in up to four parts while all run at once (eight: 200 x 1024 x 8192 17.4 us against 10.9), or pairs, whichever
-// takes less time by {fixed, per wave and block of K, per wave, joining 2 and 4 parts}, fitted to 35 shapes of 33 to 3700 tokens x 264 to 9600 x
-// 128 to 11008, 5 to 8 % rms, of which it picks the faster every time. Tiles of 128 against pairs: 128 x 4096 x 4096 in four parts 10.2 / 19.3
-// us, 512 x 4096 x 11008 30 / 47, 1444 x 1040 x 1760 7.9 / 12.1; 777 x 2752 x 1488 13.2 / 11.0, 512 x 11008 x 4096 40 / 36, 1204 x 6600 x 128 13.7 / 8.9.
+// takes less time by {fixed, per wave and block of K, per wave, joining 2 and 4 parts}, fitted to 35 shapes of 33 to 8192 tokens x 264 to 11008 x
+// 128 to 11008, 6 to 8 % rms, of which it picks one within 3 % of the fastest every time. Tiles of 128 against pairs: 128 x 4096 x 4096 in four
+// parts 9.7 / 17.0 us, 512 x 4096 x 11008 33 / 39, 1444 x 1040 x 1760 8.5 / 10.6; 777 x 2752 x 1488 13.8 / 10.6, 512 x 11008 x 4096 43 / 34,
+// 1204 x 6600 x 128 13.8 / 8.8.
 Plan plan_of(int m, int n, int k, bool vector, int sms) {
   const int num_kb = (k - 1) / 128 + 1;
   Plan plan{0, 0, 128, 1};
@@ -1030,8 +1060,8 @@ Plan plan_of(int m, int n, int k, bool vector, int sms) {
     while (plan.splits < 8 && 4 * tiles * 2 * plan.splits <= 5LL * sms && num_kb >= 4 * plan.splits) plan.splits *= 2;
     return plan;
   }
-  const double pair_us[3] = {vector ? 3.6 : 3.2, vector ? 0.71 : 0.5, 1.8};
-  const double tile_us[3] = {vector ? -0.5 : -0.8, vector ? 0.563 : 0.335, vector ? 3.3 : 3.7};
+  const double pair_us[3] = {vector ? 3.6 : 3.0, vector ? 0.633 : 0.416, vector ? 1.9 : 1.8};
+  const double tile_us[3] = {vector ? -0.4 : -0.6, vector ? 0.602 : 0.365, vector ? 3.2 : 3.4};
   const long long tiles = (static_cast<long long>(m - 1) / 128 + 1) * ((n - 1) / 128 + 1);
   const long long large = (static_cast<long long>(m - 1) / 256 + 1) * ((n - 1) / 256 + 1), pairs = sms >= 2 ? sms / 2 : 1;
   double best = pair_us[0] + static_cast<double>((large - 1) / pairs + 1) * (num_kb * pair_us[1] + pair_us[2]);
@@ -1067,6 +1097,15 @@ int launch_pair(int device, int sms, cudaStream_t st, const Fp8Params& p) {
   static bool ready[64];
   const auto kernel = fp8_pair_kernel<kVector, T>;
   if (int e = opt_in(kernel, device, Kern::SMEM_BYTES, ready)) return e;
+  // the accumulating warps would wait for ever for registers that the CTA was not launched with
+  static std::atomic<int> registers{0};
+  if (registers.load() == 0) {
+    cudaFuncAttributes attributes;
+    const cudaError_t e = cudaFuncGetAttributes(&attributes, kernel);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncGetAttributes");
+    registers.store(attributes.numRegs);
+  }
+  if (registers.load() < Kern::LAUNCH_REGS) return fail(KCG_E_BAD_CONFIG, "the 8-bit product was built with too few registers");
   const long long tiles = static_cast<long long>((p.rows_p + 255) / 256) * ((p.rows_q + 255) / 256);
   if (tiles > 0x3fffffffLL) return fail(KCG_E_TOO_LARGE, "too many tiles for one launch");
   const int pairs = static_cast<int>(tiles < sms / 2 ? tiles : sms / 2);
