@@ -843,8 +843,10 @@ struct Fp8Pair {
         uint32_t it = 0, g = 0;
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t what) {
-          if (ok) ok = mbar_wait_warp(bar, parity, &bars->abort_flag);
-          if (!ok && lane == 0) report(bars, FP8_TIMEOUT_ACCUMULATE, it, what);
+          if (!ok || mbar_wait_warp(bar, parity, &bars->abort_flag)) return;
+          ok = false;
+          if (lane == 0) report(bars, FP8_TIMEOUT_ACCUMULATE, it, what);
+          for (int i = 0; i < 1000; ++i) __nanosleep(1000);  // the halves leave the barriers at which this warp has arrived
         };
         wait(&bars->scale_full[0], 0u, 2u);
         named_bar_sync(BAR_FULL, MEETING);  // the first block's scales
