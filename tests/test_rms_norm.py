@@ -139,6 +139,28 @@ def test_forward(rows, width, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("width", [509, 511, 513, 2047, 2049, 4095, 4097, 8191, 8193, 12001, 16383, 16385])
+def test_rows_of_no_whole_pieces_either_side_of_each_form(width, dtype):
+    test_forward(3, width, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("width", [512, 2048, 4096, 8192, 16384])
+def test_rows_that_start_anywhere(width):
+    """Whole pieces, but no row on a 16-byte boundary; written over x and over the residual."""
+    x = rows_of(5, width + 1, torch.bfloat16, 1)[:, 1:]
+    r = rows_of(5, width + 1, torch.bfloat16, 2)[:, 1:]
+    w = rows_of(1, width, torch.bfloat16, 3)[0]
+    h64 = x.double() + r.double()
+    q, scales, h = matmul_op.rms_norm_fp8(x, w, r, eps=EPS)
+    near_fp8(q, scales, norm64(h64, w))
+    y, h2 = matmul_op.rms_norm(x, w, r, eps=EPS, out=x, residual_out=r)
+    assert torch.equal(h2, h) and h2.data_ptr() == r.data_ptr() and y.data_ptr() == x.data_ptr()
+    near(y, norm64(h64, w), torch.bfloat16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("rows,width", SHAPES + [(513, 1376), (1000, 264), (700, 129)])
 def test_backward_against_the_formula(rows, width, dtype):
     """dx: two terms whose difference may be small, each off by 100 u of itself (80 of the root's, and the second sum's 140 u of
