@@ -112,28 +112,29 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
 }
 
 // Eight values of a row from column c on, as they lie in memory; those past the row's end as zeros. kVec: rows start on 16-byte
-// boundaries.
+// boundaries, else the values may lie `step` apart.
 template <typename T, bool kVec>
-__device__ __forceinline__ void load_piece(const T* row, int c, int cols, Raw8<T>& v) {
+__device__ __forceinline__ void load_piece(const T* row, int c, int cols, Raw8<T>& v, int step = 1) {
   if (kVec && c + 8 <= cols) {
     v.load(row + c);
   } else {
     T e[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) e[j] = c + j < cols ? row[c + j] : T(0.f);
+    for (int j = 0; j < 8; ++j) e[j] = c + j * step < cols ? row[c + j * step] : T(0.f);
     v.set(e);
   }
 }
 
-// Eight values to a row from column c on, as far as the row goes. kWhole: rows of whole pieces on 16-byte boundaries.
+// Eight values to a row from column c on, as far as the row goes. kWhole: rows of whole pieces on 16-byte boundaries, else the values
+// may go `step` apart.
 template <typename T, bool kWhole>
-__device__ __forceinline__ void store_piece(T* row, int c, int cols, const float2 (&v)[4]) {
+__device__ __forceinline__ void store_piece(T* row, int c, int cols, const float2 (&v)[4], int step = 1) {
   if constexpr (kWhole) {
     store8(row + c, v);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (c + j < cols) row[c + j] = from_f32<T>(j & 1 ? v[j / 2].y : v[j / 2].x);
+      if (c + j * step < cols) row[c + j * step] = from_f32<T>(j & 1 ? v[j / 2].y : v[j / 2].x);
   }
 }
 

@@ -283,32 +283,35 @@ struct GradArgs {
 
 // Each CTA walks rows blockIdx.x, + gridDim.x, ...; a thread keeps its columns' share of dw in registers, the row as it lies in
 // memory, and (kAhead: rows of up to 8192 values) asks for the next row before it reduces the present one. !kWhole: rows that
-// are no whole 16-byte pieces, value by value (8192 x 4095 bf16 157 us; by threads that each own every 512th value, dw in shared memory, 300).
+// are no whole 16-byte pieces, value by value, a warp's side by side (8192 x 4095 bf16 104 us; eight of a row in each thread 156; dw in shared
+// memory 300).
 template <typename T, int kVPT, bool kDh, bool kWhole, int kThreads, int kCtas, bool kAhead>
 __global__ void __launch_bounds__(kThreads, kCtas) norm_grad_kernel(const GradArgs a) {
   constexpr int kWarps = warps_of(kThreads);
   __shared__ float scratch[2][2 * kWarps];
   griddep_launch_dependents();
   griddep_wait();
-  const int tid = threadIdx.x, threads = blockDim.x, pieces = (a.width + 7) / 8;
+  const int tid = threadIdx.x, threads = blockDim.x;
   struct Row {
     Raw8<T> h[kVPT], dy[kVPT], dh[kDh ? kVPT : 1];
   };
   float2 dw[kVPT][4];
   Raw8<T> w[kVPT];
   Row at, next;
+  // The column of a thread's piece v = i * threads + tid, whose others follow at once, or (single values) `threads` apart.
+  auto first = [&](int v) { return kWhole ? 8 * v : 8 * (v - tid) + tid; };
   auto read = [&](Raw8<T>& to, const T* from, int v) {
     if constexpr (kWhole) {
       to.load(from + 8 * v);
     } else {
-      load_piece<T, false>(from, 8 * v, a.width, to);
+      load_piece<T, false>(from, first(v), a.width, to, threads);
     }
   };
   auto ask = [&](Row& to, long long row) {
 #pragma unroll
     for (int i = 0; i < kVPT; ++i) {
       const int v = i * threads + tid;
-      if (v < pieces) {
+      if (first(v) < a.width) {
         read(to.h[i], static_cast<const T*>(a.h) + row * a.ldh, v);
         read(to.dy[i], static_cast<const T*>(a.dy) + row * a.lddy, v);
         if constexpr (kDh) read(to.dh[i], static_cast<const T*>(a.dh) + row * a.lddh, v);
@@ -319,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) norm_grad_kernel(const GradAr
   for (int i = 0; i < kVPT; ++i) {
     w[i].zero(), at.h[i].zero(), at.dy[i].zero(), next.h[i].zero(), next.dy[i].zero();
     if constexpr (kDh) at.dh[i].zero(), next.dh[i].zero();
-    if (i * threads + tid < pieces) read(w[i], static_cast<const T*>(a.w), i * threads + tid);
+    if (first(i * threads + tid) < a.width) read(w[i], static_cast<const T*>(a.w), i * threads + tid);
 #pragma unroll
     for (int j = 0; j < 4; ++j) dw[i][j] = both(0.f);
   }
@@ -364,14 +367,14 @@ __global__ void __launch_bounds__(kThreads, kCtas) norm_grad_kernel(const GradAr
         dw[i][j] = __ffma2_rn(dy[j], __fmul2_rn(h[j], both(r)), dw[i][j]);
         d[j] = kDh ? __ffma2_rn(g, both(r), d[j]) : __fmul2_rn(g, both(r));
       }
-      if (v < pieces) store_piece<T, kWhole>(static_cast<T*>(a.dx) + row * a.lddx, 8 * v, a.width, d);
+      if (first(v) < a.width) store_piece<T, kWhole>(static_cast<T*>(a.dx) + row * a.lddx, first(v), a.width, d, threads);
     }
   }
   float* mine = a.partial + static_cast<long long>(blockIdx.x) * a.width;
 #pragma unroll
   for (int i = 0; i < kVPT; ++i) {
     const int v = i * threads + tid;
-    if (v < pieces) store_piece<float, kWhole>(mine, 8 * v, a.width, dw[i]);
+    if (first(v) < a.width) store_piece<float, kWhole>(mine, first(v), a.width, dw[i], threads);
   }
 }
 
