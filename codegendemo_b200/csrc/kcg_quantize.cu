@@ -1,5 +1,5 @@
 // Quantisation to 8 bits in blocks: of each block of 1 x 128 or 128 x 128 values the scale, max(largest magnitude / 448, 2^-126)
-// (57344 for e5m2), and the values x / scale as e4m3 or e5m2; as the matrix lies, or transposed (with blocks along what were the
+// (57344 for e5m2), and the values x * (1 / scale) as e4m3 or e5m2; as the matrix lies, or transposed (with blocks along what were the
 // columns' rows), as the products of a backward pass take their operands.
 //
 // Bound by HBM: every value is read once, into registers, and leaves as one byte. Blocks of one row: 16 threads a block, no shared

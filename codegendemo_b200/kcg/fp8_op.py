@@ -126,8 +126,9 @@ def rms_norm(x, weight, residual=None, eps=1e-6, out=None, residual_out=None):
 
 
 def rms_norm_fp8(x, weight, residual=None, eps=1e-6, residual_out=None):
-    """``rms_norm`` whose result leaves in 8 bits, as ``quantize_fp8`` would make it of the unrounded norm: returns (values, scales), or
-    (values, scales, h) with a residual."""
+    """``rms_norm`` whose result leaves in 8 bits, blocks of 1 x 128 of the unrounded norm as in ``quantize_fp8``: returns (values, scales),
+    or (values, scales, h) with a residual. Scales are off by a few units of fp32's last place, as the norm itself is; a value that lies as
+    near the middle between two 8-bit ones may become either, and may become the other one where the rows lie at another alignment."""
     if _warm and residual_out is None:
         results = _warm.rms_norm_fp8(x, weight, residual, eps)
         if results is not None:
@@ -178,7 +179,8 @@ def rms_norm_backward(dy, h, weight, eps=1e-6, dh=None):
 
 def quantize_fp8(x, rows=1, transposed=False, dtype=None):
     """(values, scales) of a matrix in blocks of ``rows`` (1 or 128) x 128 values: scale = max(largest magnitude / 448, 2^-126) (e5m2:
-    57344), values x / scale rounded to nearest even. ``transposed``: of ``x.t()``, cut into blocks along what were x's rows.
+    57344), values x * (1 / scale): reciprocal and product rounded to fp32, then to the nearest 8-bit value, ties to even (x / scale may
+    give the neighbour where it lies within 2^-23 of itself of the middle between two). ``transposed``: of ``x.t()``, cut into blocks along what were x's rows.
     ``dtype`` is float8_e4m3fn (default) or float8_e5m2. Scales are (row blocks) x ceil(columns / 128), fp32."""
     if _warm and dtype is None:
         results = _warm.quantize_fp8(x, rows, transposed)

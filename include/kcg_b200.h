@@ -231,8 +231,9 @@ int kcg_attention_status(int device, uint32_t out[4]);
  * with a row pitch in elements (0 = contiguous). `dtype` is KCG_DTYPE_FLOAT16, _BFLOAT16 or _FLOAT32; sums are fp32.
  *
  * 8-bit operands come in blocks along the dimension that a product sums over: of each block scale = max(largest
- * magnitude / 448 (e5m2: 57344), 2^-126), fp32, and values x / scale, rounded to nearest even. A NaN in a block
- * makes its scale and its values NaN; an infinity makes the scale infinite and the infinite values NaN. Scales of a matrix lie row after row,
+ * magnitude / 448 (e5m2: 57344), 2^-126), fp32, and values x * (1 / scale), the reciprocal and the product rounded to fp32, then to
+ * the nearest 8-bit value, ties to even. (x / scale may give the neighbour where the quotient lies within 2^-23 of itself of the
+ * middle between two 8-bit values: with 16-bit x, one to two values in a thousand.) A NaN in a block makes its scale and its values NaN; an infinity makes the scale infinite and the infinite values NaN. Scales of a matrix lie row after row,
  * ceil(columns / 128) to a row, one row for each block row.
  *
  * Root-mean-square norm: H = X + R, Y = H / sqrt(mean(H^2) + eps) * W, each row by itself. R = 0 (no residual): H = X, and H
@@ -240,7 +241,9 @@ int kcg_attention_status(int device, uint32_t out[4]);
  * of up to 32768 values; whole 16-byte pieces (width a multiple of 8, aligned rows) are the fast case. */
 int kcg_rms_norm(int device, uint64_t stream, uint64_t X, int64_t ldx, uint64_t R, int64_t ldr, uint64_t W, uint64_t Y,
                  int64_t ldy, uint64_t H, int64_t ldh, int64_t rows, int width, float eps, int dtype);
-/* The same with Y as e4m3 values Q in blocks of 1 x 128 and their scales S, from the unrounded Y. */
+/* The same with Y as e4m3 values Q in blocks of 1 x 128 and their scales S, from the unrounded Y: the operands of a product, not
+ * to the bit those of kcg_quantize_fp8. Scales are off by a few units of fp32's last place, as Y is, and a value that lies as near the middle
+ * between two 8-bit ones may become either; which, the rows' alignment has a part in (it picks the kernel). */
 int kcg_rms_norm_fp8(int device, uint64_t stream, uint64_t X, int64_t ldx, uint64_t R, int64_t ldr, uint64_t W, uint64_t Q,
                      int64_t ldq, uint64_t S, uint64_t H, int64_t ldh, int64_t rows, int width, float eps, int dtype);
 /* Its gradient: with r = 1 / sqrt(mean(H^2) + eps) and g = DY * W, DX = DH + r * g - H * r^3 * mean(g * H) (DH = 0: no
