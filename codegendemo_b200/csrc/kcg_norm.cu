@@ -64,26 +64,24 @@ __device__ __forceinline__ float rcp_ftz(float x) {
   return y;
 }
 
-// The end of a forward pass for one piece: h is stored, y (= h * w * r) stored or quantised. kFp8: the 16 neighbouring threads that hold
-// 128 values of the row come together; the factor r goes into the scale and its reciprocal instead of into every value.
+// The end of a forward pass for one piece: h is stored, y (= h * r * w, in that order: h * w may leave fp32's range where y does not) stored
+// or quantised. kFp8: the 16 neighbouring threads that hold 128 values of the row come together.
 template <typename T, bool kRes, bool kFp8>
 __device__ __forceinline__ void finish_piece(const NormArgs& a, long long row, int v, bool in, int tid, const float2 (&h)[4],
                                              const float2 (&w)[4], float r) {
   if (kRes && in) store8(static_cast<T*>(a.h) + row * a.ldh + 8 * v, h);
   float2 y[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) y[j] = kFp8 ? __fmul2_rn(h[j], w[j]) : __fmul2_rn(__fmul2_rn(h[j], both(r)), w[j]);
+  for (int j = 0; j < 4; ++j) y[j] = __fmul2_rn(__fmul2_rn(h[j], both(r)), w[j]);
   if constexpr (kFp8) {
     uint32_t bits = in ? abs_max(y) : 0u;  // (__reduce_max_sync of a warp's halves runs them one after the other, all that follows too)
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
     const float top = __uint_as_float(bits);
-    // scale = top * r / 448 and, for r / scale, 448 / top, off by an ulp or two. Where one of them is no normal number (a block of next to
-    // nothing, an infinity or a NaN in the row) by the definition, from the values themselves.
-    float scale = top * r * (1.f / 448.f), factor = 448.f * rcp_ftz(top);
-    if (!(scale >= FLT_MIN && factor >= FLT_MIN && factor <= FLT_MAX)) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] = __fmul2_rn(y[j], both(r));
+    // scale = top / 448 and, for 1 / scale, 448 / top, off by an ulp or two. Where one of them is no normal number (a block of next to nothing,
+    // values near the largest, an infinity or a NaN in the row) by the definition.
+    float scale = top * (1.f / 448.f), factor = 448.f * rcp_ftz(top);
+    if (!(scale >= FLT_MIN && factor >= FLT_MIN)) {
       if (scale < FLT_MIN) scale = FLT_MIN;
       factor = 1.f / scale;
     }
