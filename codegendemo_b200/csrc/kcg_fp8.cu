@@ -24,6 +24,7 @@
 #include "../../include/kcg_b200.h"
 #include "fp8_common.cuh"
 #include "kernels/ptx_sm100.cuh"
+#include "kernels/store_blocks.h"
 
 namespace {
 
@@ -649,9 +650,16 @@ struct Fp8Pair {
 #pragma unroll
     for (int b = 0; b < 128 / COLS_BLOCK; ++b) {
       if (row0 >= p.rows_p || col0 + b * COLS_BLOCK >= p.rows_q) break;
-      uint8_t* block = blocks + (p.vector_store ? (b & 1) * 4096 : 0);
+      uint8_t* block = blocks + (p.vector_store ? store_block(b) * 4096 : 0);
       if (p.vector_store) {
-        if (lane == 0) tma_store_wait_read<1>();  // the store before the last has read its block
+        if (lane == 0) {
+          if (stores_reading(b) == 0) {
+            tma_store_wait_read<0>();
+          } else {
+            static_assert(stores_reading(1) == 1, "the wait below leaves one store reading");
+            tma_store_wait_read<1>();
+          }
+        }
         __syncwarp();
       }
       if constexpr (!kVector) {
