@@ -432,13 +432,14 @@ struct Fp8Tile {
       const float* sp = p.sp + (static_cast<long long>(min(p0 + row, p.rows_p - 1)) >> p.sp_shift) * p.ldsp + kb0;
       const float* sq = p.sq + (static_cast<long long>(min(q0 + (kVector ? t : 0), p.rows_q - 1)) >> p.sq_shift) * p.ldsq + kb0;
       const bool fetches = !kVector || (threadIdx.x - 64) % 128 < COLS;
-      // the scales of four blocks at a time, four blocks ahead
+      // the scales of four blocks at a time, four blocks ahead (by ordinary loads: the kernel before this one may have written them while
+      // this one was there already, so they are not read-only for its whole life, as the non-coherent path asks)
       float next_p[4], next_q[4];
       auto fetch = [&](int i) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          next_p[j] = i + j < n ? __ldg(sp + i + j) : 0.f;
-          next_q[j] = fetches && i + j < n ? __ldg(sq + i + j) : 0.f;
+          next_p[j] = i + j < n ? sp[i + j] : 0.f;
+          next_q[j] = fetches && i + j < n ? sq[i + j] : 0.f;
         }
       };
       fetch(0);
@@ -600,7 +601,7 @@ struct Fp8Pair {
   }
 
   // The scales of GROUP_KB blocks of K from block kb on, those of 32 kRows rows from `row` on: four of a row a lane, all rows under way at
-  // once, to slot[i] of each block's place.
+  // once, to slot[i] of each block's place. (Ordinary loads, as in Fp8Tile.)
   template <int kRows>
   __device__ static __forceinline__ void bring(const float* s, long long ld, int shift, int row, int rows, int kb, int num_kb, bool vec,
                                                float* slot) {
@@ -609,8 +610,8 @@ struct Fp8Pair {
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
       const float* at = s + (static_cast<long long>(min(row + i * 32 + lane, rows - 1)) >> shift) * ld + kb;
-      v[i] = vec && left >= 4 ? __ldg(reinterpret_cast<const float4*>(at))
-                              : make_float4(__ldg(at), left > 1 ? __ldg(at + 1) : 0.f, left > 2 ? __ldg(at + 2) : 0.f, left > 3 ? __ldg(at + 3) : 0.f);
+      v[i] = vec && left >= 4 ? *reinterpret_cast<const float4*>(at)
+                              : make_float4(at[0], left > 1 ? at[1] : 0.f, left > 2 ? at[2] : 0.f, left > 3 ? at[3] : 0.f);
     }
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
