@@ -144,12 +144,14 @@ __device__ __forceinline__ uint32_t over_chunk(uint32_t v, int warp, int lane, u
   return v;
 }
 
+// (Ordinary loads: this kernel may be on the GPU while the one before it still writes an operand, which is not read-only for its whole
+// life then, as the non-coherent path asks.)
 __device__ __forceinline__ float4 load_a(const kcg::SplitF32Args& q, int row, int k) {
-  return row < q.M && k < q.K ? __ldg(reinterpret_cast<const float4*>(q.A + static_cast<size_t>(row) * q.lda + k))
+  return row < q.M && k < q.K ? *reinterpret_cast<const float4*>(q.A + static_cast<size_t>(row) * q.lda + k)
                               : make_float4(0.f, 0.f, 0.f, 0.f);
 }
 __device__ __forceinline__ float4 load_b(const kcg::SplitF32Args& q, int k, int n) {
-  return k < q.K && n < q.N ? __ldg(reinterpret_cast<const float4*>(q.B + static_cast<size_t>(k) * q.ldb + n))
+  return k < q.K && n < q.N ? *reinterpret_cast<const float4*>(q.B + static_cast<size_t>(k) * q.ldb + n)
                             : make_float4(0.f, 0.f, 0.f, 0.f);
 }
 __device__ __forceinline__ int sample_row(const kcg::SplitF32Args& q, int warp) {
