@@ -154,12 +154,19 @@ __device__ __forceinline__ void add_scaled(float* acc, const uint32_t (&part)[kN
   }
 }
 
+// A NaN stays one (fmaxf would make it 0).
+__device__ __forceinline__ float relu(float x) {
+  float y;
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // One value of C from its sum.
 template <typename T>
 __device__ __forceinline__ float finish(const Fp8Params& p, float v, const T* c, float bias) {
   if (p.beta != 0.f) v = fmaf(p.beta, to_f32(*c), v);
   v += bias;
-  return p.relu ? fmaxf(v, 0.f) : v;
+  return p.relu ? relu(v) : v;
 }
 template <typename T>
 __device__ __forceinline__ float bias_at(const Fp8Params& p, int n) {
@@ -207,7 +214,7 @@ __device__ __forceinline__ void finish_row(const Fp8Params& p, float (&v)[kN], i
   }
   if (p.relu) {
 #pragma unroll
-    for (int i = 0; i < kN; ++i) v[i] = fmaxf(v[i], 0.f);
+    for (int i = 0; i < kN; ++i) v[i] = relu(v[i]);
   }
 }
 

@@ -211,7 +211,7 @@ def matmul_fp8(a, a_scale, b, b_scale, c=None, beta=0.0, bias=None, relu=False, 
     ``a_scale`` M x ceil(K / 128); ``b`` is N x K (a weight as linear layers keep it) in blocks of 128 x 128, ``b_scale``
     ceil(N / 128) x ceil(K / 128), or of 1 x 128, ``b_scale`` N x ceil(K / 128). e4m3 or e5m2, each its own. Sums in fp32, one rounding
     to ``out_dtype`` (bf16 by default; fp16, fp32) or c's type. Rows of a and b have to start on 16-byte boundaries, as
-    ``quantize_fp8`` and ``rms_norm_fp8`` lay them out. Scales may reach 2^88 (values of 1e29), and the product
+    ``quantize_fp8`` and ``rms_norm_fp8`` lay them out. ReLU leaves a NaN one. Scales may reach 2^88 (values of 1e29), and the product
     of two, but for blocks of zeros, has to be a normal fp32 number."""
     if _warm and c is None and type(beta) is float and beta == 0.0:
         c = _warm.matmul_fp8(a, a_scale, b, b_scale, bias, relu, out_dtype)

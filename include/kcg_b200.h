@@ -263,7 +263,7 @@ int kcg_quantize_fp8(int device, uint64_t stream, uint64_t X, int64_t ldx, uint6
  * B is N x K (a weight as linear layers keep it) in blocks of block_b (1 or 128) x 128. Scales may
  * reach 2^88, and the product of two, but for blocks of zeros, has to be a normal fp32 number. M, N and K up to
  * 2^31 - 256. Rows of A and B start on 16-byte boundaries; C and bias are of dtype_c. beta * C is skipped when beta
- * == 0. C must not overlap the operands. */
+ * == 0. ReLU (act) leaves a NaN one. C must not overlap the operands. */
 typedef struct kcg_fp8_product {
   uint64_t A, scale_a, B, scale_b, C, bias;
   int64_t lda, ld_scale_a, ldb, ld_scale_b, ldc;
