@@ -184,7 +184,9 @@ __device__ __forceinline__ uint8_t quantize1(float v, float inv) {
 
 // ------------------------------------------------------------------------------------------------ host side
 inline int fail(int code, const std::string& msg) { return kcg_internal_fail(code, msg.c_str()); }
+// The error also leaves the runtime, which would give it to the next call that asks how its launch went.
 inline int cuda_fail(cudaError_t e, const char* what) {
+  cudaGetLastError();
   return fail(static_cast<int>(e), std::string(what) + ": " + cudaGetErrorString(e));
 }
 inline bool known_dtype(int dt) { return dt == KCG_DTYPE_FLOAT32 || dt == KCG_DTYPE_FLOAT16 || dt == KCG_DTYPE_BFLOAT16; }

@@ -333,7 +333,9 @@ extern "C" int kcg_internal_split_f32(uint64_t stream, const kcg::SplitF32Args* 
   cfg.attrs = attr;
   cfg.numAttrs = pdl ? 1 : 0;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, split_f32_kernel, *q);
-  if (e != cudaSuccess)
+  if (e != cudaSuccess) {
+    cudaGetLastError();  // (the next launch would be told of it)
     return kcg_internal_fail(static_cast<int>(e), (std::string("operand split launch: ") + cudaGetErrorString(e)).c_str());
+  }
   return 0;  // (counted with the product that it is a part of)
 }

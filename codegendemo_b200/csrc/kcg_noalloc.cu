@@ -60,6 +60,7 @@ EncodeFn g_encode = nullptr;
 
 int fail(int code, const std::string& msg) { return kcg_internal_fail(code, msg.c_str()); }
 int cuda_fail(cudaError_t e, const char* what) {
+  cudaGetLastError();  // (the next launch would be told of it)
   return fail(static_cast<int>(e), std::string(what) + ": " + cudaGetErrorString(e));
 }
 

@@ -145,7 +145,10 @@ extern "C" int kcg_softmax_rows_ex(int device, uint64_t stream, uint64_t X, int 
   int prev = -1;
   cudaError_t e = cudaGetDevice(&prev);
   if (e == cudaSuccess && prev != device) e = cudaSetDevice(device);
-  if (e != cudaSuccess) return fail(static_cast<int>(e), std::string("cudaSetDevice: ") + cudaGetErrorString(e));
+  if (e != cudaSuccess) {
+    cudaGetLastError();  // (the next launch would be told of it)
+    return fail(static_cast<int>(e), std::string("cudaSetDevice: ") + cudaGetErrorString(e));
+  }
   const int grid = static_cast<int>(rows < 148 * 16 ? rows : 148 * 16);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (dtype_in == KCG_DTYPE_FLOAT32) {
