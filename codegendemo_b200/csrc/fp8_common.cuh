@@ -100,16 +100,6 @@ __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
   raw.load(p);
   raw.values(v);
 }
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-  } else {
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()), pack2(v[4], v[5], T()),
-                                              pack2(v[6], v[7], T()));
-  }
-}
 
 // Eight values of a row from column c on, as they lie in memory; those past the row's end as zeros. kVec: rows start on 16-byte
 // boundaries, else the values may lie `step` apart.
