@@ -105,7 +105,7 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr) {
 
 struct Fp8Params {
   CUtensorMap tmP, tmQ;  // {K, rows}: the operand whose rows are the tile's rows, and the one whose rows are its columns
-  CUtensorMap tmC;       // Fp8Pair, vector_store: {N, M}, blocks of 128 bytes x 32 rows
+  CUtensorMap tmC;       // Fp8Pair, tma_store: {N, M}, blocks of 128 bytes x 32 rows
   const float *sp, *sq;  // scale of row i at block kb: s[(i >> shift) * ld + kb]
   long long ldsp, ldsq;
   int sp_shift, sq_shift;
@@ -118,6 +118,7 @@ struct Fp8Params {
   int relu;
   int fused;  // any of the three
   int vector_store, word_store;  // rows of C start on 16-byte boundaries, on 4-byte ones
+  int tma_store;                 // and end on 16-byte ones: a TMA store writes 16 bytes or none
   int vector_sp, vector_sq;  // so do those of the scales
   int splits;        // Fp8Tile: CTAs that share a tile's K
 };
@@ -628,7 +629,9 @@ struct Fp8Pair {
   }
 
   // This warp's accumulators to C: 32 rows of 128 columns, through blocks of shared memory: 16-byte units XORed with the row, the
-  // swizzle of the tensor map, and TMA stores, two under way; or rows by RowStore where TMA cannot address them.
+  // swizzle of the tensor map, and TMA stores, two under way; or rows by RowStore where TMA cannot address them or would write past
+  // their ends (8192 x 4095 x 4096 into rows of 4096 130 us; only the last columns of such rows by RowStore 126, which cost 8192 x 8192 x 128 with
+  // no such rows 29.5 for 28.5).
   __device__ static __forceinline__ void store(const Fp8Params& p, float (&acc)[128], int row0, int col0, uint8_t* blocks) {
     using Rows = RowStore<T, COLS_BLOCK>;
     static_assert(Rows::kBytes <= 8192, "a block of rows exceeds a warp's shared memory");
@@ -658,8 +661,8 @@ struct Fp8Pair {
 #pragma unroll
     for (int b = 0; b < 128 / COLS_BLOCK; ++b) {
       if (row0 >= p.rows_p || col0 + b * COLS_BLOCK >= p.rows_q) break;
-      uint8_t* block = blocks + (p.vector_store ? store_block(b) * 4096 : 0);
-      if (p.vector_store) {
+      uint8_t* block = blocks + (p.tma_store ? store_block(b) * 4096 : 0);
+      if (p.tma_store) {
         if (lane == 0) {
           if (stores_reading(b) == 0) {
             tma_store_wait_read<0>();
@@ -672,7 +675,7 @@ struct Fp8Pair {
       }
       if constexpr (!kVector) {
         const float* v = acc + b * COLS_BLOCK;
-        if (p.vector_store) {
+        if (p.tma_store) {
 #pragma unroll
           for (int u = 0; u < 8; ++u) *reinterpret_cast<uint4*>(block + lane * 128 + ((u ^ (lane & 7)) << 4)) = unit16<T>(v, u);
         } else {
@@ -680,8 +683,8 @@ struct Fp8Pair {
         }
       } else {
         const uint32_t x = lane >> 2, t = lane & 3;  // (row within eight, pair of columns within eight)
-        const uint32_t swizzle = !p.vector_store ? 0u : (sizeof(T) == 4 ? x ^ (t >> 1) : x) << 4, pitch = p.vector_store ? 128 : Rows::kPitch;
-        uint8_t* to = block + x * pitch + (sizeof(T) == 4 ? (t & 1) * 8 + (p.vector_store ? 0 : (t >> 1) * 16) : t * 4);
+        const uint32_t swizzle = !p.tma_store ? 0u : (sizeof(T) == 4 ? x ^ (t >> 1) : x) << 4, pitch = p.tma_store ? 128 : Rows::kPitch;
+        uint8_t* to = block + x * pitch + (sizeof(T) == 4 ? (t & 1) * 8 + (p.tma_store ? 0 : (t >> 1) * 16) : t * 4);
 #pragma unroll
         for (int r = 0; r < 4; ++r, to += 8 * pitch)
 #pragma unroll
@@ -695,7 +698,7 @@ struct Fp8Pair {
             }
           }
       }
-      if (p.vector_store) {
+      if (p.tma_store) {
         send(p, block, row0, col0 + b * COLS_BLOCK);
       } else {
         Rows::copy(p, block, row0, col0 + b * COLS_BLOCK);
@@ -1026,7 +1029,7 @@ int encode(EncodeFn fn, CUtensorMap* tm, uint64_t ptr, int k, int64_t ld, int ro
   return r == CUDA_SUCCESS ? 0 : fail(static_cast<int>(r), "cuTensorMapEncodeTiled failed");
 }
 
-// C, for stores of 128 bytes x 32 rows; what lies past it is not stored.
+// C, for stores of 128 bytes x 32 rows; rows past it are not stored, columns past it are where they share 16 bytes with one inside.
 int encode_c(EncodeFn fn, CUtensorMap* tm, uint64_t ptr, int dtype, int n, int64_t ld, int m) {
   const int eb = dtype == KCG_DTYPE_FLOAT32 ? 4 : 2;
   cuuint64_t gdim[2] = {static_cast<cuuint64_t>(n), static_cast<cuuint64_t>(m)};
@@ -1204,9 +1207,10 @@ extern "C" int kcg_matmul_fp8(int device, uint64_t stream, const kcg_fp8_product
   p.beta = a->beta, p.relu = a->relu, p.splits = plan.splits;
   p.vector_store = a->C % 16 == 0 && ldc * eb % 16 == 0;
   p.word_store = a->C % 4 == 0 && ldc * eb % 4 == 0;
+  p.tma_store = plan.pair && p.vector_store && static_cast<int64_t>(a->n) * eb % 16 == 0;
   p.vector_sp = reinterpret_cast<uint64_t>(p.sp) % 16 == 0 && p.ldsp % 4 == 0;
   p.vector_sq = reinterpret_cast<uint64_t>(p.sq) % 16 == 0 && p.ldsq % 4 == 0;
-  if (plan.pair && p.vector_store)
+  if (p.tma_store)
     if (int r = encode_c(enc, &p.tmC, a->C, a->dtype_c, a->n, ldc, a->m)) return r;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool vector = a->block_b == 1;
