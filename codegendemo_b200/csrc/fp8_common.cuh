@@ -129,8 +129,10 @@ __device__ __forceinline__ void store_piece(T* row, int c, int cols, const float
 }
 
 // ---- 8-bit blocks. Of a block with largest magnitude top: scale = max(top / largest 8-bit value, 2^-126), values
-// x * (1 / scale) rounded to nearest even. The lower bound keeps 1 / scale finite, also for a block of zeros. Magnitudes are compared
-// as integers, in which a NaN is the largest: it makes the block's scale, and with it every value of the block, a NaN.
+// x * (1 / scale), reciprocal and product rounded to fp32, then to nearest even. The lower bound keeps 1 / scale finite, also for a block of
+// zeros. Magnitudes are compared as integers, in which a NaN is the largest: it makes the block's scale, and with it every value of the block,
+// a NaN.
+
 // The larger magnitude of three values, a NaN if one of them is.
 __device__ __forceinline__ float abs_max3(float a, float b, float c) {
   float r;

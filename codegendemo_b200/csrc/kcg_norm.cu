@@ -5,8 +5,16 @@
 // (dh: the gradient that reaches h past the norm, along the residual stream.) Sums and products in fp32, one rounding at the end:
 // y comes from the unrounded sum h, which is rounded only where it is stored.
 //
+// A sum of squares past fp32's largest number makes r 0 (rows of 1.8e19 and more, a single value of that size), one below its smallest, with
+// eps = 0, infinite.
+//
 // Bound by HBM: a row is read once, into registers, and written once, by a warp (forward, up to 1024 values) or by CTAs that walk rows. Rows
-// that are no whole 16-byte pieces are read value by value, forward by a kernel of their own that reads them twice.
+// that are no whole 16-byte pieces are read value by value, forward by a kernel of their own. Read twice, the second time from a
+// cache: such rows of more than 16384 values, and h and dy of every row of more than 16384 in the gradient.
+//
+// Registers: the CTAs an SM were chosen for 16-bit rows. In fp32 with a residual, up to 16384 values, 72 to 160 bytes a thread are spilled, in
+// every type past 16384 values 60 to 950, and by the gradient 36 to 264 in fp32 up to 8192 values and 320 to 644 in every type from there to
+// 16384 (four pieces of h, dy, the weight and their shares of dw in 128 registers).
 #include <cuda_runtime.h>
 
 #include <cfloat>
@@ -489,7 +497,7 @@ int launch_norm(const NormArgs& a, bool vectors, int sms, cudaStream_t st) {
   return a.scales ? launch_norm<T, false, true>(a, vectors, sms, st) : launch_norm<T, false, false>(a, vectors, sms, st);
 }
 
-constexpr int kMaxWidth = 32768;  // a row in a CTA's registers, its share of dw in shared memory
+constexpr int kMaxWidth = 32768;  // (1024 threads hold four pieces each; a CTA's share of dw takes 128 KB of shared memory)
 
 // Threads of a CTA of the backward pass: two pieces each up to 8192 values a row, then four.
 int grad_threads(int width) {

@@ -15,7 +15,9 @@ A linear layer ``y = x w^T`` in 8 bits, and its gradients::
     dw = matmul_fp8(*quantize_fp8(dy, transposed=True), *quantize_fp8(x, transposed=True), out_dtype=torch.float32)
 
 All work on CUDA tensors of any device, on torch's current stream of that device; results come from torch's allocator. Matrices
-may be views with a row pitch (contiguous rows).
+are 2-D (tokens x width: a batch of sequences is viewed as its tokens) and may be views with a row pitch (contiguous rows). Like the
+other operators of this library these are no autograd functions: results carry no gradient, and a backward pass is made of the
+calls above.
 """
 import ctypes
 
@@ -103,9 +105,9 @@ def _sum_of(x, residual, residual_out):
 
 def rms_norm(x, weight, residual=None, eps=1e-6, out=None, residual_out=None):
     """``h / sqrt(mean(h^2) + eps) * weight`` row by row, with ``h = x + residual`` (or x): returns the norm, or (norm, h) with a
-    residual. Sums in fp32, each result rounded once (the norm is taken of the unrounded sum). ``x`` and ``residual`` are
-    rows x width, fp16, bf16 or fp32, ``weight`` width values of the same type. ``out`` and ``residual_out`` take the results;
-    each may be ``x`` or ``residual`` itself (not both the same one), other overlaps are not allowed."""
+    residual. Sums in fp32 (a row whose sum of squares passes 3.4e38 gives zeros), each result rounded once (the norm is taken of
+    the unrounded sum). ``x`` and ``residual`` are rows x width, fp16, bf16 or fp32, ``weight`` width values of the same type. ``out``
+    and ``residual_out`` take the results; each may be ``x`` or ``residual`` itself (not both the same one), other overlaps are not allowed."""
     if _warm and out is None and residual_out is None:
         results = _warm.rms_norm(x, weight, residual, eps)
         if results is not None:
@@ -180,7 +182,8 @@ def rms_norm_backward(dy, h, weight, eps=1e-6, dh=None):
 def quantize_fp8(x, rows=1, transposed=False, dtype=None):
     """(values, scales) of a matrix in blocks of ``rows`` (1 or 128) x 128 values: scale = max(largest magnitude / 448, 2^-126) (e5m2:
     57344), values x * (1 / scale): reciprocal and product rounded to fp32, then to the nearest 8-bit value, ties to even (x / scale may
-    give the neighbour where it lies within 2^-23 of itself of the middle between two). ``transposed``: of ``x.t()``, cut into blocks along what were x's rows.
+    give the neighbour where it lies within 2^-23 of itself of the middle between two). ``transposed``: of ``x.t()``, cut into blocks
+    along what were x's rows.
     ``dtype`` is float8_e4m3fn (default) or float8_e5m2. Scales are (row blocks) x ceil(columns / 128), fp32."""
     if _warm and dtype is None:
         results = _warm.quantize_fp8(x, rows, transposed)

@@ -238,7 +238,8 @@ int kcg_attention_status(int device, uint32_t out[4]);
  *
  * Root-mean-square norm: H = X + R, Y = H / sqrt(mean(H^2) + eps) * W, each row by itself. R = 0 (no residual): H = X, and H
  * must be 0 too. Y and H are rounded once; Y comes from the unrounded sum. H may be X or R, Y may be X or R if H is not. Rows
- * of up to 32768 values; whole 16-byte pieces (width a multiple of 8, aligned rows) are the fast case. */
+ * of up to 32768 values; whole 16-byte pieces (width a multiple of 8, aligned rows) are the fast case. Sums are taken in
+ * fp32: a row whose sum of squares passes 3.4e38 (a value of 1.8e19) gives zeros. */
 int kcg_rms_norm(int device, uint64_t stream, uint64_t X, int64_t ldx, uint64_t R, int64_t ldr, uint64_t W, uint64_t Y,
                  int64_t ldy, uint64_t H, int64_t ldh, int64_t rows, int width, float eps, int dtype);
 /* The same with Y as e4m3 values Q in blocks of 1 x 128 and their scales S, from the unrounded Y: the operands of a product, not
@@ -255,8 +256,8 @@ int kcg_rms_norm_backward(int device, uint64_t stream, uint64_t DY, int64_t lddy
                           uint64_t DH, int64_t lddh, uint64_t DX, int64_t lddx, uint64_t DW, uint64_t workspace,
                           int64_t workspace_bytes, int64_t rows, int width, float eps, int dtype);
 /* 8-bit values and scales of a matrix in blocks of block_rows (1 or 128) x 128; `transposed`: of its transpose, whose rows (cols
- * of them) are what is cut into blocks. `dtype8`: KCG_FP8_E4M3 or _E5M2. Rows of Q start on 16-byte boundaries, and a row's last
- * 16-byte piece is written whole. */
+ * of them) are what is cut into blocks. `dtype8`: KCG_FP8_E4M3 or _E5M2. Rows of Q start on 16-byte boundaries; what lies between
+ * a row's last value and the next such boundary may be written over, in whole or in part. */
 int kcg_quantize_fp8(int device, uint64_t stream, uint64_t X, int64_t ldx, uint64_t Q, int64_t ldq, uint64_t S, int64_t rows,
                      int cols, int block_rows, int transposed, int dtype, int dtype8);
 /* C = act(sum over blocks of scale_a * scale_b * (A * B^T of the block) + beta * C + bias[col]): A is M x K in blocks of 1 x 128,
