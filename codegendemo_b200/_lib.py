@@ -27,6 +27,7 @@ EXPORTED_SYMBOLS = (
     "kcg_attention_fwd", "kcg_attention_status",
     "kcg_rms_norm", "kcg_rms_norm_fp8", "kcg_rms_norm_backward_workspace", "kcg_rms_norm_backward", "kcg_quantize_fp8",
     "kcg_matmul_fp8", "kcg_matmul_fp8_status",
+    "kcg_append_kv", "kcg_attention_paged_workspace", "kcg_attention_paged", "kcg_attention_paged_status",
     "kcg_launch_gemm_allgather", "kcg_peer_alloc", "kcg_peer_open", "kcg_peer_close",
     "kcg_peer_free", "kcg_check_status", "kcg_matmul_host", "kcg_launch_count", "kcg_trim", "kcg_shutdown",
     "kcg_last_error", "kcg_version", "kcg_gemm_bf16_splitk_noalloc",
@@ -105,6 +106,28 @@ class Fp8Product(ctypes.Structure):
                [(name, ctypes.c_int64) for name in ("lda", "ld_scale_a", "ldb", "ld_scale_b", "ldc")] + \
                [(name, ctypes.c_int32) for name in ("m", "n", "k", "block_b", "dtype_a", "dtype_b", "dtype_c")] + \
                [("beta", ctypes.c_float), ("relu", ctypes.c_int32), ("reserved", ctypes.c_int32 * 3)]
+
+
+class PagedCache(ctypes.Structure):
+    """``kcg_paged_cache``."""
+    _fields_ = [("K", ctypes.c_uint64), ("V", ctypes.c_uint64), ("k_stride", ctypes.c_int64 * 3), ("v_stride", ctypes.c_int64 * 3)] + \
+               [(name, ctypes.c_uint64) for name in ("table", "lengths", "starts")] + [("table_ld", ctypes.c_int64)] + \
+               [(name, ctypes.c_int32) for name in ("pages", "page", "width", "sequences", "kv_heads", "d", "dtype", "reserved")]
+
+
+class NewRows(ctypes.Structure):
+    """``kcg_new_rows``."""
+    _fields_ = [(name, ctypes.c_uint64) for name in ("K", "V", "Q", "QO")] + \
+               [(name, ctypes.c_int64 * 2) for name in ("k_stride", "v_stride", "q_stride", "qo_stride")] + \
+               [(name, ctypes.c_uint64) for name in ("cos", "sin", "positions")] + [("angles", ctypes.c_int64)] + \
+               [(name, ctypes.c_int32) for name in ("rows", "q_heads", "rotary", "interleaved")]
+
+
+class PagedQuery(ctypes.Structure):
+    """``kcg_paged_query``."""
+    _fields_ = [("Q", ctypes.c_uint64), ("O", ctypes.c_uint64), ("q_stride", ctypes.c_int64 * 2), ("o_stride", ctypes.c_int64 * 2),
+                ("workspace", ctypes.c_uint64), ("workspace_bytes", ctypes.c_int64)] + \
+               [(name, ctypes.c_int32) for name in ("rows", "q_heads", "window", "sinks")] + [("scale", ctypes.c_float), ("reserved", ctypes.c_int32)]
 
 
 class DeviceProps(ctypes.Structure):
@@ -188,8 +211,14 @@ def get_lib() -> ctypes.CDLL:
     lib.kcg_quantize_fp8.argtypes = [i32, u64, u64, i64, u64, i64, u64, i64, i32, i32, i32, i32, i32]
     lib.kcg_matmul_fp8.argtypes = [i32, u64, ctypes.POINTER(Fp8Product)]
     lib.kcg_matmul_fp8_status.argtypes = [i32, ctypes.POINTER(ctypes.c_uint32)]
+    cache_t, query_t = ctypes.POINTER(PagedCache), ctypes.POINTER(PagedQuery)
+    lib.kcg_append_kv.argtypes = [i32, u64, cache_t, ctypes.POINTER(NewRows)]
+    lib.kcg_attention_paged_workspace.argtypes = [i32, cache_t, query_t]
+    lib.kcg_attention_paged_workspace.restype = i64
+    lib.kcg_attention_paged.argtypes = [i32, u64, cache_t, query_t]
+    lib.kcg_attention_paged_status.argtypes = [i32, ctypes.POINTER(ctypes.c_uint32)]
     for name in ("kcg_rms_norm", "kcg_rms_norm_fp8", "kcg_rms_norm_backward", "kcg_quantize_fp8", "kcg_matmul_fp8",
-                 "kcg_matmul_fp8_status"):
+                 "kcg_matmul_fp8_status", "kcg_append_kv", "kcg_attention_paged", "kcg_attention_paged_status"):
         getattr(lib, name).restype = i32
     lib.kcg_peer_alloc.argtypes = [ctypes.c_int, u64, ctypes.POINTER(u64), ctypes.c_char_p]
     lib.kcg_peer_open.argtypes = [ctypes.c_int, ctypes.c_char_p, ctypes.POINTER(u64)]

@@ -96,10 +96,10 @@ def build_library(force: bool = False) -> str:
     deps = srcs + [os.path.join(kdir, f) for f in sorted(os.listdir(kdir))] + [
         os.path.join(os.path.dirname(HERE), "include", "kcg_b200.h")]
     # device code linked into the library itself: the allocation-free split-K entry, the row softmax, the fused attention
-    # the split of fp32 operands, and the 8-bit linear layer
+    # the split of fp32 operands, the 8-bit linear layer, and the paged cache
     extra = [os.path.join(HERE, "csrc", f) for f in ("kcg_noalloc.cu", "kcg_softmax.cu", "kcg_attention.cu", "kcg_f32split.cu",
-                                                     "kcg_norm.cu", "kcg_quantize.cu", "kcg_fp8.cu")]
-    deps += extra + [os.path.join(HERE, "csrc", "fp8_common.cuh")]
+                                                     "kcg_norm.cu", "kcg_quantize.cu", "kcg_fp8.cu", "kcg_paged.cu")]
+    deps += extra + [os.path.join(HERE, "csrc", f) for f in ("fp8_common.cuh", "paged.cuh")]
     if not force and _newer(out, deps):
         return out
     nvcc = os.path.join(CUDA_HOME, "bin", "nvcc")

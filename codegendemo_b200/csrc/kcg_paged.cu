@@ -1,0 +1,271 @@
+// The paged cache of keys and values: storing a step's rows in it, with the rotation by their positions on the way.
+//
+// Bound by HBM: each row's heads are read once and written once (a prompt), or by the latency of three dependent loads (the row's
+// sequence, its length, its page) in a decode step. A warp takes one row and four heads (d = 64: eight) at a time, a thread two
+// 16-byte pieces whose values turn together, so that it reads its angles once for all heads and needs no other thread's values;
+// where there are few rows, several warps share one.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/kcg_b200.h"
+#include "fp8_common.cuh"
+#include "kernels/ptx_sm100.cuh"
+#include "paged.cuh"
+
+namespace {
+
+using namespace kcg;
+using namespace kcg8;
+using namespace kcgp;
+
+struct AppendArgs {
+  Sequences seq;
+  const void *k, *v, *q;
+  void *k_cache, *v_cache, *qo;
+  long long k_row, k_head, v_row, v_head, q_row, q_head, qo_row, qo_head;
+  long long kc[3], vc[3];  // strides of the caches
+  const float *cos, *sin;
+  const int32_t* positions;
+  long long angles;
+  int q_heads, kv_heads, rotary, warps_log2;  // warps that share a row
+};
+
+constexpr int kAppendWarps = 8;
+
+// A thread's piece pair u of a head: halves rotary / 2 values apart (the pair turns together), neighbouring pieces when interleaved
+// or past the rotated part.
+template <typename T, int kD, bool kInterleaved>
+__global__ void __launch_bounds__(kAppendWarps * 32) append_kv_kernel(const AppendArgs a) {
+  constexpr int UNITS = kD / 16, HEADS = 32 / UNITS;  // piece pairs of a head, heads of a warp's step
+  griddep_launch_dependents();
+  griddep_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row = (static_cast<int>(blockIdx.x) << (3 - a.warps_log2)) + (warp >> a.warps_log2);
+  if (row >= a.seq.rows) return;
+  const int u = lane % UNITS;
+  const bool turned = u * 16 < a.rotary;
+  const int at0 = turned && !kInterleaved ? u * 8 : u * 16;
+  const int at1 = turned && !kInterleaved ? at0 + a.rotary / 2 : at0 + 8;
+
+  const int b = sequence_of(a.seq, row);
+  if (b < 0) return;
+  const int n = a.seq.start(b + 1) - a.seq.start(b);
+  const int position = a.seq.lengths[b] - n + (row - a.seq.start(b));
+  const int page = position >= 0 && position < a.seq.capacity() ? a.seq.page_of(b, position) : -1;
+  float c[8], s[8];
+  if (turned) {
+    const long long p = a.positions ? a.positions[row] : position;
+    if (p >= 0 && p < a.angles) {
+      const long long at = p * (a.rotary / 2) + u * 8;
+      load8(a.cos + at, c), load8(a.sin + at, s);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c[i] = s[i] = __int_as_float(0x7fffffff);
+    }
+  }
+  const long long slot = position & ((1 << a.seq.page_log2) - 1);
+  const int heads = a.q_heads + 2 * a.kv_heads;
+#pragma unroll 4
+  for (int h = ((warp & ((1 << a.warps_log2) - 1)) * HEADS) + lane / UNITS; h < heads; h += HEADS << a.warps_log2) {
+    const T* from;
+    T* to;
+    bool turn = turned;
+    if (h < a.q_heads) {
+      from = static_cast<const T*>(a.q) + row * a.q_row + h * a.q_head;
+      to = static_cast<T*>(a.qo) + row * a.qo_row + h * a.qo_head;
+    } else if (h < a.q_heads + a.kv_heads) {
+      const int kh = h - a.q_heads;
+      from = static_cast<const T*>(a.k) + row * a.k_row + kh * a.k_head;
+      to = page < 0 ? nullptr : static_cast<T*>(a.k_cache) + page * a.kc[0] + kh * a.kc[1] + slot * a.kc[2];
+    } else {
+      const int vh = h - a.q_heads - a.kv_heads;
+      from = static_cast<const T*>(a.v) + row * a.v_row + vh * a.v_head;
+      to = page < 0 ? nullptr : static_cast<T*>(a.v_cache) + page * a.vc[0] + vh * a.vc[1] + slot * a.vc[2];
+      turn = false;
+    }
+    if (!to) continue;
+    Raw8<T> x, y;
+    x.load(from + at0), y.load(from + at1);
+    if (position < 0) {
+      x.zero(), y.zero();  // (only queries come here)
+    } else if (turn) {
+      float p[8], q[8], e[8], f[8];
+      x.values(p), y.values(q);
+      if constexpr (kInterleaved) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          e[2 * i] = p[2 * i] * c[i] - p[2 * i + 1] * s[i], e[2 * i + 1] = p[2 * i + 1] * c[i] + p[2 * i] * s[i];
+          f[2 * i] = q[2 * i] * c[i + 4] - q[2 * i + 1] * s[i + 4], f[2 * i + 1] = q[2 * i + 1] * c[i + 4] + q[2 * i] * s[i + 4];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = p[i] * c[i] - q[i] * s[i], f[i] = q[i] * c[i] + p[i] * s[i];
+      }
+      float2 ev[4], fv[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ev[i] = make_float2(e[2 * i], e[2 * i + 1]), fv[i] = make_float2(f[2 * i], f[2 * i + 1]);
+      store8(to + at0, ev), store8(to + at1, fv);
+      continue;
+    }
+    *reinterpret_cast<uint4*>(to + at0) = x.v, *reinterpret_cast<uint4*>(to + at1) = y.v;
+  }
+}
+
+template <typename T>
+int append(Launch& launch, const AppendArgs& a, int d, bool interleaved) {
+  if (d == 128)
+    return interleaved ? launch(append_kv_kernel<T, 128, true>, "append_kv launch", a) : launch(append_kv_kernel<T, 128, false>, "append_kv launch", a);
+  return interleaved ? launch(append_kv_kernel<T, 64, true>, "append_kv launch", a) : launch(append_kv_kernel<T, 64, false>, "append_kv launch", a);
+}
+
+// ---------------------------------------------------------------------------------------------------- attention
+struct PagedArgs {
+  Sequences seq;
+  const void *k, *v, *q;
+  void* o;
+  long long q_row, q_head, o_row, o_head;
+  long long kc[3], vc[3];
+  int q_heads, kv_heads, window, sinks;
+  float scale_log2;
+};
+
+// A warp a row and query head, key after key.
+template <typename T, int kD>
+__global__ void __launch_bounds__(128) attention_paged_kernel(const PagedArgs a) {
+  griddep_launch_dependents();
+  griddep_wait();
+  const int lane = threadIdx.x & 31;
+  const long long unit = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  const int row = static_cast<int>(unit / a.q_heads), head = static_cast<int>(unit % a.q_heads);
+  if (row >= a.seq.rows) return;
+  const int b = sequence_of(a.seq, row);
+  if (b < 0) return;
+  constexpr int PER = kD / 32;
+  const int length = a.seq.lengths[b];
+  const int n = a.seq.start(b + 1) - a.seq.start(b);
+  const int position = length - n + (row - a.seq.start(b));
+  const int keys = min(a.seq.keys(length), position + 1);
+  const T* q = static_cast<const T*>(a.q) + row * a.q_row + head * a.q_head + lane * PER;
+  float qv[PER], acc[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) qv[i] = to_f32(q[i]) * a.scale_log2, acc[i] = 0.f;
+  const int kh = head / (a.q_heads / a.kv_heads);
+  float m = -INFINITY, sum = 0.f;
+  for (int j = 0; j < keys; ++j) {
+    if (a.window > 0 && position - j >= a.window && j >= a.sinks) {
+      j = position - a.window;  // the next key in sight comes behind it
+      continue;
+    }
+    const int page = a.seq.page_of(b, j);
+    const long long slot = j & ((1 << a.seq.page_log2) - 1);
+    float s = 0.f, v[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int c = lane * PER + i;
+      s += page < 0 ? 0.f : qv[i] * to_f32(static_cast<const T*>(a.k)[page * a.kc[0] + kh * a.kc[1] + slot * a.kc[2] + c]);
+      v[i] = page < 0 ? 0.f : to_f32(static_cast<const T*>(a.v)[page * a.vc[0] + kh * a.vc[1] + slot * a.vc[2] + c]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    const float top = fmaxf(m, s), base = top == -INFINITY ? 0.f : top;
+    const float alpha = exp2f(m - base), w = exp2f(s - base);
+    m = top, sum = sum * alpha + w;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) acc[i] = acc[i] * alpha + w * v[i];
+  }
+  T* o = static_cast<T*>(a.o) + row * a.o_row + head * a.o_head + lane * PER;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) o[i] = from_f32<T>(sum == 0.f ? 0.f : acc[i] / sum);
+}
+
+int check_query(const kcg_paged_cache* c, const kcg_paged_query* q) {
+  if (!q) return fail(KCG_E_BAD_ARG, "attention_paged: null pointer");
+  if (int r = check_cache(c, q->rows)) return r;
+  if (q->rows > 0 && (!q->Q || !q->O)) return fail(KCG_E_BAD_ARG, "attention_paged: null pointer");
+  if (q->Q % 16 || q->O % 16 || q->workspace % 16) return fail(KCG_E_BAD_ARG, "attention_paged: operands must start on 16-byte boundaries");
+  if (!aligned_rows(q->q_stride, 2, c->d) || !aligned_rows(q->o_stride, 2, c->d))
+    return fail(KCG_E_BAD_ARG, "attention_paged: strides are multiples of 8 values, at least a head's");
+  if (q->q_heads < 1 || q->q_heads % c->kv_heads || q->q_heads / c->kv_heads > 64)
+    return fail(KCG_E_BAD_ARG, "attention_paged: 1 to 64 query heads share a key head");
+  if (q->window < 0 || q->sinks < 0) return fail(KCG_E_BAD_ARG, "attention_paged: negative window or sinks");
+  if (!(q->scale > 0.f) || !(q->scale <= 3e38f)) return fail(KCG_E_BAD_ARG, "scale must be positive and finite");
+  if (static_cast<long long>(q->rows) * q->q_heads > 0x7fffff00LL) return fail(KCG_E_TOO_LARGE, "attention_paged: too many rows");
+  return 0;
+}
+
+}  // namespace
+
+extern "C" int kcg_append_kv(int device, uint64_t stream, const kcg_paged_cache* c, const kcg_new_rows* r) {
+  if (!r) return fail(KCG_E_BAD_ARG, "append_kv: null pointer");
+  if (int e = check_cache(c, r->rows)) return e;
+  const bool queries = r->Q != 0;
+  if (r->rows > 0 && (!r->K || !r->V)) return fail(KCG_E_BAD_ARG, "append_kv: null pointer");
+  if (queries != (r->QO != 0) || (queries && (r->q_heads < 1 || r->q_heads > 65535))) return fail(KCG_E_BAD_ARG, "append_kv: queries, their heads and their results go together");
+  if (!aligned_rows(r->k_stride, 2, c->d) || !aligned_rows(r->v_stride, 2, c->d) ||
+      (queries && (!aligned_rows(r->q_stride, 2, c->d) || !aligned_rows(r->qo_stride, 2, c->d))))
+    return fail(KCG_E_BAD_ARG, "append_kv: strides are multiples of 8 values, at least a head's");
+  if (r->rotary < 0 || r->rotary > c->d || r->rotary % 16) return fail(KCG_E_BAD_ARG, "append_kv: a multiple of 16 values is turned, at most a head's");
+  if (r->rotary > 0 && (!r->cos || !r->sin || r->angles < 1)) return fail(KCG_E_BAD_ARG, "append_kv: no angles");
+  if (r->K % 16 || r->V % 16 || r->Q % 16 || r->QO % 16 || r->cos % 16 || r->sin % 16 || r->positions % 4)
+    return fail(KCG_E_BAD_ARG, "append_kv: operands must start on 16-byte boundaries");
+  if (r->rows > 0x7fffff00) return fail(KCG_E_TOO_LARGE, "append_kv: too many rows");
+  if (r->rows == 0) return 0;
+  DeviceGuard guard;
+  if (cudaError_t e = guard.enter(device)) return cuda_fail(e, "cudaSetDevice");
+  int sms;
+  if (int e = sm_count(device, &sms)) return e;
+  AppendArgs a{};
+  a.seq = sequences_of(c, r->rows);
+  a.k = reinterpret_cast<const void*>(r->K), a.v = reinterpret_cast<const void*>(r->V), a.q = reinterpret_cast<const void*>(r->Q);
+  a.k_cache = reinterpret_cast<void*>(c->K), a.v_cache = reinterpret_cast<void*>(c->V), a.qo = reinterpret_cast<void*>(r->QO);
+  a.k_row = r->k_stride[0], a.k_head = r->k_stride[1], a.v_row = r->v_stride[0], a.v_head = r->v_stride[1];
+  a.q_row = r->q_stride[0], a.q_head = r->q_stride[1], a.qo_row = r->qo_stride[0], a.qo_head = r->qo_stride[1];
+  for (int i = 0; i < 3; ++i) a.kc[i] = c->k_stride[i], a.vc[i] = c->v_stride[i];
+  a.cos = reinterpret_cast<const float*>(r->cos), a.sin = reinterpret_cast<const float*>(r->sin);
+  a.positions = reinterpret_cast<const int32_t*>(r->positions);
+  a.angles = r->angles;
+  a.q_heads = queries ? r->q_heads : 0, a.kv_heads = c->kv_heads, a.rotary = r->rotary;
+  // Warps that share a row: as many as leave the GPU some 16 warps an SM, and each something to do.
+  const int steps = ((a.q_heads + 2 * a.kv_heads) * (c->d / 16) + 31) / 32;
+  while (a.warps_log2 < 3 && (r->rows << a.warps_log2) < sms * 16 && (1 << a.warps_log2) < steps) ++a.warps_log2;
+  const int per = kAppendWarps >> a.warps_log2;
+  Launch launch(reinterpret_cast<cudaStream_t>(stream));
+  launch.shape(static_cast<unsigned>((static_cast<long long>(r->rows) + per - 1) / per), kAppendWarps * 32);
+  return c->dtype == KCG_DTYPE_BFLOAT16 ? append<__nv_bfloat16>(launch, a, c->d, r->interleaved != 0) : append<__half>(launch, a, c->d, r->interleaved != 0);
+}
+
+extern "C" int64_t kcg_attention_paged_workspace(int device, const kcg_paged_cache* c, const kcg_paged_query* q) {
+  (void)device;
+  if (int r = check_query(c, q)) return r;
+  return 0;
+}
+
+extern "C" int kcg_attention_paged(int device, uint64_t stream, const kcg_paged_cache* c, const kcg_paged_query* q) {
+  if (int r = check_query(c, q)) return r;
+  if (q->rows == 0) return 0;
+  DeviceGuard guard;
+  if (cudaError_t e = guard.enter(device)) return cuda_fail(e, "cudaSetDevice");
+  PagedArgs a{};
+  a.seq = sequences_of(c, q->rows);
+  a.k = reinterpret_cast<const void*>(c->K), a.v = reinterpret_cast<const void*>(c->V), a.q = reinterpret_cast<const void*>(q->Q);
+  a.o = reinterpret_cast<void*>(q->O);
+  a.q_row = q->q_stride[0], a.q_head = q->q_stride[1], a.o_row = q->o_stride[0], a.o_head = q->o_stride[1];
+  for (int i = 0; i < 3; ++i) a.kc[i] = c->k_stride[i], a.vc[i] = c->v_stride[i];
+  a.q_heads = q->q_heads, a.kv_heads = c->kv_heads, a.window = q->window, a.sinks = q->sinks;
+  a.scale_log2 = q->scale * 1.4426950408889634f;
+  Launch launch(reinterpret_cast<cudaStream_t>(stream));
+  launch.shape(static_cast<unsigned>((static_cast<long long>(q->rows) * q->q_heads + 3) / 4), 128);
+  if (c->dtype == KCG_DTYPE_BFLOAT16)
+    return c->d == 128 ? launch(attention_paged_kernel<__nv_bfloat16, 128>, "attention_paged launch", a) : launch(attention_paged_kernel<__nv_bfloat16, 64>, "attention_paged launch", a);
+  return c->d == 128 ? launch(attention_paged_kernel<__half, 128>, "attention_paged launch", a) : launch(attention_paged_kernel<__half, 64>, "attention_paged launch", a);
+}
+
+extern "C" int kcg_attention_paged_status(int device, uint32_t out[4]) {
+  if (!out) return fail(KCG_E_BAD_ARG, "null argument");
+  DeviceGuard guard;
+  if (cudaError_t e = guard.enter(device)) return cuda_fail(e, "cudaSetDevice");
+  if (cudaError_t e = cudaDeviceSynchronize()) return cuda_fail(e, "cudaDeviceSynchronize");
+  for (int i = 0; i < 4; ++i) out[i] = 0u;
+  return 0;
+}

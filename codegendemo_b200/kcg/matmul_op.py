@@ -11,6 +11,7 @@ from codegendemo_b200.kcg.Operators.matmul import KernelArgMatmul
 from codegendemo_b200.kcg.Utils import DeviceInfo, EnumKernelDType, FromTorchType
 from codegendemo_b200.kcg.fp8_op import (matmul_fp8, matmul_fp8_status, quantize_fp8, rms_norm, rms_norm_backward,  # noqa: F401
                                          rms_norm_fp8)
+from codegendemo_b200.kcg.paged_op import append_kv, attention_paged, attention_paged_status, rotary_table  # noqa: F401
 
 
 def default_config(M: int, N: int, K: int, dtype: EnumKernelDType, out_dtype=None, **keys) -> KernelArgMatmul:

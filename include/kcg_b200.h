@@ -280,6 +280,64 @@ int kcg_matmul_fp8(int device, uint64_t stream, const kcg_fp8_product* product);
 /* As kcg_attention_status, for kcg_matmul_fp8. */
 int kcg_matmul_fp8_status(int device, uint32_t out[4]);
 
+/* ---- attention over a paged cache --------------------------------------------------------
+ * What a server that generates text does in each layer of each step: keys and values of the step's rows go into the pages of
+ * their sequences, queries and keys turned by their positions on the way (kcg_append_kv), and the rows attend over what the
+ * pages hold (kcg_attention_paged). No counterpart in the reference (see the note on kcg_softmax_rows). fp16 or bf16, head
+ * dimension 64 or 128.
+ *
+ * A cache is K and V, each pages x heads x page x d with any strides between the heads' rows of d contiguous values (in elements,
+ * multiples of 8; memory on 16-byte boundaries), page a power of two of at least 8. Position p of sequence b lies in page
+ * table[b * table_ld + p / page], at p % page. lengths[b] counts a sequence's tokens, those of the step among them; its rows of
+ * the step are starts[b] to starts[b + 1] - 1, or (starts = 0) as many as every other's, and they are its last tokens: row i of n
+ * has position lengths[b] - n + i. table, lengths, starts (int32, on the device) are read when the work runs. What they
+ * may say, whatever it is, is not read or written outside of the memory described here: a length beyond the table's width counts as far
+ * as the table goes, a page that does not exist (a number below 0 or not below `pages`) reads as zeros and is not written, rows at or
+ * behind `rows` and those of negative position (a length of 0: an empty place of the batch) have no key. */
+typedef struct kcg_paged_cache {
+  uint64_t K, V;
+  int64_t k_stride[3], v_stride[3]; /* of a page, a head, a token */
+  uint64_t table, lengths, starts;
+  int64_t table_ld;
+  int32_t pages, page, width;       /* width: of the table */
+  int32_t sequences, kv_heads, d, dtype;
+  int32_t reserved;
+} kcg_paged_cache;
+/* The step's rows: K and V rows x kv_heads x d (strides of a row and of a head, as above), and, if Q is not 0, the queries, rows
+ * x q_heads x d, whose turned rows go to QO (which may be Q). cos and sin: fp32, angles x (rotary / 2), contiguous, 16-byte aligned,
+ * of position p in row p (or of positions[row], int32, if positions is not 0); the first `rotary` values of a head (a
+ * multiple of 16, at most d) are turned, in pairs rotary / 2 apart or (interleaved) of neighbours: (x, y) becomes
+ * (x cos - y sin, y cos + x sin), each rounded once, the rest stays; rotary = 0: nothing is turned. A position that has no angles
+ * gives NaN. Rows without a place in the cache are not stored; QO is zeros where a row's position in the cache is negative, and left as it
+ * was behind the last sequence's rows. */
+typedef struct kcg_new_rows {
+  uint64_t K, V, Q, QO;
+  int64_t k_stride[2], v_stride[2], q_stride[2], qo_stride[2];
+  uint64_t cos, sin, positions;
+  int64_t angles;
+  int32_t rows, q_heads, rotary, interleaved;
+} kcg_new_rows;
+int kcg_append_kv(int device, uint64_t stream, const kcg_paged_cache* cache, const kcg_new_rows* rows);
+/* O = sum over keys of softmax(scale * q k^T) v, row by row: the query heads q_heads / kv_heads at a time share a key head; a row
+ * at position p sees the keys of its sequence up to p, of those (window > 0) the last `window` and the first `sinks`. A row that sees none is zeros;
+ * rows behind the last sequence's are left as they were. Values of keys that no row of the sequence sees may be anything, NaN
+ * too; those of keys that some row sees have to be finite. Q and O: rows x q_heads x d, strides as above. scale positive. `workspace`: device memory, 16-byte
+ * aligned, as many bytes as the function below says for the same cache and rows (0: none needed), free again when the call's work is done. */
+typedef struct kcg_paged_query {
+  uint64_t Q, O;
+  int64_t q_stride[2], o_stride[2];
+  uint64_t workspace;
+  int64_t workspace_bytes;
+  int32_t rows, q_heads;
+  int32_t window, sinks;
+  float scale;
+  int32_t reserved;
+} kcg_paged_query;
+int64_t kcg_attention_paged_workspace(int device, const kcg_paged_cache* cache, const kcg_paged_query* query);
+int kcg_attention_paged(int device, uint64_t stream, const kcg_paged_cache* cache, const kcg_paged_query* query);
+/* As kcg_attention_status, for kcg_attention_paged. */
+int kcg_attention_paged_status(int device, uint32_t out[4]);
+
 /* ---- M-sharded product with the all-gather of C fused into the kernel ---------------
  * No counterpart in the reference (it has no multi-GPU code). Rank r of G computes rows
  * [r*M/G, (r+1)*M/G) of C with the same cubin as kcg_launch_gemm; `C` is the address of that slab
