@@ -4,11 +4,14 @@
 // sequence, its length, its page) in a decode step. A warp takes one row and four heads (d = 64: eight) at a time, a thread two
 // 16-byte pieces whose values turn together, so that it reads its angles once for all heads and needs no other thread's values;
 // where there are few rows, several warps share one.
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <mutex>
 
 #include "../../include/kcg_b200.h"
+#include "attn_common.cuh"
 #include "fp8_common.cuh"
 #include "kernels/ptx_sm100.cuh"
 #include "paged.cuh"
@@ -130,6 +133,11 @@ struct PagedArgs {
   float scale_log2;
 };
 
+__device__ unsigned int g_paged_status[4];  // {code, block, detail, detail}; 0 = no wait ran out
+enum : uint32_t { PAGED_TIMEOUT_LOADS = 1, PAGED_TIMEOUT_ATTENTION = 2 };
+
+#include "paged_tokens.cuh"
+
 // A warp a row and query head, key after key.
 template <typename T, int kD>
 __global__ void __launch_bounds__(128) attention_paged_kernel(const PagedArgs a) {
@@ -194,6 +202,98 @@ int check_query(const kcg_paged_cache* c, const kcg_paged_query* q) {
   return 0;
 }
 
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+std::mutex g_mutex;
+
+int encoder(EncodeFn* out) {
+  static EncodeFn known = nullptr;
+  std::lock_guard<std::mutex> lock(g_mutex);
+  if (!known) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found);
+    if (e != cudaSuccess || found != cudaDriverEntryPointSuccess || !fn) {
+      cudaGetLastError();
+      return fail(KCG_E_NO_DRIVER, "cuTensorMapEncodeTiled not available from the driver");
+    }
+    known = reinterpret_cast<EncodeFn>(fn);
+  }
+  *out = known;
+  return 0;
+}
+
+// {d, token of a page, head, page} view of a cache; boxes of 64 values x `box_rows` tokens of one head and page. What is outside reads as zero.
+int encode_cache(EncodeFn encode, CUtensorMap* tm, const kcg_paged_cache* c, uint64_t ptr, const int64_t* stride, int box_rows) {
+  cuuint64_t dim[4] = {static_cast<cuuint64_t>(c->d), static_cast<cuuint64_t>(c->page), static_cast<cuuint64_t>(c->kv_heads), static_cast<cuuint64_t>(c->pages)};
+  cuuint64_t step[3] = {static_cast<cuuint64_t>(stride[2]) * 2, static_cast<cuuint64_t>(stride[1]) * 2, static_cast<cuuint64_t>(stride[0]) * 2};
+  cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), 1, 1}, one[4] = {1, 1, 1, 1};
+  const CUresult r = encode(tm, c->dtype == KCG_DTYPE_BFLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                            reinterpret_cast<void*>(ptr), dim, step, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : fail(static_cast<int>(r), "cuTensorMapEncodeTiled failed");
+}
+
+// Dynamic shared memory of a kernel, opted in to once on each device.
+template <auto kKernel>
+int opt_in(int device, int bytes) {
+  static std::atomic<unsigned long long> done{0};
+  if (done.load() >> device & 1ull) return 0;
+  const cudaError_t e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(MaxDynamicSharedMemorySize)");
+  done.fetch_or(1ull << device);
+  return 0;
+}
+
+// Rows that share a key head, where every sequence has as many new tokens; those of up to 64 go by tokens (paged_tokens.cuh).
+int shared_rows(const kcg_paged_cache* c, const kcg_paged_query* q) {
+  if (c->starts) return 0;
+  const long long n = static_cast<long long>(q->rows / c->sequences) * (q->q_heads / c->kv_heads);
+  return n <= 64 ? static_cast<int>(n) : 0;
+}
+
+int64_t tokens_workspace(int sms, int rows, int d) { return 2ll * sms * (2ll * rows * (d + 2) * 4 + 16); }
+
+template <int kD, bool kBf16, int kRowGroups>
+int launch_tokens(int device, int sms, cudaStream_t st, const kcg_paged_cache* c, const TokensArgs& p) {
+  using Kern = AttnTokens<kD, kBf16, kRowGroups>;
+  if (int r = opt_in<attention_tokens_kernel<kD, kBf16, kRowGroups>>(device, Kern::SMEM_BYTES)) return r;
+  Launch launch(st);
+  launch.shape(2 * sms, Kern::NUM_THREADS, Kern::SMEM_BYTES);
+  if (int r = launch(attention_tokens_kernel<kD, kBf16, kRowGroups>, "attention_paged launch", p)) return r;
+  launch.shape(2 * sms, 256);
+  return launch(attention_tokens_join_kernel<kD, kBf16>, "attention_paged join launch", p, 2 * sms);
+}
+
+template <int kRowGroups>
+int launch_tokens_of(int device, int sms, cudaStream_t st, const kcg_paged_cache* c, const TokensArgs& p) {
+  if (c->d == 128)
+    return c->dtype == KCG_DTYPE_BFLOAT16 ? launch_tokens<128, true, kRowGroups>(device, sms, st, c, p) : launch_tokens<128, false, kRowGroups>(device, sms, st, c, p);
+  return c->dtype == KCG_DTYPE_BFLOAT16 ? launch_tokens<64, true, kRowGroups>(device, sms, st, c, p) : launch_tokens<64, false, kRowGroups>(device, sms, st, c, p);
+}
+
+int attention_tokens(int device, cudaStream_t st, const kcg_paged_cache* c, const kcg_paged_query* q, int rows) {
+  int sms;
+  if (int r = sm_count(device, &sms)) return r;
+  if (!q->workspace || q->workspace_bytes < tokens_workspace(sms, rows, c->d)) return fail(KCG_E_BAD_ARG, "attention_paged: workspace too small");
+  EncodeFn encode;
+  if (int r = encoder(&encode)) return r;
+  TokensArgs p{};
+  const int box = c->page < 64 ? c->page : 64;
+  if (int r = encode_cache(encode, &p.tmK, c, c->K, c->k_stride, box)) return r;
+  if (int r = encode_cache(encode, &p.tmV, c, c->V, c->v_stride, box)) return r;
+  p.seq = sequences_of(c, q->rows);
+  p.q = reinterpret_cast<const void*>(q->Q), p.o = reinterpret_cast<void*>(q->O);
+  p.q_row = q->q_stride[0], p.q_head = q->q_stride[1], p.o_row = q->o_stride[0], p.o_head = q->o_stride[1];
+  p.parts = reinterpret_cast<float*>(q->workspace);
+  p.kv_heads = c->kv_heads, p.group = q->q_heads / c->kv_heads, p.window = q->window, p.sinks = q->sinks;
+  while ((1 << p.box_log2) < box) ++p.box_log2;
+  p.scale_log2 = q->scale * 1.4426950408889634f;
+  if (rows <= 16) return launch_tokens_of<1>(device, sms, st, c, p);
+  if (rows <= 32) return launch_tokens_of<2>(device, sms, st, c, p);
+  return launch_tokens_of<4>(device, sms, st, c, p);
+}
+
 }  // namespace
 
 extern "C" int kcg_append_kv(int device, uint64_t stream, const kcg_paged_cache* c, const kcg_new_rows* r) {
@@ -236,9 +336,12 @@ extern "C" int kcg_append_kv(int device, uint64_t stream, const kcg_paged_cache*
 }
 
 extern "C" int64_t kcg_attention_paged_workspace(int device, const kcg_paged_cache* c, const kcg_paged_query* q) {
-  (void)device;
   if (int r = check_query(c, q)) return r;
-  return 0;
+  const int rows = shared_rows(c, q);
+  if (rows == 0) return 0;
+  int sms;
+  if (int r = sm_count(device, &sms)) return r < 0 ? r : KCG_E_BAD_ARG;
+  return tokens_workspace(sms, rows, c->d);
 }
 
 extern "C" int kcg_attention_paged(int device, uint64_t stream, const kcg_paged_cache* c, const kcg_paged_query* q) {
@@ -246,6 +349,7 @@ extern "C" int kcg_attention_paged(int device, uint64_t stream, const kcg_paged_
   if (q->rows == 0) return 0;
   DeviceGuard guard;
   if (cudaError_t e = guard.enter(device)) return cuda_fail(e, "cudaSetDevice");
+  if (const int rows = shared_rows(c, q)) return attention_tokens(device, reinterpret_cast<cudaStream_t>(stream), c, q, rows);
   PagedArgs a{};
   a.seq = sequences_of(c, q->rows);
   a.k = reinterpret_cast<const void*>(c->K), a.v = reinterpret_cast<const void*>(c->V), a.q = reinterpret_cast<const void*>(q->Q);
@@ -266,6 +370,9 @@ extern "C" int kcg_attention_paged_status(int device, uint32_t out[4]) {
   DeviceGuard guard;
   if (cudaError_t e = guard.enter(device)) return cuda_fail(e, "cudaSetDevice");
   if (cudaError_t e = cudaDeviceSynchronize()) return cuda_fail(e, "cudaDeviceSynchronize");
-  for (int i = 0; i < 4; ++i) out[i] = 0u;
-  return 0;
+  if (cudaError_t e = cudaMemcpyFromSymbol(out, g_paged_status, sizeof(uint32_t) * 4)) return cuda_fail(e, "cudaMemcpyFromSymbol");
+  if (out[0] == 0u) return 0;
+  const uint32_t zero[4] = {0u, 0u, 0u, 0u};
+  if (cudaError_t e = cudaMemcpyToSymbol(g_paged_status, zero, sizeof(zero))) return cuda_fail(e, "cudaMemcpyToSymbol");
+  return fail(KCG_E_DEVICE_TIMEOUT, "a bounded wait of the paged attention ran out");
 }

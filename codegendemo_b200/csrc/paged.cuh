@@ -39,6 +39,22 @@ struct Sequences {
   }
 };
 
+// The tiles of `tile` keys that the rows at positions p_lo .. of a sequence of `keys` keys see some of: those of the first `sinks`
+// keys that lie before the window of the first row, then those from that window's start on.
+struct TileList {
+  int first, window0, count;  // tiles of the sinks; first tile behind them; all
+  int lo;                     // first key of the first row's window
+  __device__ __forceinline__ TileList(int keys, int p_lo, int window, int sinks, int tile) {
+    lo = window > 0 && p_lo >= window ? p_lo - window + 1 : 0;
+    const int s = min(min(sinks, lo), keys);
+    first = s / tile + (s % tile ? 1 : 0);
+    window0 = max(lo / tile, first);
+    const int end = keys / tile + (keys % tile ? 1 : 0);
+    count = first + max(0, end - window0);
+  }
+  __device__ __forceinline__ int tile_at(int i) const { return i < first ? i : window0 + i - first; }
+};
+
 // The sequence whose rows hold `row`, or -1; asked by a whole (converged) warp, 32 places at a time. (The last sequence that starts at
 // or before the row, if it has not ended there: empty ones start where the next one does.)
 __device__ __forceinline__ int sequence_of(const Sequences& s, int row) {

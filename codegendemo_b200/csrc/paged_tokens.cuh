@@ -1,0 +1,509 @@
+// Attention of one or a few new tokens of each sequence over its keys in the paged cache: up to 64 rows (tokens x query heads that share a
+// key head) meet every key of a sequence and key head.
+//
+// Each key is read once, 2 * d values, for at most 64 rows, so HBM bounds it. Sequences differ in length, and one of them may be all there is: so
+// the 64-key tiles of all sequences and key heads are laid end to end and cut into equal ranges, one for each CTA, two CTAs an SM; a range may
+// cover the end of one (sequence, head) and the beginning of others. What a range covers whole leaves as a result, a part as
+// unnormalised fp32 rows with their maximum and sum in a workspace; a second kernel, already on the GPU when the first one ends, joins the
+// parts of a (sequence, head) in the order of its keys. No atomics: the order of every sum follows from the lengths.
+//   warp 4     loads: a lane a box of a page (16 keys of K, say), its page's number fetched while the tile before is waited for; tells the others
+//              through the stage which rows and keys it holds
+//   warps 0-3  mma.sync m16n8k16 with 16 rows each. kRowGroups = 1 (up to 16 rows): each warp 16 of a tile's 64 keys; 2 (up to 32): two groups
+//              of rows, 32 keys each; 4 (up to 64): all 64 keys. (tcgen05 needs 128 rows: see kernels/attn_decode.cuh.)
+// Keys that no row sees, but a box holds (behind the last token of a page, before a window), may be anything: their scores are replaced
+// and their values overwritten with zeros, as 0 x NaN would not vanish.
+#pragma once
+
+struct TokensArgs {
+  CUtensorMap tmK, tmV;  // {d, token of a page, head, page}, boxes of {64, min(page, 64), 1, 1}, 128-byte swizzle
+  Sequences seq;
+  const void* q;
+  void* o;
+  long long q_row, q_head, o_row, o_head;
+  float* parts;  // [2 * CTAs][rows][d], then [2 * CTAs][rows] {maximum, sum}, then [CTAs] {sequence, head, last CTA, 0}
+  int kv_heads, group, window, sinks;
+  int box_log2;  // keys of a box
+  float scale_log2;
+};
+
+// Tiles that a CTA takes at least, where there are enough CTAs for less.
+constexpr int kTokensMinTiles = 2;
+
+// How `total` tiles are cut into ranges: the CTAs that have one, the first tile of a CTA's, the CTA that has a tile.
+struct Ranges {
+  long long total;
+  int ctas;
+  __device__ __forceinline__ Ranges(long long t, int most) : total(t) {
+    const long long n = t / kTokensMinTiles;
+    ctas = n < 1 ? 1 : n < most ? static_cast<int>(n) : most;
+  }
+  __device__ __forceinline__ long long begin(int cta) const { return total * cta / ctas; }
+  __device__ __forceinline__ int owner(long long tile) const { return static_cast<int>(((tile + 1) * ctas - 1) / total); }
+};
+
+template <int kD, bool kBf16, int kRowGroups>
+struct AttnTokens {
+  static constexpr int BC = 64;
+  static constexpr int STAGES = kD == 128 ? 3 : 6;
+  static constexpr int KEY_GROUPS = 4 / kRowGroups, WKEYS = BC / KEY_GROUPS, ROWS = 16 * kRowGroups;
+  static constexpr int NUM_THREADS = 160;
+  static constexpr int HALVES = kD / 64;
+  static constexpr int HALF_BYTES = BC * 128;  // 64 keys x 64 values
+  static constexpr int KV_BYTES = BC * kD * 2, STAGE_BYTES = 2 * KV_BYTES, RING_BYTES = STAGES * STAGE_BYTES;
+  static constexpr int JOIN_BYTES = 4 * 16 * 32 * 4;  // 32 columns of the warps' rows
+  static constexpr int SMEM_BYTES = RING_BYTES + JOIN_BYTES + 1024 + 2048;
+  static_assert(2 * (SMEM_BYTES + 1024) <= 228 * 1024, "two CTAs an SM");
+  using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
+
+  // What a stage holds, for the warps that read it.
+  struct Tile {
+    int b, h;      // sequence, key head
+    int key0;      // first key of the tile
+    int keys;      // of the sequence
+    int p_lo;      // position of the first row's token
+    int lo;        // first key of the first row's window
+    int flags;     // MASKED: some row does not see some key; FIRST, LAST of a (sequence, head)'s keys in this CTA; WHOLE: all of them
+    int slot;      // where a part goes
+  };
+  enum : int { MASKED = 1, FIRST = 2, LAST = 4, WHOLE = 8 };
+  struct Shared {
+    uint64_t full[STAGES], empty[STAGES];
+    Tile tile[STAGES];
+    float2 warp_ml[4][16];
+    long long before[5];  // tiles of the sequences before each warp's
+    long long range[2];
+    int found[3];         // sequence, head and tile that the range begins with
+    volatile uint32_t abort_flag;
+  };
+  static_assert(sizeof(Shared) <= 2048, "barrier block exceeds its shared-memory slot");
+
+  __device__ static __forceinline__ void report(Shared* sh, uint32_t code, uint32_t d0) {
+    sh->abort_flag = 1u;
+    if (atomicCAS(&g_paged_status[0], 0u, code) == 0u) {
+      g_paged_status[1] = blockIdx.x;
+      g_paged_status[2] = d0;
+      g_paged_status[3] = 0u;
+    }
+  }
+  __device__ static __forceinline__ float weight(float x, float base) { return x == -INFINITY ? 0.f : ex2(x - base); }
+
+  // A sequence's tiles; one without a key has one too, in which no row sees anything.
+  __device__ static __forceinline__ TileList tiles_of(const TokensArgs& p, int length, int* keys, int* p_lo) {
+    *keys = p.seq.keys(length);
+    *p_lo = max(length, 0) - p.seq.each;
+    TileList t(*keys, *p_lo, p.window, p.sinks, BC);
+    t.count = max(t.count, 1);
+    return t;
+  }
+
+  __device__ static void run(const TokensArgs& p) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    float* join = reinterpret_cast<float*>(smem + RING_BYTES);
+    Shared* sh = reinterpret_cast<Shared*>(smem + RING_BYTES + JOIN_BYTES);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rows = p.seq.each * p.group;
+
+    griddep_launch_dependents();
+    if (threadIdx.x == 0) {
+      for (int s = 0; s < STAGES; ++s) {
+        mbar_init(&sh->full[s], 1);
+        mbar_init(&sh->empty[s], 4);
+      }
+      sh->abort_flag = 0u;
+      sh->range[0] = sh->range[1] = 0;
+      fence_mbar_init();
+    }
+    if (threadIdx.x == 128) {
+      tma_prefetch_desc(&p.tmK);
+      tma_prefetch_desc(&p.tmV);
+    }
+    griddep_wait();
+
+    // All sequences' tiles, and where this CTA's range begins: a thread counts those of its run of sequences.
+    const int per = (p.seq.count + NUM_THREADS - 1) / NUM_THREADS;
+    const int b0 = min(static_cast<int>(threadIdx.x) * per, p.seq.count), b1 = min(b0 + per, p.seq.count);
+    long long mine = 0;
+    int keys, p_lo;
+    for (int b = b0; b < b1; ++b) mine += tiles_of(p, p.seq.lengths[b], &keys, &p_lo).count;
+    mine *= p.kv_heads;
+    long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    if (lane == 31) sh->before[warp] = upto;
+    __syncthreads();
+    long long total = 0, base = 0;
+#pragma unroll
+    for (int w = 0; w < 5; ++w) {
+      if (w < warp) base += sh->before[w];
+      total += sh->before[w];
+    }
+    const Ranges ranges(total, gridDim.x);
+    const int cta = static_cast<int>(blockIdx.x);
+    const long long g0 = cta < ranges.ctas ? ranges.begin(cta) : 0, g1 = cta < ranges.ctas ? ranges.begin(cta + 1) : 0;
+    base += upto - mine;
+    if (g0 < g1 && g0 >= base && g0 < base + mine) {
+      long long at = g0 - base;
+      for (int b = b0; b < b1; ++b) {
+        const int n = tiles_of(p, p.seq.lengths[b], &keys, &p_lo).count;
+        if (at < static_cast<long long>(n) * p.kv_heads) {
+          sh->found[0] = b, sh->found[1] = static_cast<int>(at / n), sh->found[2] = static_cast<int>(at % n);
+          break;
+        }
+        at -= static_cast<long long>(n) * p.kv_heads;
+      }
+    }
+    __syncthreads();
+    const int count = static_cast<int>(g1 - g0);
+
+    if (warp == 4) {
+      // ------------------------------------------------------------------ loads
+      int4 meta = make_int4(-1, 0, 0, 0);
+      if (count > 0) {
+        int b = sh->found[0], h = sh->found[1], t = sh->found[2];
+        TileList list = tiles_of(p, p.seq.lengths[b], &keys, &p_lo);
+        int next_length = b + 1 < p.seq.count ? p.seq.lengths[b + 1] : 0;
+        const int boxes = BC >> p.box_log2;            // of 64 columns, in a tile of K or of V
+        const int loads = boxes * HALVES * 2;          // at most 32: a lane each
+        const int box = lane % boxes, half = lane / boxes % HALVES, is_v = lane / (boxes * HALVES);
+        // this lane's page of tile t of sequence b; -1 (zeros) where no row sees any of the box
+        auto page_of = [&](int b_, const TileList& list_, int keys_, int t_) {
+          const int key = list_.tile_at(t_) * BC + (box << p.box_log2);
+          const bool seen = key < keys_ && (key + (1 << p.box_log2) > list_.lo || key < p.sinks);
+          return lane < loads && seen ? p.seq.page_of(b_, key) : -1;
+        };
+        int page = page_of(b, list, keys, t);
+        long long unit_begin = g0 - t;
+        for (int i = 0; i < count; ++i) {
+          const int s = i % STAGES;
+          const int key0 = list.tile_at(t) * BC;
+          const int this_page = page;
+          Tile tile;
+          tile.b = b, tile.h = h, tile.key0 = key0, tile.keys = keys, tile.p_lo = p_lo, tile.lo = list.lo;
+          const int p_hi = p_lo + p.seq.each - 1;
+          const bool near = p.window <= 0 || key0 > p_hi - p.window || key0 + BC <= p.sinks;
+          const bool whole = unit_begin >= g0 && unit_begin + list.count <= g1;
+          tile.flags = (key0 + BC > keys || key0 + BC > p_lo + 1 || !near ? MASKED : 0) | (i == 0 || t == 0 ? FIRST : 0) |
+                       (i == count - 1 || t == list.count - 1 ? LAST : 0) | (whole ? WHOLE : 0);
+          tile.slot = 2 * cta + (unit_begin >= g0 ? 1 : 0);
+          if (!whole && unit_begin >= g0) meta = make_int4(b, h, ranges.owner(unit_begin + list.count - 1), 0);
+          const int this_h = h;
+          // the next tile, and its pages while this one's stage is waited for
+          if (++t == list.count) {
+            t = 0;
+            unit_begin += list.count;
+            if (++h == p.kv_heads) {
+              h = 0;
+              if (++b < p.seq.count) {
+                list = tiles_of(p, next_length, &keys, &p_lo);
+                next_length = b + 1 < p.seq.count ? p.seq.lengths[b + 1] : 0;
+              }
+            }
+          }
+          if (i + 1 < count) page = page_of(b, list, keys, t);
+          const bool free = mbar_wait(&sh->empty[s], ((i / STAGES) & 1u) ^ 1u, &sh->abort_flag);
+          if (!__all_sync(0xffffffffu, free)) {
+            if (lane == 0) report(sh, PAGED_TIMEOUT_LOADS, static_cast<uint32_t>(i));
+            break;
+          }
+          uint8_t* st = smem + s * STAGE_BYTES;
+          if (lane == 0) {
+            sh->tile[s] = tile;
+            mbar_expect_tx(&sh->full[s], STAGE_BYTES);
+          }
+          __syncwarp();
+          if (lane < loads) {
+            const int in_page = (key0 + (box << p.box_log2)) & ((1 << p.seq.page_log2) - 1);
+            tma_load_4d(st + is_v * KV_BYTES + half * HALF_BYTES + (box << p.box_log2) * 128, is_v ? &p.tmV : &p.tmK, &sh->full[s], half * 64,
+                        in_page, this_h, this_page);
+          }
+        }
+      }
+      if (lane == 0) {
+        float* end = p.parts + 2ll * gridDim.x * rows * (kD + 2);
+        reinterpret_cast<int4*>(end)[cta] = meta;
+      }
+      __syncwarp();
+    } else if (count > 0) {
+      const int q = lane >> 2, t = lane & 3;  // row and column pair of this lane in an accumulator tile
+      const int rg = warp / KEY_GROUPS, kg = warp % KEY_GROUPS;
+      const int mat = lane >> 3, mrow = lane & 7;
+      uint32_t qf[kD / 16][4];
+      float o[kD / 8][4];
+      float m[2], l[2];
+      int see[2], near[2];  // keys below `see`, of those from `near` on (and the sinks)
+      for (int i = 0; i < count; ++i) {
+        const int s = i % STAGES;
+        const bool got = mbar_wait(&sh->full[s], (i / STAGES) & 1u, &sh->abort_flag);
+        // (one outcome for all four: they meet again at the end of a (sequence, head))
+        if (!named_bar_all(1, 128, got)) {
+          if (!got && lane == 0) report(sh, PAGED_TIMEOUT_ATTENTION, static_cast<uint32_t>(i));
+          break;
+        }
+        const Tile tile = sh->tile[s];
+        if (tile.flags & FIRST) {
+          const T* Q = static_cast<const T*>(p.q);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int r = rg * 16 + q + 8 * e, i_tok = r / p.group;
+            const bool live = r < rows;
+            const T* from = Q + (static_cast<long long>(tile.b) * p.seq.each + i_tok) * p.q_row + (tile.h * p.group + r - i_tok * p.group) * p.q_head;
+#pragma unroll
+            for (int ks = 0; ks < kD / 16; ++ks) {
+              qf[ks][e] = live ? *reinterpret_cast<const uint32_t*>(from + ks * 16 + 2 * t) : 0u;
+              qf[ks][e + 2] = live ? *reinterpret_cast<const uint32_t*>(from + ks * 16 + 2 * t + 8) : 0u;
+            }
+            const int position = tile.p_lo + (live ? i_tok : 0);
+            see[e] = min(position + 1, tile.keys);
+            near[e] = p.window > 0 && position >= p.window ? position - p.window + 1 : 0;
+            m[e] = -INFINITY, l[e] = 0.f;
+          }
+#pragma unroll
+          for (int n = 0; n < kD / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+        }
+        const uint32_t kaddr = smem_u32(smem + s * STAGE_BYTES), vaddr = kaddr + KV_BYTES;
+        // two accumulators per 8 keys (even and odd 16 values of d): twice as many independent chains
+        float c[WKEYS / 8][4], c2[WKEYS / 8][4];
+#pragma unroll
+        for (int n = 0; n < WKEYS / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c[n][e] = c2[n][e] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < kD / 32; ++ks) {
+          const int unit = ks * 4 + mat;
+#pragma unroll
+          for (int n = 0; n < WKEYS / 8; ++n) {
+            const int key = kg * WKEYS + n * 8 + mrow;
+            uint32_t b[4];
+            ldmatrix_x4(b, kaddr + key * 128 + (unit >> 3) * HALF_BYTES + (((unit & 7) ^ (key & 7)) << 4));
+            mma_16816<kBf16>(c[n], qf[2 * ks][0], qf[2 * ks][1], qf[2 * ks][2], qf[2 * ks][3], b[0], b[1]);
+            mma_16816<kBf16>(c2[n], qf[2 * ks + 1][0], qf[2 * ks + 1][1], qf[2 * ks + 1][2], qf[2 * ks + 1][3], b[2], b[3]);
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < WKEYS / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c[n][e] += c2[n][e];
+        if (tile.flags & MASKED) {
+          const int first = tile.key0 + kg * WKEYS;
+#pragma unroll
+          for (int n = 0; n < WKEYS / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int key = first + n * 8 + 2 * t + (e & 1);
+              if (key >= see[e >> 1] || (key < near[e >> 1] && key >= p.sinks)) c[n][e] = -INFINITY;
+            }
+          // values of keys that no row sees
+          bool zeroed = false;
+          for (int u = lane; u < WKEYS * (kD / 8); u += 32) {
+            const int k = u / (kD / 8), piece = u % (kD / 8), key = first + k, at = kg * WKEYS + k;
+            if (key >= tile.keys || (key < tile.lo && key >= p.sinks)) {
+              *reinterpret_cast<uint4*>(smem + s * STAGE_BYTES + KV_BYTES + (piece >> 3) * HALF_BYTES + at * 128 + (((piece & 7) ^ (at & 7)) << 4)) =
+                  make_uint4(0u, 0u, 0u, 0u);
+              zeroed = true;
+            }
+          }
+          if (zeroed) fence_proxy_async_smem();  // (the stage's next load comes behind these stores)
+          __syncwarp();
+        }
+        float base_[2], alpha[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int n = 0; n < WKEYS / 8; ++n) mx = fmaxf(mx, fmaxf(c[n][2 * h], c[n][2 * h + 1]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          mx = fmaxf(m[h], mx * p.scale_log2);  // (the scale is positive: checked by the host)
+          base_[h] = mx == -INFINITY ? 0.f : mx;
+          alpha[h] = ex2(m[h] - base_[h]);
+          m[h] = mx;
+        }
+        if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+          for (int n = 0; n < kD / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][e] *= alpha[e >> 1];
+        }
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int n = 0; n < WKEYS / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            c[n][e] = ex2(fmaf(c[n][e], p.scale_log2, -base_[e >> 1]));
+            sum[e >> 1] += c[n][e];
+          }
+        l[0] = l[0] * alpha[0] + sum[0];
+        l[1] = l[1] * alpha[1] + sum[1];
+#pragma unroll
+        for (int ks = 0; ks < WKEYS / 16; ++ks) {
+          const uint32_t a0 = pack_pair<kBf16>(c[2 * ks][0], c[2 * ks][1]);
+          const uint32_t a1 = pack_pair<kBf16>(c[2 * ks][2], c[2 * ks][3]);
+          const uint32_t a2 = pack_pair<kBf16>(c[2 * ks + 1][0], c[2 * ks + 1][1]);
+          const uint32_t a3 = pack_pair<kBf16>(c[2 * ks + 1][2], c[2 * ks + 1][3]);
+          const int key = kg * WKEYS + ks * 16 + (mat & 1) * 8 + mrow;
+          const uint32_t vrow = vaddr + key * 128;
+#pragma unroll
+          for (int n = 0; n < kD / 8; n += 2) {
+            const int unit = n + (mat >> 1);
+            uint32_t b[4];
+            ldmatrix_x4_trans(b, vrow + (unit >> 3) * HALF_BYTES + (((unit & 7) ^ (key & 7)) << 4));
+            mma_16816<kBf16>(o[n], a0, a1, a2, a3, b[0], b[1]);
+            mma_16816<kBf16>(o[n + 1], a0, a1, a2, a3, b[2], b[3]);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->empty[s]);
+        if (!(tile.flags & LAST)) continue;
+
+        // ---- the end of these rows' keys in this CTA: the warps' sums, 32 columns at a time
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+          l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+          if (t == 0) sh->warp_ml[warp][q + 8 * h] = make_float2(m[h], l[h]);
+        }
+        named_bar_sync(1, 128);
+        float f[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < KEY_GROUPS; ++k) top = fmaxf(top, sh->warp_ml[rg * KEY_GROUPS + k][q + 8 * h].x);
+          f[h] = weight(m[h], top);
+        }
+#pragma unroll
+        for (int cc = 0; cc < kD / 32; ++cc) {
+          float* mine_o = join + warp * 16 * 32;
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            *reinterpret_cast<float2*>(mine_o + q * 32 + n * 8 + 2 * t) = make_float2(o[cc * 4 + n][0] * f[0], o[cc * 4 + n][1] * f[0]);
+            *reinterpret_cast<float2*>(mine_o + (q + 8) * 32 + n * 8 + 2 * t) = make_float2(o[cc * 4 + n][2] * f[1], o[cc * 4 + n][3] * f[1]);
+          }
+          named_bar_sync(1, 128);
+          const int row = threadIdx.x >> 3, c4 = threadIdx.x & 7;  // of a group of 16 rows
+#pragma unroll
+          for (int g = 0; g < kRowGroups; ++g) {
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+            float top = -INFINITY, sum_l = 0.f;
+#pragma unroll
+            for (int k = 0; k < KEY_GROUPS; ++k) {
+              const float4 x = reinterpret_cast<const float4*>(join + ((g * KEY_GROUPS + k) * 16 + row) * 32)[c4];
+              a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
+              top = fmaxf(top, sh->warp_ml[g * KEY_GROUPS + k][row].x);
+            }
+#pragma unroll
+            for (int k = 0; k < KEY_GROUPS; ++k) {
+              const float2 ml = sh->warp_ml[g * KEY_GROUPS + k][row];
+              sum_l = fmaf(ml.y, weight(ml.x, top), sum_l);
+            }
+            const int r = g * 16 + row;
+            if (r >= rows) continue;
+            const int col = cc * 32 + c4 * 4;
+            if (tile.flags & WHOLE) {
+              const float inv = sum_l == 0.f ? 0.f : 1.f / sum_l;
+              const int i_tok = r / p.group;
+              T* to = static_cast<T*>(p.o) + (static_cast<long long>(tile.b) * p.seq.each + i_tok) * p.o_row + (tile.h * p.group + r - i_tok * p.group) * p.o_head + col;
+              *reinterpret_cast<uint2*>(to) = make_uint2(pack_pair<kBf16>(a.x * inv, a.y * inv), pack_pair<kBf16>(a.z * inv, a.w * inv));
+            } else {
+              const long long part = static_cast<long long>(tile.slot) * rows + r;
+              *reinterpret_cast<float4*>(p.parts + part * kD + col) = a;
+              if (cc == 0 && c4 == 0)
+                reinterpret_cast<float2*>(p.parts + 2ll * gridDim.x * rows * kD)[part] = make_float2(top, sum_l);
+            }
+          }
+          named_bar_sync(1, 128);
+        }
+      }
+    }
+    if (sh->abort_flag != 0u) {  // loads still in flight land before the ring is given up
+      const uint64_t w0 = global_timer_ns();
+      while (global_timer_ns() - w0 < 200000ull) __nanosleep(1000);
+    }
+    __syncthreads();
+  }
+};
+
+template <int kD, bool kBf16, int kRowGroups>
+__global__ void __launch_bounds__(160, 2) attention_tokens_kernel(const __grid_constant__ TokensArgs p) {
+  AttnTokens<kD, kBf16, kRowGroups>::run(p);
+}
+
+// The parts of a (sequence, key head) whose keys began in CTA blockIdx.x of the kernel above and ended in a later one's. A warp takes a
+// row at a time, or, of few rows, a share of a row's parts.
+template <int kD, bool kBf16>
+__global__ void __launch_bounds__(256) attention_tokens_join_kernel(const __grid_constant__ TokensArgs p, int ctas) {
+  using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
+  using Vec = typename std::conditional<kD == 128, float4, float2>::type;
+  constexpr int PER = kD / 32;
+  __shared__ float acc[8][kD];
+  __shared__ float2 ml_of[8];
+  griddep_wait();
+  griddep_launch_dependents();
+  const int rows = p.seq.each * p.group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float2* ml = reinterpret_cast<const float2*>(p.parts + 2ll * ctas * rows * kD);
+  const int4 meta = reinterpret_cast<const int4*>(p.parts + 2ll * ctas * rows * (kD + 2))[blockIdx.x];
+  if (meta.x < 0) return;
+  const int first = static_cast<int>(blockIdx.x), n = meta.z - first + 1;  // CTAs with a part: slot 1 of the first, slot 0 of the others
+  int shares = 1;  // warps of a row
+  while (shares < 8 && rows * shares < 8 && n > shares) shares *= 2;
+  const int at_once = 8 / shares;
+  for (int r0 = 0; r0 < rows; r0 += at_once) {
+    const int r = r0 + warp / shares, share = warp % shares;
+    const bool live = r < rows;
+    float top = -INFINITY, sum = 0.f, a[PER];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) a[e] = 0.f;
+    if (live) {
+      auto part = [&](int i) { return (2ll * (first + i) + (i == 0 ? 1 : 0)) * rows + r; };
+      for (int i = share + lane * shares; i < n; i += 32 * shares) top = fmaxf(top, ml[part(i)].x);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll 4
+      for (int i = share; i < n; i += shares) {
+        const float2 s = ml[part(i)];
+        const Vec v = reinterpret_cast<const Vec*>(p.parts + part(i) * kD)[lane];
+        const float f = s.x == -INFINITY ? 0.f : ex2(s.x - top);
+        sum = fmaf(f, s.y, sum);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) a[e] = fmaf(f, reinterpret_cast<const float*>(&v)[e], a[e]);
+      }
+    }
+    if (shares > 1) {
+#pragma unroll
+      for (int e = 0; e < PER; ++e) acc[warp][lane * PER + e] = a[e];
+      if (lane == 0) ml_of[warp] = make_float2(top, sum);
+      __syncthreads();
+      if (live && share == 0) {
+        float all = -INFINITY;
+        for (int w = 0; w < shares; ++w) all = fmaxf(all, ml_of[warp + w].x);
+        sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) a[e] = 0.f;
+        for (int w = 0; w < shares; ++w) {
+          const float2 s = ml_of[warp + w];
+          const float f = s.x == -INFINITY ? 0.f : ex2(s.x - all);
+          sum = fmaf(f, s.y, sum);
+#pragma unroll
+          for (int e = 0; e < PER; ++e) a[e] = fmaf(f, acc[warp + w][lane * PER + e], a[e]);
+        }
+      }
+      __syncthreads();
+    }
+    if (live && share == 0) {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const int i_tok = r / p.group;
+      T* to = static_cast<T*>(p.o) + (static_cast<long long>(meta.x) * p.seq.each + i_tok) * p.o_row + (meta.y * p.group + r - i_tok * p.group) * p.o_head + lane * PER;
+      if constexpr (PER == 4) {
+        *reinterpret_cast<uint2*>(to) = make_uint2(pack_pair<kBf16>(a[0] * inv, a[1] * inv), pack_pair<kBf16>(a[2] * inv, a[3] * inv));
+      } else {
+        *reinterpret_cast<uint32_t*>(to) = pack_pair<kBf16>(a[0] * inv, a[1] * inv);
+      }
+    }
+  }
+}
