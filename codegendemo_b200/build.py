@@ -99,7 +99,8 @@ def build_library(force: bool = False) -> str:
     # the split of fp32 operands, the 8-bit linear layer, and the paged cache
     extra = [os.path.join(HERE, "csrc", f) for f in ("kcg_noalloc.cu", "kcg_softmax.cu", "kcg_attention.cu", "kcg_f32split.cu",
                                                      "kcg_norm.cu", "kcg_quantize.cu", "kcg_fp8.cu", "kcg_paged.cu")]
-    deps += extra + [os.path.join(HERE, "csrc", f) for f in ("attn_common.cuh", "fp8_common.cuh", "paged.cuh", "paged_tokens.cuh")]
+    deps += extra + [os.path.join(HERE, "csrc", f) for f in ("attn_common.cuh", "fp8_common.cuh", "paged.cuh", "paged_prompt.cuh",
+                                                              "paged_tokens.cuh")]
     if not force and _newer(out, deps):
         return out
     nvcc = os.path.join(CUDA_HOME, "bin", "nvcc")

@@ -7,6 +7,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <mutex>
 
@@ -123,69 +124,11 @@ int append(Launch& launch, const AppendArgs& a, int d, bool interleaved) {
 }
 
 // ---------------------------------------------------------------------------------------------------- attention
-struct PagedArgs {
-  Sequences seq;
-  const void *k, *v, *q;
-  void* o;
-  long long q_row, q_head, o_row, o_head;
-  long long kc[3], vc[3];
-  int q_heads, kv_heads, window, sinks;
-  float scale_log2;
-};
-
 __device__ unsigned int g_paged_status[4];  // {code, block, detail, detail}; 0 = no wait ran out
 enum : uint32_t { PAGED_TIMEOUT_LOADS = 1, PAGED_TIMEOUT_ATTENTION = 2 };
 
+#include "paged_prompt.cuh"
 #include "paged_tokens.cuh"
-
-// A warp a row and query head, key after key.
-template <typename T, int kD>
-__global__ void __launch_bounds__(128) attention_paged_kernel(const PagedArgs a) {
-  griddep_launch_dependents();
-  griddep_wait();
-  const int lane = threadIdx.x & 31;
-  const long long unit = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  const int row = static_cast<int>(unit / a.q_heads), head = static_cast<int>(unit % a.q_heads);
-  if (row >= a.seq.rows) return;
-  const int b = sequence_of(a.seq, row);
-  if (b < 0) return;
-  constexpr int PER = kD / 32;
-  const int length = a.seq.lengths[b];
-  const int n = a.seq.start(b + 1) - a.seq.start(b);
-  const int position = length - n + (row - a.seq.start(b));
-  const int keys = min(a.seq.keys(length), position + 1);
-  const T* q = static_cast<const T*>(a.q) + row * a.q_row + head * a.q_head + lane * PER;
-  float qv[PER], acc[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) qv[i] = to_f32(q[i]) * a.scale_log2, acc[i] = 0.f;
-  const int kh = head / (a.q_heads / a.kv_heads);
-  float m = -INFINITY, sum = 0.f;
-  for (int j = 0; j < keys; ++j) {
-    if (a.window > 0 && position - j >= a.window && j >= a.sinks) {
-      j = position - a.window;  // the next key in sight comes behind it
-      continue;
-    }
-    const int page = a.seq.page_of(b, j);
-    const long long slot = j & ((1 << a.seq.page_log2) - 1);
-    float s = 0.f, v[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int c = lane * PER + i;
-      s += page < 0 ? 0.f : qv[i] * to_f32(static_cast<const T*>(a.k)[page * a.kc[0] + kh * a.kc[1] + slot * a.kc[2] + c]);
-      v[i] = page < 0 ? 0.f : to_f32(static_cast<const T*>(a.v)[page * a.vc[0] + kh * a.vc[1] + slot * a.vc[2] + c]);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    const float top = fmaxf(m, s), base = top == -INFINITY ? 0.f : top;
-    const float alpha = exp2f(m - base), w = exp2f(s - base);
-    m = top, sum = sum * alpha + w;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) acc[i] = acc[i] * alpha + w * v[i];
-  }
-  T* o = static_cast<T*>(a.o) + row * a.o_row + head * a.o_head + lane * PER;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) o[i] = from_f32<T>(sum == 0.f ? 0.f : acc[i] / sum);
-}
 
 int check_query(const kcg_paged_cache* c, const kcg_paged_query* q) {
   if (!q) return fail(KCG_E_BAD_ARG, "attention_paged: null pointer");
@@ -294,6 +237,83 @@ int attention_tokens(int device, cudaStream_t st, const kcg_paged_cache* c, cons
   return launch_tokens_of<4>(device, sms, st, c, p);
 }
 
+// How many clusters of 2 .. 8 CTAs of the key-split prompt kernel run at once (asked once per device and kernel; 0: not known yet).
+template <auto kKernel>
+int prompt_clusters(int device, int threads, int smem, int size) {
+  static std::atomic<int> known[64][9];
+  int n = known[device][size].load();
+  if (n == 0) {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = size, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(size), cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem, cfg.attrs = attr, cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, kKernel, &cfg) != cudaSuccess || n <= 0) {
+      cudaGetLastError();
+      n = -1;  // this size is not used
+    }
+    known[device][size].store(n);
+  }
+  return n;
+}
+
+template <int kD, bool kBf16>
+int launch_prompt(int device, cudaStream_t st, PromptArgs& p, int max_steps) {
+  using Kern = AttnPrompt<kD, kBf16, false>;
+  constexpr auto whole = attention_prompt_kernel<kD, kBf16, false>;
+  constexpr auto split = attention_prompt_kernel<kD, kBf16, true>;
+  if (int r = opt_in<whole>(device, Kern::SMEM_BYTES)) return r;
+  if (int r = opt_in<split>(device, Kern::SMEM_BYTES)) return r;
+  const long long units = static_cast<long long>(p.slots) * p.kv_heads;
+  if (units > 0x7fffffffLL / 8) return fail(KCG_E_TOO_LARGE, "attention_paged: too many rows");
+  // The largest number of CTAs, 2 to 8, that can share the keys of a pair of tiles with every cluster running at once and, where the
+  // sequences are as long as the table, four tiles of keys each (joining costs what two do).
+  p.splits = 1;
+  for (int s = 8; s >= 2 && p.splits == 1; --s)
+    if (max_steps >= 4 * s && units <= prompt_clusters<split>(device, Kern::NUM_THREADS, Kern::SMEM_BYTES, s)) p.splits = s;
+  Launch launch(st);
+  launch.shape(static_cast<unsigned>(units * p.splits), Kern::NUM_THREADS, Kern::SMEM_BYTES, p.splits);
+  return p.splits > 1 ? launch(split, "attention_paged launch", p) : launch(whole, "attention_paged launch", p);
+}
+
+int attention_prompt(int device, cudaStream_t st, const kcg_paged_cache* c, const kcg_paged_query* q) {
+  if (device < 0 || device >= 64) return fail(KCG_E_BAD_ARG, "device index out of range");
+  EncodeFn encode;
+  if (int r = encoder(&encode)) return r;
+  PromptArgs p{};
+  p.seq = sequences_of(c, q->rows);
+  p.o = reinterpret_cast<void*>(q->O);
+  p.o_row = q->o_stride[0], p.o_head = q->o_stride[1];
+  p.kv_heads = c->kv_heads, p.group = q->q_heads / c->kv_heads, p.window = q->window, p.sinks = q->sinks;
+  p.tile_tokens = 128 / p.group;
+  p.scale_log2 = q->scale * 1.4426950408889634f;
+  const int pair = 2 * p.tile_tokens;
+  // (first row) / pair + sequence + tiles of the sequence, at most: see AttnPrompt::place()
+  const long long slots = c->starts ? (static_cast<long long>(q->rows) + pair - 1) / pair + c->sequences - 1
+                                    : static_cast<long long>((p.seq.each + pair - 1) / pair) * c->sequences;
+  if (slots > 0x7fffffffLL) return fail(KCG_E_TOO_LARGE, "attention_paged: too many rows");
+  p.slots = static_cast<int>(slots);
+  const int box = c->page < 128 ? c->page : 128;
+  while ((1 << p.box_log2) < box) ++p.box_log2;
+  const bool bf16 = c->dtype == KCG_DTYPE_BFLOAT16;
+  {
+    cuuint64_t dim[3] = {static_cast<cuuint64_t>(c->d), static_cast<cuuint64_t>(q->q_heads), static_cast<cuuint64_t>(q->rows)};
+    cuuint64_t step[2] = {static_cast<cuuint64_t>(q->q_stride[1]) * 2, static_cast<cuuint64_t>(q->q_stride[0]) * 2};
+    cuuint32_t box3[3] = {64, static_cast<cuuint32_t>(p.group), static_cast<cuuint32_t>(p.tile_tokens)}, one[3] = {1, 1, 1};
+    const CUresult r = encode(&p.tmQ, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, reinterpret_cast<void*>(q->Q), dim,
+                              step, box3, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(static_cast<int>(r), "cuTensorMapEncodeTiled failed");
+  }
+  if (int r = encode_cache(encode, &p.tmK, c, c->K, c->k_stride, box)) return r;
+  if (int r = encode_cache(encode, &p.tmV, c, c->V, c->v_stride, box)) return r;
+  long long keys = static_cast<long long>(c->width) * c->page;
+  if (q->window > 0) keys = std::min(keys, static_cast<long long>(q->window) + pair + q->sinks);
+  const int max_steps = static_cast<int>(std::min((keys + 127) / 128, 1000000LL));
+  if (c->d == 128) return bf16 ? launch_prompt<128, true>(device, st, p, max_steps) : launch_prompt<128, false>(device, st, p, max_steps);
+  return bf16 ? launch_prompt<64, true>(device, st, p, max_steps) : launch_prompt<64, false>(device, st, p, max_steps);
+}
+
 }  // namespace
 
 extern "C" int kcg_append_kv(int device, uint64_t stream, const kcg_paged_cache* c, const kcg_new_rows* r) {
@@ -350,19 +370,7 @@ extern "C" int kcg_attention_paged(int device, uint64_t stream, const kcg_paged_
   DeviceGuard guard;
   if (cudaError_t e = guard.enter(device)) return cuda_fail(e, "cudaSetDevice");
   if (const int rows = shared_rows(c, q)) return attention_tokens(device, reinterpret_cast<cudaStream_t>(stream), c, q, rows);
-  PagedArgs a{};
-  a.seq = sequences_of(c, q->rows);
-  a.k = reinterpret_cast<const void*>(c->K), a.v = reinterpret_cast<const void*>(c->V), a.q = reinterpret_cast<const void*>(q->Q);
-  a.o = reinterpret_cast<void*>(q->O);
-  a.q_row = q->q_stride[0], a.q_head = q->q_stride[1], a.o_row = q->o_stride[0], a.o_head = q->o_stride[1];
-  for (int i = 0; i < 3; ++i) a.kc[i] = c->k_stride[i], a.vc[i] = c->v_stride[i];
-  a.q_heads = q->q_heads, a.kv_heads = c->kv_heads, a.window = q->window, a.sinks = q->sinks;
-  a.scale_log2 = q->scale * 1.4426950408889634f;
-  Launch launch(reinterpret_cast<cudaStream_t>(stream));
-  launch.shape(static_cast<unsigned>((static_cast<long long>(q->rows) * q->q_heads + 3) / 4), 128);
-  if (c->dtype == KCG_DTYPE_BFLOAT16)
-    return c->d == 128 ? launch(attention_paged_kernel<__nv_bfloat16, 128>, "attention_paged launch", a) : launch(attention_paged_kernel<__nv_bfloat16, 64>, "attention_paged launch", a);
-  return c->d == 128 ? launch(attention_paged_kernel<__half, 128>, "attention_paged launch", a) : launch(attention_paged_kernel<__half, 64>, "attention_paged launch", a);
+  return attention_prompt(device, reinterpret_cast<cudaStream_t>(stream), c, q);
 }
 
 extern "C" int kcg_attention_paged_status(int device, uint32_t out[4]) {

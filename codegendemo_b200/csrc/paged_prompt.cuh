@@ -1,0 +1,538 @@
+// Attention of prompts, or pieces of prompts, over their sequences' keys in the paged cache: causal, optionally with a sliding window and first
+// tokens that stay visible. The form of the fused attention kernel (AttnFwd2 in kcg_attention.cu, where its roles, meetings and figures are
+// described) over pages:
+//
+// One CTA takes two tiles of 128 rows: the query heads that share a key head, of as many tokens as fit (32 tokens x 4 heads, say), so that every
+// key tile is loaded once for all of them. It walks the 128-key tiles that its rows see: those of the sinks, then from the first row's window to
+// the last row's position; a warp masks a tile only where one of its 32 rows does not see all of it.
+//   warp 0    loads: both Q tiles once, then K and V tiles through two-stage rings, a lane a box of a page; page numbers one tile ahead
+//   warp 1    tcgen05.mma: S = Q K^T, O += P V with P in tensor memory
+//   warp 2    waits for K and V in the issuer's place, and overwrites values that no row sees with zeros (0 x NaN would not vanish)
+//   warps 4-7 softmax of tile 0, warps 8-11 of tile 1, a row a thread
+// Bound by what bounds that kernel, the chain scores - softmax - product of a tile against the other tile's, and the power cap.
+// kKeySplit: where the tiles do not fill the GPU, the CTAs of a cluster share the keys of one, and join their results in shared memory.
+#pragma once
+
+struct PromptArgs {
+  CUtensorMap tmQ;       // {d, head, row}, boxes of {64, group, tokens of a tile}
+  CUtensorMap tmK, tmV;  // {d, token of a page, head, page}, boxes of {64, min(page, 128), 1, 1}; 128-byte swizzle all
+  Sequences seq;
+  void* o;
+  long long o_row, o_head;
+  int kv_heads, group, tile_tokens, window, sinks;
+  int box_log2;  // keys of a box
+  int slots;     // pairs of tiles: see place()
+  int splits;    // CTAs that share a pair's keys
+  float scale_log2;
+};
+
+template <int kD, bool kBf16, bool kKeySplit>
+struct AttnPrompt {
+  static constexpr int BR = 128, BC = 128, TILES = 2;
+  static constexpr int K_STAGES = 2, V_STAGES = 2;
+  static constexpr int NUM_THREADS = 384;
+  static constexpr int HALVES = kD / 64;
+  static constexpr int BOX_BYTES = 128 * 128;  // 128 rows x 64 values
+  static constexpr int Q_BYTES = BR * kD * 2, KV_BYTES = BC * kD * 2;
+  static constexpr int OFF_K = TILES * Q_BYTES, OFF_V = OFF_K + K_STAGES * KV_BYTES, RING_BYTES = OFF_V + V_STAGES * KV_BYTES;
+  static constexpr int SMEM_BYTES = RING_BYTES + 2048;  // 1 KB alignment slack + barriers
+  static constexpr int P_PART = kD == 128 ? 96 : 64;    // keys of a step after which P V starts
+  static constexpr bool kApart = kD == 64;              // tile 1 starts half a step after tile 0
+  static constexpr uint32_t COL_O = TILES * BC, TMEM_COLS = 512;
+  static constexpr uint32_t FMT = kBf16 ? FMT_BF16 : FMT_F16;
+  static constexpr uint32_t IDESC_S = make_instr_desc(FMT, 0u, 0u, 128u, BC);
+  static constexpr uint32_t IDESC_O = make_instr_desc(FMT, 0u, 1u, 128u, kD);
+  using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
+
+  struct Barriers {
+    uint64_t q_full;
+    uint64_t k_full[K_STAGES], k_empty[K_STAGES], v_full[V_STAGES], v_empty[V_STAGES];
+    uint64_t s_full[TILES];  // S_t of the current step is complete
+    uint64_t o_full[TILES];  // the last P_t V has retired
+    uint32_t tmem_base;
+    volatile uint32_t abort_flag;
+  };
+
+  // Named barriers: see AttnFwd2. Every meeting takes place in every step whatever else happened.
+  static constexpr uint32_t BAR_PART = 1;  // + t: the first P_PART keys of P_t are in tensor memory and O_t is rescaled
+  static constexpr uint32_t BAR_FULL = 3;  // + t: all of P_t is
+  static constexpr uint32_t BAR_KV = 5;    // the V tile of a step and the K tile of the next are there
+  static constexpr uint32_t PT_THREADS = 160, KV_THREADS = 64;
+
+  __device__ static __forceinline__ void report(Barriers* bars, uint32_t code, uint32_t d0, uint32_t d1) {
+    bars->abort_flag = 1u;
+    if (atomicCAS(&g_paged_status[0], 0u, code) == 0u) {
+      g_paged_status[1] = blockIdx.x;
+      g_paged_status[2] = d0;
+      g_paged_status[3] = d1;
+    }
+  }
+
+  // What a CTA works on: tokens token0 .. of sequence b, `rows` of them. The pairs of tiles of sequence b take the slots from
+  // (its first row) / (tokens of a pair) + b on, of which there are enough: so the slot's sequence is found by a search over the first rows
+  // alone, and some slots have no tokens.
+  struct Place {
+    int b, row0, tokens;  // sequence, first row of the step, tokens (0: none)
+    int p_lo;             // position of the first
+    int hi;               // keys that the last one sees (or some, at the table's end)
+    int keys;             // of the sequence
+  };
+  __device__ static __forceinline__ Place place(const PromptArgs& p, int slot) {
+    const Sequences& s = p.seq;
+    const int pair = TILES * p.tile_tokens, lane = threadIdx.x & 31;
+    Place x{};
+    int t;
+    if (!s.starts) {
+      const int each = (s.each + pair - 1) / pair;
+      x.b = slot / each, t = slot % each;
+    } else {
+      int lo = 0, hi = s.count;
+      while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+        const unsigned there = __ballot_sync(0xffffffffu, at < hi && s.start(at) / pair + at <= slot);
+        const int last = there ? 31 - __clz(there) : 0;
+        lo += last * step;
+        hi = min(lo + step, hi);
+      }
+      x.b = lo;
+      t = slot - (s.start(lo) / pair + lo);
+    }
+    const int first = s.start(x.b), n = s.start(x.b + 1) - first;
+    if (t < 0 || t >= (n + pair - 1) / pair || n <= 0) return x;
+    const int length = s.lengths[x.b];
+    x.tokens = min(pair, n - t * pair);
+    x.row0 = first + t * pair;
+    x.keys = s.keys(length);
+    x.p_lo = max(length, 0) - n + t * pair;  // (a negative length: no keys)
+    x.hi = max(0, min(x.keys, x.p_lo + x.tokens));
+    return x;
+  }
+
+  __device__ static void run(const PromptArgs& p) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    Barriers* bars = reinterpret_cast<Barriers*>(smem + RING_BYTES);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = kKeySplit ? static_cast<int>(cluster_cta_rank()) : 0;
+    const int unit = static_cast<int>(blockIdx.x) / (kKeySplit ? p.splits : 1);
+    const int head = unit % p.kv_heads;
+
+    griddep_launch_dependents();
+    if (threadIdx.x == 0) {
+      tma_prefetch_desc(&p.tmQ);
+      tma_prefetch_desc(&p.tmK);
+      tma_prefetch_desc(&p.tmV);
+      mbar_init(&bars->q_full, 1);
+      for (int s = 0; s < K_STAGES; ++s) mbar_init(&bars->k_full[s], 1), mbar_init(&bars->k_empty[s], 1);
+      for (int s = 0; s < V_STAGES; ++s) mbar_init(&bars->v_full[s], 1), mbar_init(&bars->v_empty[s], 1);
+      for (int t = 0; t < TILES; ++t) mbar_init(&bars->s_full[t], 1), mbar_init(&bars->o_full[t], 1);
+      bars->abort_flag = 0u;
+      fence_mbar_init();
+      fence_proxy_async_smem();
+    }
+    if (warp == 1) {
+      tmem_alloc(&bars->tmem_base, TMEM_COLS);
+      tmem_relinquish();
+    }
+    griddep_wait();
+    // (the last tokens of a sequence, which see the most keys, first)
+    const Place at = place(p, p.slots - 1 - unit / p.kv_heads);
+    const TileList list(at.hi, at.p_lo, p.window, p.sinks, BC);
+    const int steps = at.tokens > 0 ? list.count : 0;
+    const int step0 = kKeySplit ? static_cast<int>(static_cast<long long>(steps) * rank / p.splits) : 0;
+    const int nkv = (kKeySplit ? static_cast<int>(static_cast<long long>(steps) * (rank + 1) / p.splits) : steps) - step0;
+    const int tiles = at.tokens > p.tile_tokens ? 2 : 1;
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem_base = bars->tmem_base;
+
+    // Registers: 384 threads are launched with 168 each; the control warpgroup keeps 56, the softmax warpgroups take
+    // 224 (56 + 2 * 224 = 3 * 168), which a row's 128 scores need.
+    if (warp < 4) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+      if (warp == 0 && nkv > 0) {
+        // ------------------------------------------------------------------ loads
+        if (lane == 0) {
+          mbar_expect_tx(&bars->q_full, tiles * HALVES * p.tile_tokens * p.group * 128);
+          for (int t = 0; t < tiles; ++t)
+#pragma unroll
+            for (int b = 0; b < HALVES; ++b)
+              tma_load_3d(smem + t * Q_BYTES + b * BOX_BYTES, &p.tmQ, &bars->q_full, b * 64, head * p.group, at.row0 + t * p.tile_tokens);
+        }
+        const int boxes = BC >> p.box_log2, loads = boxes * HALVES;  // (at most 32)
+        const int box = lane % boxes, half = lane / boxes;
+        // this lane's page of a step; -1 (zeros) where no row sees any of the box
+        auto page_of = [&](int j) {
+          const int key = list.tile_at(step0 + j) * BC + (box << p.box_log2);
+          const bool seen = key < at.hi && (key + (1 << p.box_log2) > list.lo || key < p.sinks);
+          return lane < loads && seen ? p.seq.page_of(at.b, key) : -1;
+        };
+        int page = page_of(0);
+        for (int j = 0; j < nkv; ++j) {
+          const int ks = j % K_STAGES, vs = j % V_STAGES;
+          const int in_page = (list.tile_at(step0 + j) * BC + (box << p.box_log2)) & ((1 << p.seq.page_log2) - 1);
+          const int this_page = page;
+          if (j + 1 < nkv) page = page_of(j + 1);
+          const uint32_t to = half * BOX_BYTES + (box << p.box_log2) * 128;
+          bool free = mbar_wait(&bars->k_empty[ks], ((j / K_STAGES) & 1u) ^ 1u, &bars->abort_flag);
+          if (!__all_sync(0xffffffffu, free)) {
+            if (lane == 0) report(bars, PAGED_TIMEOUT_LOADS, j, 0u);
+            break;
+          }
+          if (lane == 0) mbar_expect_tx(&bars->k_full[ks], KV_BYTES);
+          __syncwarp();
+          if (lane < loads) tma_load_4d(smem + OFF_K + ks * KV_BYTES + to, &p.tmK, &bars->k_full[ks], half * 64, in_page, head, this_page);
+          free = mbar_wait(&bars->v_empty[vs], ((j / V_STAGES) & 1u) ^ 1u, &bars->abort_flag);
+          if (!__all_sync(0xffffffffu, free)) {
+            if (lane == 0) report(bars, PAGED_TIMEOUT_LOADS, j, 1u);
+            break;
+          }
+          if (lane == 0) mbar_expect_tx(&bars->v_full[vs], KV_BYTES);
+          __syncwarp();
+          if (lane < loads) tma_load_4d(smem + OFF_V + vs * KV_BYTES + to, &p.tmV, &bars->v_full[vs], half * 64, in_page, head, this_page);
+        }
+      } else if (warp == 1 && nkv > 0) {
+        // ---------------------------------------------------------------- products
+        const bool q_there = mbar_wait(&bars->q_full, 0u, &bars->abort_flag);
+        if (!q_there && lane == 0) report(bars, PAGED_TIMEOUT_ATTENTION, 0u, 0u);
+        __syncwarp();
+        const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+        const uint64_t qdesc = make_smem_desc(smem_u32(smem), 16, 1024, SWZ_128B);
+        const uint64_t kdesc = make_smem_desc(smem_u32(smem + OFF_K), 16, 1024, SWZ_128B);
+        const uint64_t vdesc = make_smem_desc(smem_u32(smem + OFF_V), BOX_BYTES, 1024, SWZ_128B);
+        auto issue_s = [&](int t, int i) {
+          const uint64_t ad = qdesc + t * (Q_BYTES >> 4), bd = kdesc + (i % K_STAGES) * (KV_BYTES >> 4);
+#pragma unroll
+          for (int ks = 0; ks < kD / 16; ++ks) {
+            const uint32_t in_row = (ks * 32) % 128, box = (ks * 32) / 128;
+            umma_ss<false>(tmem + t * BC, ad + ((box * BOX_BYTES + in_row) >> 4), bd + ((box * BOX_BYTES + in_row) >> 4), IDESC_S, ks > 0 ? 1u : 0u);
+          }
+          umma_commit(&bars->s_full[t]);
+          if (t == tiles - 1) umma_commit(&bars->k_empty[i % K_STAGES]);
+        };
+        auto issue_pv = [&](int t, int j, int ks0, int ks1) {
+          const uint64_t vd = vdesc + (j % V_STAGES) * (KV_BYTES >> 4);
+#pragma unroll
+          for (int ks = 0; ks < BC / 16; ++ks)
+            if (ks >= ks0 && ks < ks1)
+              umma_ts<false>(tmem + COL_O + t * kD, tmem + t * BC + ks * 8, vd + ((ks * 16 * 128) >> 4), IDESC_O, (j > 0 || ks > 0) ? 1u : 0u);
+        };
+        named_bar_sync(BAR_KV, KV_THREADS);  // the first K tile
+        tc_fence_after_sync();
+        if (elect_one()) {
+          issue_s(0, 0);
+          if (!kApart && tiles == 2) issue_s(1, 0);
+        }
+        __syncwarp();
+        for (int j = 0; j < nkv; ++j) {
+          named_bar_sync(BAR_KV, KV_THREADS);
+#pragma unroll
+          for (int t = 0; t < TILES; ++t) {
+            if (t >= tiles) continue;
+            named_bar_sync(BAR_PART + t, PT_THREADS);
+            tc_fence_after_sync();
+            if (elect_one()) {
+              if (kApart && j == 0 && t == 0 && tiles == 2) issue_s(1, 0);
+              issue_pv(t, j, 0, P_PART / 16);
+            }
+            __syncwarp();
+            named_bar_sync(BAR_FULL + t, PT_THREADS);
+            tc_fence_after_sync();
+            if (elect_one()) {
+              issue_pv(t, j, P_PART / 16, BC / 16);
+              if (t == tiles - 1) umma_commit(&bars->v_empty[j % V_STAGES]);
+              if (j + 1 < nkv) {
+                issue_s(t, j + 1);
+              } else {
+                umma_commit(&bars->o_full[t]);
+              }
+            }
+            __syncwarp();
+          }
+        }
+      } else if (warp == 2 && nkv > 0) {
+        // ------------------------------------------- waits for K and V in the issuer's place
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t what, int i) {
+          if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, &bars->abort_flag));
+          if (!ok && lane == 0) report(bars, PAGED_TIMEOUT_ATTENTION, what, static_cast<uint32_t>(i));
+        };
+        wait(&bars->k_full[0], 0u, 1u, 0);
+        named_bar_sync(BAR_KV, KV_THREADS);
+        for (int j = 0; j < nkv; ++j) {
+          wait(&bars->v_full[j % V_STAGES], (j / V_STAGES) & 1u, 2u, j);
+          // values of keys that none of the rows sees: behind the last one's, and between the sinks and the first one's window
+          const int key0 = list.tile_at(step0 + j) * BC;
+          const int end = max(0, min(BC, at.hi - key0)), gap0 = max(0, min(BC, p.sinks - key0)), gap1 = max(0, min(BC, list.lo - key0));
+          if (end < BC || gap0 < gap1) {
+            uint8_t* v = smem + OFF_V + (j % V_STAGES) * KV_BYTES;
+            for (int u = lane; u < BC * 8 * HALVES; u += 32) {
+              const int k = u / 8 % BC;
+              if (k >= end || (k >= gap0 && k < gap1)) *reinterpret_cast<uint4*>(v + u * 16) = make_uint4(0u, 0u, 0u, 0u);  // (whole rows: in any order)
+            }
+            fence_proxy_async_smem();
+          }
+          if (j + 1 < nkv) wait(&bars->k_full[(j + 1) % K_STAGES], ((j + 1) / K_STAGES) & 1u, 1u, j + 1);
+          __syncwarp();
+          named_bar_sync(BAR_KV, KV_THREADS);
+        }
+      }  // (warp 3 only gives its registers)
+      if constexpr (kKeySplit) {  // the two meetings of the cluster that join the partial results
+        __syncwarp();
+        cluster_sync_all();
+        cluster_sync_all();
+      }
+    } else {
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+      // ------------------------------------------------- softmax, correction, epilogue
+      const int q = warp & 3;           // TMEM lane quarter this warp may access
+      const int t = (warp - 4) >> 2;    // query tile of this warp
+      const int row = q * 32 + lane;    // query row of this thread inside its tile
+      const uint32_t lane_addr = static_cast<uint32_t>(q * 32) << 16;
+      const uint32_t col_s = tmem_base + lane_addr + t * BC, col_o = tmem_base + lane_addr + COL_O + t * kD;
+      const int token = t * p.tile_tokens + row / p.group;
+      const bool live = row < p.tile_tokens * p.group && token < at.tokens;
+      // keys below `see`, of those from `near` on and the sinks; rows without a token (whose scores are of whatever lies there) are not masked
+      const int position = at.p_lo + token;
+      const int see = live ? min(position + 1, at.keys) : 0x7fffffff;
+      const int near = live && p.window > 0 && position >= p.window ? position - p.window + 1 : 0;
+      // m: the row's running maximum, which the exponentials of a step are taken against, in the exp2 domain: the maximum itself, so that
+      // the largest probability is exactly 1 and does not lose a bit to the 16-bit P.
+      float m = -INFINITY;
+      uint64_t sum2[2] = {f32x2(0.f, 0.f), f32x2(0.f, 0.f)};
+      bool ok = nkv > 0 && t < tiles;
+      const int mine = ok ? nkv : 0;
+      const uint64_t scale2 = f32x2(p.scale_log2, p.scale_log2);
+      int j = 0;
+      for (; j < mine; ++j) {
+        const bool got = mbar_wait_for(&bars->s_full[t], j & 1u, 4 * KCG_WAIT_LIMIT_NS);
+        if (!__all_sync(0xffffffffu, got)) {
+          if (lane == 0) report(bars, PAGED_TIMEOUT_ATTENTION, 3u, static_cast<uint32_t>(j));
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+        uint32_t sr[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(col_s + c * 32, sr[c]);
+        const int key0 = list.tile_at(step0 + j) * BC;
+        const int end = see - key0, gap0 = p.sinks - key0, gap1 = near - key0;
+        const bool masked = __any_sync(0xffffffffu, end < BC || (gap1 > 0 && gap0 < BC));
+        tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) pin_32(sr[c]);
+        if (masked) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c * 32 + i >= end || (c * 32 + i >= gap0 && c * 32 + i < gap1)) sr[c][i] = __float_as_uint(-INFINITY);
+        }
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        auto max_of = [&](int c) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 2)
+            mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(sr[c][i]), __uint_as_float(sr[c][i + 1]));
+        };
+#pragma unroll
+        for (int c = 0; c < 4; ++c) max_of(c);
+        // (the scale is positive: checked by the host)
+        const float mx = fmaxf(m, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2);
+        // (without a finite score so far the probabilities are 0, not -inf - -inf)
+        const float base = mx == -INFINITY ? 0.f : mx;
+        const float alpha = ex2(m - base);
+        m = mx;
+        const uint64_t alpha2 = f32x2(alpha, alpha), zero2 = f32x2(0.f, 0.f), base2 = f32x2(-base, -base);
+        sum2[0] = fma_f32x2(sum2[0], alpha2, zero2);
+        sum2[1] = fma_f32x2(sum2[1], alpha2, zero2);
+        // Exponentials and P of 32 keys: packed pairs over the S columns this thread has read.
+        auto exponentials = [&](int c) {
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float2 e = f32x2_split(fma_f32x2(f32x2(__uint_as_float(sr[c][2 * i]), __uint_as_float(sr[c][2 * i + 1])), scale2, base2));
+            e.x = ex2(e.x);
+            e.y = ex2(e.y);
+            sum2[i & 1] = add_f32x2(sum2[i & 1], f32x2(e.x, e.y));
+            w[i] = pack_pair<kBf16>(e.x, e.y);
+          }
+          tmem_st_32x32b_x16(col_s + c * 16, w);
+        };
+        // O_t <- alpha * O_t, where a row of the warp has a new maximum (the previous P_t V has retired: the scores just read were issued
+        // behind it).
+        if (j > 0 && __any_sync(0xffffffffu, live && alpha != 1.f)) {
+          auto scale_store = [&](uint32_t (&o)[32], int c) {
+            pin_32(o);
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const float2 v = f32x2_split(mul_f32x2(f32x2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), alpha2));
+              o[i] = __float_as_uint(v.x);
+              o[i + 1] = __float_as_uint(v.y);
+            }
+            tmem_st_32x32b_x32(col_o + c * 32, o);
+          };
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(col_o + c * 32, o);
+            exponentials(c);
+            tmem_ld_wait();
+            scale_store(o, c);
+          }
+          if constexpr (kD == 128) {
+            static_assert(P_PART == 96, "the third piece of 32 keys comes before the publication");
+            uint32_t o[2][32];
+            tmem_ld_32x32b_x32(col_o + 64, o[0]);
+            tmem_ld_32x32b_x32(col_o + 96, o[1]);
+            exponentials(2);
+            tmem_ld_wait();
+            scale_store(o[0], 2);
+            scale_store(o[1], 3);
+          }
+        } else {
+          exponentials(0);
+          exponentials(1);
+          if constexpr (P_PART == 96) exponentials(2);
+        }
+        auto publish = [&](uint32_t bar) {
+          tmem_st_wait();
+          tc_fence_before_sync();
+          named_bar_arrive(bar, PT_THREADS);
+        };
+        publish(BAR_PART + t);
+        if constexpr (P_PART == 64) exponentials(2);
+        exponentials(3);
+        publish(BAR_FULL + t);
+      }
+      for (; j < mine; ++j) {  // (given up)
+        __syncwarp();
+        named_bar_sync(BAR_PART + t, PT_THREADS);
+        named_bar_sync(BAR_FULL + t, PT_THREADS);
+      }
+      const float2 s01 = f32x2_split(add_f32x2(sum2[0], sum2[1]));
+      const float l = s01.x + s01.y;
+      if (ok) {
+        const bool got = mbar_wait(&bars->o_full[t], 0u, &bars->abort_flag);
+        if (!__all_sync(0xffffffffu, got)) {
+          if (lane == 0) report(bars, PAGED_TIMEOUT_ATTENTION, 4u, 0u);
+          ok = false;
+        }
+      }
+      const bool gave_up = mine > 0 && !ok;
+      if constexpr (kKeySplit) {
+        // Partial results: once the products of both tiles have retired, the operand ring holds this CTA's O rows (fp32, not normalised,
+        // 16-byte units XOR-swizzled by the row: a warp writes 32 rows at a time) and their {maximum, sum}; then each CTA joins an equal
+        // share of the output over the cluster's shared memories.
+        constexpr int UNITS = kD / 4;  // 16-byte units of a row
+        constexpr int OFF_ML = TILES * BR * kD * 4;
+        static_assert(OFF_ML + TILES * BR * 8 <= RING_BYTES, "the partial result must fit the ring");
+        bool both = true;
+        if (ok && tiles == 2) {
+          both = __all_sync(0xffffffffu, mbar_wait(&bars->o_full[t ^ 1], 0u, &bars->abort_flag));
+          if (!both && lane == 0) report(bars, PAGED_TIMEOUT_ATTENTION, 5u, 0u);
+        }
+        if (t < tiles && both && !gave_up) {
+          tc_fence_after_sync();
+          const int r = t * BR + row;
+          uint8_t* to = smem + r * kD * 4;
+#pragma unroll
+          for (int c = 0; c < kD / 32; ++c) {
+            uint32_t o[32];
+            if (mine > 0) {
+              tmem_ld_32x32b_x32(col_o + c * 32, o);
+              tmem_ld_wait();
+              pin_32(o);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = 0u;
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+              *reinterpret_cast<uint4*>(to + (((c * 8 + u) ^ (r & (UNITS - 1))) << 4)) = make_uint4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
+          }
+          reinterpret_cast<float2*>(smem + OFF_ML)[r] = make_float2(m, l);
+        }
+        __syncwarp();
+        cluster_sync_all();
+        {
+          const int all = tiles * BR * UNITS;
+          const int u0 = all / p.splits * rank + min(rank, all % p.splits), u1 = u0 + all / p.splits + (rank < all % p.splits ? 1 : 0);
+          const uint32_t base_addr = smem_u32(smem);
+          for (int i = u0 + static_cast<int>(threadIdx.x) - 128; i < u1; i += TILES * 128) {
+            const int r = i / UNITS, u = i % UNITS, in_tile = r % BR;
+            const int tok = r / BR * p.tile_tokens + in_tile / p.group;
+            if (in_tile >= p.tile_tokens * p.group || tok >= at.tokens) continue;
+            const uint32_t ml_addr = base_addr + OFF_ML + r * 8;
+            const uint32_t o_addr = base_addr + r * kD * 4 + ((u ^ (r & (UNITS - 1))) << 4);
+            float top = -INFINITY;
+            for (int c = 0; c < p.splits; ++c) top = fmaxf(top, ld_cluster_f2(map_to_cta(ml_addr, c)).x);
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+            float sum = 0.f;
+#pragma unroll 4
+            for (int c = 0; c < p.splits; ++c) {
+              const float2 ml = ld_cluster_f2(map_to_cta(ml_addr, c));
+              const float4 x = ld_cluster_f4(map_to_cta(o_addr, c));
+              const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+              a.x = fmaf(f, x.x, a.x);
+              a.y = fmaf(f, x.y, a.y);
+              a.z = fmaf(f, x.z, a.z);
+              a.w = fmaf(f, x.w, a.w);
+              sum = fmaf(f, ml.y, sum);
+            }
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            T* out = reinterpret_cast<T*>(p.o) + static_cast<long long>(at.row0 + tok) * p.o_row +
+                     static_cast<long long>(head * p.group + in_tile % p.group) * p.o_head + u * 4;
+            *reinterpret_cast<uint2*>(out) = make_uint2(pack_pair<kBf16>(a.x * inv, a.y * inv), pack_pair<kBf16>(a.z * inv, a.w * inv));
+          }
+        }
+        __syncwarp();
+        cluster_sync_all();  // the other CTAs read this one's shared memory until here
+      } else {
+        tc_fence_after_sync();
+        const float inv = mine == 0 || l == 0.f ? 0.f : 1.f / l;
+        T* out = reinterpret_cast<T*>(p.o) + static_cast<long long>(at.row0 + token) * p.o_row +
+                 static_cast<long long>(head * p.group + row % p.group) * p.o_head;
+#pragma unroll
+        for (int c = 0; c < kD / 32; ++c) {
+          uint32_t r[32];
+          if (mine > 0 && !gave_up) {
+            tmem_ld_32x32b_x32(col_o + c * 32, r);
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = 0u;
+          }
+          if (live) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                w[e] = pack_pair<kBf16>(__uint_as_float(r[u * 8 + 2 * e]) * inv, __uint_as_float(r[u * 8 + 2 * e + 1]) * inv);
+              *reinterpret_cast<uint4*>(out + c * 32 + u * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
+      }
+    }
+
+    // ---------------------------------------------------------------- common exit
+    __syncwarp();
+    if (bars->abort_flag != 0u) {  // loads and products still in flight end before their memory is given up
+      const uint64_t t0 = global_timer_ns();
+      while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 1) {
+      tc_fence_after_sync();
+      tmem_dealloc(tmem_base, TMEM_COLS);
+    }
+  }
+};
+
+template <int kD, bool kBf16, bool kKeySplit>
+__global__ void __launch_bounds__(384, 1) attention_prompt_kernel(const __grid_constant__ PromptArgs p) {
+  AttnPrompt<kD, kBf16, kKeySplit>::run(p);
+}
