@@ -18,6 +18,7 @@
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <cstdint>
@@ -402,6 +403,159 @@ PyObject* bind_fp8(PyObject*, PyObject* args) {
   Py_RETURN_NONE;
 }
 
+// ---- the paged cache (kcg/paged_op.py): as the 8-bit linear layer's, right arguments or the operator's own way.
+struct PagedEntries {
+  int (*append)(int, uint64_t, const kcg_paged_cache*, const kcg_new_rows*);
+  int64_t (*workspace)(int, const kcg_paged_cache*, const kcg_paged_query*);
+  int (*attention)(int, uint64_t, const kcg_paged_cache*, const kcg_paged_query*);
+};
+PagedEntries g_paged{};
+
+// A CUDA tensor of `dims` dimensions whose innermost one is contiguous, on a 16-byte boundary, and the strides of the others.
+const at::Tensor* heads(PyObject* o, int64_t dims, int64_t* strides) {
+  if (!THPVariable_CheckExact(o)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_cuda() || t.dim() != dims || t.layout() != at::kStrided || !t.has_storage() || t.numel() == 0 || t.stride(dims - 1) != 1 ||
+      address(t) % 16)
+    return nullptr;
+  const int64_t d = t.size(dims - 1);
+  int64_t inner = d;
+  for (int64_t i = dims - 2; i >= 0; --i) {
+    const int64_t n = t.size(i), s = n > 1 ? t.stride(i) : inner;
+    if (n > INT32_MAX || s < d || s % 8) return nullptr;
+    strides[i] = s;
+    inner = std::max(inner, s * n);
+  }
+  return &t;
+}
+const at::Tensor* ints(PyObject* o, const at::Tensor& like, int64_t dims) {
+  if (!THPVariable_CheckExact(o)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  return t.is_cuda() && t.scalar_type() == at::kInt && t.dim() == dims && t.layout() == at::kStrided && t.has_storage() && t.device() == like.device() &&
+                 t.numel() > 0 && (t.size(dims - 1) == 1 || t.stride(dims - 1) == 1)
+             ? &t
+             : nullptr;
+}
+bool like_cache(const at::Tensor& t, const at::Tensor& cache) {
+  return t.scalar_type() == cache.scalar_type() && t.device() == cache.device() && t.size(t.dim() - 1) == cache.size(3);
+}
+
+// The cache of args: k_cache, v_cache, page_table, lengths, starts. False: not this path's.
+bool paged_cache(PyObject* const* args, int64_t rows, kcg_paged_cache* c, const at::Tensor** k) {
+  const at::Tensor *kc = heads(args[0], 4, c->k_stride), *vc = heads(args[1], 4, c->v_stride);
+  if (!kc || !vc || vc->sizes() != kc->sizes() || !like_cache(*vc, *kc)) return false;
+  const at::Tensor *table = ints(args[2], *kc, 2), *lengths = ints(args[3], *kc, 1), *starts = nullptr;
+  if (!table || !lengths || lengths->size(0) != table->size(0)) return false;
+  const int64_t sequences = table->size(0), width = table->size(1), page = kc->size(2);
+  if (args[4] != Py_None) {
+    starts = ints(args[4], *kc, 1);
+    if (!starts || starts->size(0) != sequences + 1) return false;
+  } else if (rows % sequences) {
+    return false;
+  }
+  c->dtype = dtype_of(*kc);
+  c->table_ld = sequences > 1 ? table->stride(0) : width;
+  if ((c->dtype != KCG_DTYPE_FLOAT16 && c->dtype != KCG_DTYPE_BFLOAT16) || (kc->size(3) != 64 && kc->size(3) != 128) || page < 8 || (page & (page - 1)) ||
+      c->table_ld < width || width * page > INT32_MAX - 255 || sequences > 1 << 24 || kc->size(1) > 65535)
+    return false;
+  c->K = address(*kc), c->V = address(*vc), c->table = address(*table), c->lengths = address(*lengths), c->starts = starts ? address(*starts) : 0;
+  c->pages = static_cast<int32_t>(kc->size(0)), c->page = static_cast<int32_t>(page), c->width = static_cast<int32_t>(width);
+  c->sequences = static_cast<int32_t>(sequences), c->kv_heads = static_cast<int32_t>(kc->size(1)), c->d = static_cast<int32_t>(kc->size(3));
+  *k = kc;
+  return true;
+}
+
+// attention_paged(q, k_cache, v_cache, page_table, lengths, starts, scale, window, sinks) -> tensor or None
+PyObject* attention_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  kcg_paged_cache c{};
+  kcg_paged_query a{};
+  if (n != 9 || !g_paged.attention) Py_RETURN_NONE;
+  const at::Tensor *q = heads(args[0], 3, a.q_stride), *k;
+  if (!q || !paged_cache(args + 1, q->size(0), &c, &k) || !like_cache(*q, *k) || watched()) Py_RETURN_NONE;
+  a.rows = static_cast<int32_t>(q->size(0)), a.q_heads = static_cast<int32_t>(q->size(1));
+  if (a.q_heads % c.kv_heads || a.q_heads / c.kv_heads > 64) Py_RETURN_NONE;
+  a.scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(c.d)));
+  if (args[6] != Py_None) {
+    if (!PyFloat_CheckExact(args[6])) Py_RETURN_NONE;
+    const double scale = PyFloat_AS_DOUBLE(args[6]);
+    a.scale = static_cast<float>(scale);
+    if (!(scale > 0.0 && scale < 3e38) || !(a.scale > 0.f)) Py_RETURN_NONE;
+  }
+  auto size_of = [](PyObject* o, long least, int32_t* out) {
+    if (!PyLong_CheckExact(o)) return false;
+    const long v = PyLong_AsLong(o);
+    if (v == -1 && PyErr_Occurred()) PyErr_Clear();
+    *out = static_cast<int32_t>(v);
+    return v >= least && v <= INT32_MAX;
+  };
+  if ((args[7] != Py_None && !size_of(args[7], 1, &a.window)) || !size_of(args[8], 0, &a.sinks)) Py_RETURN_NONE;
+  const int device = q->device().index();
+  at::Tensor o = empty_like_on(*q, q->sizes(), q->scalar_type()), workspace;
+  a.Q = address(*q), a.O = out_address(o);
+  a.o_stride[0] = q->size(1) * q->size(2), a.o_stride[1] = q->size(2);
+  const int64_t bytes = g_paged.workspace(device, &c, &a);
+  if (bytes < 0) Py_RETURN_NONE;
+  if (bytes > 0) {
+    workspace = empty_like_on(*q, {bytes}, at::kByte);
+    a.workspace = out_address(workspace), a.workspace_bytes = bytes;
+  }
+  const uint64_t stream = stream_of(*q);
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = g_paged.attention(device, stream, &c, &a);
+  Py_END_ALLOW_THREADS
+  return finish(status, std::move(o));
+  END_HANDLE_TH_ERRORS
+}
+
+// append_kv(k, v, k_cache, v_cache, page_table, lengths, starts, q, (cos, sin), interleaved, positions) -> the turned queries, or None
+PyObject* append_kv(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  kcg_paged_cache c{};
+  kcg_new_rows r{};
+  if (n != 11 || !g_paged.append || !PyTuple_CheckExact(args[8]) || PyTuple_GET_SIZE(args[8]) != 2 || (args[9] != Py_False && args[9] != Py_True))
+    Py_RETURN_NONE;
+  const at::Tensor *k = heads(args[0], 3, r.k_stride), *v = heads(args[1], 3, r.v_stride), *q = heads(args[7], 3, r.q_stride), *cache;
+  const at::Tensor *cos = plain(PyTuple_GET_ITEM(args[8], 0), 2), *sin = plain(PyTuple_GET_ITEM(args[8], 1), 2);
+  if (!k || !v || !q || !cos || !sin || !paged_cache(args + 2, k->size(0), &c, &cache) || !like_cache(*k, *cache) || !like_cache(*v, *cache) ||
+      !like_cache(*q, *cache) || k->size(1) != c.kv_heads || v->size(1) != c.kv_heads || v->size(0) != k->size(0) || q->size(0) != k->size(0) || watched())
+    Py_RETURN_NONE;
+  const int64_t half = cos->size(1);
+  if (cos->scalar_type() != at::kFloat || sin->scalar_type() != at::kFloat || cos->device() != k->device() || sin->device() != k->device() ||
+      cos->sizes() != sin->sizes() || cos->size(0) < 1 || half < 8 || half % 8 || half > c.d / 2 || address(*cos) % 16 || address(*sin) % 16 ||
+      q->size(1) > 65535)
+    Py_RETURN_NONE;
+  if (args[10] != Py_None) {
+    const at::Tensor* positions = ints(args[10], *k, 1);
+    if (!positions || positions->size(0) != k->size(0)) Py_RETURN_NONE;
+    r.positions = address(*positions);
+  }
+  at::Tensor o = empty_like_on(*q, q->sizes(), q->scalar_type());
+  r.K = address(*k), r.V = address(*v), r.Q = address(*q), r.QO = out_address(o);
+  r.qo_stride[0] = q->size(1) * q->size(2), r.qo_stride[1] = q->size(2);
+  r.cos = address(*cos), r.sin = address(*sin), r.angles = cos->size(0);
+  r.rows = static_cast<int32_t>(k->size(0)), r.q_heads = static_cast<int32_t>(q->size(1)), r.rotary = static_cast<int32_t>(2 * half);
+  r.interleaved = args[9] == Py_True ? 1 : 0;
+  const int device = k->device().index();
+  const uint64_t stream = stream_of(*k);
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = g_paged.append(device, stream, &c, &r);
+  Py_END_ALLOW_THREADS
+  return finish(status, std::move(o));
+  END_HANDLE_TH_ERRORS
+}
+
+// bind_paged(kcg_append_kv, kcg_attention_paged_workspace, kcg_attention_paged): addresses
+PyObject* bind_paged(PyObject*, PyObject* args) {
+  unsigned long long f[3];
+  if (!PyArg_ParseTuple(args, "KKK", &f[0], &f[1], &f[2])) return nullptr;
+  auto set = [&](auto& entry, int i) { entry = reinterpret_cast<std::decay_t<decltype(entry)>>(static_cast<uintptr_t>(f[i])); };
+  set(g_paged.append, 0), set(g_paged.workspace, 1), set(g_paged.attention, 2);
+  Py_RETURN_NONE;
+}
+
 // remember(m, n, k, batch, dtype, device, b_transposed, function, info, owner)
 PyObject* remember(PyObject*, PyObject* args) {
   Shape s{};
@@ -447,6 +601,7 @@ PyCFunction fast(F f) {
 PyMethodDef g_methods[] = {{"bind", bind, METH_VARARGS, "addresses of the library's entries"},
                            {"bind_trim", bind_trim, METH_VARARGS, "address of the function that gives memory back"},
                            {"bind_fp8", bind_fp8, METH_VARARGS, "addresses of the 8-bit linear layer's entries"},
+                           {"bind_paged", bind_paged, METH_VARARGS, "addresses of the paged cache's entries"},
                            {"remember", remember, METH_VARARGS, "a shape's kernel"},
                            {"matmul", fast(matmul), METH_FASTCALL, "a product whose kernel is known, or None"},
                            {"bmm", fast(bmm), METH_FASTCALL, "a batched one"},
@@ -456,6 +611,8 @@ PyMethodDef g_methods[] = {{"bind", bind, METH_VARARGS, "addresses of the librar
                            {"rms_norm_backward", fast(rms_norm_backward), METH_FASTCALL, "gradients of the norm, or None"},
                            {"quantize_fp8", fast(quantize_fp8), METH_FASTCALL, "8-bit values and scales, or None"},
                            {"matmul_fp8", fast(matmul_fp8), METH_FASTCALL, "an 8-bit product, or None"},
+                           {"attention_paged", fast(attention_paged), METH_FASTCALL, "attention over a paged cache, or None"},
+                           {"append_kv", fast(append_kv), METH_FASTCALL, "rows into a paged cache, or None"},
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_torchcall", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -386,6 +386,8 @@ def _warm_calls():
             found.bind_fp8(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
                 lib.kcg_rms_norm, lib.kcg_rms_norm_fp8, lib.kcg_rms_norm_backward_workspace, lib.kcg_rms_norm_backward,
                 lib.kcg_quantize_fp8, lib.kcg_matmul_fp8)))
+            found.bind_paged(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
+                lib.kcg_append_kv, lib.kcg_attention_paged_workspace, lib.kcg_attention_paged)))
             found.bind_trim(ctypes.cast(lib.kcg_internal_trim_if_low, ctypes.c_void_p).value)
         _warm = found
     return _warm

@@ -29,6 +29,18 @@ import math
 from codegendemo_b200 import _lib
 from codegendemo_b200.kcg.Utils import DeviceInfo
 
+_warm = None  # csrc/kcg_torchcall.cpp once something was launched, False where it was not built for this torch
+
+
+def _launched(status):
+    """The end of a call that went this way: its error, or the next call's shorter way."""
+    global _warm
+    if status:
+        _lib.check(status)
+    if _warm is None:
+        from codegendemo_b200.kcg import matmul_op
+        _warm = matmul_op._warm_calls()
+
 
 def rotary_table(positions, dim, base=10000.0, device="cuda"):
     """(cos, sin) of the angles ``p * base ** (-2 i / dim)`` of positions p = 0 .. positions - 1, each (positions, dim / 2) in fp32; the
@@ -120,6 +132,10 @@ def append_kv(k, v, k_cache, v_cache, page_table, lengths, starts=None, q=None, 
     (x cos - y sin, y cos + x sin), rounded once. ``positions`` (rows, int32): angles of other positions than the cache's. k, v and q may be parts of
     one projection's result. Where two rows have one place in the cache, it holds values of either. A position without angles gives NaN.
     Rows of the queries whose position is negative become zeros, those behind the last sequence's are not written."""
+    if _warm and q is not None and rotary is not None and q_out is None:
+        turned = _warm.append_kv(k, v, k_cache, v_cache, page_table, lengths, starts, q, rotary, interleaved, positions)
+        if turned is not None:
+            return turned
     import torch
     cache_rows = k.shape[0] if k.dim() == 3 else 0
     c = _cache(k_cache, v_cache, page_table, lengths, starts, cache_rows)
@@ -154,7 +170,7 @@ def append_kv(k, v, k_cache, v_cache, page_table, lengths, starts=None, q=None, 
             r.positions = positions.data_ptr()
     if r.rows > 0:
         dev = k_cache.device.index or 0
-        _lib.check(_lib.get_lib().kcg_append_kv(dev, DeviceInfo.get_cuda_stream(dev), ctypes.byref(c), ctypes.byref(r)))
+        _launched(_lib.get_lib().kcg_append_kv(dev, DeviceInfo.get_cuda_stream(dev), ctypes.byref(c), ctypes.byref(r)))
     return q_out
 
 
@@ -165,6 +181,10 @@ def attention_paged(q, k_cache, v_cache, page_table, lengths, starts=None, scale
     any key gives zeros (a negative position: an empty place of the batch); rows behind the last sequence's are not written. Sums and
     softmax in fp32, the weights rounded to the inputs' type in front of their product with the values. Values of keys that no row of the
     sequence sees may be anything; those of keys that some row sees have to be finite."""
+    if _warm and out is None:
+        out = _warm.attention_paged(q, k_cache, v_cache, page_table, lengths, starts, scale, window, sinks)
+        if out is not None:
+            return out
     if q.dim() != 3:
         raise ValueError("q must be rows x heads x d")
     c = _cache(k_cache, v_cache, page_table, lengths, starts, q.shape[0])
@@ -195,7 +215,7 @@ def attention_paged(q, k_cache, v_cache, page_table, lengths, starts=None, scale
         import torch
         workspace = q.new_empty(size, dtype=torch.uint8)
         a.workspace, a.workspace_bytes = workspace.data_ptr(), size
-    _lib.check(lib.kcg_attention_paged(dev, DeviceInfo.get_cuda_stream(dev), ctypes.byref(c), ctypes.byref(a)))
+    _launched(lib.kcg_attention_paged(dev, DeviceInfo.get_cuda_stream(dev), ctypes.byref(c), ctypes.byref(a)))
     return out
 
 
