@@ -204,7 +204,7 @@ int launch_tokens(int device, int sms, cudaStream_t st, const kcg_paged_cache* c
   Launch launch(st);
   launch.shape(2 * sms, Kern::NUM_THREADS, Kern::SMEM_BYTES);
   if (int r = launch(attention_tokens_kernel<kD, kBf16, kRowGroups>, "attention_paged launch", p)) return r;
-  launch.shape(2 * sms, 256);
+  launch.shape(2 * sms, 512);
   return launch(attention_tokens_join_kernel<kD, kBf16>, "attention_paged join launch", p, 2 * sms);
 }
 
@@ -222,7 +222,7 @@ int attention_tokens(int device, cudaStream_t st, const kcg_paged_cache* c, cons
   EncodeFn encode;
   if (int r = encoder(&encode)) return r;
   TokensArgs p{};
-  const int box = c->page < 64 ? c->page : 64;
+  const int tile = c->d == 128 ? 64 : 128, box = c->page < tile ? c->page : tile;
   if (int r = encode_cache(encode, &p.tmK, c, c->K, c->k_stride, box)) return r;
   if (int r = encode_cache(encode, &p.tmV, c, c->V, c->v_stride, box)) return r;
   p.seq = sequences_of(c, q->rows);

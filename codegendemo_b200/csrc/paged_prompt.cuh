@@ -473,7 +473,7 @@ struct AttnPrompt {
             for (int c = 0; c < p.splits; ++c) {
               const float2 ml = ld_cluster_f2(map_to_cta(ml_addr, c));
               const float4 x = ld_cluster_f4(map_to_cta(o_addr, c));
-              const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+              const float f = ml.y == 0.f ? 0.f : ex2(ml.x - top);  // (a part of no key; a sum of NaN has to reach the result)
               a.x = fmaf(f, x.x, a.x);
               a.y = fmaf(f, x.y, a.y);
               a.z = fmaf(f, x.z, a.z);

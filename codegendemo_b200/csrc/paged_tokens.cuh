@@ -2,8 +2,9 @@
 // key head) meet every key of a sequence and key head.
 //
 // Each key is read once, 2 * d values, for at most 64 rows, so HBM bounds it. Sequences differ in length, and one of them may be all there is: so
-// the 64-key tiles of all sequences and key heads are laid end to end and cut into equal ranges, one for each CTA, two CTAs an SM; a range may
-// cover the end of one (sequence, head) and the beginning of others. What a range covers whole leaves as a result, a part as
+// the tiles of 64 keys (d = 64: 128) of all sequences and key heads are laid end to end, kTokensPause places apart for what the end of
+// one costs, and cut into equal ranges, one for each CTA, two CTAs an SM; a range may cover the end of one (sequence, head) and the
+// beginning of others. What a range covers whole leaves as a result, a part as
 // unnormalised fp32 rows with their maximum and sum in a workspace; a second kernel, already on the GPU when the first one ends, joins the
 // parts of a (sequence, head) in the order of its keys. No atomics: the order of every sum follows from the lengths.
 //   warp 4     loads: a lane a box of a page (16 keys of K, say), its page's number fetched while the tile before is waited for; tells the others
@@ -15,7 +16,7 @@
 #pragma once
 
 struct TokensArgs {
-  CUtensorMap tmK, tmV;  // {d, token of a page, head, page}, boxes of {64, min(page, 64), 1, 1}, 128-byte swizzle
+  CUtensorMap tmK, tmV;  // {d, token of a page, head, page}, boxes of {64, min(page, tile), 1, 1}, 128-byte swizzle
   Sequences seq;
   const void* q;
   void* o;
@@ -26,32 +27,42 @@ struct TokensArgs {
   float scale_log2;
 };
 
-// Tiles that a CTA takes at least, where there are enough CTAs for less.
-constexpr int kTokensMinTiles = 2;
+// Places that a CTA takes at least, where there are enough CTAs for less.
+constexpr int kTokensMinPlaces = 2;
+// Places without a tile behind each (sequence, head)'s: joining the warps' results and beginning with other rows takes as long as a tile or
+// two. (48 sequences x 4 tokens with a window of 1024, three of them empty: 73 us without, as many empty ones' ends in one CTA.)
+constexpr int kTokensPause = 2;
 
-// How `total` tiles are cut into ranges: the CTAs that have one, the first tile of a CTA's, the CTA that has a tile.
+// How `total` places are cut into ranges: the CTAs that have one, the first place of a CTA's, the CTA that has a place.
 struct Ranges {
   long long total;
   int ctas;
   __device__ __forceinline__ Ranges(long long t, int most) : total(t) {
-    const long long n = t / kTokensMinTiles;
+    const long long n = t / kTokensMinPlaces;
     ctas = n < 1 ? 1 : n < most ? static_cast<int>(n) : most;
   }
   __device__ __forceinline__ long long begin(int cta) const { return total * cta / ctas; }
-  __device__ __forceinline__ int owner(long long tile) const { return static_cast<int>(((tile + 1) * ctas - 1) / total); }
+  __device__ __forceinline__ int owner(long long place) const { return static_cast<int>(((place + 1) * ctas - 1) / total); }
 };
 
 template <int kD, bool kBf16, int kRowGroups>
 struct AttnTokens {
-  static constexpr int BC = 64;
-  static constexpr int STAGES = kD == 128 ? 3 : 6;
+  // Keys of a tile: 32 KB of K and V. (64 keys of d = 64 left each warp one short chain of products and exponentials a tile, 0.84 us for 16 KB:
+  // 16 sequences x 32 heads of 2049 keys 48 us, bound by that.)
+  static constexpr int BC = kD == 128 ? 64 : 128;
+  static constexpr int STAGES = 3;
   static constexpr int KEY_GROUPS = 4 / kRowGroups, WKEYS = BC / KEY_GROUPS, ROWS = 16 * kRowGroups;
   static constexpr int NUM_THREADS = 160;
   static constexpr int HALVES = kD / 64;
-  static constexpr int HALF_BYTES = BC * 128;  // 64 keys x 64 values
+  static constexpr int HALF_BYTES = BC * 128;  // a tile's keys x 64 values
   static constexpr int KV_BYTES = BC * kD * 2, STAGE_BYTES = 2 * KV_BYTES, RING_BYTES = STAGES * STAGE_BYTES;
   static constexpr int JOIN_BYTES = 4 * 16 * 32 * 4;  // 32 columns of the warps' rows
-  static constexpr int SMEM_BYTES = RING_BYTES + JOIN_BYTES + 1024 + 2048;
+  // Up to 16 rows of queries come through shared memory with the first tile of their keys, rows 16 bytes apart (no two of a fragment in one
+  // bank); more are read by the warps themselves.
+  static constexpr bool kQueriesAhead = kRowGroups == 1;
+  static constexpr int Q_PITCH = kD * 2 + 16, Q_BYTES = kQueriesAhead ? 16 * Q_PITCH : 0;
+  static constexpr int CHAINS = WKEYS <= 32 ? 2 : 1;  // accumulators per 8 keys (even and odd 16 values of d)
+  static constexpr int SMEM_BYTES = RING_BYTES + JOIN_BYTES + Q_BYTES + 1024 + 1024;
   static_assert(2 * (SMEM_BYTES + 1024) <= 228 * 1024, "two CTAs an SM");
   using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
 
@@ -62,20 +73,20 @@ struct AttnTokens {
     int keys;      // of the sequence
     int p_lo;      // position of the first row's token
     int lo;        // first key of the first row's window
-    int flags;     // MASKED: some row does not see some key; FIRST, LAST of a (sequence, head)'s keys in this CTA; WHOLE: all of them
+    int flags;     // MASKED: some row does not see some key; FIRST, LAST of a (sequence, head)'s keys in this CTA; WHOLE: all of them; END: of all
     int slot;      // where a part goes
   };
-  enum : int { MASKED = 1, FIRST = 2, LAST = 4, WHOLE = 8 };
+  enum : int { MASKED = 1, FIRST = 2, LAST = 4, WHOLE = 8, END = 16 };
   struct Shared {
-    uint64_t full[STAGES], empty[STAGES];
+    uint64_t full[STAGES], empty[STAGES], q_empty;
     Tile tile[STAGES];
     float2 warp_ml[4][16];
-    long long before[5];  // tiles of the sequences before each warp's
-    long long range[2];
-    int found[3];         // sequence, head and tile that the range begins with
+    long long before[5];  // places of each warp's sequences
+    long long begin;      // the first place with a tile in this CTA's range
+    int found[3];         // its sequence (-1: there is none), head and tile
     volatile uint32_t abort_flag;
   };
-  static_assert(sizeof(Shared) <= 2048, "barrier block exceeds its shared-memory slot");
+  static_assert(sizeof(Shared) <= 1024, "barrier block exceeds its shared-memory slot");
 
   __device__ static __forceinline__ void report(Shared* sh, uint32_t code, uint32_t d0) {
     sh->abort_flag = 1u;
@@ -85,7 +96,9 @@ struct AttnTokens {
       g_paged_status[3] = 0u;
     }
   }
-  __device__ static __forceinline__ float weight(float x, float base) { return x == -INFINITY ? 0.f : ex2(x - base); }
+  // Weight of a partial result with maximum and sum ml; one of no key weighs nothing. (Scores that are all NaN leave a maximum of -inf and a sum
+  // of NaN, which has to reach the result.)
+  __device__ static __forceinline__ float weight(float2 ml, float base) { return ml.y == 0.f ? 0.f : ex2(ml.x - base); }
 
   // A sequence's tiles; one without a key has one too, in which no row sees anything.
   __device__ static __forceinline__ TileList tiles_of(const TokensArgs& p, int length, int* keys, int* p_lo) {
@@ -100,7 +113,8 @@ struct AttnTokens {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     float* join = reinterpret_cast<float*>(smem + RING_BYTES);
-    Shared* sh = reinterpret_cast<Shared*>(smem + RING_BYTES + JOIN_BYTES);
+    uint8_t* queries = smem + RING_BYTES + JOIN_BYTES;
+    Shared* sh = reinterpret_cast<Shared*>(queries + Q_BYTES);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rows = p.seq.each * p.group;
 
@@ -110,8 +124,9 @@ struct AttnTokens {
         mbar_init(&sh->full[s], 1);
         mbar_init(&sh->empty[s], 4);
       }
+      mbar_init(&sh->q_empty, 4);
       sh->abort_flag = 0u;
-      sh->range[0] = sh->range[1] = 0;
+      sh->found[0] = -1;
       fence_mbar_init();
     }
     if (threadIdx.x == 128) {
@@ -120,12 +135,12 @@ struct AttnTokens {
     }
     griddep_wait();
 
-    // All sequences' tiles, and where this CTA's range begins: a thread counts those of its run of sequences.
+    // All sequences' places, and where this CTA's range begins: a thread counts those of its run of sequences.
     const int per = (p.seq.count + NUM_THREADS - 1) / NUM_THREADS;
     const int b0 = min(static_cast<int>(threadIdx.x) * per, p.seq.count), b1 = min(b0 + per, p.seq.count);
     long long mine = 0;
     int keys, p_lo;
-    for (int b = b0; b < b1; ++b) mine += tiles_of(p, p.seq.lengths[b], &keys, &p_lo).count;
+    for (int b = b0; b < b1; ++b) mine += tiles_of(p, p.seq.lengths[b], &keys, &p_lo).count + kTokensPause;
     mine *= p.kv_heads;
     long long upto = mine;
 #pragma unroll
@@ -148,27 +163,37 @@ struct AttnTokens {
     if (g0 < g1 && g0 >= base && g0 < base + mine) {
       long long at = g0 - base;
       for (int b = b0; b < b1; ++b) {
-        const int n = tiles_of(p, p.seq.lengths[b], &keys, &p_lo).count;
-        if (at < static_cast<long long>(n) * p.kv_heads) {
-          sh->found[0] = b, sh->found[1] = static_cast<int>(at / n), sh->found[2] = static_cast<int>(at % n);
+        const int n = tiles_of(p, p.seq.lengths[b], &keys, &p_lo).count, places = n + kTokensPause;
+        if (at < static_cast<long long>(places) * p.kv_heads) {
+          int h = static_cast<int>(at / places), t = static_cast<int>(at % places), to = b;
+          long long begin = g0;
+          if (t >= n) {  // behind the last tile: the next (sequence, head)'s first one
+            begin += places - t;
+            t = 0;
+            if (++h == p.kv_heads) h = 0, ++to;
+          }
+          if (begin < g1) sh->found[0] = to, sh->found[1] = h, sh->found[2] = t, sh->begin = begin;
           break;
         }
-        at -= static_cast<long long>(n) * p.kv_heads;
+        at -= static_cast<long long>(places) * p.kv_heads;
       }
     }
     __syncthreads();
-    const int count = static_cast<int>(g1 - g0);
+    const bool any = sh->found[0] >= 0;
 
     if (warp == 4) {
       // ------------------------------------------------------------------ loads
       int4 meta = make_int4(-1, 0, 0, 0);
-      if (count > 0) {
-        int b = sh->found[0], h = sh->found[1], t = sh->found[2];
+      if (any) {
+        int b = sh->found[0], h = sh->found[1], t = sh->found[2], units = 0;
+        long long place = sh->begin;
         TileList list = tiles_of(p, p.seq.lengths[b], &keys, &p_lo);
         int next_length = b + 1 < p.seq.count ? p.seq.lengths[b + 1] : 0;
         const int boxes = BC >> p.box_log2;            // of 64 columns, in a tile of K or of V
         const int loads = boxes * HALVES * 2;          // at most 32: a lane each
         const int box = lane % boxes, half = lane / boxes % HALVES, is_v = lane / (boxes * HALVES);
+        const int tok = lane / p.group;                // of this lane's row of queries
+        const T* q_from = static_cast<const T*>(p.q) + tok * p.q_row + (lane - tok * p.group) * p.q_head;
         // this lane's page of tile t of sequence b; -1 (zeros) where no row sees any of the box
         auto page_of = [&](int b_, const TileList& list_, int keys_, int t_) {
           const int key = list_.tile_at(t_) * BC + (box << p.box_log2);
@@ -176,25 +201,29 @@ struct AttnTokens {
           return lane < loads && seen ? p.seq.page_of(b_, key) : -1;
         };
         int page = page_of(b, list, keys, t);
-        long long unit_begin = g0 - t;
-        for (int i = 0; i < count; ++i) {
+        long long unit_begin = place - t;
+        bool more = true;
+        for (int i = 0; more; ++i) {
           const int s = i % STAGES;
           const int key0 = list.tile_at(t) * BC;
-          const int this_page = page;
+          const int this_page = page, this_b = b, this_h = h;
           Tile tile;
           tile.b = b, tile.h = h, tile.key0 = key0, tile.keys = keys, tile.p_lo = p_lo, tile.lo = list.lo;
           const int p_hi = p_lo + p.seq.each - 1;
           const bool near = p.window <= 0 || key0 > p_hi - p.window || key0 + BC <= p.sinks;
           const bool whole = unit_begin >= g0 && unit_begin + list.count <= g1;
-          tile.flags = (key0 + BC > keys || key0 + BC > p_lo + 1 || !near ? MASKED : 0) | (i == 0 || t == 0 ? FIRST : 0) |
-                       (i == count - 1 || t == list.count - 1 ? LAST : 0) | (whole ? WHOLE : 0);
+          const bool first = i == 0 || t == 0;
+          tile.flags = (key0 + BC > keys || key0 + BC > p_lo + 1 || !near ? MASKED : 0) | (first ? FIRST : 0) | (whole ? WHOLE : 0);
           tile.slot = 2 * cta + (unit_begin >= g0 ? 1 : 0);
           if (!whole && unit_begin >= g0) meta = make_int4(b, h, ranges.owner(unit_begin + list.count - 1), 0);
-          const int this_h = h;
           // the next tile, and its pages while this one's stage is waited for
+          ++place;
+          bool last = false;
           if (++t == list.count) {
+            last = true;
             t = 0;
-            unit_begin += list.count;
+            place += kTokensPause;
+            unit_begin = place;
             if (++h == p.kv_heads) {
               h = 0;
               if (++b < p.seq.count) {
@@ -203,8 +232,14 @@ struct AttnTokens {
               }
             }
           }
-          if (i + 1 < count) page = page_of(b, list, keys, t);
-          const bool free = mbar_wait(&sh->empty[s], ((i / STAGES) & 1u) ^ 1u, &sh->abort_flag);
+          more = place < g1;
+          tile.flags |= (last || !more ? LAST : 0) | (more ? 0 : END);
+          if (more) page = page_of(b, list, keys, t);
+          bool free = mbar_wait(&sh->empty[s], ((i / STAGES) & 1u) ^ 1u, &sh->abort_flag);
+          if (kQueriesAhead && first) {
+            if (free) free = mbar_wait(&sh->q_empty, (units & 1u) ^ 1u, &sh->abort_flag);
+            ++units;
+          }
           if (!__all_sync(0xffffffffu, free)) {
             if (lane == 0) report(sh, PAGED_TIMEOUT_LOADS, static_cast<uint32_t>(i));
             break;
@@ -212,7 +247,7 @@ struct AttnTokens {
           uint8_t* st = smem + s * STAGE_BYTES;
           if (lane == 0) {
             sh->tile[s] = tile;
-            mbar_expect_tx(&sh->full[s], STAGE_BYTES);
+            mbar_expect_tx(&sh->full[s], STAGE_BYTES + (kQueriesAhead && first ? rows * kD * 2 : 0));
           }
           __syncwarp();
           if (lane < loads) {
@@ -220,6 +255,9 @@ struct AttnTokens {
             tma_load_4d(st + is_v * KV_BYTES + half * HALF_BYTES + (box << p.box_log2) * 128, is_v ? &p.tmV : &p.tmK, &sh->full[s], half * 64,
                         in_page, this_h, this_page);
           }
+          if (kQueriesAhead && first && lane < rows)
+            bulk_load_1d(queries + lane * Q_PITCH, q_from + static_cast<long long>(this_b) * p.seq.each * p.q_row + this_h * p.group * p.q_head, kD * 2,
+                         &sh->full[s]);
         }
       }
       if (lane == 0) {
@@ -227,7 +265,7 @@ struct AttnTokens {
         reinterpret_cast<int4*>(end)[cta] = meta;
       }
       __syncwarp();
-    } else if (count > 0) {
+    } else if (any) {
       const int q = lane >> 2, t = lane & 3;  // row and column pair of this lane in an accumulator tile
       const int rg = warp / KEY_GROUPS, kg = warp % KEY_GROUPS;
       const int mat = lane >> 3, mrow = lane & 7;
@@ -235,7 +273,7 @@ struct AttnTokens {
       float o[kD / 8][4];
       float m[2], l[2];
       int see[2], near[2];  // keys below `see`, of those from `near` on (and the sinks)
-      for (int i = 0; i < count; ++i) {
+      for (int i = 0;; ++i) {
         const int s = i % STAGES;
         const bool got = mbar_wait(&sh->full[s], (i / STAGES) & 1u, &sh->abort_flag);
         // (one outcome for all four: they meet again at the end of a (sequence, head))
@@ -250,7 +288,8 @@ struct AttnTokens {
           for (int e = 0; e < 2; ++e) {
             const int r = rg * 16 + q + 8 * e, i_tok = r / p.group;
             const bool live = r < rows;
-            const T* from = Q + (static_cast<long long>(tile.b) * p.seq.each + i_tok) * p.q_row + (tile.h * p.group + r - i_tok * p.group) * p.q_head;
+            const T* from = kQueriesAhead ? reinterpret_cast<const T*>(queries + r * Q_PITCH)
+                                          : Q + (static_cast<long long>(tile.b) * p.seq.each + i_tok) * p.q_row + (tile.h * p.group + r - i_tok * p.group) * p.q_head;
 #pragma unroll
             for (int ks = 0; ks < kD / 16; ++ks) {
               qf[ks][e] = live ? *reinterpret_cast<const uint32_t*>(from + ks * 16 + 2 * t) : 0u;
@@ -265,14 +304,20 @@ struct AttnTokens {
           for (int n = 0; n < kD / 8; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+          if (kQueriesAhead) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->q_empty);
+          }
         }
         const uint32_t kaddr = smem_u32(smem + s * STAGE_BYTES), vaddr = kaddr + KV_BYTES;
-        // two accumulators per 8 keys (even and odd 16 values of d): twice as many independent chains
-        float c[WKEYS / 8][4], c2[WKEYS / 8][4];
+        float c[WKEYS / 8][4], c2[CHAINS == 2 ? WKEYS / 8 : 1][4];
 #pragma unroll
         for (int n = 0; n < WKEYS / 8; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) c[n][e] = c2[n][e] = 0.f;
+          for (int e = 0; e < 4; ++e) {
+            c[n][e] = 0.f;
+            if (CHAINS == 2) c2[n][e] = 0.f;
+          }
 #pragma unroll
         for (int ks = 0; ks < kD / 32; ++ks) {
           const int unit = ks * 4 + mat;
@@ -282,13 +327,15 @@ struct AttnTokens {
             uint32_t b[4];
             ldmatrix_x4(b, kaddr + key * 128 + (unit >> 3) * HALF_BYTES + (((unit & 7) ^ (key & 7)) << 4));
             mma_16816<kBf16>(c[n], qf[2 * ks][0], qf[2 * ks][1], qf[2 * ks][2], qf[2 * ks][3], b[0], b[1]);
-            mma_16816<kBf16>(c2[n], qf[2 * ks + 1][0], qf[2 * ks + 1][1], qf[2 * ks + 1][2], qf[2 * ks + 1][3], b[2], b[3]);
+            mma_16816<kBf16>(CHAINS == 2 ? c2[n] : c[n], qf[2 * ks + 1][0], qf[2 * ks + 1][1], qf[2 * ks + 1][2], qf[2 * ks + 1][3], b[2], b[3]);
           }
         }
+        if constexpr (CHAINS == 2) {
 #pragma unroll
-        for (int n = 0; n < WKEYS / 8; ++n)
+          for (int n = 0; n < WKEYS / 8; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) c[n][e] += c2[n][e];
+            for (int e = 0; e < 4; ++e) c[n][e] += c2[n][e];
+        }
         if (tile.flags & MASKED) {
           const int first = tile.key0 + kg * WKEYS;
 #pragma unroll
@@ -359,7 +406,7 @@ struct AttnTokens {
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->empty[s]);
-        if (!(tile.flags & LAST)) continue;
+        if (!(tile.flags & LAST)) continue;  // (the CTA's last tile is the last of its rows)
 
         // ---- the end of these rows' keys in this CTA: the warps' sums, 32 columns at a time
 #pragma unroll
@@ -375,7 +422,7 @@ struct AttnTokens {
           float top = -INFINITY;
 #pragma unroll
           for (int k = 0; k < KEY_GROUPS; ++k) top = fmaxf(top, sh->warp_ml[rg * KEY_GROUPS + k][q + 8 * h].x);
-          f[h] = weight(m[h], top);
+          f[h] = weight(make_float2(m[h], l[h]), top);
         }
 #pragma unroll
         for (int cc = 0; cc < kD / 32; ++cc) {
@@ -400,7 +447,7 @@ struct AttnTokens {
 #pragma unroll
             for (int k = 0; k < KEY_GROUPS; ++k) {
               const float2 ml = sh->warp_ml[g * KEY_GROUPS + k][row];
-              sum_l = fmaf(ml.y, weight(ml.x, top), sum_l);
+              sum_l = fmaf(ml.y, weight(ml, top), sum_l);
             }
             const int r = g * 16 + row;
             if (r >= rows) continue;
@@ -419,6 +466,7 @@ struct AttnTokens {
           }
           named_bar_sync(1, 128);
         }
+        if (tile.flags & END) break;
       }
     }
     if (sh->abort_flag != 0u) {  // loads still in flight land before the ring is given up
@@ -434,15 +482,15 @@ __global__ void __launch_bounds__(160, 2) attention_tokens_kernel(const __grid_c
   AttnTokens<kD, kBf16, kRowGroups>::run(p);
 }
 
-// The parts of a (sequence, key head) whose keys began in CTA blockIdx.x of the kernel above and ended in a later one's. A warp takes a
-// row at a time, or, of few rows, a share of a row's parts.
+// The parts of a (sequence, key head) whose keys began in CTA blockIdx.x of the kernel above and ended in a later one's. 16 warps: as many to a row
+// as there are for it, each with a share of the parts, eight at a time.
 template <int kD, bool kBf16>
-__global__ void __launch_bounds__(256) attention_tokens_join_kernel(const __grid_constant__ TokensArgs p, int ctas) {
+__global__ void __launch_bounds__(512) attention_tokens_join_kernel(const __grid_constant__ TokensArgs p, int ctas) {
   using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
   using Vec = typename std::conditional<kD == 128, float4, float2>::type;
-  constexpr int PER = kD / 32;
-  __shared__ float acc[8][kD];
-  __shared__ float2 ml_of[8];
+  constexpr int PER = kD / 32, WARPS = 16, AT_ONCE = 8;
+  __shared__ float acc[WARPS][kD];
+  __shared__ float2 ml_of[WARPS];
   griddep_wait();
   griddep_launch_dependents();
   const int rows = p.seq.each * p.group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -451,27 +499,39 @@ __global__ void __launch_bounds__(256) attention_tokens_join_kernel(const __grid
   if (meta.x < 0) return;
   const int first = static_cast<int>(blockIdx.x), n = meta.z - first + 1;  // CTAs with a part: slot 1 of the first, slot 0 of the others
   int shares = 1;  // warps of a row
-  while (shares < 8 && rows * shares < 8 && n > shares) shares *= 2;
-  const int at_once = 8 / shares;
-  for (int r0 = 0; r0 < rows; r0 += at_once) {
+  while (shares < WARPS && rows * shares < WARPS && n > shares) shares *= 2;
+  const int rows_at_once = WARPS / shares;
+  for (int r0 = 0; r0 < rows; r0 += rows_at_once) {
     const int r = r0 + warp / shares, share = warp % shares;
     const bool live = r < rows;
     float top = -INFINITY, sum = 0.f, a[PER];
 #pragma unroll
     for (int e = 0; e < PER; ++e) a[e] = 0.f;
-    if (live) {
-      auto part = [&](int i) { return (2ll * (first + i) + (i == 0 ? 1 : 0)) * rows + r; };
-      for (int i = share + lane * shares; i < n; i += 32 * shares) top = fmaxf(top, ml[part(i)].x);
+    for (int i0 = share; live && i0 < n; i0 += shares * AT_ONCE) {
+      float2 s[AT_ONCE];
+      Vec v[AT_ONCE];
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-#pragma unroll 4
-      for (int i = share; i < n; i += shares) {
-        const float2 s = ml[part(i)];
-        const Vec v = reinterpret_cast<const Vec*>(p.parts + part(i) * kD)[lane];
-        const float f = s.x == -INFINITY ? 0.f : ex2(s.x - top);
-        sum = fmaf(f, s.y, sum);
+      for (int u = 0; u < AT_ONCE; ++u) {
+        const int i = i0 + u * shares;
+        const long long part = (2ll * (first + i) + (i == 0 ? 1 : 0)) * rows + r;
+        s[u] = i < n ? ml[part] : make_float2(-INFINITY, 0.f);
+        if (i < n) v[u] = reinterpret_cast<const Vec*>(p.parts + part * kD)[lane];
+      }
+      float now = top;
 #pragma unroll
-        for (int e = 0; e < PER; ++e) a[e] = fmaf(f, reinterpret_cast<const float*>(&v)[e], a[e]);
+      for (int u = 0; u < AT_ONCE; ++u) now = fmaxf(now, s[u].x);
+      const float old = sum == 0.f ? 0.f : ex2(top - now);
+      top = now;
+      sum *= old;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) a[e] *= old;
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+        if (s[u].y == 0.f) continue;  // (no key in sight: zeros, or no part)
+        const float f = ex2(s[u].x - top);
+        sum = fmaf(f, s[u].y, sum);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) a[e] = fmaf(f, reinterpret_cast<const float*>(&v[u])[e], a[e]);
       }
     }
     if (shares > 1) {
@@ -487,7 +547,7 @@ __global__ void __launch_bounds__(256) attention_tokens_join_kernel(const __grid
         for (int e = 0; e < PER; ++e) a[e] = 0.f;
         for (int w = 0; w < shares; ++w) {
           const float2 s = ml_of[warp + w];
-          const float f = s.x == -INFINITY ? 0.f : ex2(s.x - all);
+          const float f = s.y == 0.f ? 0.f : ex2(s.x - all);
           sum = fmaf(f, s.y, sum);
 #pragma unroll
           for (int e = 0; e < PER; ++e) a[e] = fmaf(f, acc[warp + w][lane * PER + e], a[e]);

@@ -195,6 +195,32 @@ def test_other_streams_at_once():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("case", [([900, 64], 1, 8, 2, 128, 16, BF), ([20], 1, 4, 4, 64, 16, FP), ([900, 64], [40, 64], 8, 2, 64, 16, FP), ([3000], [1], 8, 2, 128, 16, BF)], ids=ids)
+def test_queries_and_scores_that_are_no_numbers(case):
+    """A query of NaN gives NaN, a row by itself; scores of +inf give NaN as the formula's inf - inf does, of -inf no weight."""
+    step = Step(*case)
+    want, tol = step.oracle()
+    step.q[0, 1] = float("nan")
+    got = matmul_op.attention_paged(*step.args())
+    assert bool(got[0, 1].isnan().all())
+    got[0, 1], want[0, 1] = 0, 0
+    assert_close(got, want, tol)
+    step = Step(*case)
+    step.k[0][0, -1], step.q[0, 0] = float("inf"), step.q[0, 0].abs() + 0.25
+    step.put(0)
+    if sum(step.new) == 1 or step.new[0] == 1:  # (the last key: the first row sees it)
+        got = matmul_op.attention_paged(*step.args())
+        assert bool(got[0, 0].isnan().all())
+    step.q[0, 0] = -step.q[0, 0]
+    step.k[0][0, -1] = float("inf")
+    got = matmul_op.attention_paged(*step.args())
+    step.k[0][0, -1] = 60000.0  # a finite key of no weight, in place of one of none
+    want, tol = step.oracle()
+    if step.lens[0] > 1:
+        assert bool(((got[0, 0].double() - want[0, 0]).abs() <= tol[0, 0]).all())
+
+
+@pytest.mark.gpu
 def test_no_rows():
     step = Step([10, 20], 1, 8, 2, 128, 16, BF)
     got = matmul_op.attention_paged(step.q[:0], *step.args()[1:5])
