@@ -125,7 +125,7 @@ int append(Launch& launch, const AppendArgs& a, int d, bool interleaved) {
 
 // ---------------------------------------------------------------------------------------------------- attention
 __device__ unsigned int g_paged_status[4];  // {code, block, detail, detail}; 0 = no wait ran out
-enum : uint32_t { PAGED_TIMEOUT_LOADS = 1, PAGED_TIMEOUT_ATTENTION = 2 };
+enum : uint32_t { PAGED_TIMEOUT_LOADS = 1, PAGED_TIMEOUT_ATTENTION = 2, PAGED_TIMEOUT_UNIT = 3 };
 
 #include "paged_prompt.cuh"
 #include "paged_tokens.cuh"
@@ -222,7 +222,7 @@ int attention_tokens(int device, cudaStream_t st, const kcg_paged_cache* c, cons
   EncodeFn encode;
   if (int r = encoder(&encode)) return r;
   TokensArgs p{};
-  const int tile = c->d == 128 ? 64 : 128, box = c->page < tile ? c->page : tile;
+  const int most = q->window > 0 ? 16 : c->d == 128 ? 64 : 128, box = c->page < most ? c->page : most;  // keys of a box: see attention_prompt()
   if (int r = encode_cache(encode, &p.tmK, c, c->K, c->k_stride, box)) return r;
   if (int r = encode_cache(encode, &p.tmV, c, c->V, c->v_stride, box)) return r;
   p.seq = sequences_of(c, q->rows);
@@ -293,7 +293,8 @@ int attention_prompt(int device, cudaStream_t st, const kcg_paged_cache* c, cons
                                     : static_cast<long long>((p.seq.each + pair - 1) / pair) * c->sequences;
   if (slots > 0x7fffffffLL) return fail(KCG_E_TOO_LARGE, "attention_paged: too many rows");
   p.slots = static_cast<int>(slots);
-  const int box = c->page < 128 ? c->page : 128;
+  // Keys of a box: of a page, or of 32 where a window's keys begin anywhere and are laid out from a box's border on.
+  const int most = q->window > 0 ? 32 : 128, box = c->page < most ? c->page : most;
   while ((1 << p.box_log2) < box) ++p.box_log2;
   const bool bf16 = c->dtype == KCG_DTYPE_BFLOAT16;
   {

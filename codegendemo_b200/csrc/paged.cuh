@@ -39,20 +39,28 @@ struct Sequences {
   }
 };
 
-// The tiles of `tile` keys that the rows at positions p_lo .. of a sequence of `keys` keys see some of: those of the first `sinks`
-// keys that lie before the window of the first row, then those from that window's start on.
-struct TileList {
-  int first, window0, count;  // tiles of the sinks; first tile behind them; all
-  int lo;                     // first key of the first row's window
-  __device__ __forceinline__ TileList(int keys, int p_lo, int window, int sinks, int tile) {
-    lo = window > 0 && p_lo >= window ? p_lo - window + 1 : 0;
-    const int s = min(min(sinks, lo), keys);
-    first = s / tile + (s % tile ? 1 : 0);
-    window0 = max(lo / tile, first);
-    const int end = keys / tile + (keys % tile ? 1 : 0);
-    count = first + max(0, end - window0);
+// The keys that rows at positions p_lo .. see some of, laid end to end in whole boxes (parts of pages, `box` keys, a power of two): those of the first
+// `sinks` keys that lie before the first row's window, then those from that window on, up to `end`. A place v below `lead` is key v, others key
+// v + shift. (With a window of 1024 and 4 sinks 64 tokens see 9 tiles of 128; as tiles of a sequence's keys the same are 10 or 11.)
+struct KeyList {
+  int lead, shift;  // places of the sinks, when they are apart; keys between them and the others
+  int lo;           // place of the first key of the first row's window: places from `sinks` to here are of no row's keys
+  int count;        // places
+  __device__ __forceinline__ KeyList() {}
+  __device__ __forceinline__ KeyList(int end, int p_lo, int window, int sinks, int box) {
+    const int first = window > 0 && p_lo >= window ? p_lo - window + 1 : 0;
+    const int from = first & -box;
+    lead = sinks < from ? (sinks + box - 1) & -box : from;
+    shift = from - lead;
+    if (shift == 0) lead = 0;  // (one piece)
+    lo = first - shift;
+    count = place(end);
   }
-  __device__ __forceinline__ int tile_at(int i) const { return i < first ? i : window0 + i - first; }
+  // Keys below x as places.
+  __device__ __forceinline__ int place(int x) const { return x - shift > lead ? x - shift : min(x, lead); }
+  __device__ __forceinline__ int key(int v) const { return v < lead ? v : v + shift; }
+  // Whether some row may see a key of the box at place v.
+  __device__ __forceinline__ bool seen(int v, int box, int sinks) const { return v < count && (v < sinks || v + box > lo); }
 };
 
 // The sequence whose rows hold `row`, or -1; asked by a whole (converged) warp, 32 places at a time. (The last sequence that starts at

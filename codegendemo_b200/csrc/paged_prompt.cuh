@@ -2,15 +2,19 @@
 // tokens that stay visible. The form of the fused attention kernel (AttnFwd2 in kcg_attention.cu, where its roles, meetings and figures are
 // described) over pages:
 //
-// One CTA takes two tiles of 128 rows: the query heads that share a key head, of as many tokens as fit (32 tokens x 4 heads, say), so that every
-// key tile is loaded once for all of them. It walks the 128-key tiles that its rows see: those of the sinks, then from the first row's window to
+// A CTA takes two tiles of 128 rows at a time: the query heads that share a key head, of as many tokens as fit (32 tokens x 4 heads, say), so that
+// every key tile is loaded once for all of them. It walks the keys that its rows see in tiles of 128: the sinks, then from the first row's window to
 // the last row's position; a warp masks a tile only where one of its 32 rows does not see all of it.
-//   warp 0    loads: both Q tiles once, then K and V tiles through two-stage rings, a lane a box of a page; page numbers one tile ahead
+//   warp 0    loads: both Q tiles, then K and V tiles through two-stage rings, a lane a box of a page; page numbers one tile ahead
 //   warp 1    tcgen05.mma: S = Q K^T, O += P V with P in tensor memory
 //   warp 2    waits for K and V in the issuer's place, and overwrites values that no row sees with zeros (0 x NaN would not vanish)
+//   warp 3    the next pair of tiles, while the loads of this one end
 //   warps 4-7 softmax of tile 0, warps 8-11 of tile 1, a row a thread
-// Bound by what bounds that kernel, the chain scores - softmax - product of a tile against the other tile's, and the power cap.
-// kKeySplit: where the tiles do not fill the GPU, the CTAs of a cluster share the keys of one, and join their results in shared memory.
+// Bound by what bounds that kernel, the chain scores - softmax - product of a tile against the other tile's, and the power cap. A window makes
+// a pair of tiles short, nine steps of 1.7 us at a window of 1024: then what comes before the first step and behind the last one counts. So a CTA
+// stays where it is and takes over a CTA that has not been launched yet (cluster launch control) as its next pair: the queries and keys of that one
+// are loaded, and its first scores computed, while this one's rows are finished.
+// kKeySplit: where the tiles do not fill the GPU, the CTAs of a cluster share the keys of one pair, and join their results in shared memory.
 #pragma once
 
 struct PromptArgs {
@@ -44,14 +48,29 @@ struct AttnPrompt {
   static constexpr uint32_t IDESC_O = make_instr_desc(FMT, 0u, 1u, 128u, kD);
   using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
 
+  // A pair of tiles (and, with others, a share of its keys).
+  struct Unit {
+    KeyList list;
+    int b, head, row0, tokens;  // sequence, key head, first row of the step, tokens (0: none)
+    int p_lo, keys;             // position of the first token; keys of the sequence
+    int v0, steps, tiles;       // first place of the keys, tiles of keys, tiles of rows
+    int end;                    // there is no further unit, and this is none
+  };
   struct Barriers {
-    uint64_t q_full;
+    uint64_t q_full, q_empty;
     uint64_t k_full[K_STAGES], k_empty[K_STAGES], v_full[V_STAGES], v_empty[V_STAGES];
     uint64_t s_full[TILES];  // S_t of the current step is complete
-    uint64_t o_full[TILES];  // the last P_t V has retired
+    uint64_t o_full[TILES];  // the last P_t V of a unit has retired
+    uint64_t unit_full[2], unit_empty[2];  // a unit is there, every warp has read it
+    uint64_t unit_wanted;                  // the loads of the current unit come to their end
+    uint64_t taken;                        // the answer to a request for another CTA's work
+    uint4 answer;                          // (16-byte aligned: barriers stand before it)
+    Unit unit[2];
     uint32_t tmem_base;
     volatile uint32_t abort_flag;
   };
+  static_assert(sizeof(Barriers) <= 1024, "barrier block exceeds its shared-memory slot");
+  static constexpr int UNIT_WARPS = 11;  // that read a unit
 
   // Named barriers: see AttnFwd2. Every meeting takes place in every step whatever else happened.
   static constexpr uint32_t BAR_PART = 1;  // + t: the first P_PART keys of P_t are in tensor memory and O_t is rescaled
@@ -68,19 +87,16 @@ struct AttnPrompt {
     }
   }
 
-  // What a CTA works on: tokens token0 .. of sequence b, `rows` of them. The pairs of tiles of sequence b take the slots from
-  // (its first row) / (tokens of a pair) + b on, of which there are enough: so the slot's sequence is found by a search over the first rows
-  // alone, and some slots have no tokens.
-  struct Place {
-    int b, row0, tokens;  // sequence, first row of the step, tokens (0: none)
-    int p_lo;             // position of the first
-    int hi;               // keys that the last one sees (or some, at the table's end)
-    int keys;             // of the sequence
-  };
-  __device__ static __forceinline__ Place place(const PromptArgs& p, int slot) {
+  // The pairs of tiles of sequence b take the slots from (its first row) / (tokens of a pair) + b on, of which there are enough: so a slot's
+  // sequence is found by a search over the first rows alone, and some slots have no tokens. Asked by a whole warp.
+  __device__ static __forceinline__ Unit unit_of(const PromptArgs& p, int index, int rank) {
     const Sequences& s = p.seq;
     const int pair = TILES * p.tile_tokens, lane = threadIdx.x & 31;
-    Place x{};
+    const int slot = p.slots - 1 - index / p.kv_heads;  // (the last tokens of a sequence, which see the most keys, first)
+    Unit x;
+    x.head = index % p.kv_heads;
+    x.end = x.tokens = x.steps = x.v0 = x.row0 = x.p_lo = x.keys = 0;
+    x.tiles = 1;
     int t;
     if (!s.starts) {
       const int each = (s.each + pair - 1) / pair;
@@ -98,13 +114,48 @@ struct AttnPrompt {
       t = slot - (s.start(lo) / pair + lo);
     }
     const int first = s.start(x.b), n = s.start(x.b + 1) - first;
-    if (t < 0 || t >= (n + pair - 1) / pair || n <= 0) return x;
-    const int length = s.lengths[x.b];
-    x.tokens = min(pair, n - t * pair);
-    x.row0 = first + t * pair;
-    x.keys = s.keys(length);
-    x.p_lo = max(length, 0) - n + t * pair;  // (a negative length: no keys)
-    x.hi = max(0, min(x.keys, x.p_lo + x.tokens));
+    if (t >= 0 && n > 0 && t < (n + pair - 1) / pair) {
+      const int length = s.lengths[x.b];
+      x.tokens = min(pair, n - t * pair);
+      x.tiles = x.tokens > p.tile_tokens ? 2 : 1;
+      x.row0 = first + t * pair;
+      x.keys = s.keys(length);
+      x.p_lo = max(length, 0) - n + t * pair;  // (a negative length: no keys)
+    }
+    x.list = KeyList(x.tokens > 0 ? max(0, min(x.keys, x.p_lo + x.tokens)) : 0, x.p_lo, p.window, p.sinks, 1 << p.box_log2);
+    const int steps = x.list.count / BC + (x.list.count % BC ? 1 : 0);
+    const int step0 = kKeySplit ? static_cast<int>(static_cast<long long>(steps) * rank / p.splits) : 0;
+    x.steps = (kKeySplit ? static_cast<int>(static_cast<long long>(steps) * (rank + 1) / p.splits) : steps) - step0;
+    x.v0 = step0 * BC;
+    return x;
+  }
+
+  // Bits below n, of 32.
+  __device__ static __forceinline__ uint32_t below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
+
+  // Takes over a CTA of this grid that has not been launched yet, if there is one; 16 bytes of answer.
+  __device__ static __forceinline__ void request_cta(uint4* answer, uint64_t* bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+                 :
+                 : "r"(smem_u32(answer)), "r"(smem_u32(bar))
+                 : "memory");
+  }
+  // Its blockIdx.x, or -1: there was none (and none may be asked for again).
+  __device__ static __forceinline__ int requested_cta(const uint4* answer) {
+    int x;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        ".reg .b128 a;\n\t"
+        ".reg .b32 y, z, w;\n\t"
+        "ld.shared.b128 a, [%1];\n\t"
+        "mov.b32 %0, -1;\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, y, z, w}, a;\n\t"
+        "}\n"
+        : "=&r"(x)
+        : "r"(smem_u32(answer))
+        : "memory");
     return x;
   }
 
@@ -114,8 +165,6 @@ struct AttnPrompt {
     Barriers* bars = reinterpret_cast<Barriers*>(smem + RING_BYTES);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = kKeySplit ? static_cast<int>(cluster_cta_rank()) : 0;
-    const int unit = static_cast<int>(blockIdx.x) / (kKeySplit ? p.splits : 1);
-    const int head = unit % p.kv_heads;
 
     griddep_launch_dependents();
     if (threadIdx.x == 0) {
@@ -123,9 +172,13 @@ struct AttnPrompt {
       tma_prefetch_desc(&p.tmK);
       tma_prefetch_desc(&p.tmV);
       mbar_init(&bars->q_full, 1);
+      mbar_init(&bars->q_empty, 1);
       for (int s = 0; s < K_STAGES; ++s) mbar_init(&bars->k_full[s], 1), mbar_init(&bars->k_empty[s], 1);
       for (int s = 0; s < V_STAGES; ++s) mbar_init(&bars->v_full[s], 1), mbar_init(&bars->v_empty[s], 1);
       for (int t = 0; t < TILES; ++t) mbar_init(&bars->s_full[t], 1), mbar_init(&bars->o_full[t], 1);
+      for (int s = 0; s < 2; ++s) mbar_init(&bars->unit_full[s], 1), mbar_init(&bars->unit_empty[s], UNIT_WARPS);
+      mbar_init(&bars->unit_wanted, 1);
+      mbar_init(&bars->taken, 1);
       bars->abort_flag = 0u;
       fence_mbar_init();
       fence_proxy_async_smem();
@@ -134,150 +187,222 @@ struct AttnPrompt {
       tmem_alloc(&bars->tmem_base, TMEM_COLS);
       tmem_relinquish();
     }
-    griddep_wait();
-    // (the last tokens of a sequence, which see the most keys, first)
-    const Place at = place(p, p.slots - 1 - unit / p.kv_heads);
-    const TileList list(at.hi, at.p_lo, p.window, p.sinks, BC);
-    const int steps = at.tokens > 0 ? list.count : 0;
-    const int step0 = kKeySplit ? static_cast<int>(static_cast<long long>(steps) * rank / p.splits) : 0;
-    const int nkv = (kKeySplit ? static_cast<int>(static_cast<long long>(steps) * (rank + 1) / p.splits) : steps) - step0;
-    const int tiles = at.tokens > p.tile_tokens ? 2 : 1;
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
+    griddep_wait();
     const uint32_t tmem_base = bars->tmem_base;
+
+    // The next unit, for each warp that works on it. All read the same ones, whatever went wrong (the wait does not look at the abort flag and is
+    // longer than those that it follows from), so that the meetings on the way come out even.
+    int taken = 0;
+    auto next_unit = [&](Unit* x) {
+      const int slot = taken & 1;
+      const bool got = __all_sync(0xffffffffu, mbar_wait_for(&bars->unit_full[slot], (taken >> 1) & 1u, 8 * KCG_WAIT_LIMIT_NS));
+      if (!got) {
+        if (lane == 0) report(bars, PAGED_TIMEOUT_UNIT, static_cast<uint32_t>(taken), warp);
+        return false;
+      }
+      *x = bars->unit[slot];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->unit_empty[slot]);
+      ++taken;
+      return x->end == 0;
+    };
 
     // Registers: 384 threads are launched with 168 each; the control warpgroup keeps 56, the softmax warpgroups take
     // 224 (56 + 2 * 224 = 3 * 168), which a row's 128 scores need.
     if (warp < 4) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-      if (warp == 0 && nkv > 0) {
+      if (warp == 0) {
         // ------------------------------------------------------------------ loads
-        if (lane == 0) {
-          mbar_expect_tx(&bars->q_full, tiles * HALVES * p.tile_tokens * p.group * 128);
-          for (int t = 0; t < tiles; ++t)
-#pragma unroll
-            for (int b = 0; b < HALVES; ++b)
-              tma_load_3d(smem + t * Q_BYTES + b * BOX_BYTES, &p.tmQ, &bars->q_full, b * 64, head * p.group, at.row0 + t * p.tile_tokens);
-        }
         const int boxes = BC >> p.box_log2, loads = boxes * HALVES;  // (at most 32)
         const int box = lane % boxes, half = lane / boxes;
-        // this lane's page of a step; -1 (zeros) where no row sees any of the box
-        auto page_of = [&](int j) {
-          const int key = list.tile_at(step0 + j) * BC + (box << p.box_log2);
-          const bool seen = key < at.hi && (key + (1 << p.box_log2) > list.lo || key < p.sinks);
-          return lane < loads && seen ? p.seq.page_of(at.b, key) : -1;
-        };
-        int page = page_of(0);
-        for (int j = 0; j < nkv; ++j) {
-          const int ks = j % K_STAGES, vs = j % V_STAGES;
-          const int in_page = (list.tile_at(step0 + j) * BC + (box << p.box_log2)) & ((1 << p.seq.page_log2) - 1);
-          const int this_page = page;
-          if (j + 1 < nkv) page = page_of(j + 1);
-          const uint32_t to = half * BOX_BYTES + (box << p.box_log2) * 128;
-          bool free = mbar_wait(&bars->k_empty[ks], ((j / K_STAGES) & 1u) ^ 1u, &bars->abort_flag);
-          if (!__all_sync(0xffffffffu, free)) {
-            if (lane == 0) report(bars, PAGED_TIMEOUT_LOADS, j, 0u);
-            break;
+        const uint32_t to = half * BOX_BYTES + (box << p.box_log2) * 128;
+        uint32_t it = 0, queries = 0;  // steps and units with keys so far
+        bool ok = true;
+        for (Unit x; next_unit(&x);) {
+          // this lane's key and page of a step; page -1 (zeros) where no row sees any of the box
+          auto page_of = [&](int j, int* key) {
+            const int v = x.v0 + j * BC + (box << p.box_log2);
+            *key = x.list.key(v);
+            return lane < loads && x.list.seen(v, 1 << p.box_log2, p.sinks) ? p.seq.page_of(x.b, *key) : -1;
+          };
+          int key = 0, page = x.steps > 0 ? page_of(0, &key) : -1;
+          if (x.steps == 0 && lane == 0) mbar_arrive(&bars->unit_wanted);
+          if (x.steps > 0 && ok) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&bars->q_empty, (queries & 1u) ^ 1u, &bars->abort_flag));
+            ++queries;
+            if (!ok && lane == 0) report(bars, PAGED_TIMEOUT_LOADS, it, 2u);
+            if (ok && lane == 0) {
+              mbar_expect_tx(&bars->q_full, x.tiles * HALVES * p.tile_tokens * p.group * 128);
+              for (int t = 0; t < x.tiles; ++t)
+#pragma unroll
+                for (int b = 0; b < HALVES; ++b)
+                  tma_load_3d(smem + t * Q_BYTES + b * BOX_BYTES, &p.tmQ, &bars->q_full, b * 64, x.head * p.group, x.row0 + t * p.tile_tokens);
+            }
+            __syncwarp();
           }
-          if (lane == 0) mbar_expect_tx(&bars->k_full[ks], KV_BYTES);
-          __syncwarp();
-          if (lane < loads) tma_load_4d(smem + OFF_K + ks * KV_BYTES + to, &p.tmK, &bars->k_full[ks], half * 64, in_page, head, this_page);
-          free = mbar_wait(&bars->v_empty[vs], ((j / V_STAGES) & 1u) ^ 1u, &bars->abort_flag);
-          if (!__all_sync(0xffffffffu, free)) {
-            if (lane == 0) report(bars, PAGED_TIMEOUT_LOADS, j, 1u);
-            break;
+          for (int j = 0; j < x.steps; ++j, ++it) {
+            if (j == max(0, x.steps - 2) && lane == 0) mbar_arrive(&bars->unit_wanted);
+            if (!ok) continue;
+            const int ks = it % K_STAGES, vs = it % V_STAGES;
+            const int in_page = key & ((1 << p.seq.page_log2) - 1), this_page = page;
+            if (j + 1 < x.steps) page = page_of(j + 1, &key);
+            ok = __all_sync(0xffffffffu, mbar_wait(&bars->k_empty[ks], ((it / K_STAGES) & 1u) ^ 1u, &bars->abort_flag));
+            if (!ok) {
+              if (lane == 0) report(bars, PAGED_TIMEOUT_LOADS, it, 0u);
+              continue;
+            }
+            if (lane == 0) mbar_expect_tx(&bars->k_full[ks], KV_BYTES);
+            __syncwarp();
+            if (lane < loads) tma_load_4d(smem + OFF_K + ks * KV_BYTES + to, &p.tmK, &bars->k_full[ks], half * 64, in_page, x.head, this_page);
+            ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_empty[vs], ((it / V_STAGES) & 1u) ^ 1u, &bars->abort_flag));
+            if (!ok) {
+              if (lane == 0) report(bars, PAGED_TIMEOUT_LOADS, it, 1u);
+              continue;
+            }
+            if (lane == 0) mbar_expect_tx(&bars->v_full[vs], KV_BYTES);
+            __syncwarp();
+            if (lane < loads) tma_load_4d(smem + OFF_V + vs * KV_BYTES + to, &p.tmV, &bars->v_full[vs], half * 64, in_page, x.head, this_page);
           }
-          if (lane == 0) mbar_expect_tx(&bars->v_full[vs], KV_BYTES);
-          __syncwarp();
-          if (lane < loads) tma_load_4d(smem + OFF_V + vs * KV_BYTES + to, &p.tmV, &bars->v_full[vs], half * 64, in_page, head, this_page);
         }
-      } else if (warp == 1 && nkv > 0) {
+      } else if (warp == 1) {
         // ---------------------------------------------------------------- products
-        const bool q_there = mbar_wait(&bars->q_full, 0u, &bars->abort_flag);
-        if (!q_there && lane == 0) report(bars, PAGED_TIMEOUT_ATTENTION, 0u, 0u);
-        __syncwarp();
         const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
         const uint64_t qdesc = make_smem_desc(smem_u32(smem), 16, 1024, SWZ_128B);
         const uint64_t kdesc = make_smem_desc(smem_u32(smem + OFF_K), 16, 1024, SWZ_128B);
         const uint64_t vdesc = make_smem_desc(smem_u32(smem + OFF_V), BOX_BYTES, 1024, SWZ_128B);
-        auto issue_s = [&](int t, int i) {
-          const uint64_t ad = qdesc + t * (Q_BYTES >> 4), bd = kdesc + (i % K_STAGES) * (KV_BYTES >> 4);
+        uint32_t it0 = 0, queries = 0;
+        for (Unit x; next_unit(&x);) {
+          const int nkv = x.steps, tiles = x.tiles;
+          if (nkv == 0) continue;
+          auto issue_s = [&](int t, int i) {
+            const uint64_t ad = qdesc + t * (Q_BYTES >> 4), bd = kdesc + ((it0 + i) % K_STAGES) * (KV_BYTES >> 4);
 #pragma unroll
-          for (int ks = 0; ks < kD / 16; ++ks) {
-            const uint32_t in_row = (ks * 32) % 128, box = (ks * 32) / 128;
-            umma_ss<false>(tmem + t * BC, ad + ((box * BOX_BYTES + in_row) >> 4), bd + ((box * BOX_BYTES + in_row) >> 4), IDESC_S, ks > 0 ? 1u : 0u);
-          }
-          umma_commit(&bars->s_full[t]);
-          if (t == tiles - 1) umma_commit(&bars->k_empty[i % K_STAGES]);
-        };
-        auto issue_pv = [&](int t, int j, int ks0, int ks1) {
-          const uint64_t vd = vdesc + (j % V_STAGES) * (KV_BYTES >> 4);
-#pragma unroll
-          for (int ks = 0; ks < BC / 16; ++ks)
-            if (ks >= ks0 && ks < ks1)
-              umma_ts<false>(tmem + COL_O + t * kD, tmem + t * BC + ks * 8, vd + ((ks * 16 * 128) >> 4), IDESC_O, (j > 0 || ks > 0) ? 1u : 0u);
-        };
-        named_bar_sync(BAR_KV, KV_THREADS);  // the first K tile
-        tc_fence_after_sync();
-        if (elect_one()) {
-          issue_s(0, 0);
-          if (!kApart && tiles == 2) issue_s(1, 0);
-        }
-        __syncwarp();
-        for (int j = 0; j < nkv; ++j) {
-          named_bar_sync(BAR_KV, KV_THREADS);
-#pragma unroll
-          for (int t = 0; t < TILES; ++t) {
-            if (t >= tiles) continue;
-            named_bar_sync(BAR_PART + t, PT_THREADS);
-            tc_fence_after_sync();
-            if (elect_one()) {
-              if (kApart && j == 0 && t == 0 && tiles == 2) issue_s(1, 0);
-              issue_pv(t, j, 0, P_PART / 16);
+            for (int ks = 0; ks < kD / 16; ++ks) {
+              const uint32_t in_row = (ks * 32) % 128, box = (ks * 32) / 128;
+              umma_ss<false>(tmem + t * BC, ad + ((box * BOX_BYTES + in_row) >> 4), bd + ((box * BOX_BYTES + in_row) >> 4), IDESC_S, ks > 0 ? 1u : 0u);
             }
-            __syncwarp();
-            named_bar_sync(BAR_FULL + t, PT_THREADS);
-            tc_fence_after_sync();
-            if (elect_one()) {
-              issue_pv(t, j, P_PART / 16, BC / 16);
-              if (t == tiles - 1) umma_commit(&bars->v_empty[j % V_STAGES]);
-              if (j + 1 < nkv) {
-                issue_s(t, j + 1);
-              } else {
-                umma_commit(&bars->o_full[t]);
+            umma_commit(&bars->s_full[t]);
+            if (t == tiles - 1) {
+              umma_commit(&bars->k_empty[(it0 + i) % K_STAGES]);
+              if (i == nkv - 1) umma_commit(&bars->q_empty);
+            }
+          };
+          auto issue_pv = [&](int t, int j, int ks0, int ks1) {
+            const uint64_t vd = vdesc + ((it0 + j) % V_STAGES) * (KV_BYTES >> 4);
+#pragma unroll
+            for (int ks = 0; ks < BC / 16; ++ks)
+              if (ks >= ks0 && ks < ks1)
+                umma_ts<false>(tmem + COL_O + t * kD, tmem + t * BC + ks * 8, vd + ((ks * 16 * 128) >> 4), IDESC_O, (j > 0 || ks > 0) ? 1u : 0u);
+          };
+          const bool q_there = __all_sync(0xffffffffu, mbar_wait(&bars->q_full, queries & 1u, &bars->abort_flag));
+          ++queries;
+          if (!q_there && lane == 0) report(bars, PAGED_TIMEOUT_ATTENTION, 0u, 0u);
+          __syncwarp();
+          named_bar_sync(BAR_KV, KV_THREADS);  // the first K tile
+          tc_fence_after_sync();
+          if (elect_one()) {
+            issue_s(0, 0);
+            if (!kApart && tiles == 2) issue_s(1, 0);
+          }
+          __syncwarp();
+          for (int j = 0; j < nkv; ++j) {
+            named_bar_sync(BAR_KV, KV_THREADS);
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+              if (t >= tiles) continue;
+              named_bar_sync(BAR_PART + t, PT_THREADS);
+              tc_fence_after_sync();
+              if (elect_one()) {
+                if (kApart && j == 0 && t == 0 && tiles == 2) issue_s(1, 0);
+                issue_pv(t, j, 0, P_PART / 16);
               }
+              __syncwarp();
+              named_bar_sync(BAR_FULL + t, PT_THREADS);
+              tc_fence_after_sync();
+              if (elect_one()) {
+                issue_pv(t, j, P_PART / 16, BC / 16);
+                if (t == tiles - 1) umma_commit(&bars->v_empty[(it0 + j) % V_STAGES]);
+                if (j + 1 < nkv) {
+                  issue_s(t, j + 1);
+                } else {
+                  umma_commit(&bars->o_full[t]);
+                }
+              }
+              __syncwarp();
             }
-            __syncwarp();
           }
+          it0 += nkv;
         }
-      } else if (warp == 2 && nkv > 0) {
+      } else if (warp == 2) {
         // ------------------------------------------- waits for K and V in the issuer's place
         bool ok = true;
-        auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t what, int i) {
+        auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t what, uint32_t i) {
           if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, &bars->abort_flag));
-          if (!ok && lane == 0) report(bars, PAGED_TIMEOUT_ATTENTION, what, static_cast<uint32_t>(i));
+          if (!ok && lane == 0) report(bars, PAGED_TIMEOUT_ATTENTION, what, i);
         };
-        wait(&bars->k_full[0], 0u, 1u, 0);
-        named_bar_sync(BAR_KV, KV_THREADS);
-        for (int j = 0; j < nkv; ++j) {
-          wait(&bars->v_full[j % V_STAGES], (j / V_STAGES) & 1u, 2u, j);
-          // values of keys that none of the rows sees: behind the last one's, and between the sinks and the first one's window
-          const int key0 = list.tile_at(step0 + j) * BC;
-          const int end = max(0, min(BC, at.hi - key0)), gap0 = max(0, min(BC, p.sinks - key0)), gap1 = max(0, min(BC, list.lo - key0));
-          if (end < BC || gap0 < gap1) {
-            uint8_t* v = smem + OFF_V + (j % V_STAGES) * KV_BYTES;
-            for (int u = lane; u < BC * 8 * HALVES; u += 32) {
-              const int k = u / 8 % BC;
-              if (k >= end || (k >= gap0 && k < gap1)) *reinterpret_cast<uint4*>(v + u * 16) = make_uint4(0u, 0u, 0u, 0u);  // (whole rows: in any order)
-            }
-            fence_proxy_async_smem();
-          }
-          if (j + 1 < nkv) wait(&bars->k_full[(j + 1) % K_STAGES], ((j + 1) / K_STAGES) & 1u, 1u, j + 1);
-          __syncwarp();
+        uint32_t it = 0;
+        for (Unit x; next_unit(&x);) {
+          if (x.steps == 0) continue;
+          wait(&bars->k_full[it % K_STAGES], (it / K_STAGES) & 1u, 1u, it);
           named_bar_sync(BAR_KV, KV_THREADS);
+          for (int j = 0; j < x.steps; ++j, ++it) {
+            wait(&bars->v_full[it % V_STAGES], (it / V_STAGES) & 1u, 2u, it);
+            // values of keys that none of the rows sees: behind the last one's, and between the sinks and the first one's window
+            const int v0 = x.v0 + j * BC;
+            const int end = max(0, min(BC, x.list.count - v0)), gap0 = max(0, min(BC, p.sinks - v0)), gap1 = max(0, min(BC, x.list.lo - v0));
+            if (end < BC || gap0 < gap1) {
+              uint8_t* v = smem + OFF_V + (it % V_STAGES) * KV_BYTES;
+              for (int u = lane; u < BC * 8 * HALVES; u += 32) {
+                const int k = u / 8 % BC;
+                if (k >= end || (k >= gap0 && k < gap1)) *reinterpret_cast<uint4*>(v + u * 16) = make_uint4(0u, 0u, 0u, 0u);  // (whole rows: in any order)
+              }
+              fence_proxy_async_smem();
+            }
+            if (j + 1 < x.steps) wait(&bars->k_full[(it + 1) % K_STAGES], ((it + 1) / K_STAGES) & 1u, 1u, it + 1);
+            __syncwarp();
+            named_bar_sync(BAR_KV, KV_THREADS);
+          }
         }
-      }  // (warp 3 only gives its registers)
+      } else {
+        // ------------------------------------------------------------------ units
+        // One after the other into two slots. A slot is free once every warp has read the unit in it; what has gone wrong ends the row of units with
+        // one that says so, and where a slot does not become free, with none: the warps' wait for it ends by itself.
+        int index = static_cast<int>(blockIdx.x) / (kKeySplit ? p.splits : 1);
+        bool more = true;
+        for (uint32_t u = 0; more; ++u) {
+          Unit x = unit_of(p, index < 0 ? 0 : index, rank);
+          if (index < 0 || bars->abort_flag != 0u) x.end = 1;
+          bool free = u < 2 || mbar_wait_for(&bars->unit_empty[u & 1], ((u >> 1) & 1u) ^ 1u, KCG_WAIT_LIMIT_NS);
+          if (!__all_sync(0xffffffffu, free)) {
+            if (lane == 0) report(bars, PAGED_TIMEOUT_UNIT, u, 32u);
+            break;
+          }
+          if (lane == 0) {
+            bars->unit[u & 1] = x;
+            mbar_arrive(&bars->unit_full[u & 1]);
+          }
+          __syncwarp();
+          if (x.end) break;
+          free = mbar_wait(&bars->unit_wanted, u & 1u, &bars->abort_flag);
+          if (kKeySplit || !__all_sync(0xffffffffu, free)) {
+            index = -1;
+            continue;
+          }
+          if (lane == 0) {
+            mbar_expect_tx(&bars->taken, 16);
+            request_cta(&bars->answer, &bars->taken);
+          }
+          __syncwarp();
+          const bool answered = __all_sync(0xffffffffu, mbar_wait(&bars->taken, u & 1u, &bars->abort_flag));
+          index = answered ? requested_cta(&bars->answer) : -1;
+          if (!answered && lane == 0) report(bars, PAGED_TIMEOUT_UNIT, u, 33u);
+          fence_proxy_async_smem();  // (the next answer is written behind this reading)
+          __syncwarp();
+        }
+      }
       if constexpr (kKeySplit) {  // the two meetings of the cluster that join the partial results
         __syncwarp();
         cluster_sync_all();
@@ -291,43 +416,50 @@ struct AttnPrompt {
       const int row = q * 32 + lane;    // query row of this thread inside its tile
       const uint32_t lane_addr = static_cast<uint32_t>(q * 32) << 16;
       const uint32_t col_s = tmem_base + lane_addr + t * BC, col_o = tmem_base + lane_addr + COL_O + t * kD;
-      const int token = t * p.tile_tokens + row / p.group;
-      const bool live = row < p.tile_tokens * p.group && token < at.tokens;
-      // keys below `see`, of those from `near` on and the sinks; rows without a token (whose scores are of whatever lies there) are not masked
-      const int position = at.p_lo + token;
-      const int see = live ? min(position + 1, at.keys) : 0x7fffffff;
-      const int near = live && p.window > 0 && position >= p.window ? position - p.window + 1 : 0;
+      const int token = row < p.tile_tokens * p.group ? t * p.tile_tokens + row / p.group : 0x40000000;  // of the unit's (which has less than that)
+      const uint64_t scale2 = f32x2(p.scale_log2, p.scale_log2);
+      uint32_t scores = 0, results = 0;  // of this tile so far
+      bool alive = true;                 // no wait of this warp has run out
+      for (Unit x; next_unit(&x);) {
+      const bool live = token < x.tokens;
+      // places of keys below `see`, of those from `near` on and the sinks; rows without a token (whose scores are of whatever lies there) are not masked
+      const int position = x.p_lo + token;
+      const int see = live ? x.list.place(min(position + 1, x.keys)) : 0x7fffffff;
+      const int near = live && p.window > 0 && position >= p.window ? position - p.window + 1 - x.list.shift : 0;
       // m: the row's running maximum, which the exponentials of a step are taken against, in the exp2 domain: the maximum itself, so that
       // the largest probability is exactly 1 and does not lose a bit to the 16-bit P.
       float m = -INFINITY;
       uint64_t sum2[2] = {f32x2(0.f, 0.f), f32x2(0.f, 0.f)};
-      bool ok = nkv > 0 && t < tiles;
-      const int mine = ok ? nkv : 0;
-      const uint64_t scale2 = f32x2(p.scale_log2, p.scale_log2);
+      const int mine = t < x.tiles ? x.steps : 0;
       int j = 0;
-      for (; j < mine; ++j) {
-        const bool got = mbar_wait_for(&bars->s_full[t], j & 1u, 4 * KCG_WAIT_LIMIT_NS);
-        if (!__all_sync(0xffffffffu, got)) {
+      for (; j < mine && alive; ++j) {
+        alive = __all_sync(0xffffffffu, mbar_wait_for(&bars->s_full[t], scores & 1u, 4 * KCG_WAIT_LIMIT_NS));
+        if (!alive) {
           if (lane == 0) report(bars, PAGED_TIMEOUT_ATTENTION, 3u, static_cast<uint32_t>(j));
-          ok = false;
           break;
         }
+        ++scores;
         tc_fence_after_sync();
         uint32_t sr[4][32];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(col_s + c * 32, sr[c]);
-        const int key0 = list.tile_at(step0 + j) * BC;
-        const int end = see - key0, gap0 = p.sinks - key0, gap1 = near - key0;
+        const int v0 = x.v0 + j * BC;
+        const int end = see - v0, gap0 = p.sinks - v0, gap1 = near - v0;
         const bool masked = __any_sync(0xffffffffu, end < BC || (gap1 > 0 && gap0 < BC));
         tmem_ld_wait();
 #pragma unroll
         for (int c = 0; c < 4; ++c) pin_32(sr[c]);
         if (masked) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < 4; ++c) {
+            // a bit a key that the row sees (a test of a bit and a select each, where 32 comparisons with three borders are five)
+            const uint32_t bits = below(end - c * 32) & (below(gap0 - c * 32) | ~below(gap1 - c * 32));
+            if (__any_sync(0xffffffffu, bits != 0xffffffffu)) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (c * 32 + i >= end || (c * 32 + i >= gap0 && c * 32 + i < gap1)) sr[c][i] = __float_as_uint(-INFINITY);
+              for (int i = 0; i < 32; ++i)
+                if (!(bits >> i & 1u)) sr[c][i] = __float_as_uint(-INFINITY);
+            }
+          }
         }
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         auto max_of = [&](int c) {
@@ -412,14 +544,12 @@ struct AttnPrompt {
       }
       const float2 s01 = f32x2_split(add_f32x2(sum2[0], sum2[1]));
       const float l = s01.x + s01.y;
-      if (ok) {
-        const bool got = mbar_wait(&bars->o_full[t], 0u, &bars->abort_flag);
-        if (!__all_sync(0xffffffffu, got)) {
-          if (lane == 0) report(bars, PAGED_TIMEOUT_ATTENTION, 4u, 0u);
-          ok = false;
-        }
+      if (mine > 0 && alive) {
+        alive = __all_sync(0xffffffffu, mbar_wait(&bars->o_full[t], results & 1u, &bars->abort_flag));
+        if (!alive && lane == 0) report(bars, PAGED_TIMEOUT_ATTENTION, 4u, 0u);
+        ++results;
       }
-      const bool gave_up = mine > 0 && !ok;
+      const bool gave_up = mine > 0 && !alive;
       if constexpr (kKeySplit) {
         // Partial results: once the products of both tiles have retired, the operand ring holds this CTA's O rows (fp32, not normalised,
         // 16-byte units XOR-swizzled by the row: a warp writes 32 rows at a time) and their {maximum, sum}; then each CTA joins an equal
@@ -428,11 +558,11 @@ struct AttnPrompt {
         constexpr int OFF_ML = TILES * BR * kD * 4;
         static_assert(OFF_ML + TILES * BR * 8 <= RING_BYTES, "the partial result must fit the ring");
         bool both = true;
-        if (ok && tiles == 2) {
+        if (mine > 0 && !gave_up && x.tiles == 2) {
           both = __all_sync(0xffffffffu, mbar_wait(&bars->o_full[t ^ 1], 0u, &bars->abort_flag));
           if (!both && lane == 0) report(bars, PAGED_TIMEOUT_ATTENTION, 5u, 0u);
         }
-        if (t < tiles && both && !gave_up) {
+        if (t < x.tiles && both && !gave_up) {
           tc_fence_after_sync();
           const int r = t * BR + row;
           uint8_t* to = smem + r * kD * 4;
@@ -456,13 +586,13 @@ struct AttnPrompt {
         __syncwarp();
         cluster_sync_all();
         {
-          const int all = tiles * BR * UNITS;
+          const int all = x.tiles * BR * UNITS;
           const int u0 = all / p.splits * rank + min(rank, all % p.splits), u1 = u0 + all / p.splits + (rank < all % p.splits ? 1 : 0);
           const uint32_t base_addr = smem_u32(smem);
           for (int i = u0 + static_cast<int>(threadIdx.x) - 128; i < u1; i += TILES * 128) {
             const int r = i / UNITS, u = i % UNITS, in_tile = r % BR;
             const int tok = r / BR * p.tile_tokens + in_tile / p.group;
-            if (in_tile >= p.tile_tokens * p.group || tok >= at.tokens) continue;
+            if (in_tile >= p.tile_tokens * p.group || tok >= x.tokens) continue;
             const uint32_t ml_addr = base_addr + OFF_ML + r * 8;
             const uint32_t o_addr = base_addr + r * kD * 4 + ((u ^ (r & (UNITS - 1))) << 4);
             float top = -INFINITY;
@@ -481,8 +611,8 @@ struct AttnPrompt {
               sum = fmaf(f, ml.y, sum);
             }
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            T* out = reinterpret_cast<T*>(p.o) + static_cast<long long>(at.row0 + tok) * p.o_row +
-                     static_cast<long long>(head * p.group + in_tile % p.group) * p.o_head + u * 4;
+            T* out = reinterpret_cast<T*>(p.o) + static_cast<long long>(x.row0 + tok) * p.o_row +
+                     static_cast<long long>(x.head * p.group + in_tile % p.group) * p.o_head + u * 4;
             *reinterpret_cast<uint2*>(out) = make_uint2(pack_pair<kBf16>(a.x * inv, a.y * inv), pack_pair<kBf16>(a.z * inv, a.w * inv));
           }
         }
@@ -491,8 +621,8 @@ struct AttnPrompt {
       } else {
         tc_fence_after_sync();
         const float inv = mine == 0 || l == 0.f ? 0.f : 1.f / l;
-        T* out = reinterpret_cast<T*>(p.o) + static_cast<long long>(at.row0 + token) * p.o_row +
-                 static_cast<long long>(head * p.group + row % p.group) * p.o_head;
+        T* out = reinterpret_cast<T*>(p.o) + static_cast<long long>(x.row0 + token) * p.o_row +
+                 static_cast<long long>(x.head * p.group + row % p.group) * p.o_head;
 #pragma unroll
         for (int c = 0; c < kD / 32; ++c) {
           uint32_t r[32];
@@ -515,6 +645,7 @@ struct AttnPrompt {
           }
         }
       }
+      }  // (units; a cluster has one, and its meetings are in it)
     }
 
     // ---------------------------------------------------------------- common exit

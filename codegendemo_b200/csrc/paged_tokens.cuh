@@ -62,17 +62,17 @@ struct AttnTokens {
   static constexpr bool kQueriesAhead = kRowGroups == 1;
   static constexpr int Q_PITCH = kD * 2 + 16, Q_BYTES = kQueriesAhead ? 16 * Q_PITCH : 0;
   static constexpr int CHAINS = WKEYS <= 32 ? 2 : 1;  // accumulators per 8 keys (even and odd 16 values of d)
-  static constexpr int SMEM_BYTES = RING_BYTES + JOIN_BYTES + Q_BYTES + 1024 + 1024;
+  static constexpr int SMEM_BYTES = RING_BYTES + JOIN_BYTES + Q_BYTES + 1024 + 1280;
   static_assert(2 * (SMEM_BYTES + 1024) <= 228 * 1024, "two CTAs an SM");
   using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
 
   // What a stage holds, for the warps that read it.
   struct Tile {
     int b, h;      // sequence, key head
-    int key0;      // first key of the tile
+    int v0;        // first place of the tile's keys
     int keys;      // of the sequence
     int p_lo;      // position of the first row's token
-    int lo;        // first key of the first row's window
+    KeyList list;
     int flags;     // MASKED: some row does not see some key; FIRST, LAST of a (sequence, head)'s keys in this CTA; WHOLE: all of them; END: of all
     int slot;      // where a part goes
   };
@@ -86,7 +86,7 @@ struct AttnTokens {
     int found[3];         // its sequence (-1: there is none), head and tile
     volatile uint32_t abort_flag;
   };
-  static_assert(sizeof(Shared) <= 1024, "barrier block exceeds its shared-memory slot");
+  static_assert(sizeof(Shared) <= 1280, "barrier block exceeds its shared-memory slot");
 
   __device__ static __forceinline__ void report(Shared* sh, uint32_t code, uint32_t d0) {
     sh->abort_flag = 1u;
@@ -100,14 +100,17 @@ struct AttnTokens {
   // of NaN, which has to reach the result.)
   __device__ static __forceinline__ float weight(float2 ml, float base) { return ml.y == 0.f ? 0.f : ex2(ml.x - base); }
 
-  // A sequence's tiles; one without a key has one too, in which no row sees anything.
-  __device__ static __forceinline__ TileList tiles_of(const TokensArgs& p, int length, int* keys, int* p_lo) {
-    *keys = p.seq.keys(length);
-    *p_lo = max(length, 0) - p.seq.each;
-    TileList t(*keys, *p_lo, p.window, p.sinks, BC);
-    t.count = max(t.count, 1);
-    return t;
-  }
+  // A sequence's keys and tiles; one without a key has a tile too, in which no row sees anything.
+  struct Keys {
+    KeyList list;
+    int keys, p_lo, count;  // of the sequence; position of the first row's token; tiles
+    __device__ __forceinline__ Keys(const TokensArgs& p, int length) {
+      keys = p.seq.keys(length);
+      p_lo = max(length, 0) - p.seq.each;
+      list = KeyList(keys, p_lo, p.window, p.sinks, 1 << p.box_log2);
+      count = max(1, list.count / BC + (list.count % BC ? 1 : 0));
+    }
+  };
 
   __device__ static void run(const TokensArgs& p) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -139,8 +142,7 @@ struct AttnTokens {
     const int per = (p.seq.count + NUM_THREADS - 1) / NUM_THREADS;
     const int b0 = min(static_cast<int>(threadIdx.x) * per, p.seq.count), b1 = min(b0 + per, p.seq.count);
     long long mine = 0;
-    int keys, p_lo;
-    for (int b = b0; b < b1; ++b) mine += tiles_of(p, p.seq.lengths[b], &keys, &p_lo).count + kTokensPause;
+    for (int b = b0; b < b1; ++b) mine += Keys(p, p.seq.lengths[b]).count + kTokensPause;
     mine *= p.kv_heads;
     long long upto = mine;
 #pragma unroll
@@ -163,7 +165,7 @@ struct AttnTokens {
     if (g0 < g1 && g0 >= base && g0 < base + mine) {
       long long at = g0 - base;
       for (int b = b0; b < b1; ++b) {
-        const int n = tiles_of(p, p.seq.lengths[b], &keys, &p_lo).count, places = n + kTokensPause;
+        const int n = Keys(p, p.seq.lengths[b]).count, places = n + kTokensPause;
         if (at < static_cast<long long>(places) * p.kv_heads) {
           int h = static_cast<int>(at / places), t = static_cast<int>(at % places), to = b;
           long long begin = g0;
@@ -187,39 +189,41 @@ struct AttnTokens {
       if (any) {
         int b = sh->found[0], h = sh->found[1], t = sh->found[2], units = 0;
         long long place = sh->begin;
-        TileList list = tiles_of(p, p.seq.lengths[b], &keys, &p_lo);
+        Keys seq(p, p.seq.lengths[b]);
         int next_length = b + 1 < p.seq.count ? p.seq.lengths[b + 1] : 0;
         const int boxes = BC >> p.box_log2;            // of 64 columns, in a tile of K or of V
         const int loads = boxes * HALVES * 2;          // at most 32: a lane each
         const int box = lane % boxes, half = lane / boxes % HALVES, is_v = lane / (boxes * HALVES);
         const int tok = lane / p.group;                // of this lane's row of queries
         const T* q_from = static_cast<const T*>(p.q) + tok * p.q_row + (lane - tok * p.group) * p.q_head;
-        // this lane's page of tile t of sequence b; -1 (zeros) where no row sees any of the box
-        auto page_of = [&](int b_, const TileList& list_, int keys_, int t_) {
-          const int key = list_.tile_at(t_) * BC + (box << p.box_log2);
-          const bool seen = key < keys_ && (key + (1 << p.box_log2) > list_.lo || key < p.sinks);
-          return lane < loads && seen ? p.seq.page_of(b_, key) : -1;
+        // this lane's key and page of tile t of sequence b; page -1 (zeros) where no row sees any of the box
+        int key;
+        auto page_of = [&]() {
+          const int v = t * BC + (box << p.box_log2);
+          key = seq.list.key(v);
+          return lane < loads && seq.list.seen(v, 1 << p.box_log2, p.sinks) ? p.seq.page_of(b, key) : -1;
         };
-        int page = page_of(b, list, keys, t);
+        int page = page_of();
         long long unit_begin = place - t;
         bool more = true;
         for (int i = 0; more; ++i) {
           const int s = i % STAGES;
-          const int key0 = list.tile_at(t) * BC;
-          const int this_page = page, this_b = b, this_h = h;
+          const int v0 = t * BC;
+          const int this_page = page, in_page = key & ((1 << p.seq.page_log2) - 1), this_b = b, this_h = h;
           Tile tile;
-          tile.b = b, tile.h = h, tile.key0 = key0, tile.keys = keys, tile.p_lo = p_lo, tile.lo = list.lo;
-          const int p_hi = p_lo + p.seq.each - 1;
-          const bool near = p.window <= 0 || key0 > p_hi - p.window || key0 + BC <= p.sinks;
-          const bool whole = unit_begin >= g0 && unit_begin + list.count <= g1;
+          tile.b = b, tile.h = h, tile.v0 = v0, tile.keys = seq.keys, tile.p_lo = seq.p_lo, tile.list = seq.list;
+          // every row sees every key: up to the first row's position, from the last one's window on or among the sinks
+          const int p_hi = seq.p_lo + p.seq.each - 1, near = p.window > 0 && p_hi >= p.window ? p_hi - p.window + 1 - seq.list.shift : 0;
+          const bool all = v0 + BC <= seq.list.place(min(seq.keys, seq.p_lo + 1)) && (v0 >= near || v0 + BC <= p.sinks);
+          const bool whole = unit_begin >= g0 && unit_begin + seq.count <= g1;
           const bool first = i == 0 || t == 0;
-          tile.flags = (key0 + BC > keys || key0 + BC > p_lo + 1 || !near ? MASKED : 0) | (first ? FIRST : 0) | (whole ? WHOLE : 0);
+          tile.flags = (all ? 0 : MASKED) | (first ? FIRST : 0) | (whole ? WHOLE : 0);
           tile.slot = 2 * cta + (unit_begin >= g0 ? 1 : 0);
-          if (!whole && unit_begin >= g0) meta = make_int4(b, h, ranges.owner(unit_begin + list.count - 1), 0);
+          if (!whole && unit_begin >= g0) meta = make_int4(b, h, ranges.owner(unit_begin + seq.count - 1), 0);
           // the next tile, and its pages while this one's stage is waited for
           ++place;
           bool last = false;
-          if (++t == list.count) {
+          if (++t == seq.count) {
             last = true;
             t = 0;
             place += kTokensPause;
@@ -227,14 +231,14 @@ struct AttnTokens {
             if (++h == p.kv_heads) {
               h = 0;
               if (++b < p.seq.count) {
-                list = tiles_of(p, next_length, &keys, &p_lo);
+                seq = Keys(p, next_length);
                 next_length = b + 1 < p.seq.count ? p.seq.lengths[b + 1] : 0;
               }
             }
           }
           more = place < g1;
           tile.flags |= (last || !more ? LAST : 0) | (more ? 0 : END);
-          if (more) page = page_of(b, list, keys, t);
+          if (more) page = page_of();
           bool free = mbar_wait(&sh->empty[s], ((i / STAGES) & 1u) ^ 1u, &sh->abort_flag);
           if (kQueriesAhead && first) {
             if (free) free = mbar_wait(&sh->q_empty, (units & 1u) ^ 1u, &sh->abort_flag);
@@ -250,11 +254,9 @@ struct AttnTokens {
             mbar_expect_tx(&sh->full[s], STAGE_BYTES + (kQueriesAhead && first ? rows * kD * 2 : 0));
           }
           __syncwarp();
-          if (lane < loads) {
-            const int in_page = (key0 + (box << p.box_log2)) & ((1 << p.seq.page_log2) - 1);
+          if (lane < loads)
             tma_load_4d(st + is_v * KV_BYTES + half * HALF_BYTES + (box << p.box_log2) * 128, is_v ? &p.tmV : &p.tmK, &sh->full[s], half * 64,
                         in_page, this_h, this_page);
-          }
           if (kQueriesAhead && first && lane < rows)
             bulk_load_1d(queries + lane * Q_PITCH, q_from + static_cast<long long>(this_b) * p.seq.each * p.q_row + this_h * p.group * p.q_head, kD * 2,
                          &sh->full[s]);
@@ -272,7 +274,7 @@ struct AttnTokens {
       uint32_t qf[kD / 16][4];
       float o[kD / 8][4];
       float m[2], l[2];
-      int see[2], near[2];  // keys below `see`, of those from `near` on (and the sinks)
+      int see[2], near[2];  // places of keys below `see`, of those from `near` on (and the sinks)
       for (int i = 0;; ++i) {
         const int s = i % STAGES;
         const bool got = mbar_wait(&sh->full[s], (i / STAGES) & 1u, &sh->abort_flag);
@@ -296,8 +298,8 @@ struct AttnTokens {
               qf[ks][e + 2] = live ? *reinterpret_cast<const uint32_t*>(from + ks * 16 + 2 * t + 8) : 0u;
             }
             const int position = tile.p_lo + (live ? i_tok : 0);
-            see[e] = min(position + 1, tile.keys);
-            near[e] = p.window > 0 && position >= p.window ? position - p.window + 1 : 0;
+            see[e] = tile.list.place(min(position + 1, tile.keys));
+            near[e] = p.window > 0 && position >= p.window ? position - p.window + 1 - tile.list.shift : 0;
             m[e] = -INFINITY, l[e] = 0.f;
           }
 #pragma unroll
@@ -337,7 +339,7 @@ struct AttnTokens {
             for (int e = 0; e < 4; ++e) c[n][e] += c2[n][e];
         }
         if (tile.flags & MASKED) {
-          const int first = tile.key0 + kg * WKEYS;
+          const int first = tile.v0 + kg * WKEYS;
 #pragma unroll
           for (int n = 0; n < WKEYS / 8; ++n)
 #pragma unroll
@@ -349,7 +351,7 @@ struct AttnTokens {
           bool zeroed = false;
           for (int u = lane; u < WKEYS * (kD / 8); u += 32) {
             const int k = u / (kD / 8), piece = u % (kD / 8), key = first + k, at = kg * WKEYS + k;
-            if (key >= tile.keys || (key < tile.lo && key >= p.sinks)) {
+            if (key >= tile.list.count || (key < tile.list.lo && key >= p.sinks)) {
               *reinterpret_cast<uint4*>(smem + s * STAGE_BYTES + KV_BYTES + (piece >> 3) * HALF_BYTES + at * 128 + (((piece & 7) ^ (at & 7)) << 4)) =
                   make_uint4(0u, 0u, 0u, 0u);
               zeroed = true;
