@@ -5,10 +5,11 @@
 // A CTA takes two tiles of 128 rows at a time: the query heads that share a key head, of as many tokens as fit (32 tokens x 4 heads, say), so that
 // every key tile is loaded once for all of them. It walks the keys that its rows see in tiles of 128: the sinks, then from the first row's window to
 // the last row's position; a warp masks a tile only where one of its 32 rows does not see all of it.
-//   warp 0    loads: both Q tiles, then K and V tiles through two-stage rings, a lane a box of a page; page numbers one tile ahead
+//   warp 0    loads: both Q tiles and K tiles through a two-stage ring, a lane a box of a page; page numbers one tile ahead
 //   warp 1    tcgen05.mma: S = Q K^T, O += P V with P in tensor memory
 //   warp 2    waits for K and V in the issuer's place, and overwrites values that no row sees with zeros (0 x NaN would not vanish)
-//   warp 3    the next pair of tiles, while the loads of this one end
+//   warp 3    loads V tiles in the same way (one warp for both was the limit with pages of 16 tokens, 32 boxes a step); the next pair of tiles,
+//             while the loads of this one end
 //   warps 4-7 softmax of tile 0, warps 8-11 of tile 1, a row a thread
 // Bound by what bounds that kernel, the chain scores - softmax - product of a tile against the other tile's, and the power cap. A window makes
 // a pair of tiles short, nine steps of 1.7 us at a window of 1024: then what comes before the first step and behind the last one counts. So a CTA
@@ -39,7 +40,10 @@ struct AttnPrompt {
   static constexpr int BOX_BYTES = 128 * 128;  // 128 rows x 64 values
   static constexpr int Q_BYTES = BR * kD * 2, KV_BYTES = BC * kD * 2;
   static constexpr int OFF_K = TILES * Q_BYTES, OFF_V = OFF_K + K_STAGES * KV_BYTES, RING_BYTES = OFF_V + V_STAGES * KV_BYTES;
-  static constexpr int SMEM_BYTES = RING_BYTES + 2048;  // 1 KB alignment slack + barriers
+  // Results leave through shared memory, 32 rows x 128 bytes of a warp at a time, as whole 128-byte lines. (A row a thread, 16 bytes of 32 rows a
+  // store, kept the load-store unit busy for 4000 cycles a pair of tiles.)
+  static constexpr int OUT_BYTES = 8 * 32 * 128;
+  static constexpr int SMEM_BYTES = RING_BYTES + OUT_BYTES + 2048;  // 1 KB alignment slack + barriers
   static constexpr int P_PART = kD == 128 ? 96 : 64;    // keys of a step after which P V starts
   static constexpr bool kApart = kD == 64;              // tile 1 starts half a step after tile 0
   static constexpr uint32_t COL_O = TILES * BC, TMEM_COLS = 512;
@@ -62,7 +66,6 @@ struct AttnPrompt {
     uint64_t s_full[TILES];  // S_t of the current step is complete
     uint64_t o_full[TILES];  // the last P_t V of a unit has retired
     uint64_t unit_full[2], unit_empty[2];  // a unit is there, every warp has read it
-    uint64_t unit_wanted;                  // the loads of the current unit come to their end
     uint64_t taken;                        // the answer to a request for another CTA's work
     uint4 answer;                          // (16-byte aligned: barriers stand before it)
     Unit unit[2];
@@ -70,7 +73,7 @@ struct AttnPrompt {
     volatile uint32_t abort_flag;
   };
   static_assert(sizeof(Barriers) <= 1024, "barrier block exceeds its shared-memory slot");
-  static constexpr int UNIT_WARPS = 11;  // that read a unit
+  static constexpr int UNIT_WARPS = 11;  // that read a unit (warp 3 makes them)
 
   // Named barriers: see AttnFwd2. Every meeting takes place in every step whatever else happened.
   static constexpr uint32_t BAR_PART = 1;  // + t: the first P_PART keys of P_t are in tensor memory and O_t is rescaled
@@ -162,7 +165,7 @@ struct AttnPrompt {
   __device__ static void run(const PromptArgs& p) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    Barriers* bars = reinterpret_cast<Barriers*>(smem + RING_BYTES);
+    Barriers* bars = reinterpret_cast<Barriers*>(smem + RING_BYTES + OUT_BYTES);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = kKeySplit ? static_cast<int>(cluster_cta_rank()) : 0;
 
@@ -177,7 +180,6 @@ struct AttnPrompt {
       for (int s = 0; s < V_STAGES; ++s) mbar_init(&bars->v_full[s], 1), mbar_init(&bars->v_empty[s], 1);
       for (int t = 0; t < TILES; ++t) mbar_init(&bars->s_full[t], 1), mbar_init(&bars->o_full[t], 1);
       for (int s = 0; s < 2; ++s) mbar_init(&bars->unit_full[s], 1), mbar_init(&bars->unit_empty[s], UNIT_WARPS);
-      mbar_init(&bars->unit_wanted, 1);
       mbar_init(&bars->taken, 1);
       bars->abort_flag = 0u;
       fence_mbar_init();
@@ -214,57 +216,46 @@ struct AttnPrompt {
     // 224 (56 + 2 * 224 = 3 * 168), which a row's 128 scores need.
     if (warp < 4) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+      // This lane's box of a tile of K or V: its place in the tile and in shared memory; a load of it from a page (-1: zeros).
+      const int boxes = BC >> p.box_log2, loads = boxes * HALVES;  // (at most 32)
+      const int box = lane % boxes, half = lane / boxes;
+      const uint32_t to = half * BOX_BYTES + (box << p.box_log2) * 128;
+      auto page_of = [&](const Unit& x, int j, int* key) {
+        const int v = x.v0 + j * BC + (box << p.box_log2);
+        *key = x.list.key(v);
+        return lane < loads && x.list.seen(v, 1 << p.box_log2, p.sinks) ? p.seq.page_of(x.b, *key) : -1;
+      };
+      auto load = [&](uint8_t* tile, const CUtensorMap* tm, uint64_t* bar, const Unit& x, int key, int page) {
+        if (lane == 0) mbar_expect_tx(bar, KV_BYTES);
+        __syncwarp();
+        if (lane < loads) tma_load_4d(tile + to, tm, bar, half * 64, key & ((1 << p.seq.page_log2) - 1), x.head, page);
+      };
       if (warp == 0) {
-        // ------------------------------------------------------------------ loads
-        const int boxes = BC >> p.box_log2, loads = boxes * HALVES;  // (at most 32)
-        const int box = lane % boxes, half = lane / boxes;
-        const uint32_t to = half * BOX_BYTES + (box << p.box_log2) * 128;
+        // ------------------------------------------------------------------ loads of Q and K
         uint32_t it = 0, queries = 0;  // steps and units with keys so far
         bool ok = true;
         for (Unit x; next_unit(&x);) {
-          // this lane's key and page of a step; page -1 (zeros) where no row sees any of the box
-          auto page_of = [&](int j, int* key) {
-            const int v = x.v0 + j * BC + (box << p.box_log2);
-            *key = x.list.key(v);
-            return lane < loads && x.list.seen(v, 1 << p.box_log2, p.sinks) ? p.seq.page_of(x.b, *key) : -1;
-          };
-          int key = 0, page = x.steps > 0 ? page_of(0, &key) : -1;
-          if (x.steps == 0 && lane == 0) mbar_arrive(&bars->unit_wanted);
-          if (x.steps > 0 && ok) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&bars->q_empty, (queries & 1u) ^ 1u, &bars->abort_flag));
-            ++queries;
-            if (!ok && lane == 0) report(bars, PAGED_TIMEOUT_LOADS, it, 2u);
-            if (ok && lane == 0) {
-              mbar_expect_tx(&bars->q_full, x.tiles * HALVES * p.tile_tokens * p.group * 128);
-              for (int t = 0; t < x.tiles; ++t)
-#pragma unroll
-                for (int b = 0; b < HALVES; ++b)
-                  tma_load_3d(smem + t * Q_BYTES + b * BOX_BYTES, &p.tmQ, &bars->q_full, b * 64, x.head * p.group, x.row0 + t * p.tile_tokens);
-            }
-            __syncwarp();
-          }
+          if (x.steps == 0) continue;
+          int key = 0, page = page_of(x, 0, &key);
           for (int j = 0; j < x.steps; ++j, ++it) {
-            if (j == max(0, x.steps - 2) && lane == 0) mbar_arrive(&bars->unit_wanted);
             if (!ok) continue;
-            const int ks = it % K_STAGES, vs = it % V_STAGES;
-            const int in_page = key & ((1 << p.seq.page_log2) - 1), this_page = page;
-            if (j + 1 < x.steps) page = page_of(j + 1, &key);
+            const int ks = it % K_STAGES, this_key = key, this_page = page;
+            if (j + 1 < x.steps) page = page_of(x, j + 1, &key);
             ok = __all_sync(0xffffffffu, mbar_wait(&bars->k_empty[ks], ((it / K_STAGES) & 1u) ^ 1u, &bars->abort_flag));
-            if (!ok) {
-              if (lane == 0) report(bars, PAGED_TIMEOUT_LOADS, it, 0u);
-              continue;
+            if (ok) load(smem + OFF_K + ks * KV_BYTES, &p.tmK, &bars->k_full[ks], x, this_key, this_page);
+            if (ok && j == 0) {  // (behind the first K tile: the queries' place is free later)
+              ok = __all_sync(0xffffffffu, mbar_wait(&bars->q_empty, (queries & 1u) ^ 1u, &bars->abort_flag));
+              ++queries;
+              if (ok && lane == 0) {
+                mbar_expect_tx(&bars->q_full, x.tiles * HALVES * p.tile_tokens * p.group * 128);
+                for (int t = 0; t < x.tiles; ++t)
+#pragma unroll
+                  for (int b = 0; b < HALVES; ++b)
+                    tma_load_3d(smem + t * Q_BYTES + b * BOX_BYTES, &p.tmQ, &bars->q_full, b * 64, x.head * p.group, x.row0 + t * p.tile_tokens);
+              }
+              __syncwarp();
             }
-            if (lane == 0) mbar_expect_tx(&bars->k_full[ks], KV_BYTES);
-            __syncwarp();
-            if (lane < loads) tma_load_4d(smem + OFF_K + ks * KV_BYTES + to, &p.tmK, &bars->k_full[ks], half * 64, in_page, x.head, this_page);
-            ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_empty[vs], ((it / V_STAGES) & 1u) ^ 1u, &bars->abort_flag));
-            if (!ok) {
-              if (lane == 0) report(bars, PAGED_TIMEOUT_LOADS, it, 1u);
-              continue;
-            }
-            if (lane == 0) mbar_expect_tx(&bars->v_full[vs], KV_BYTES);
-            __syncwarp();
-            if (lane < loads) tma_load_4d(smem + OFF_V + vs * KV_BYTES + to, &p.tmV, &bars->v_full[vs], half * 64, in_page, x.head, this_page);
+            if (!ok && lane == 0) report(bars, PAGED_TIMEOUT_LOADS, it, 0u);
           }
         }
       } else if (warp == 1) {
@@ -367,40 +358,70 @@ struct AttnPrompt {
           }
         }
       } else {
-        // ------------------------------------------------------------------ units
-        // One after the other into two slots. A slot is free once every warp has read the unit in it; what has gone wrong ends the row of units with
-        // one that says so, and where a slot does not become free, with none: the warps' wait for it ends by itself.
-        int index = static_cast<int>(blockIdx.x) / (kKeySplit ? p.splits : 1);
-        bool more = true;
-        for (uint32_t u = 0; more; ++u) {
-          Unit x = unit_of(p, index < 0 ? 0 : index, rank);
-          if (index < 0 || bars->abort_flag != 0u) x.end = 1;
-          bool free = u < 2 || mbar_wait_for(&bars->unit_empty[u & 1], ((u >> 1) & 1u) ^ 1u, KCG_WAIT_LIMIT_NS);
+        // ------------------------------------------------------------------ loads of V, and the units
+        // Units one after the other into two slots. A slot is free once every warp has read the unit in it; what has gone wrong ends the row of units
+        // with one that says so, and where a slot does not become free, with none: the warps' wait for it ends by itself.
+        uint32_t it = 0, made = 0, asked = 0;
+        bool ok = true;
+        auto publish = [&](Unit& x) {
+          if (bars->abort_flag != 0u) x.end = 1;
+          const int slot = made & 1;
+          const bool free = made < 2 || mbar_wait_for(&bars->unit_empty[slot], ((made >> 1) & 1u) ^ 1u, KCG_WAIT_LIMIT_NS);
           if (!__all_sync(0xffffffffu, free)) {
-            if (lane == 0) report(bars, PAGED_TIMEOUT_UNIT, u, 32u);
-            break;
+            if (lane == 0) report(bars, PAGED_TIMEOUT_UNIT, made, 32u);
+            x.end = 1;
+            return;
           }
           if (lane == 0) {
-            bars->unit[u & 1] = x;
-            mbar_arrive(&bars->unit_full[u & 1]);
+            bars->unit[slot] = x;
+            mbar_arrive(&bars->unit_full[slot]);
           }
           __syncwarp();
-          if (x.end) break;
-          free = mbar_wait(&bars->unit_wanted, u & 1u, &bars->abort_flag);
-          if (kKeySplit || !__all_sync(0xffffffffu, free)) {
-            index = -1;
-            continue;
-          }
-          if (lane == 0) {
+          ++made;
+        };
+        auto ask = [&]() {
+          if (!kKeySplit && lane == 0) {
             mbar_expect_tx(&bars->taken, 16);
             request_cta(&bars->answer, &bars->taken);
           }
           __syncwarp();
-          const bool answered = __all_sync(0xffffffffu, mbar_wait(&bars->taken, u & 1u, &bars->abort_flag));
-          index = answered ? requested_cta(&bars->answer) : -1;
-          if (!answered && lane == 0) report(bars, PAGED_TIMEOUT_UNIT, u, 33u);
-          fence_proxy_async_smem();  // (the next answer is written behind this reading)
-          __syncwarp();
+        };
+        // the unit behind this one, published
+        auto answered = [&]() {
+          int index = -1;
+          if (!kKeySplit) {
+            const bool there = __all_sync(0xffffffffu, mbar_wait(&bars->taken, asked & 1u, &bars->abort_flag));
+            ++asked;
+            if (there) index = requested_cta(&bars->answer);
+            if (!there && lane == 0) report(bars, PAGED_TIMEOUT_UNIT, made, 33u);
+            fence_proxy_async_smem();  // (the next answer is written behind this reading)
+            __syncwarp();
+          }
+          Unit next = unit_of(p, index < 0 ? 0 : index, rank);
+          if (index < 0) next.end = 1;
+          publish(next);
+          return next;
+        };
+        Unit x = unit_of(p, static_cast<int>(blockIdx.x) / (kKeySplit ? p.splits : 1), rank);
+        publish(x);
+        while (!x.end) {
+          Unit next;
+          if (x.steps == 0) {
+            ask();
+            next = answered();
+          }
+          int key = 0, page = x.steps > 0 ? page_of(x, 0, &key) : -1;
+          for (int j = 0; j < x.steps; ++j, ++it) {
+            const int vs = it % V_STAGES, this_key = key, this_page = page;
+            if (j + 1 < x.steps) page = page_of(x, j + 1, &key);
+            if (j == max(0, x.steps - 3)) ask();
+            if (j == max(0, x.steps - 2)) next = answered();
+            if (!ok) continue;
+            ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_empty[vs], ((it / V_STAGES) & 1u) ^ 1u, &bars->abort_flag));
+            if (ok) load(smem + OFF_V + vs * KV_BYTES, &p.tmV, &bars->v_full[vs], x, this_key, this_page);
+            if (!ok && lane == 0) report(bars, PAGED_TIMEOUT_LOADS, it, 1u);
+          }
+          x = next;
         }
       }
       if constexpr (kKeySplit) {  // the two meetings of the cluster that join the partial results
@@ -621,27 +642,38 @@ struct AttnPrompt {
       } else {
         tc_fence_after_sync();
         const float inv = mine == 0 || l == 0.f ? 0.f : 1.f / l;
-        T* out = reinterpret_cast<T*>(p.o) + static_cast<long long>(x.row0 + token) * p.o_row +
-                 static_cast<long long>(x.head * p.group + row % p.group) * p.o_head;
+        // (this thread's row, from the result's first byte on; -1: none)
+        const long long at = live ? (static_cast<long long>(x.row0 + token) * p.o_row + static_cast<long long>(x.head * p.group + row % p.group) * p.o_head) : -1;
+        uint8_t* stage = smem + RING_BYTES + (warp - 4) * (32 * 128);
 #pragma unroll
-        for (int c = 0; c < kD / 32; ++c) {
-          uint32_t r[32];
+        for (int c2 = 0; c2 < HALVES; ++c2) {
+          uint32_t o[2][32];
           if (mine > 0 && !gave_up) {
-            tmem_ld_32x32b_x32(col_o + c * 32, r);
+            tmem_ld_32x32b_x32(col_o + c2 * 64, o[0]);
+            tmem_ld_32x32b_x32(col_o + c2 * 64 + 32, o[1]);
             tmem_ld_wait();
+            pin_32(o[0]);
+            pin_32(o[1]);
           } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) r[i] = 0u;
+            for (int i = 0; i < 64; ++i) o[i / 32][i % 32] = 0u;
           }
-          if (live) {
+          __syncwarp();  // (the warp has read what the last round left here)
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              uint32_t w[4];
+          for (int u = 0; u < 8; ++u) {
+            uint32_t w[4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                w[e] = pack_pair<kBf16>(__uint_as_float(r[u * 8 + 2 * e]) * inv, __uint_as_float(r[u * 8 + 2 * e + 1]) * inv);
-              *reinterpret_cast<uint4*>(out + c * 32 + u * 8) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
+            for (int e = 0; e < 4; ++e)
+              w[e] = pack_pair<kBf16>(__uint_as_float(o[u / 4][u % 4 * 8 + 2 * e]) * inv, __uint_as_float(o[u / 4][u % 4 * 8 + 2 * e + 1]) * inv);
+            *reinterpret_cast<uint4*>(stage + lane * 128 + ((u ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int r = k * 4 + lane / 8, u = lane & 7;
+            const long long to = __shfl_sync(0xffffffffu, at, r);
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((u ^ (r & 7)) << 4));
+            if (to >= 0) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.o) + to + c2 * 64 + u * 8) = v;
           }
         }
       }
