@@ -116,9 +116,8 @@ struct AttnPrompt {
       x.b = lo;
       t = slot - (s.start(lo) / pair + lo);
     }
-    const int first = s.start(x.b), n = s.start(x.b + 1) - first;
+    const int first = s.start(x.b), n = s.start(x.b + 1) - first, length = s.lengths[x.b];
     if (t >= 0 && n > 0 && t < (n + pair - 1) / pair) {
-      const int length = s.lengths[x.b];
       x.tokens = min(pair, n - t * pair);
       x.tiles = x.tokens > p.tile_tokens ? 2 : 1;
       x.row0 = first + t * pair;
@@ -198,17 +197,20 @@ struct AttnPrompt {
     // The next unit, for each warp that works on it. All read the same ones, whatever went wrong (the wait does not look at the abort flag and is
     // longer than those that it follows from), so that the meetings on the way come out even.
     int taken = 0;
-    auto next_unit = [&](Unit* x) {
-      const int slot = taken & 1;
-      const bool got = __all_sync(0xffffffffu, mbar_wait_for(&bars->unit_full[slot], (taken >> 1) & 1u, 8 * KCG_WAIT_LIMIT_NS));
-      if (!got) {
-        if (lane == 0) report(bars, PAGED_TIMEOUT_UNIT, static_cast<uint32_t>(taken), warp);
-        return false;
-      }
-      *x = bars->unit[slot];
+    auto unit_there = [&]() {
+      const bool got = __all_sync(0xffffffffu, mbar_wait_for(&bars->unit_full[taken & 1], (taken >> 1) & 1u, 8 * KCG_WAIT_LIMIT_NS));
+      if (!got && lane == 0) report(bars, PAGED_TIMEOUT_UNIT, static_cast<uint32_t>(taken), warp);
+      return got;
+    };
+    auto unit_read = [&]() {
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->unit_empty[slot]);
+      if (lane == 0) mbar_arrive(&bars->unit_empty[taken & 1]);
       ++taken;
+    };
+    auto next_unit = [&](Unit* x) {
+      if (!unit_there()) return false;
+      *x = bars->unit[taken & 1];
+      unit_read();
       return x->end == 0;
     };
 
@@ -234,26 +236,31 @@ struct AttnPrompt {
         // ------------------------------------------------------------------ loads of Q and K
         uint32_t it = 0, queries = 0;  // steps and units with keys so far
         bool ok = true;
+        auto load_queries = [&](const Unit& x) {
+          ++queries;
+          if (lane == 0) {
+            mbar_expect_tx(&bars->q_full, x.tiles * HALVES * p.tile_tokens * p.group * 128);
+            for (int t = 0; t < x.tiles; ++t)
+#pragma unroll
+              for (int b = 0; b < HALVES; ++b)
+                tma_load_3d(smem + t * Q_BYTES + b * BOX_BYTES, &p.tmQ, &bars->q_full, b * 64, x.head * p.group, x.row0 + t * p.tile_tokens);
+          }
+          __syncwarp();
+        };
         for (Unit x; next_unit(&x);) {
           if (x.steps == 0) continue;
           int key = 0, page = page_of(x, 0, &key);
+          const bool queries_on = ok && mbar_test_warp(&bars->q_empty, (queries & 1u) ^ 1u);
+          if (queries_on) load_queries(x);
           for (int j = 0; j < x.steps; ++j, ++it) {
             if (!ok) continue;
             const int ks = it % K_STAGES, this_key = key, this_page = page;
             if (j + 1 < x.steps) page = page_of(x, j + 1, &key);
             ok = __all_sync(0xffffffffu, mbar_wait(&bars->k_empty[ks], ((it / K_STAGES) & 1u) ^ 1u, &bars->abort_flag));
             if (ok) load(smem + OFF_K + ks * KV_BYTES, &p.tmK, &bars->k_full[ks], x, this_key, this_page);
-            if (ok && j == 0) {  // (behind the first K tile: the queries' place is free later)
+            if (ok && j == 0 && !queries_on) {  // (behind the first K tile: the queries' place was not free before)
               ok = __all_sync(0xffffffffu, mbar_wait(&bars->q_empty, (queries & 1u) ^ 1u, &bars->abort_flag));
-              ++queries;
-              if (ok && lane == 0) {
-                mbar_expect_tx(&bars->q_full, x.tiles * HALVES * p.tile_tokens * p.group * 128);
-                for (int t = 0; t < x.tiles; ++t)
-#pragma unroll
-                  for (int b = 0; b < HALVES; ++b)
-                    tma_load_3d(smem + t * Q_BYTES + b * BOX_BYTES, &p.tmQ, &bars->q_full, b * 64, x.head * p.group, x.row0 + t * p.tile_tokens);
-              }
-              __syncwarp();
+              if (ok) load_queries(x);
             }
             if (!ok && lane == 0) report(bars, PAGED_TIMEOUT_LOADS, it, 0u);
           }
@@ -264,65 +271,94 @@ struct AttnPrompt {
         const uint64_t qdesc = make_smem_desc(smem_u32(smem), 16, 1024, SWZ_128B);
         const uint64_t kdesc = make_smem_desc(smem_u32(smem + OFF_K), 16, 1024, SWZ_128B);
         const uint64_t vdesc = make_smem_desc(smem_u32(smem + OFF_V), BOX_BYTES, 1024, SWZ_128B);
-        uint32_t it0 = 0, queries = 0;
-        for (Unit x; next_unit(&x);) {
-          const int nkv = x.steps, tiles = x.tiles;
+        uint32_t it0 = 0, queries = 0;  // steps and units with keys before the current one's
+        // S_t of step it0 + i, of a unit of `tiles` tiles; `last`: it is the unit's last
+        auto issue_s = [&](int t, int i, int tiles, bool last) {
+          const uint64_t ad = qdesc + t * (Q_BYTES >> 4), bd = kdesc + ((it0 + i) % K_STAGES) * (KV_BYTES >> 4);
+#pragma unroll
+          for (int ks = 0; ks < kD / 16; ++ks) {
+            const uint32_t in_row = (ks * 32) % 128, box = (ks * 32) / 128;
+            umma_ss<false>(tmem + t * BC, ad + ((box * BOX_BYTES + in_row) >> 4), bd + ((box * BOX_BYTES + in_row) >> 4), IDESC_S, ks > 0 ? 1u : 0u);
+          }
+          umma_commit(&bars->s_full[t]);
+          if (t == tiles - 1) {
+            umma_commit(&bars->k_empty[(it0 + i) % K_STAGES]);
+            if (last) umma_commit(&bars->q_empty);
+          }
+        };
+        auto issue_pv = [&](int t, int j, int ks0, int ks1) {
+          const uint64_t vd = vdesc + ((it0 + j) % V_STAGES) * (KV_BYTES >> 4);
+#pragma unroll
+          for (int ks = 0; ks < BC / 16; ++ks)
+            if (ks >= ks0 && ks < ks1)
+              umma_ts<false>(tmem + COL_O + t * kD, tmem + t * BC + ks * 8, vd + ((ks * 16 * 128) >> 4), IDESC_O, (j > 0 || ks > 0) ? 1u : 0u);
+        };
+        int begun = 0;  // tiles of the current unit whose first scores are on their way
+        for (bool known = false; known || unit_there();) {
+          const int nkv = bars->unit[taken & 1].steps, tiles = bars->unit[taken & 1].tiles;
+          const bool end = bars->unit[taken & 1].end != 0;
+          unit_read();
+          known = false;
+          if (end) break;
           if (nkv == 0) continue;
-          auto issue_s = [&](int t, int i) {
-            const uint64_t ad = qdesc + t * (Q_BYTES >> 4), bd = kdesc + ((it0 + i) % K_STAGES) * (KV_BYTES >> 4);
-#pragma unroll
-            for (int ks = 0; ks < kD / 16; ++ks) {
-              const uint32_t in_row = (ks * 32) % 128, box = (ks * 32) / 128;
-              umma_ss<false>(tmem + t * BC, ad + ((box * BOX_BYTES + in_row) >> 4), bd + ((box * BOX_BYTES + in_row) >> 4), IDESC_S, ks > 0 ? 1u : 0u);
-            }
-            umma_commit(&bars->s_full[t]);
-            if (t == tiles - 1) {
-              umma_commit(&bars->k_empty[(it0 + i) % K_STAGES]);
-              if (i == nkv - 1) umma_commit(&bars->q_empty);
-            }
-          };
-          auto issue_pv = [&](int t, int j, int ks0, int ks1) {
-            const uint64_t vd = vdesc + ((it0 + j) % V_STAGES) * (KV_BYTES >> 4);
-#pragma unroll
-            for (int ks = 0; ks < BC / 16; ++ks)
-              if (ks >= ks0 && ks < ks1)
-                umma_ts<false>(tmem + COL_O + t * kD, tmem + t * BC + ks * 8, vd + ((ks * 16 * 128) >> 4), IDESC_O, (j > 0 || ks > 0) ? 1u : 0u);
-          };
-          const bool q_there = __all_sync(0xffffffffu, mbar_wait(&bars->q_full, queries & 1u, &bars->abort_flag));
+          if (begun == 0) {
+            const bool q_there = __all_sync(0xffffffffu, mbar_wait(&bars->q_full, queries & 1u, &bars->abort_flag));
+            if (!q_there && lane == 0) report(bars, PAGED_TIMEOUT_ATTENTION, 0u, 0u);
+          }
           ++queries;
-          if (!q_there && lane == 0) report(bars, PAGED_TIMEOUT_ATTENTION, 0u, 0u);
           __syncwarp();
           named_bar_sync(BAR_KV, KV_THREADS);  // the first K tile
           tc_fence_after_sync();
-          if (elect_one()) {
-            issue_s(0, 0);
-            if (!kApart && tiles == 2) issue_s(1, 0);
+          const int first = kApart && begun == 0 ? 1 : tiles;  // (the second tile's follow the first one's first weights)
+#pragma unroll 1
+          for (int t = begun; t < first; ++t) {
+            if (elect_one()) issue_s(t, 0, tiles, nkv == 1);
+            __syncwarp();
           }
-          __syncwarp();
+          const bool second = first < tiles;
+          begun = 0;  // (of the next unit, from here on)
+          bool ready = false;
+          int next_steps = 0, next_tiles = 0;
           for (int j = 0; j < nkv; ++j) {
             named_bar_sync(BAR_KV, KV_THREADS);
-#pragma unroll
-            for (int t = 0; t < TILES; ++t) {
-              if (t >= tiles) continue;
+            const bool last = j + 1 == nkv;
+#pragma unroll 1
+            for (int t = 0; t < tiles; ++t) {
               named_bar_sync(BAR_PART + t, PT_THREADS);
               tc_fence_after_sync();
-              if (elect_one()) {
-                if (kApart && j == 0 && t == 0 && tiles == 2) issue_s(1, 0);
-                issue_pv(t, j, 0, P_PART / 16);
+              if (second && j == 0 && t == 0) {
+                if (elect_one()) issue_s(1, 0, tiles, nkv == 1);
+                __syncwarp();
               }
+              if (elect_one()) issue_pv(t, j, 0, P_PART / 16);
               __syncwarp();
+              if (last && !known && mbar_test_warp(&bars->unit_full[taken & 1], (taken >> 1) & 1u)) {  // (while the last weights are waited for)
+                known = true;
+                next_steps = bars->unit[taken & 1].end ? 0 : bars->unit[taken & 1].steps;
+                next_tiles = bars->unit[taken & 1].tiles;
+              }
               named_bar_sync(BAR_FULL + t, PT_THREADS);
               tc_fence_after_sync();
               if (elect_one()) {
                 issue_pv(t, j, P_PART / 16, BC / 16);
                 if (t == tiles - 1) umma_commit(&bars->v_empty[(it0 + j) % V_STAGES]);
-                if (j + 1 < nkv) {
-                  issue_s(t, j + 1);
-                } else {
-                  umma_commit(&bars->o_full[t]);
-                }
+                if (last) umma_commit(&bars->o_full[t]);
               }
               __syncwarp();
+              // The next scores of this tile: of the next step, or of the next unit's first if its operands have come (the other tile has
+              // still to finish then, and this one's warps their rows).
+              if (last && next_steps > 0 && t < next_tiles && begun == t) {
+                if (!ready)
+                  ready = mbar_test_warp(&bars->q_full, queries & 1u) &&
+                          mbar_test_warp(&bars->k_full[(it0 + nkv) % K_STAGES], ((it0 + nkv) / K_STAGES) & 1u);
+                tc_fence_after_sync();
+              }
+              const bool ahead = last && ready && t < next_tiles && begun == t;
+              if (!last || ahead) {
+                if (elect_one()) issue_s(t, j + 1, last ? next_tiles : tiles, last ? next_steps == 1 : j + 2 == nkv);
+                __syncwarp();
+                begun += ahead ? 1 : 0;
+              }
             }
           }
           it0 += nkv;
@@ -363,14 +399,13 @@ struct AttnPrompt {
         // with one that says so, and where a slot does not become free, with none: the warps' wait for it ends by itself.
         uint32_t it = 0, made = 0, asked = 0;
         bool ok = true;
-        auto publish = [&](Unit& x) {
+        auto publish = [&](Unit& x) {  // false: the row ends
           if (bars->abort_flag != 0u) x.end = 1;
           const int slot = made & 1;
           const bool free = made < 2 || mbar_wait_for(&bars->unit_empty[slot], ((made >> 1) & 1u) ^ 1u, KCG_WAIT_LIMIT_NS);
           if (!__all_sync(0xffffffffu, free)) {
             if (lane == 0) report(bars, PAGED_TIMEOUT_UNIT, made, 32u);
-            x.end = 1;
-            return;
+            return false;
           }
           if (lane == 0) {
             bars->unit[slot] = x;
@@ -378,6 +413,7 @@ struct AttnPrompt {
           }
           __syncwarp();
           ++made;
+          return x.end == 0;
         };
         auto ask = [&]() {
           if (!kKeySplit && lane == 0) {
@@ -399,29 +435,32 @@ struct AttnPrompt {
           }
           Unit next = unit_of(p, index < 0 ? 0 : index, rank);
           if (index < 0) next.end = 1;
-          publish(next);
-          return next;
+          return publish(next);
         };
-        Unit x = unit_of(p, static_cast<int>(blockIdx.x) / (kKeySplit ? p.splits : 1), rank);
-        publish(x);
-        while (!x.end) {
-          Unit next;
+        bool more;
+        {
+          Unit first = unit_of(p, static_cast<int>(blockIdx.x) / (kKeySplit ? p.splits : 1), rank);
+          more = publish(first);
+        }
+        while (more) {
+          const Unit x = bars->unit[(made - 1) & 1];
           if (x.steps == 0) {
             ask();
-            next = answered();
+            more = answered();
+            continue;
           }
-          int key = 0, page = x.steps > 0 ? page_of(x, 0, &key) : -1;
+          int key = 0, page = page_of(x, 0, &key);
           for (int j = 0; j < x.steps; ++j, ++it) {
             const int vs = it % V_STAGES, this_key = key, this_page = page;
             if (j + 1 < x.steps) page = page_of(x, j + 1, &key);
             if (j == max(0, x.steps - 3)) ask();
-            if (j == max(0, x.steps - 2)) next = answered();
-            if (!ok) continue;
-            ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_empty[vs], ((it / V_STAGES) & 1u) ^ 1u, &bars->abort_flag));
-            if (ok) load(smem + OFF_V + vs * KV_BYTES, &p.tmV, &bars->v_full[vs], x, this_key, this_page);
-            if (!ok && lane == 0) report(bars, PAGED_TIMEOUT_LOADS, it, 1u);
+            if (ok) {
+              ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_empty[vs], ((it / V_STAGES) & 1u) ^ 1u, &bars->abort_flag));
+              if (ok) load(smem + OFF_V + vs * KV_BYTES, &p.tmV, &bars->v_full[vs], x, this_key, this_page);
+              if (!ok && lane == 0) report(bars, PAGED_TIMEOUT_LOADS, it, 1u);
+            }
+            if (j == max(0, x.steps - 2)) more = answered();
           }
-          x = next;
         }
       }
       if constexpr (kKeySplit) {  // the two meetings of the cluster that join the partial results
@@ -437,11 +476,18 @@ struct AttnPrompt {
       const int row = q * 32 + lane;    // query row of this thread inside its tile
       const uint32_t lane_addr = static_cast<uint32_t>(q * 32) << 16;
       const uint32_t col_s = tmem_base + lane_addr + t * BC, col_o = tmem_base + lane_addr + COL_O + t * kD;
-      const int token = row < p.tile_tokens * p.group ? t * p.tile_tokens + row / p.group : 0x40000000;  // of the unit's (which has less than that)
+      const int in_tile = row / p.group, head_row = row - in_tile * p.group;
+      const int token = row < p.tile_tokens * p.group ? t * p.tile_tokens + in_tile : 0x40000000;  // of the unit's (which has less than that)
       const uint64_t scale2 = f32x2(p.scale_log2, p.scale_log2);
       uint32_t scores = 0, results = 0;  // of this tile so far
       bool alive = true;                 // no wait of this warp has run out
-      for (Unit x; next_unit(&x);) {
+      while (unit_there()) {
+      const Unit& unit = bars->unit[taken & 1];
+      if (unit.end) {
+        unit_read();
+        break;
+      }
+      const Unit x = unit;
       const bool live = token < x.tokens;
       // places of keys below `see`, of those from `near` on and the sinks; rows without a token (whose scores are of whatever lies there) are not masked
       const int position = x.p_lo + token;
@@ -632,8 +678,8 @@ struct AttnPrompt {
               sum = fmaf(f, ml.y, sum);
             }
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            T* out = reinterpret_cast<T*>(p.o) + static_cast<long long>(x.row0 + tok) * p.o_row +
-                     static_cast<long long>(x.head * p.group + in_tile % p.group) * p.o_head + u * 4;
+            T* out = reinterpret_cast<T*>(p.o) + static_cast<long long>(unit.row0 + tok) * p.o_row +
+                     static_cast<long long>(unit.head * p.group + in_tile % p.group) * p.o_head + u * 4;
             *reinterpret_cast<uint2*>(out) = make_uint2(pack_pair<kBf16>(a.x * inv, a.y * inv), pack_pair<kBf16>(a.z * inv, a.w * inv));
           }
         }
@@ -643,40 +689,45 @@ struct AttnPrompt {
         tc_fence_after_sync();
         const float inv = mine == 0 || l == 0.f ? 0.f : 1.f / l;
         // (this thread's row, from the result's first byte on; -1: none)
-        const long long at = live ? (static_cast<long long>(x.row0 + token) * p.o_row + static_cast<long long>(x.head * p.group + row % p.group) * p.o_head) : -1;
+        const long long at = live ? static_cast<long long>(unit.row0 + token) * p.o_row + static_cast<long long>(unit.head * p.group + head_row) * p.o_head : -1;
         uint8_t* stage = smem + RING_BYTES + (warp - 4) * (32 * 128);
+        uint32_t o[kD / 32][32];
+        if (mine > 0 && !gave_up) {
+#pragma unroll
+          for (int c = 0; c < kD / 32; ++c) tmem_ld_32x32b_x32(col_o + c * 32, o[c]);
+          tmem_ld_wait();
+#pragma unroll
+          for (int c = 0; c < kD / 32; ++c) pin_32(o[c]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kD; ++i) o[i / 32][i % 32] = 0u;
+        }
 #pragma unroll
         for (int c2 = 0; c2 < HALVES; ++c2) {
-          uint32_t o[2][32];
-          if (mine > 0 && !gave_up) {
-            tmem_ld_32x32b_x32(col_o + c2 * 64, o[0]);
-            tmem_ld_32x32b_x32(col_o + c2 * 64 + 32, o[1]);
-            tmem_ld_wait();
-            pin_32(o[0]);
-            pin_32(o[1]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 64; ++i) o[i / 32][i % 32] = 0u;
-          }
           __syncwarp();  // (the warp has read what the last round left here)
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              w[e] = pack_pair<kBf16>(__uint_as_float(o[u / 4][u % 4 * 8 + 2 * e]) * inv, __uint_as_float(o[u / 4][u % 4 * 8 + 2 * e + 1]) * inv);
+              w[e] = pack_pair<kBf16>(__uint_as_float(o[c2 * 2 + u / 4][u % 4 * 8 + 2 * e]) * inv, __uint_as_float(o[c2 * 2 + u / 4][u % 4 * 8 + 2 * e + 1]) * inv);
             *reinterpret_cast<uint4*>(stage + lane * 128 + ((u ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
           }
           __syncwarp();
+          uint4 v[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const int r = k * 4 + lane / 8, u = lane & 7;
-            const long long to = __shfl_sync(0xffffffffu, at, r);
-            const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((u ^ (r & 7)) << 4));
-            if (to >= 0) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.o) + to + c2 * 64 + u * 8) = v;
+            v[k] = *reinterpret_cast<const uint4*>(stage + r * 128 + ((u ^ (r & 7)) << 4));
+          }
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const long long to = __shfl_sync(0xffffffffu, at, k * 4 + lane / 8);
+            if (to >= 0) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.o) + to + c2 * 64 + (lane & 7) * 8) = v[k];
           }
         }
       }
+      unit_read();
       }  // (units; a cluster has one, and its meetings are in it)
     }
 
