@@ -258,13 +258,13 @@ int prompt_clusters(int device, int threads, int smem, int size) {
 }
 
 template <int kD, bool kBf16>
-int launch_prompt(int device, cudaStream_t st, PromptArgs& p, int max_steps) {
+int launch_prompt(int device, cudaStream_t st, PromptArgs& p, long long pairs, int max_steps) {
   using Kern = AttnPrompt<kD, kBf16, false>;
   constexpr auto whole = attention_prompt_kernel<kD, kBf16, false>;
   constexpr auto split = attention_prompt_kernel<kD, kBf16, true>;
   if (int r = opt_in<whole>(device, Kern::SMEM_BYTES)) return r;
   if (int r = opt_in<split>(device, Kern::SMEM_BYTES)) return r;
-  const long long units = static_cast<long long>(p.slots) * p.kv_heads;
+  const long long units = pairs * p.kv_heads;
   if (units > 0x7fffffffLL / 8) return fail(KCG_E_TOO_LARGE, "attention_paged: too many rows");
   // The largest number of CTAs, 2 to 8, that can share the keys of a pair of tiles with every cluster running at once and, where the
   // sequences are as long as the table, four tiles of keys each (joining costs what two do).
@@ -288,11 +288,11 @@ int attention_prompt(int device, cudaStream_t st, const kcg_paged_cache* c, cons
   p.tile_tokens = 128 / p.group;
   p.scale_log2 = q->scale * 1.4426950408889634f;
   const int pair = 2 * p.tile_tokens;
-  // (first row) / pair + sequence + tiles of the sequence, at most: see AttnPrompt::place()
-  const long long slots = c->starts ? (static_cast<long long>(q->rows) + pair - 1) / pair + c->sequences - 1
+  // Pairs of tiles, at most: a sequence has one that is not full.
+  const long long pairs = c->starts ? (static_cast<long long>(q->rows) + pair - 1) / pair + c->sequences - 1
                                     : static_cast<long long>((p.seq.each + pair - 1) / pair) * c->sequences;
-  if (slots > 0x7fffffffLL) return fail(KCG_E_TOO_LARGE, "attention_paged: too many rows");
-  p.slots = static_cast<int>(slots);
+  if (pairs > 0x7fffffffLL) return fail(KCG_E_TOO_LARGE, "attention_paged: too many rows");
+  p.pairs = static_cast<int>(pairs);
   // Keys of a box: of a page, or of 32 where a window's keys begin anywhere and are laid out from a box's border on.
   const int most = q->window > 0 ? 32 : 128, box = c->page < most ? c->page : most;
   while ((1 << p.box_log2) < box) ++p.box_log2;
@@ -311,8 +311,8 @@ int attention_prompt(int device, cudaStream_t st, const kcg_paged_cache* c, cons
   long long keys = static_cast<long long>(c->width) * c->page;
   if (q->window > 0) keys = std::min(keys, static_cast<long long>(q->window) + pair + q->sinks);
   const int max_steps = static_cast<int>(std::min((keys + 127) / 128, 1000000LL));
-  if (c->d == 128) return bf16 ? launch_prompt<128, true>(device, st, p, max_steps) : launch_prompt<128, false>(device, st, p, max_steps);
-  return bf16 ? launch_prompt<64, true>(device, st, p, max_steps) : launch_prompt<64, false>(device, st, p, max_steps);
+  if (c->d == 128) return bf16 ? launch_prompt<128, true>(device, st, p, pairs, max_steps) : launch_prompt<128, false>(device, st, p, pairs, max_steps);
+  return bf16 ? launch_prompt<64, true>(device, st, p, pairs, max_steps) : launch_prompt<64, false>(device, st, p, pairs, max_steps);
 }
 
 }  // namespace

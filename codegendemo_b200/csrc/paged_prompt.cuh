@@ -26,7 +26,7 @@ struct PromptArgs {
   long long o_row, o_head;
   int kv_heads, group, tile_tokens, window, sinks;
   int box_log2;  // keys of a box
-  int slots;     // pairs of tiles: see place()
+  int pairs;     // of tiles, at most
   int splits;    // CTAs that share a pair's keys
   float scale_log2;
 };
@@ -90,39 +90,91 @@ struct AttnPrompt {
     }
   }
 
-  // The pairs of tiles of sequence b take the slots from (its first row) / (tokens of a pair) + b on, of which there are enough: so a slot's
-  // sequence is found by a search over the first rows alone, and some slots have no tokens. Asked by a whole warp.
+  // A sequence's pairs of tiles: its tokens are counted from the last one, whose pair sees the most keys; the first may have fewer tokens.
+  // ends_from(h): of `pairs` pairs of a sequence of `length` tokens those whose last token has at least h tokens before it.
+  __device__ static __forceinline__ int ends_from(int length, int pairs, int pair, int h) {
+    return h >= length ? 0 : min(pairs, (length - 1 - h) / pair + 1);
+  }
+  // The unit of a place in the row of units. Asked by a whole warp. Up to kOrdered sequences: those with the most keys come first, over all
+  // sequences, so that none of the long ones begins last (ORDERED_MEASURED); for a place's keys,
+  // bisected, the warp counts the pairs of all sequences that have more. Of more sequences that would take longer than a unit, and many short
+  // units even out by themselves: the pairs of sequence b take the places from (its first row) / (tokens of a pair) + b on, of which there are
+  // enough (some have no tokens), so a search over the first rows alone finds the sequence; the last ones first.
+  static constexpr int kOrdered = 64;
   __device__ static __forceinline__ Unit unit_of(const PromptArgs& p, int index, int rank) {
     const Sequences& s = p.seq;
     const int pair = TILES * p.tile_tokens, lane = threadIdx.x & 31;
-    const int slot = p.slots - 1 - index / p.kv_heads;  // (the last tokens of a sequence, which see the most keys, first)
+    int e = index / p.kv_heads;  // in the end: which of the sequence's pairs, from the last one on
     Unit x;
     x.head = index % p.kv_heads;
-    x.end = x.tokens = x.steps = x.v0 = x.row0 = x.p_lo = x.keys = 0;
+    x.end = x.tokens = x.steps = x.v0 = x.row0 = x.p_lo = x.keys = x.b = 0;
     x.tiles = 1;
-    int t;
-    if (!s.starts) {
-      const int each = (s.each + pair - 1) / pair;
-      x.b = slot / each, t = slot % each;
-    } else {
+    if (s.count > kOrdered) {
+      const int place = p.pairs - 1 - e;
       int lo = 0, hi = s.count;
       while (hi - lo > 1) {
         const int step = (hi - lo + 31) / 32, at = lo + lane * step;
-        const unsigned there = __ballot_sync(0xffffffffu, at < hi && s.start(at) / pair + at <= slot);
+        const unsigned there = __ballot_sync(0xffffffffu, at < hi && s.start(at) / pair + at <= place);
         const int last = there ? 31 - __clz(there) : 0;
         lo += last * step;
         hi = min(lo + step, hi);
       }
       x.b = lo;
-      t = slot - (s.start(lo) / pair + lo);
+      e = max(0, s.start(lo + 1) - s.start(lo) + pair - 1) / pair - 1 - (place - (s.start(lo) / pair + lo));
+    } else if (s.count > 1) {
+      auto count = [&](int b, int h) {
+        if (b >= s.count) return 0;
+        const int n = s.start(b + 1) - s.start(b);
+        return n > 0 ? ends_from(max(s.lengths[b], n), (n + pair - 1) / pair, pair, h) : 0;  // (no pair's last token is before the first)
+      };
+      int hi = 0;
+      for (int b = lane; b < s.count; b += 32) hi = max(hi, max(s.lengths[b], s.start(b + 1) - s.start(b)));
+      hi = __reduce_max_sync(0xffffffffu, hi);
+      int lo = -1;  // all pairs' last tokens have more before them, none has `hi`; as many as e do not have lo + 1 in the end
+      while (hi - lo > 1) {
+        const int mid = lo + (hi - lo) / 2;
+        int n = 0;
+        for (int b0 = 0; b0 < s.count; b0 += 32) n += count(b0 + lane, mid);
+        n = __reduce_add_sync(0xffffffffu, n);
+        if (n > e) {
+          lo = mid;
+        } else {
+          hi = mid;
+        }
+      }
+      // pairs with more come first; then those that have just as many, in the order of the sequences
+      int more = 0;
+      for (int b0 = 0; b0 < s.count; b0 += 32) more += count(b0 + lane, lo + 1);
+      e -= __reduce_add_sync(0xffffffffu, more);
+      int found = -1;
+      for (int b0 = 0; b0 < s.count && found < 0; b0 += 32) {
+        const int mine = count(b0 + lane, lo) - count(b0 + lane, lo + 1);
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += v;
+        }
+        const unsigned there = __ballot_sync(0xffffffffu, e < upto && e >= upto - mine);
+        if (there) {
+          const int l = __ffs(there) - 1;
+          found = b0 + l;
+          e = count(found, lo + 1) + (e - __shfl_sync(0xffffffffu, upto - mine, l));
+        } else {
+          e -= __shfl_sync(0xffffffffu, upto, 31);
+        }
+      }
+      x.b = max(found, 0);
+      if (found < 0) e = -1;
     }
     const int first = s.start(x.b), n = s.start(x.b + 1) - first, length = s.lengths[x.b];
-    if (t >= 0 && n > 0 && t < (n + pair - 1) / pair) {
-      x.tokens = min(pair, n - t * pair);
+    if (n > 0 && e >= 0 && e < (n + pair - 1) / pair) {
+      const int from = n - (e + 1) * pair;  // (the first pair has what is left)
+      x.tokens = from < 0 ? pair + from : pair;
       x.tiles = x.tokens > p.tile_tokens ? 2 : 1;
-      x.row0 = first + t * pair;
+      x.row0 = first + max(from, 0);
       x.keys = s.keys(length);
-      x.p_lo = max(length, 0) - n + t * pair;  // (a negative length: no keys)
+      x.p_lo = max(length, 0) - n + max(from, 0);  // (a negative length: no keys)
     }
     x.list = KeyList(x.tokens > 0 ? max(0, min(x.keys, x.p_lo + x.tokens)) : 0, x.p_lo, p.window, p.sinks, 1 << p.box_log2);
     const int steps = x.list.count / BC + (x.list.count % BC ? 1 : 0);
@@ -653,34 +705,60 @@ struct AttnPrompt {
         __syncwarp();
         cluster_sync_all();
         {
-          const int all = x.tiles * BR * UNITS;
-          const int u0 = all / p.splits * rank + min(rank, all % p.splits), u1 = u0 + all / p.splits + (rank < all % p.splits ? 1 : 0);
+          // This CTA's rows, as many to a warp: a lane first takes the weights of one of them, then the warp whole rows (d = 64: two), four loads of other CTAs'
+          // rows in flight for each of them. (An element at a time, with its row's weights each time, was 13 us of latency for two CTAs.)
+          const int all = x.tiles * BR, r0 = all * rank / p.splits, r1 = all * (rank + 1) / p.splits;
+          const int per = (r1 - r0 + 7) / 8, first = r0 + (warp - 4) * per, mine_rows = max(0, min(per, r1 - first));  // (at most 16)
           const uint32_t base_addr = smem_u32(smem);
-          for (int i = u0 + static_cast<int>(threadIdx.x) - 128; i < u1; i += TILES * 128) {
-            const int r = i / UNITS, u = i % UNITS, in_tile = r % BR;
-            const int tok = r / BR * p.tile_tokens + in_tile / p.group;
-            if (in_tile >= p.tile_tokens * p.group || tok >= x.tokens) continue;
-            const uint32_t ml_addr = base_addr + OFF_ML + r * 8;
-            const uint32_t o_addr = base_addr + r * kD * 4 + ((u ^ (r & (UNITS - 1))) << 4);
-            float top = -INFINITY;
-            for (int c = 0; c < p.splits; ++c) top = fmaxf(top, ld_cluster_f2(map_to_cta(ml_addr, c)).x);
-            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-            float sum = 0.f;
-#pragma unroll 4
-            for (int c = 0; c < p.splits; ++c) {
-              const float2 ml = ld_cluster_f2(map_to_cta(ml_addr, c));
-              const float4 x = ld_cluster_f4(map_to_cta(o_addr, c));
-              const float f = ml.y == 0.f ? 0.f : ex2(ml.x - top);  // (a part of no key; a sum of NaN has to reach the result)
-              a.x = fmaf(f, x.x, a.x);
-              a.y = fmaf(f, x.y, a.y);
-              a.z = fmaf(f, x.z, a.z);
-              a.w = fmaf(f, x.w, a.w);
-              sum = fmaf(f, ml.y, sum);
+          float f[8], inv = 0.f;
+          {
+            const uint32_t ml_addr = base_addr + OFF_ML + (first + min(lane, max(mine_rows - 1, 0))) * 8;
+            float2 ml[8];
+            float top = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) ml[c] = c < p.splits && mine_rows > 0 ? ld_cluster_f2(map_to_cta(ml_addr, c)) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) top = fmaxf(top, ml[c].x);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              f[c] = ml[c].y == 0.f ? 0.f : ex2(ml[c].x - top);  // (a part of no key; a sum of NaN has to reach the result)
+              sum = fmaf(f[c], ml[c].y, sum);
             }
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            T* out = reinterpret_cast<T*>(p.o) + static_cast<long long>(unit.row0 + tok) * p.o_row +
-                     static_cast<long long>(unit.head * p.group + in_tile % p.group) * p.o_head + u * 4;
-            *reinterpret_cast<uint2*>(out) = make_uint2(pack_pair<kBf16>(a.x * inv, a.y * inv), pack_pair<kBf16>(a.z * inv, a.w * inv));
+            inv = sum == 0.f ? 0.f : 1.f / sum;
+          }
+          constexpr int ROWS = 128 / kD, AT_ONCE = 4;  // rows a warp takes with one load, loads in flight
+          const int u = lane % UNITS;
+          for (int k0 = 0; k0 < mine_rows; k0 += ROWS * AT_ONCE) {
+            float4 sums[AT_ONCE];
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) sums[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              if (c >= p.splits) break;
+              float4 v[AT_ONCE];
+#pragma unroll
+              for (int i = 0; i < AT_ONCE; ++i) {
+                const int r = first + min(k0 + i * ROWS + lane / UNITS, mine_rows - 1);
+                v[i] = ld_cluster_f4(map_to_cta(base_addr + r * kD * 4 + ((u ^ (r & (UNITS - 1))) << 4), c));
+              }
+#pragma unroll
+              for (int i = 0; i < AT_ONCE; ++i) {
+                const float w = __shfl_sync(0xffffffffu, f[c], min(k0 + i * ROWS + lane / UNITS, mine_rows - 1));
+                if (w == 0.f) continue;  // (what a part of no key holds)
+                sums[i].x = fmaf(w, v[i].x, sums[i].x), sums[i].y = fmaf(w, v[i].y, sums[i].y);
+                sums[i].z = fmaf(w, v[i].z, sums[i].z), sums[i].w = fmaf(w, v[i].w, sums[i].w);
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+              const int k = k0 + i * ROWS + lane / UNITS, r = first + k, in_tile = r % BR;
+              const float scale = __shfl_sync(0xffffffffu, inv, min(k, mine_rows - 1));
+              const int tok = r / BR * p.tile_tokens + in_tile / p.group;
+              if (k >= mine_rows || in_tile >= p.tile_tokens * p.group || tok >= x.tokens) continue;
+              T* out = reinterpret_cast<T*>(p.o) + static_cast<long long>(unit.row0 + tok) * p.o_row +
+                       static_cast<long long>(unit.head * p.group + in_tile % p.group) * p.o_head + u * 4;
+              *reinterpret_cast<uint2*>(out) = make_uint2(pack_pair<kBf16>(sums[i].x * scale, sums[i].y * scale), pack_pair<kBf16>(sums[i].z * scale, sums[i].w * scale));
+            }
           }
         }
         __syncwarp();
