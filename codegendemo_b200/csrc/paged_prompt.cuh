@@ -61,7 +61,7 @@ struct AttnPrompt {
     int end;                    // there is no further unit, and this is none
   };
   struct Barriers {
-    uint64_t q_full, q_empty;
+    uint64_t q_full[TILES], q_empty[TILES];
     uint64_t k_full[K_STAGES], k_empty[K_STAGES], v_full[V_STAGES], v_empty[V_STAGES];
     uint64_t s_full[TILES];  // S_t of the current step is complete
     uint64_t o_full[TILES];  // the last P_t V of a unit has retired
@@ -90,99 +90,92 @@ struct AttnPrompt {
     }
   }
 
-  // A sequence's pairs of tiles: its tokens are counted from the last one, whose pair sees the most keys; the first may have fewer tokens.
-  // ends_from(h): of `pairs` pairs of a sequence of `length` tokens those whose last token has at least h tokens before it.
-  __device__ static __forceinline__ int ends_from(int length, int pairs, int pair, int h) {
-    return h >= length ? 0 : min(pairs, (length - 1 - h) / pair + 1);
-  }
-  // The unit of a place in the row of units. Asked by a whole warp. Up to kOrdered sequences: those with the most keys come first, over all
-  // sequences, so that none of the long ones begins last (ORDERED_MEASURED); for a place's keys,
-  // bisected, the warp counts the pairs of all sequences that have more. Of more sequences that would take longer than a unit, and many short
-  // units even out by themselves: the pairs of sequence b take the places from (its first row) / (tokens of a pair) + b on, of which there are
-  // enough (some have no tokens), so a search over the first rows alone finds the sequence; the last ones first.
+  // The row of units, as warp 3 walks it. A sequence's pairs of tiles are counted from its last token, whose pair sees the most keys; the first may
+  // have fewer tokens. Up to kOrdered sequences: pairs with the most keys come first, over all sequences, so that none of the long ones begins
+  // last; a pair's level is the keys of its last token over a pair's tokens. For a place in the row the warp bisects its level, a lane one or two
+  // sequences, whose facts it has read once. Of more sequences that would take longer than a unit, and many short units even out by themselves:
+  // the pairs of sequence b take the places from (its first row) / (tokens of a pair) + b on, of which there are enough (some have no
+  // tokens), so a search over the first rows alone finds the sequence; the last ones first.
   static constexpr int kOrdered = 64;
-  __device__ static __forceinline__ Unit unit_of(const PromptArgs& p, int index, int rank) {
-    const Sequences& s = p.seq;
-    const int pair = TILES * p.tile_tokens, lane = threadIdx.x & 31;
-    int e = index / p.kv_heads;  // in the end: which of the sequence's pairs, from the last one on
-    Unit x;
-    x.head = index % p.kv_heads;
-    x.end = x.tokens = x.steps = x.v0 = x.row0 = x.p_lo = x.keys = x.b = 0;
-    x.tiles = 1;
-    if (s.count > kOrdered) {
-      const int place = p.pairs - 1 - e;
-      int lo = 0, hi = s.count;
-      while (hi - lo > 1) {
-        const int step = (hi - lo + 31) / 32, at = lo + lane * step;
-        const unsigned there = __ballot_sync(0xffffffffu, at < hi && s.start(at) / pair + at <= place);
-        const int last = there ? 31 - __clz(there) : 0;
-        lo += last * step;
-        hi = min(lo + step, hi);
-      }
-      x.b = lo;
-      e = max(0, s.start(lo + 1) - s.start(lo) + pair - 1) / pair - 1 - (place - (s.start(lo) / pair + lo));
-    } else if (s.count > 1) {
-      auto count = [&](int b, int h) {
-        if (b >= s.count) return 0;
-        const int n = s.start(b + 1) - s.start(b);
-        return n > 0 ? ends_from(max(s.lengths[b], n), (n + pair - 1) / pair, pair, h) : 0;  // (no pair's last token is before the first)
-      };
-      int hi = 0;
-      for (int b = lane; b < s.count; b += 32) hi = max(hi, max(s.lengths[b], s.start(b + 1) - s.start(b)));
-      hi = __reduce_max_sync(0xffffffffu, hi);
-      int lo = -1;  // all pairs' last tokens have more before them, none has `hi`; as many as e do not have lo + 1 in the end
-      while (hi - lo > 1) {
-        const int mid = lo + (hi - lo) / 2;
-        int n = 0;
-        for (int b0 = 0; b0 < s.count; b0 += 32) n += count(b0 + lane, mid);
-        n = __reduce_add_sync(0xffffffffu, n);
-        if (n > e) {
-          lo = mid;
-        } else {
-          hi = mid;
-        }
-      }
-      // pairs with more come first; then those that have just as many, in the order of the sequences
-      int more = 0;
-      for (int b0 = 0; b0 < s.count; b0 += 32) more += count(b0 + lane, lo + 1);
-      e -= __reduce_add_sync(0xffffffffu, more);
-      int found = -1;
-      for (int b0 = 0; b0 < s.count && found < 0; b0 += 32) {
-        const int mine = count(b0 + lane, lo) - count(b0 + lane, lo + 1);
-        int upto = mine;
+  struct Row {
+    int first[2], rows[2], length[2];  // of sequences lane and lane + 32: first row, rows, tokens
+    int pairs[2], level[2];            // pairs of tiles, level of the last one
+
+    __device__ __forceinline__ explicit Row(const PromptArgs& p) {
+      const int pair = TILES * p.tile_tokens, lane = threadIdx.x & 31;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int v = __shfl_up_sync(0xffffffffu, upto, o);
-          if (lane >= o) upto += v;
-        }
-        const unsigned there = __ballot_sync(0xffffffffu, e < upto && e >= upto - mine);
-        if (there) {
-          const int l = __ffs(there) - 1;
-          found = b0 + l;
-          e = count(found, lo + 1) + (e - __shfl_sync(0xffffffffu, upto - mine, l));
-        } else {
-          e -= __shfl_sync(0xffffffffu, upto, 31);
+      for (int i = 0; i < 2; ++i) {
+        const int b = lane + 32 * i;
+        first[i] = rows[i] = length[i] = pairs[i] = level[i] = 0;
+        if (p.seq.count <= kOrdered && b < p.seq.count) {
+          first[i] = p.seq.start(b), rows[i] = max(0, p.seq.start(b + 1) - first[i]), length[i] = p.seq.lengths[b];
+          pairs[i] = (rows[i] + pair - 1) / pair;
+          level[i] = (max(max(length[i], rows[i]), 1) - 1) / pair;  // (no pair's last token is before the first)
         }
       }
-      x.b = max(found, 0);
-      if (found < 0) e = -1;
     }
-    const int first = s.start(x.b), n = s.start(x.b + 1) - first, length = s.lengths[x.b];
-    if (n > 0 && e >= 0 && e < (n + pair - 1) / pair) {
-      const int from = n - (e + 1) * pair;  // (the first pair has what is left)
-      x.tokens = from < 0 ? pair + from : pair;
-      x.tiles = x.tokens > p.tile_tokens ? 2 : 1;
-      x.row0 = first + max(from, 0);
-      x.keys = s.keys(length);
-      x.p_lo = max(length, 0) - n + max(from, 0);  // (a negative length: no keys)
+    // Pairs of sequence lane + 32 i of at least a level.
+    __device__ __forceinline__ int from(int i, int l) const { return max(0, min(pairs[i], level[i] - l + 1)); }
+
+    __device__ __forceinline__ Unit unit(const PromptArgs& p, int index, int rank) const {
+      const int pair = TILES * p.tile_tokens, lane = threadIdx.x & 31;
+      int e = index / p.kv_heads;  // in the end: which of the sequence's pairs, from the last one on
+      int row0, n, tokens;
+      Unit x;
+      x.head = index - e * p.kv_heads;
+      if (p.seq.count > kOrdered) {
+        const int place = p.pairs - 1 - e;
+        int lo = 0, hi = p.seq.count;
+        while (hi - lo > 1) {
+          const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+          const unsigned there = __ballot_sync(0xffffffffu, at < hi && p.seq.start(at) / pair + at <= place);
+          const int last = there ? 31 - __clz(there) : 0;
+          lo += last * step;
+          hi = min(lo + step, hi);
+        }
+        x.b = lo;
+        row0 = p.seq.start(lo), n = max(0, p.seq.start(lo + 1) - row0), tokens = p.seq.lengths[lo];
+        e = (n + pair - 1) / pair - 1 - (place - (row0 / pair + lo));
+      } else {
+        int lo = -1, hi = __reduce_max_sync(0xffffffffu, max(level[0], level[1])) + 1;  // all pairs are of level lo at least, none of level hi
+        while (hi - lo > 1) {
+          const int mid = lo + (hi - lo) / 2;
+          if (__reduce_add_sync(0xffffffffu, from(0, mid) + from(1, mid)) > e) {
+            lo = mid;
+          } else {
+            hi = mid;
+          }
+        }
+        e -= __reduce_add_sync(0xffffffffu, from(0, hi) + from(1, hi));  // among those of level lo, one of a sequence at most
+        const unsigned at0 = __ballot_sync(0xffffffffu, from(0, lo) > from(0, hi)), at1 = __ballot_sync(0xffffffffu, from(1, lo) > from(1, hi));
+        const int i = e < __popc(at0) ? 0 : 1;
+        unsigned at = i ? at1 : at0;
+        for (int nth = e - (i ? __popc(at0) : 0); nth > 0 && at; --nth) at &= at - 1u;
+        const int l = __ffs(at) - 1, from_l = max(l, 0);
+        x.b = from_l + 32 * i;
+        row0 = __shfl_sync(0xffffffffu, i ? first[1] : first[0], from_l);
+        n = __shfl_sync(0xffffffffu, i ? rows[1] : rows[0], from_l);
+        tokens = __shfl_sync(0xffffffffu, i ? length[1] : length[0], from_l);
+        e = l < 0 ? -1 : __shfl_sync(0xffffffffu, i ? level[1] : level[0], from_l) - lo;
+      }
+      x.end = x.tokens = x.p_lo = x.keys = x.row0 = 0;
+      x.tiles = 1;
+      const int begin = n - (e + 1) * pair;  // (the first pair has what is left)
+      if (e >= 0 && begin > -pair) {
+        x.tokens = begin < 0 ? pair + begin : pair;
+        x.tiles = x.tokens > p.tile_tokens ? 2 : 1;
+        x.row0 = row0 + max(begin, 0);
+        x.keys = p.seq.keys(tokens);
+        x.p_lo = max(tokens, 0) - n + max(begin, 0);  // (a negative length: no keys)
+      }
+      x.list = KeyList(x.tokens > 0 ? max(0, min(x.keys, x.p_lo + x.tokens)) : 0, x.p_lo, p.window, p.sinks, 1 << p.box_log2);
+      const int steps = x.list.count / BC + (x.list.count % BC ? 1 : 0);
+      const int step0 = kKeySplit ? static_cast<int>(static_cast<long long>(steps) * rank / p.splits) : 0;
+      x.steps = (kKeySplit ? static_cast<int>(static_cast<long long>(steps) * (rank + 1) / p.splits) : steps) - step0;
+      x.v0 = step0 * BC;
+      return x;
     }
-    x.list = KeyList(x.tokens > 0 ? max(0, min(x.keys, x.p_lo + x.tokens)) : 0, x.p_lo, p.window, p.sinks, 1 << p.box_log2);
-    const int steps = x.list.count / BC + (x.list.count % BC ? 1 : 0);
-    const int step0 = kKeySplit ? static_cast<int>(static_cast<long long>(steps) * rank / p.splits) : 0;
-    x.steps = (kKeySplit ? static_cast<int>(static_cast<long long>(steps) * (rank + 1) / p.splits) : steps) - step0;
-    x.v0 = step0 * BC;
-    return x;
-  }
+  };
 
   // Bits below n, of 32.
   __device__ static __forceinline__ uint32_t below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
@@ -225,11 +218,12 @@ struct AttnPrompt {
       tma_prefetch_desc(&p.tmQ);
       tma_prefetch_desc(&p.tmK);
       tma_prefetch_desc(&p.tmV);
-      mbar_init(&bars->q_full, 1);
-      mbar_init(&bars->q_empty, 1);
       for (int s = 0; s < K_STAGES; ++s) mbar_init(&bars->k_full[s], 1), mbar_init(&bars->k_empty[s], 1);
       for (int s = 0; s < V_STAGES; ++s) mbar_init(&bars->v_full[s], 1), mbar_init(&bars->v_empty[s], 1);
-      for (int t = 0; t < TILES; ++t) mbar_init(&bars->s_full[t], 1), mbar_init(&bars->o_full[t], 1);
+      for (int t = 0; t < TILES; ++t) {
+        mbar_init(&bars->q_full[t], 1), mbar_init(&bars->q_empty[t], 1);
+        mbar_init(&bars->s_full[t], 1), mbar_init(&bars->o_full[t], 1);
+      }
       for (int s = 0; s < 2; ++s) mbar_init(&bars->unit_full[s], 1), mbar_init(&bars->unit_empty[s], UNIT_WARPS);
       mbar_init(&bars->taken, 1);
       bars->abort_flag = 0u;
@@ -286,33 +280,37 @@ struct AttnPrompt {
       };
       if (warp == 0) {
         // ------------------------------------------------------------------ loads of Q and K
-        uint32_t it = 0, queries = 0;  // steps and units with keys so far
+        uint32_t it = 0, queries[TILES] = {0, 0};  // steps and tiles of queries so far
         bool ok = true;
-        auto load_queries = [&](const Unit& x) {
-          ++queries;
+        // A tile of queries into its place, once the last scores of the one before are done: of tile 0 half a step earlier than of tile 1.
+        auto load_queries = [&](const Unit& x, int t) {
           if (lane == 0) {
-            mbar_expect_tx(&bars->q_full, x.tiles * HALVES * p.tile_tokens * p.group * 128);
-            for (int t = 0; t < x.tiles; ++t)
+            mbar_expect_tx(&bars->q_full[t], HALVES * p.tile_tokens * p.group * 128);
 #pragma unroll
-              for (int b = 0; b < HALVES; ++b)
-                tma_load_3d(smem + t * Q_BYTES + b * BOX_BYTES, &p.tmQ, &bars->q_full, b * 64, x.head * p.group, x.row0 + t * p.tile_tokens);
+            for (int b = 0; b < HALVES; ++b)
+              tma_load_3d(smem + t * Q_BYTES + b * BOX_BYTES, &p.tmQ, &bars->q_full[t], b * 64, x.head * p.group, x.row0 + t * p.tile_tokens);
           }
           __syncwarp();
         };
         for (Unit x; next_unit(&x);) {
           if (x.steps == 0) continue;
-          int key = 0, page = page_of(x, 0, &key);
-          const bool queries_on = ok && mbar_test_warp(&bars->q_empty, (queries & 1u) ^ 1u);
-          if (queries_on) load_queries(x);
+          int key = 0, page = page_of(x, 0, &key), on = 0;  // on: tiles of queries under way
+          if (ok && mbar_test_warp(&bars->q_empty[0], (queries[0] & 1u) ^ 1u)) load_queries(x, on++);
           for (int j = 0; j < x.steps; ++j, ++it) {
-            if (!ok) continue;
             const int ks = it % K_STAGES, this_key = key, this_page = page;
-            if (j + 1 < x.steps) page = page_of(x, j + 1, &key);
-            ok = __all_sync(0xffffffffu, mbar_wait(&bars->k_empty[ks], ((it / K_STAGES) & 1u) ^ 1u, &bars->abort_flag));
+            if (ok && j + 1 < x.steps) page = page_of(x, j + 1, &key);
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&bars->k_empty[ks], ((it / K_STAGES) & 1u) ^ 1u, &bars->abort_flag));
             if (ok) load(smem + OFF_K + ks * KV_BYTES, &p.tmK, &bars->k_full[ks], x, this_key, this_page);
-            if (ok && j == 0 && !queries_on) {  // (behind the first K tile: the queries' place was not free before)
-              ok = __all_sync(0xffffffffu, mbar_wait(&bars->q_empty, (queries & 1u) ^ 1u, &bars->abort_flag));
-              if (ok) load_queries(x);
+            if (j == 0) {
+#pragma unroll
+              for (int t = 0; t < TILES; ++t) {
+                if (t >= x.tiles) continue;
+                if (ok && on == t) {
+                  ok = __all_sync(0xffffffffu, mbar_wait(&bars->q_empty[t], (queries[t] & 1u) ^ 1u, &bars->abort_flag));
+                  if (ok) load_queries(x, on++);
+                }
+                ++queries[t];
+              }
             }
             if (!ok && lane == 0) report(bars, PAGED_TIMEOUT_LOADS, it, 0u);
           }
@@ -323,7 +321,7 @@ struct AttnPrompt {
         const uint64_t qdesc = make_smem_desc(smem_u32(smem), 16, 1024, SWZ_128B);
         const uint64_t kdesc = make_smem_desc(smem_u32(smem + OFF_K), 16, 1024, SWZ_128B);
         const uint64_t vdesc = make_smem_desc(smem_u32(smem + OFF_V), BOX_BYTES, 1024, SWZ_128B);
-        uint32_t it0 = 0, queries = 0;  // steps and units with keys before the current one's
+        uint32_t it0 = 0, queries[TILES] = {0, 0};  // steps before the current unit's, tiles of queries before its own
         // S_t of step it0 + i, of a unit of `tiles` tiles; `last`: it is the unit's last
         auto issue_s = [&](int t, int i, int tiles, bool last) {
           const uint64_t ad = qdesc + t * (Q_BYTES >> 4), bd = kdesc + ((it0 + i) % K_STAGES) * (KV_BYTES >> 4);
@@ -333,10 +331,8 @@ struct AttnPrompt {
             umma_ss<false>(tmem + t * BC, ad + ((box * BOX_BYTES + in_row) >> 4), bd + ((box * BOX_BYTES + in_row) >> 4), IDESC_S, ks > 0 ? 1u : 0u);
           }
           umma_commit(&bars->s_full[t]);
-          if (t == tiles - 1) {
-            umma_commit(&bars->k_empty[(it0 + i) % K_STAGES]);
-            if (last) umma_commit(&bars->q_empty);
-          }
+          if (last) umma_commit(&bars->q_empty[t]);
+          if (t == tiles - 1) umma_commit(&bars->k_empty[(it0 + i) % K_STAGES]);
         };
         auto issue_pv = [&](int t, int j, int ks0, int ks1) {
           const uint64_t vd = vdesc + ((it0 + j) % V_STAGES) * (KV_BYTES >> 4);
@@ -353,23 +349,24 @@ struct AttnPrompt {
           known = false;
           if (end) break;
           if (nkv == 0) continue;
-          if (begun == 0) {
-            const bool q_there = __all_sync(0xffffffffu, mbar_wait(&bars->q_full, queries & 1u, &bars->abort_flag));
-            if (!q_there && lane == 0) report(bars, PAGED_TIMEOUT_ATTENTION, 0u, 0u);
-          }
-          ++queries;
-          __syncwarp();
           named_bar_sync(BAR_KV, KV_THREADS);  // the first K tile
-          tc_fence_after_sync();
-          const int first = kApart && begun == 0 ? 1 : tiles;  // (the second tile's follow the first one's first weights)
-#pragma unroll 1
-          for (int t = begun; t < first; ++t) {
+          const uint32_t q_parity = (queries[0] & 1u) | (queries[1] & 1u) << 1;
+          auto begin = [&](int t) {
+            const bool q_there = __all_sync(0xffffffffu, mbar_wait(&bars->q_full[t], q_parity >> t & 1u, &bars->abort_flag));
+            if (!q_there && lane == 0) report(bars, PAGED_TIMEOUT_ATTENTION, 0u, t);
+            __syncwarp();
+            tc_fence_after_sync();
             if (elect_one()) issue_s(t, 0, tiles, nkv == 1);
             __syncwarp();
-          }
+          };
+          const int first = kApart && begun == 0 ? 1 : tiles;  // (the second tile's follow the first one's first weights)
+#pragma unroll 1
+          for (int t = begun; t < first; ++t) begin(t);
           const bool second = first < tiles;
+          ++queries[0];
+          queries[1] += tiles - 1;
           begun = 0;  // (of the next unit, from here on)
-          bool ready = false;
+          bool keys_there = false;
           int next_steps = 0, next_tiles = 0;
           for (int j = 0; j < nkv; ++j) {
             named_bar_sync(BAR_KV, KV_THREADS);
@@ -378,10 +375,7 @@ struct AttnPrompt {
             for (int t = 0; t < tiles; ++t) {
               named_bar_sync(BAR_PART + t, PT_THREADS);
               tc_fence_after_sync();
-              if (second && j == 0 && t == 0) {
-                if (elect_one()) issue_s(1, 0, tiles, nkv == 1);
-                __syncwarp();
-              }
+              if (second && j == 0 && t == 0) begin(1);
               if (elect_one()) issue_pv(t, j, 0, P_PART / 16);
               __syncwarp();
               if (last && !known && mbar_test_warp(&bars->unit_full[taken & 1], (taken >> 1) & 1u)) {  // (while the last weights are waited for)
@@ -399,13 +393,12 @@ struct AttnPrompt {
               __syncwarp();
               // The next scores of this tile: of the next step, or of the next unit's first if its operands have come (the other tile has
               // still to finish then, and this one's warps their rows).
+              bool ahead = false;
               if (last && next_steps > 0 && t < next_tiles && begun == t) {
-                if (!ready)
-                  ready = mbar_test_warp(&bars->q_full, queries & 1u) &&
-                          mbar_test_warp(&bars->k_full[(it0 + nkv) % K_STAGES], ((it0 + nkv) / K_STAGES) & 1u);
+                keys_there = keys_there || mbar_test_warp(&bars->k_full[(it0 + nkv) % K_STAGES], ((it0 + nkv) / K_STAGES) & 1u);
+                ahead = keys_there && mbar_test_warp(&bars->q_full[t], (t ? queries[1] : queries[0]) & 1u);
                 tc_fence_after_sync();
               }
-              const bool ahead = last && ready && t < next_tiles && begun == t;
               if (!last || ahead) {
                 if (elect_one()) issue_s(t, j + 1, last ? next_tiles : tiles, last ? next_steps == 1 : j + 2 == nkv);
                 __syncwarp();
@@ -451,6 +444,7 @@ struct AttnPrompt {
         // with one that says so, and where a slot does not become free, with none: the warps' wait for it ends by itself.
         uint32_t it = 0, made = 0, asked = 0;
         bool ok = true;
+        const Row row(p);
         auto publish = [&](Unit& x) {  // false: the row ends
           if (bars->abort_flag != 0u) x.end = 1;
           const int slot = made & 1;
@@ -485,13 +479,13 @@ struct AttnPrompt {
             fence_proxy_async_smem();  // (the next answer is written behind this reading)
             __syncwarp();
           }
-          Unit next = unit_of(p, index < 0 ? 0 : index, rank);
+          Unit next = row.unit(p, index < 0 ? 0 : index, rank);
           if (index < 0) next.end = 1;
           return publish(next);
         };
         bool more;
         {
-          Unit first = unit_of(p, static_cast<int>(blockIdx.x) / (kKeySplit ? p.splits : 1), rank);
+          Unit first = row.unit(p, static_cast<int>(blockIdx.x) / (kKeySplit ? p.splits : 1), rank);
           more = publish(first);
         }
         while (more) {
@@ -505,14 +499,14 @@ struct AttnPrompt {
           for (int j = 0; j < x.steps; ++j, ++it) {
             const int vs = it % V_STAGES, this_key = key, this_page = page;
             if (j + 1 < x.steps) page = page_of(x, j + 1, &key);
-            if (j == max(0, x.steps - 3)) ask();
+            if (j == max(0, x.steps - 2)) ask();
             if (ok) {
               ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_empty[vs], ((it / V_STAGES) & 1u) ^ 1u, &bars->abort_flag));
               if (ok) load(smem + OFF_V + vs * KV_BYTES, &p.tmV, &bars->v_full[vs], x, this_key, this_page);
               if (!ok && lane == 0) report(bars, PAGED_TIMEOUT_LOADS, it, 1u);
             }
-            if (j == max(0, x.steps - 2)) more = answered();
           }
+          more = answered();  // (behind the last V tile, which the products wait for: about a step and a half before the end)
         }
       }
       if constexpr (kKeySplit) {  // the two meetings of the cluster that join the partial results
