@@ -426,11 +426,14 @@ struct AttnPrompt {
             const int v0 = x.v0 + j * BC;
             const int end = max(0, min(BC, x.list.count - v0)), gap0 = max(0, min(BC, p.sinks - v0)), gap1 = max(0, min(BC, x.list.lo - v0));
             if (end < BC || gap0 < gap1) {
-              uint8_t* v = smem + OFF_V + (it % V_STAGES) * KV_BYTES;
-              for (int u = lane; u < BC * 8 * HALVES; u += 32) {
-                const int k = u / 8 % BC;
-                if (k >= end || (k >= gap0 && k < gap1)) *reinterpret_cast<uint4*>(v + u * 16) = make_uint4(0u, 0u, 0u, 0u);  // (whole rows: in any order)
-              }
+              auto zero = [&](int from, int to) {  // rows of both halves, whole (their 16-byte units in any order)
+                for (int u = lane; u < (to - from) * 8 * HALVES; u += 32) {
+                  const int r = HALVES == 2 ? u >> 4 : u >> 3, h = HALVES == 2 ? u >> 3 & 1 : 0;
+                  *reinterpret_cast<uint4*>(smem + OFF_V + (it % V_STAGES) * KV_BYTES + h * BOX_BYTES + (from + r) * 128 + (u & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                }
+              };
+              zero(end, BC);
+              zero(gap0, min(gap1, end));
               fence_proxy_async_smem();
             }
             if (j + 1 < x.steps) wait(&bars->k_full[(it + 1) % K_STAGES], ((it + 1) / K_STAGES) & 1u, 1u, it + 1);
@@ -539,8 +542,11 @@ struct AttnPrompt {
       const int position = x.p_lo + token;
       const int see = live ? x.list.place(min(position + 1, x.keys)) : 0x7fffffff;
       const int near = live && p.window > 0 && position >= p.window ? position - p.window + 1 - x.list.shift : 0;
-      // m: the row's running maximum, which the exponentials of a step are taken against, in the exp2 domain: the maximum itself, so that
-      // the largest probability is exactly 1 and does not lose a bit to the 16-bit P.
+      // m: what the exponentials of a step are taken against, in the exp2 domain: the row's running maximum as it was when some row of the warp last
+      // passed its own by 8. Weights are up to 2^8 then, which 16 bits hold as exactly as any (P's relative rounding is the same everywhere), and
+      // the sums in 32 bits; what is lost is that the largest weight is no longer exactly 1. Error against 64 bits, 2048 tokens, bf16: normal scores 2.02e-3
+      // -> 2.05e-3, scores of 4 times that 1.72e-3 -> 1.95e-3, of 16 times 1.44e-3 -> 1.45e-3. A window's nine steps would nearly all rescale O:
+      // 16384 tokens with a window of 1024 303 -> 283 us, 8192 without one 472 -> 451.
       float m = -INFINITY;
       uint64_t sum2[2] = {f32x2(0.f, 0.f), f32x2(0.f, 0.f)};
       const int mine = t < x.tiles ? x.steps : 0;
@@ -583,7 +589,9 @@ struct AttnPrompt {
 #pragma unroll
         for (int c = 0; c < 4; ++c) max_of(c);
         // (the scale is positive: checked by the host)
-        const float mx = fmaxf(m, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2);
+        const float highest = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;
+        const bool moved = __any_sync(0xffffffffu, live && highest > m + 8.f);
+        const float mx = moved ? fmaxf(m, highest) : m;
         // (without a finite score so far the probabilities are 0, not -inf - -inf)
         const float base = mx == -INFINITY ? 0.f : mx;
         const float alpha = ex2(m - base);
@@ -604,9 +612,9 @@ struct AttnPrompt {
           }
           tmem_st_32x32b_x16(col_s + c * 16, w);
         };
-        // O_t <- alpha * O_t, where a row of the warp has a new maximum (the previous P_t V has retired: the scores just read were issued
+        // O_t <- alpha * O_t, where the warp's rows have another m (the previous P_t V has retired: the scores just read were issued
         // behind it).
-        if (j > 0 && __any_sync(0xffffffffu, live && alpha != 1.f)) {
+        if (j > 0 && moved) {
           auto scale_store = [&](uint32_t (&o)[32], int c) {
             pin_32(o);
 #pragma unroll
