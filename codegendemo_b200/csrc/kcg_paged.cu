@@ -3,7 +3,9 @@
 // Bound by HBM: each row's heads are read once and written once (a prompt), or by the latency of three dependent loads (the row's
 // sequence, its length, its page) in a decode step. A warp takes one row and four heads (d = 64: eight) at a time, a thread two
 // 16-byte pieces whose values turn together, so that it reads its angles once for all heads and needs no other thread's values;
-// where there are few rows, several warps share one.
+// where there are few rows, several warps share one. 12085 rows of 32 + 2 x 8 heads of 128 values, bf16: 53.6 us, 5.7 TB/s, with four CTAs an
+// SM (64 registers; three of 74: 59.9, five or six, with spills, 58.8 and 62.7; the rows towards L2 while their places are looked up: 56.0);
+// 32 rows 3.2 us.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -40,7 +42,7 @@ constexpr int kAppendWarps = 8;
 // A thread's piece pair u of a head: halves rotary / 2 values apart (the pair turns together), neighbouring pieces when interleaved
 // or past the rotated part.
 template <typename T, int kD, bool kInterleaved>
-__global__ void __launch_bounds__(kAppendWarps * 32) append_kv_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kAppendWarps * 32, 4) append_kv_kernel(const AppendArgs a) {
   constexpr int UNITS = kD / 16, HEADS = 32 / UNITS;  // piece pairs of a head, heads of a warp's step
   griddep_launch_dependents();
   griddep_wait();
@@ -179,11 +181,12 @@ int encode_cache(EncodeFn encode, CUtensorMap* tm, const kcg_paged_cache* c, uin
 
 // Dynamic shared memory of a kernel, opted in to once on each device.
 template <auto kKernel>
-int opt_in(int device, int bytes) {
+int opt_in(int device, int bytes, bool large_clusters = false) {
   static std::atomic<unsigned long long> done{0};
   if (done.load() >> device & 1ull) return 0;
-  const cudaError_t e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(MaxDynamicSharedMemorySize)");
+  cudaError_t e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && large_clusters) e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
   done.fetch_or(1ull << device);
   return 0;
 }
@@ -195,21 +198,67 @@ int shared_rows(const kcg_paged_cache* c, const kcg_paged_query* q) {
   return n <= 64 ? static_cast<int>(n) : 0;
 }
 
+// How many clusters of a size run at once (asked once per device and kernel; -1: the size is not to be had).
+template <auto kKernel>
+int clusters_at_once(int device, int threads, int smem, int size) {
+  static std::atomic<int> known[64][17];
+  int n = known[device][size].load();
+  if (n == 0) {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = size, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(size), cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem, cfg.attrs = attr, cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, kKernel, &cfg) != cudaSuccess || n <= 0) {
+      cudaGetLastError();
+      n = -1;
+    }
+    known[device][size].store(n);
+  }
+  return n;
+}
+
+// CTAs of a cluster that share the keys of one (sequence, key head) of `units`, where each has one of its own, and no second kernel joins their
+// parts: where the table is so short that each has four tiles at most, and all clusters run at once; two tiles at least, if there are
+// four. 0: the keys of all sequences are cut into ranges. Bf16, 32 heads over 8 of 128 values, cluster against ranges: 1 sequence of 128 keys 7.2 us /
+// 9.6, of 1024 8.7 / 10.1, of 2048 9.9 / 11.4, 4 of 512 9.1 / 11.3; with eight tiles each and more 4 of 4096 16.8 / 15.7, 1 of 32768 46 / 32.
+template <typename Active>
+int tokens_cluster(long long units, int max_tiles, Active&& active) {
+  if (max_tiles <= 4) return 1;
+  const int s = max_tiles / 2 < 16 ? max_tiles / 2 : 16, least = (max_tiles + 3) / 4;
+  for (int n = s; n >= least; --n)
+    if (units <= active(n)) return n;
+  return 0;
+}
+
 int64_t tokens_workspace(int sms, int rows, int d) { return 2ll * sms * (2ll * rows * (d + 2) * 4 + 16); }
 
 template <int kD, bool kBf16, int kRowGroups>
-int launch_tokens(int device, int sms, cudaStream_t st, const kcg_paged_cache* c, const TokensArgs& p) {
-  using Kern = AttnTokens<kD, kBf16, kRowGroups>;
-  if (int r = opt_in<attention_tokens_kernel<kD, kBf16, kRowGroups>>(device, Kern::SMEM_BYTES)) return r;
+int launch_tokens(int device, int sms, cudaStream_t st, const kcg_paged_cache* c, TokensArgs& p) {
+  using Kern = AttnTokens<kD, kBf16, kRowGroups, false>;
+  constexpr auto ranges = attention_tokens_kernel<kD, kBf16, kRowGroups, false>;
+  constexpr auto cluster = attention_tokens_kernel<kD, kBf16, kRowGroups, true>;
+  if (int r = opt_in<ranges>(device, Kern::SMEM_BYTES)) return r;
+  if (int r = opt_in<cluster>(device, Kern::SMEM_BYTES, true)) return r;
+  const long long units = static_cast<long long>(c->sequences) * c->kv_heads;
+  long long keys = static_cast<long long>(c->width) * c->page;
+  if (p.window > 0) keys = std::min(keys, static_cast<long long>(p.window) + p.seq.each + p.sinks + 2 * (1 << p.box_log2));
+  const int max_tiles = static_cast<int>(std::min((keys + Kern::BC - 1) / Kern::BC, 1000000LL));
+  p.splits = tokens_cluster(units, max_tiles, [&](int s) { return clusters_at_once<cluster>(device, Kern::NUM_THREADS, Kern::SMEM_BYTES, s); });
   Launch launch(st);
+  if (p.splits > 0) {
+    if (units * p.splits > 0x7fffffffLL) return fail(KCG_E_TOO_LARGE, "attention_paged: too many rows");
+    launch.shape(static_cast<unsigned>(units * p.splits), Kern::NUM_THREADS, Kern::SMEM_BYTES, p.splits);
+    return launch(cluster, "attention_paged launch", p);
+  }
   launch.shape(2 * sms, Kern::NUM_THREADS, Kern::SMEM_BYTES);
-  if (int r = launch(attention_tokens_kernel<kD, kBf16, kRowGroups>, "attention_paged launch", p)) return r;
+  if (int r = launch(ranges, "attention_paged launch", p)) return r;
   launch.shape(2 * sms, 512);
   return launch(attention_tokens_join_kernel<kD, kBf16>, "attention_paged join launch", p, 2 * sms);
 }
 
 template <int kRowGroups>
-int launch_tokens_of(int device, int sms, cudaStream_t st, const kcg_paged_cache* c, const TokensArgs& p) {
+int launch_tokens_of(int device, int sms, cudaStream_t st, const kcg_paged_cache* c, TokensArgs& p) {
   if (c->d == 128)
     return c->dtype == KCG_DTYPE_BFLOAT16 ? launch_tokens<128, true, kRowGroups>(device, sms, st, c, p) : launch_tokens<128, false, kRowGroups>(device, sms, st, c, p);
   return c->dtype == KCG_DTYPE_BFLOAT16 ? launch_tokens<64, true, kRowGroups>(device, sms, st, c, p) : launch_tokens<64, false, kRowGroups>(device, sms, st, c, p);
@@ -237,26 +286,6 @@ int attention_tokens(int device, cudaStream_t st, const kcg_paged_cache* c, cons
   return launch_tokens_of<4>(device, sms, st, c, p);
 }
 
-// How many clusters of 2 .. 8 CTAs of the key-split prompt kernel run at once (asked once per device and kernel; 0: not known yet).
-template <auto kKernel>
-int prompt_clusters(int device, int threads, int smem, int size) {
-  static std::atomic<int> known[64][9];
-  int n = known[device][size].load();
-  if (n == 0) {
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = size, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.gridDim = dim3(size), cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem, cfg.attrs = attr, cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&n, kKernel, &cfg) != cudaSuccess || n <= 0) {
-      cudaGetLastError();
-      n = -1;  // this size is not used
-    }
-    known[device][size].store(n);
-  }
-  return n;
-}
-
 template <int kD, bool kBf16>
 int launch_prompt(int device, cudaStream_t st, PromptArgs& p, long long pairs, int max_steps) {
   using Kern = AttnPrompt<kD, kBf16, false>;
@@ -270,7 +299,7 @@ int launch_prompt(int device, cudaStream_t st, PromptArgs& p, long long pairs, i
   // sequences are as long as the table, four tiles of keys each (joining costs what two do).
   p.splits = 1;
   for (int s = 8; s >= 2 && p.splits == 1; --s)
-    if (max_steps >= 4 * s && units <= prompt_clusters<split>(device, Kern::NUM_THREADS, Kern::SMEM_BYTES, s)) p.splits = s;
+    if (max_steps >= 4 * s && units <= clusters_at_once<split>(device, Kern::NUM_THREADS, Kern::SMEM_BYTES, s)) p.splits = s;
   Launch launch(st);
   launch.shape(static_cast<unsigned>(units * p.splits), Kern::NUM_THREADS, Kern::SMEM_BYTES, p.splits);
   return p.splits > 1 ? launch(split, "attention_paged launch", p) : launch(whole, "attention_paged launch", p);

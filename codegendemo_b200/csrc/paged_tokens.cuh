@@ -21,9 +21,10 @@ struct TokensArgs {
   const void* q;
   void* o;
   long long q_row, q_head, o_row, o_head;
-  float* parts;  // [2 * CTAs][rows][d], then [2 * CTAs][rows] {maximum, sum}, then [CTAs] {sequence, head, last CTA, 0}
+  float* parts;  // [2 * CTAs][rows][d], then [2 * CTAs][rows] {maximum, sum}, then [CTAs] {sequence, head, first CTA, last CTA}
   int kv_heads, group, window, sinks;
   int box_log2;  // keys of a box
+  int splits;    // the cluster form: CTAs that share a (sequence, head)'s keys
   float scale_log2;
 };
 
@@ -45,7 +46,8 @@ struct Ranges {
   __device__ __forceinline__ int owner(long long place) const { return static_cast<int>(((place + 1) * ctas - 1) / total); }
 };
 
-template <int kD, bool kBf16, int kRowGroups>
+// kCluster: a cluster of `splits` CTAs has the keys of one (sequence, head), and joins its parts in shared memory; no second kernel.
+template <int kD, bool kBf16, int kRowGroups, bool kCluster>
 struct AttnTokens {
   // Keys of a tile: 32 KB of K and V. (64 keys of d = 64 left each warp one short chain of products and exponentials a tile, 0.84 us for 16 KB:
   // 16 sequences x 32 heads of 2049 keys 48 us, bound by that.)
@@ -62,7 +64,7 @@ struct AttnTokens {
   static constexpr bool kQueriesAhead = kRowGroups == 1;
   static constexpr int Q_PITCH = kD * 2 + 16, Q_BYTES = kQueriesAhead ? 16 * Q_PITCH : 0;
   static constexpr int CHAINS = WKEYS <= 32 ? 2 : 1;  // accumulators per 8 keys (even and odd 16 values of d)
-  static constexpr int SMEM_BYTES = RING_BYTES + JOIN_BYTES + Q_BYTES + 1024 + 1280;
+  static constexpr int SMEM_BYTES = RING_BYTES + JOIN_BYTES + Q_BYTES + 1024 + 1792;
   static_assert(2 * (SMEM_BYTES + 1024) <= 228 * 1024, "two CTAs an SM");
   using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
 
@@ -81,12 +83,13 @@ struct AttnTokens {
     uint64_t full[STAGES], empty[STAGES], q_empty;
     Tile tile[STAGES];
     float2 warp_ml[4][16];
+    float2 cta_ml[ROWS];  // (the cluster form)
     long long before[5];  // places of each warp's sequences
     long long begin;      // the first place with a tile in this CTA's range
     int found[3];         // its sequence (-1: there is none), head and tile
     volatile uint32_t abort_flag;
   };
-  static_assert(sizeof(Shared) <= 1280, "barrier block exceeds its shared-memory slot");
+  static_assert(sizeof(Shared) <= 1792, "barrier block exceeds its shared-memory slot");
 
   __device__ static __forceinline__ void report(Shared* sh, uint32_t code, uint32_t d0) {
     sh->abort_flag = 1u;
@@ -138,6 +141,20 @@ struct AttnTokens {
     }
     griddep_wait();
 
+    int cta = static_cast<int>(blockIdx.x);
+    long long g0 = 0, g1 = 0, total = 0;
+    if constexpr (kCluster) {
+      // this CTA's share of its (sequence, head)'s tiles
+      if (threadIdx.x == 0) {
+        const int unit = cta / p.splits, rank = static_cast<int>(cluster_cta_rank());
+        const int n = Keys(p, p.seq.lengths[unit / p.kv_heads]).count;
+        const int t0 = static_cast<int>(static_cast<long long>(n) * rank / p.splits), t1 = static_cast<int>(static_cast<long long>(n) * (rank + 1) / p.splits);
+        if (t0 < t1) sh->found[0] = unit / p.kv_heads, sh->found[1] = unit % p.kv_heads, sh->found[2] = t0, sh->begin = t0;
+        sh->before[0] = t1;
+      }
+      __syncthreads();
+      g0 = sh->begin, g1 = sh->before[0];
+    } else {
     // All sequences' places, and where this CTA's range begins: a thread counts those of its run of sequences.
     const int per = (p.seq.count + NUM_THREADS - 1) / NUM_THREADS;
     const int b0 = min(static_cast<int>(threadIdx.x) * per, p.seq.count), b1 = min(b0 + per, p.seq.count);
@@ -152,15 +169,14 @@ struct AttnTokens {
     }
     if (lane == 31) sh->before[warp] = upto;
     __syncthreads();
-    long long total = 0, base = 0;
+    long long base = 0;
 #pragma unroll
     for (int w = 0; w < 5; ++w) {
       if (w < warp) base += sh->before[w];
       total += sh->before[w];
     }
     const Ranges ranges(total, gridDim.x);
-    const int cta = static_cast<int>(blockIdx.x);
-    const long long g0 = cta < ranges.ctas ? ranges.begin(cta) : 0, g1 = cta < ranges.ctas ? ranges.begin(cta + 1) : 0;
+    if (cta < ranges.ctas) g0 = ranges.begin(cta), g1 = ranges.begin(cta + 1);
     base += upto - mine;
     if (g0 < g1 && g0 >= base && g0 < base + mine) {
       long long at = g0 - base;
@@ -181,6 +197,7 @@ struct AttnTokens {
       }
     }
     __syncthreads();
+    }
     const bool any = sh->found[0] >= 0;
 
     if (warp == 4) {
@@ -215,11 +232,14 @@ struct AttnTokens {
           // every row sees every key: up to the first row's position, from the last one's window on or among the sinks
           const int p_hi = seq.p_lo + p.seq.each - 1, near = p.window > 0 && p_hi >= p.window ? p_hi - p.window + 1 - seq.list.shift : 0;
           const bool all = v0 + BC <= seq.list.place(min(seq.keys, seq.p_lo + 1)) && (v0 >= near || v0 + BC <= p.sinks);
-          const bool whole = unit_begin >= g0 && unit_begin + seq.count <= g1;
+          const bool whole = kCluster ? p.splits == 1 : unit_begin >= g0 && unit_begin + seq.count <= g1;
           const bool first = i == 0 || t == 0;
           tile.flags = (all ? 0 : MASKED) | (first ? FIRST : 0) | (whole ? WHOLE : 0);
           tile.slot = 2 * cta + (unit_begin >= g0 ? 1 : 0);
-          if (!whole && unit_begin >= g0) meta = make_int4(b, h, ranges.owner(unit_begin + seq.count - 1), 0);
+          if (!kCluster && i == 0 && unit_begin < g0) {
+            const Ranges ranges(total, gridDim.x);
+            meta = make_int4(b, h, ranges.owner(unit_begin), ranges.owner(unit_begin + seq.count - 1));
+          }
           // the next tile, and its pages while this one's stage is waited for
           ++place;
           bool last = false;
@@ -262,7 +282,7 @@ struct AttnTokens {
                          &sh->full[s]);
         }
       }
-      if (lane == 0) {
+      if (!kCluster && lane == 0) {
         float* end = p.parts + 2ll * gridDim.x * rows * (kD + 2);
         reinterpret_cast<int4*>(end)[cta] = meta;
       }
@@ -459,6 +479,9 @@ struct AttnTokens {
               const int i_tok = r / p.group;
               T* to = static_cast<T*>(p.o) + (static_cast<long long>(tile.b) * p.seq.each + i_tok) * p.o_row + (tile.h * p.group + r - i_tok * p.group) * p.o_head + col;
               *reinterpret_cast<uint2*>(to) = make_uint2(pack_pair<kBf16>(a.x * inv, a.y * inv), pack_pair<kBf16>(a.z * inv, a.w * inv));
+            } else if (kCluster) {  // (the ring is idle: the CTA's last tile has been read)
+              reinterpret_cast<float4*>(smem)[r * (kD / 4) + col / 4] = a;
+              if (cc == 0 && c4 == 0) sh->cta_ml[r] = make_float2(top, sum_l);
             } else {
               const long long part = static_cast<long long>(tile.slot) * rows + r;
               *reinterpret_cast<float4*>(p.parts + part * kD + col) = a;
@@ -471,6 +494,50 @@ struct AttnTokens {
         if (tile.flags & END) break;
       }
     }
+    if constexpr (kCluster) {
+      if (p.splits > 1) {
+        if (!any)
+          for (int r = threadIdx.x; r < rows; r += NUM_THREADS) sh->cta_ml[r] = make_float2(-INFINITY, 0.f);
+        __syncwarp();
+        cluster_sync_all();
+        // this CTA's share of the result, 16-byte units of fp32 rows, joined over the cluster
+        constexpr int UNITS = kD / 4;
+        static_assert(ROWS * kD * 4 <= RING_BYTES, "the CTA's rows fit the ring");
+        const int rank = static_cast<int>(cluster_cta_rank()), unit = cta / p.splits, b = unit / p.kv_heads, h = unit % p.kv_heads;
+        const int u0 = rows * UNITS * rank / p.splits, u1 = rows * UNITS * (rank + 1) / p.splits;
+        const uint32_t o_addr = smem_u32(smem), ml_addr = smem_u32(&sh->cta_ml[0]);
+        for (int i = u0 + threadIdx.x; i < u1; i += NUM_THREADS) {
+          const int r = i / UNITS;
+          float2 ml[16];
+          float top = -INFINITY, sum = 0.f;
+#pragma unroll
+          for (int c = 0; c < 16; ++c) ml[c] = c < p.splits ? ld_cluster_f2(map_to_cta(ml_addr + r * 8, c)) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+          for (int c = 0; c < 16; ++c) top = fmaxf(top, ml[c].x);
+          float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int c0 = 0; c0 < 16; c0 += 8) {
+            float4 x[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              if (c0 + c < p.splits) x[c] = ld_cluster_f4(map_to_cta(o_addr + i * 16, c0 + c));
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              const float f = weight(ml[c0 + c], top);
+              if (f == 0.f) continue;  // (no part, or one of no key: whatever lies there)
+              a.x = fmaf(f, x[c].x, a.x), a.y = fmaf(f, x[c].y, a.y), a.z = fmaf(f, x[c].z, a.z), a.w = fmaf(f, x[c].w, a.w);
+              sum = fmaf(f, ml[c0 + c].y, sum);
+            }
+          }
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          const int i_tok = r / p.group;
+          T* to = static_cast<T*>(p.o) + (static_cast<long long>(b) * p.seq.each + i_tok) * p.o_row + (h * p.group + r - i_tok * p.group) * p.o_head + i % UNITS * 4;
+          *reinterpret_cast<uint2*>(to) = make_uint2(pack_pair<kBf16>(a.x * inv, a.y * inv), pack_pair<kBf16>(a.z * inv, a.w * inv));
+        }
+        __syncwarp();
+        cluster_sync_all();  // the other CTAs read this one's shared memory until here
+      }
+    }
     if (sh->abort_flag != 0u) {  // loads still in flight land before the ring is given up
       const uint64_t w0 = global_timer_ns();
       while (global_timer_ns() - w0 < 200000ull) __nanosleep(1000);
@@ -479,13 +546,15 @@ struct AttnTokens {
   }
 };
 
-template <int kD, bool kBf16, int kRowGroups>
+template <int kD, bool kBf16, int kRowGroups, bool kCluster>
 __global__ void __launch_bounds__(160, 2) attention_tokens_kernel(const __grid_constant__ TokensArgs p) {
-  AttnTokens<kD, kBf16, kRowGroups>::run(p);
+  AttnTokens<kD, kBf16, kRowGroups, kCluster>::run(p);
 }
 
-// The parts of a (sequence, key head) whose keys began in CTA blockIdx.x of the kernel above and ended in a later one's. 16 warps: as many to a row
-// as there are for it, each with a share of the parts, eight at a time.
+// The parts of the (sequence, key head) whose keys came into CTA blockIdx.x of the kernel above from the one before. A unit of n parts has n - 1 such
+// blocks, which share out its rows (one (sequence, head) of 65536 keys x 32 rows: 97 -> 22 us, in one block before); the 16 warps of a block share out a row's parts, if
+// there are not as many rows, eight at a time. (Blocks of 256 threads and 40 registers, small enough to wait beside the kernel above, were slower, 18
+// against 14 us for one sequence of 4097: they take what the next call's CTAs need.)
 template <int kD, bool kBf16>
 __global__ void __launch_bounds__(512) attention_tokens_join_kernel(const __grid_constant__ TokensArgs p, int ctas) {
   using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
@@ -495,17 +564,19 @@ __global__ void __launch_bounds__(512) attention_tokens_join_kernel(const __grid
   __shared__ float2 ml_of[WARPS];
   griddep_wait();
   griddep_launch_dependents();
-  const int rows = p.seq.each * p.group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const float2* ml = reinterpret_cast<const float2*>(p.parts + 2ll * ctas * rows * kD);
-  const int4 meta = reinterpret_cast<const int4*>(p.parts + 2ll * ctas * rows * (kD + 2))[blockIdx.x];
+  const int all_rows = p.seq.each * p.group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float2* ml = reinterpret_cast<const float2*>(p.parts + 2ll * ctas * all_rows * kD);
+  const int4 meta = reinterpret_cast<const int4*>(p.parts + 2ll * ctas * all_rows * (kD + 2))[blockIdx.x];
   if (meta.x < 0) return;
-  const int first = static_cast<int>(blockIdx.x), n = meta.z - first + 1;  // CTAs with a part: slot 1 of the first, slot 0 of the others
+  const int first = meta.z, n = meta.w - first + 1;  // CTAs with a part: slot 1 of the first, slot 0 of the others
+  const int helper = static_cast<int>(blockIdx.x) - first - 1, helpers = n - 1;
+  const int rows = (all_rows - helper + helpers - 1) / helpers;  // this block's: every helpers-th from helper on
   int shares = 1;  // warps of a row
   while (shares < WARPS && rows * shares < WARPS && n > shares) shares *= 2;
   const int rows_at_once = WARPS / shares;
   for (int r0 = 0; r0 < rows; r0 += rows_at_once) {
-    const int r = r0 + warp / shares, share = warp % shares;
-    const bool live = r < rows;
+    const int r = helper + (r0 + warp / shares) * helpers, share = warp % shares;
+    const bool live = r < all_rows;
     float top = -INFINITY, sum = 0.f, a[PER];
 #pragma unroll
     for (int e = 0; e < PER; ++e) a[e] = 0.f;
@@ -515,7 +586,7 @@ __global__ void __launch_bounds__(512) attention_tokens_join_kernel(const __grid
 #pragma unroll
       for (int u = 0; u < AT_ONCE; ++u) {
         const int i = i0 + u * shares;
-        const long long part = (2ll * (first + i) + (i == 0 ? 1 : 0)) * rows + r;
+        const long long part = (2ll * (first + i) + (i == 0 ? 1 : 0)) * all_rows + r;
         s[u] = i < n ? ml[part] : make_float2(-INFINITY, 0.f);
         if (i < n) v[u] = reinterpret_cast<const Vec*>(p.parts + part * kD)[lane];
       }
