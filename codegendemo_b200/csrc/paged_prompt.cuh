@@ -8,13 +8,15 @@
 //   warp 0    loads: both Q tiles and K tiles through a two-stage ring, a lane a box of a page; page numbers one tile ahead
 //   warp 1    tcgen05.mma: S = Q K^T, O += P V with P in tensor memory
 //   warp 2    waits for K and V in the issuer's place, and overwrites values that no row sees with zeros (0 x NaN would not vanish)
-//   warp 3    loads V tiles in the same way (one warp for both was the limit with pages of 16 tokens, 32 boxes a step); the next pair of tiles,
-//             while the loads of this one end
+//   warp 3    loads V tiles in the same way; finds the next pair of tiles when the loads of this one end
 //   warps 4-7 softmax of tile 0, warps 8-11 of tile 1, a row a thread
-// Bound by what bounds that kernel, the chain scores - softmax - product of a tile against the other tile's, and the power cap. A window makes
-// a pair of tiles short, nine steps of 1.7 us at a window of 1024: then what comes before the first step and behind the last one counts. So a CTA
-// stays where it is and takes over a CTA that has not been launched yet (cluster launch control) as its next pair: the queries and keys of that one
-// are loaded, and its first scores computed, while this one's rows are finished.
+// Bound by what bounds that kernel, the chain scores - softmax - product of a tile against the other tile's (1.8 us for both tiles' steps), and the
+// power cap: 8192 tokens, 32 heads over 8 of 128 values, bf16, 451 us (1220 TFLOP/s of the pairs seen). A window makes a pair of tiles short,
+// nine steps at a window of 1024: then what comes before the first step and behind the last one counts. So a CTA stays where it is and
+// takes over a CTA that has not been launched yet (cluster launch control) as its next pair: the queries and keys of that one are loaded, and
+// its first scores computed, while this one's rows are finished. 16384 tokens, a window of 1024, 4 sinks: 408 us with a launch a pair, then 340, 314 with
+// first scores ahead and fewer registers in the control warps, 283 with weights against a lagging maximum. In what is left a pair has 16 us of
+// steps and 4.5 of ends: masked steps at both of them, the results' stores, the first step's wait for its scores.
 // kKeySplit: where the tiles do not fill the GPU, the CTAs of a cluster share the keys of one pair, and join their results in shared memory.
 #pragma once
 
@@ -40,8 +42,9 @@ struct AttnPrompt {
   static constexpr int BOX_BYTES = 128 * 128;  // 128 rows x 64 values
   static constexpr int Q_BYTES = BR * kD * 2, KV_BYTES = BC * kD * 2;
   static constexpr int OFF_K = TILES * Q_BYTES, OFF_V = OFF_K + K_STAGES * KV_BYTES, RING_BYTES = OFF_V + V_STAGES * KV_BYTES;
-  // Results leave through shared memory, 32 rows x 128 bytes of a warp at a time, as whole 128-byte lines. (A row a thread, 16 bytes of 32 rows a
-  // store, kept the load-store unit busy for 4000 cycles a pair of tiles.)
+  // Results leave through shared memory, 32 rows x 128 bytes of a warp at a time, as whole 128-byte lines: 3000 cycles a tile, beside the other
+  // tile's products. (A row a thread, 16 bytes of 32 rows a store: 3700; 32 bytes a store cost the steps more, in registers, than it gained here: 8192
+  // tokens 471 us / 482.)
   static constexpr int OUT_BYTES = 8 * 32 * 128;
   static constexpr int SMEM_BYTES = RING_BYTES + OUT_BYTES + 2048;  // 1 KB alignment slack + barriers
   static constexpr int P_PART = kD == 128 ? 96 : 64;    // keys of a step after which P V starts
@@ -92,8 +95,9 @@ struct AttnPrompt {
 
   // The row of units, as warp 3 walks it. A sequence's pairs of tiles are counted from its last token, whose pair sees the most keys; the first may
   // have fewer tokens. Up to kOrdered sequences: pairs with the most keys come first, over all sequences, so that none of the long ones begins
-  // last; a pair's level is the keys of its last token over a pair's tokens. For a place in the row the warp bisects its level, a lane one or two
-  // sequences, whose facts it has read once. Of more sequences that would take longer than a unit, and many short units even out by themselves:
+  // last (6 prompts of up to 1501 tokens, 14 heads over 2 of 64 values: 37 us in the order of the sequences, 31); a pair's level is the keys of its last
+  // token over a pair's tokens. For a place in the row the warp bisects its level, a lane one or two
+  // sequences, whose facts it has read once (read and divided for every step of it, a place took 6 us). Of more sequences that would take longer than a unit, and many short units even out by themselves:
   // the pairs of sequence b take the places from (its first row) / (tokens of a pair) + b on, of which there are enough (some have no
   // tokens), so a search over the first rows alone finds the sequence; the last ones first.
   static constexpr int kOrdered = 64;
@@ -539,7 +543,7 @@ struct AttnPrompt {
       const Unit x = unit;
       const bool live = token < x.tokens;
       // places of keys below `see`, of those from `near` on and the sinks; rows without a token (whose scores are of whatever lies there) are not masked
-      const int position = x.p_lo + token;
+      const int position = x.p_lo + (live ? token : 0);
       const int see = live ? x.list.place(min(position + 1, x.keys)) : 0x7fffffff;
       const int near = live && p.window > 0 && position >= p.window ? position - p.window + 1 - x.list.shift : 0;
       // m: what the exponentials of a step are taken against, in the exp2 domain: the row's running maximum as it was when some row of the warp last

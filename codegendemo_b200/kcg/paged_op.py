@@ -176,7 +176,7 @@ def append_kv(k, v, k_cache, v_cache, page_table, lengths, starts=None, q=None, 
 
 def attention_paged(q, k_cache, v_cache, page_table, lengths, starts=None, scale=None, window=None, sinks=0, out=None):
     """``softmax(scale * q k^T) v`` of a step's rows over their sequences' keys in the cache: ``q`` (rows, heads, d), the heads a multiple
-    of the cache's (up to 64 share a key head), returns (rows, heads, d), in ``out`` if given. A row sees its sequence's keys up to its own position; with ``window`` only the
+    of the cache's (up to 64 share a key head), returns (rows, heads, d), in ``out`` if given (which may be ``q``). A row sees its sequence's keys up to its own position; with ``window`` only the
     last that many (itself among them), and the first ``sinks`` of the sequence. ``scale`` is 1 / sqrt(d) if not given. A row without
     any key gives zeros (a negative position: an empty place of the batch); rows behind the last sequence's are not written. Sums and
     softmax in fp32, the weights rounded to the inputs' type in front of their product with the values. Values of keys that no row of the

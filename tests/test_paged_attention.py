@@ -1,5 +1,8 @@
 """Attention over a paged cache against 64 bits, where its splits, tiles, masks and pages can go wrong."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -16,12 +19,15 @@ TOKENS = [
     ([1], 1, 1, 1, 64, 16, BF), ([1, 0, 2], 1, 4, 2, 128, 16, FP), ([63, 64, 65], 1, 8, 8, 64, 8, BF), ([127, 128, 129, 1], 1, 32, 8, 128, 32, BF),
     ([4097], 1, 32, 8, 128, 16, BF), ([4097], 1, 64, 1, 128, 64, FP), ([2048, 5, 0, 700, 33], 1, 14, 2, 64, 128, FP), ([5000] * 3, 1, 16, 16, 128, 256, BF),
     ([300, 1, 2, 5, 4], 4, 32, 8, 128, 16, BF), ([1000, 77], 5, 24, 8, 64, 32, FP), ([600, 2], 3, 63, 3, 128, 64, BF), ([900], 16, 4, 1, 128, 16, FP),
+    ([9000, 300], 2, 24, 2, 128, 64, BF), ([9000, 10], 8, 8, 1, 64, 16, FP), ([30000], 1, 64, 1, 128, 128, BF), ([250] * 7, 1, 8, 1, 128, 32, BF),
     ([130] * 40, 1, 8, 4, 128, 16, BF), ([20000, 1, 64], 1, 8, 2, 64, 1024, BF), ([513] * 150, 1, 3, 3, 64, 16, FP), ([0, 0], 1, 8, 2, 128, 16, BF),
 ]
 PROMPTS = [
     ([1], [1], 1, 1, 64, 16, BF), ([127], [127], 1, 1, 128, 16, BF), ([128, 1, 129], [128, 1, 129], 8, 8, 64, 8, FP), ([300, 0, 257], [300, 0, 257], 32, 8, 128, 32, BF),
     ([1000], [1000], 14, 2, 64, 64, FP), ([777, 40], [100, 40], 5, 1, 128, 16, BF), ([2500], [3], 32, 8, 128, 128, FP), ([50, 60, 9], [60, 60, 12], 12, 4, 64, 16, BF),
     ([640, 2, 700], [640, 0, 1], 63, 1, 128, 256, BF), ([3000, 1500], [513, 1500], 4, 4, 128, 64, BF), ([400] * 9, [400] * 9, 3, 1, 64, 32, FP),
+    ([5 * i + 1 for i in range(33)], [(7 * i) % (5 * i + 1) for i in range(33)], 8, 8, 64, 16, BF), ([90 - i for i in range(64)], [90 - i for i in range(64)], 4, 1, 128, 16, FP),
+    ([i % 50 for i in range(65)], [i % 50 for i in range(65)], 8, 2, 64, 8, BF), ([(37 * i) % 200 + 1 for i in range(150)], [(i * i) % ((37 * i) % 200 + 1) for i in range(150)], 32, 8, 128, 32, BF),
 ]
 
 
@@ -76,6 +82,47 @@ def test_views_and_places_of_results(case):
     assert_close(got, want, tol)
     behind = want.isnan()
     assert bool((out[behind] == 7.0).all()) and bool((wide[:, 2 * step.q_heads + 1:] == 7.0).all()) and bool((wide[:, step.q_heads] == 7.0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [TOKENS[3], TOKENS[9], TOKENS[13], TOKENS[15], PROMPTS[3], PROMPTS[5], PROMPTS[6], PROMPTS[9]], ids=ids)
+def test_in_the_queries_place(case):
+    step = Step(*case)
+    want, tol = step.oracle()
+    got = matmul_op.attention_paged(*step.args(), out=step.q)
+    matmul_op.attention_paged_status(0)
+    assert got is step.q
+    assert_close(got, want, tol)
+
+
+_FIRST_CALL = """
+import sys
+import torch
+from tests.helpers_paged import Step, assert_close
+from codegendemo_b200.kcg import matmul_op
+step = Step(*eval(sys.argv[1]))
+cos, sin = matmul_op.rotary_table(1000, step.d)
+k = step.k_cache.clone(), step.v_cache.clone()
+rows = sum(step.new)
+new = torch.randn(rows, step.kv_heads, step.d, device="cuda").to(step.dtype)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    matmul_op.append_kv(new, new, *k, step.table, step.lengths, step.starts, q=step.q, rotary=(cos, sin))
+    out = matmul_op.attention_paged(*step.args())
+graph.replay()
+torch.cuda.synchronize()
+assert_close(out, *step.oracle())
+print("the same")
+"""
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", ["[700, 3], 1, 8, 2, 128, 16, torch.bfloat16", "[20000, 3], 1, 8, 2, 128, 16, torch.bfloat16", "[700, 300], [300, 300], 8, 2, 64, 16, torch.float16",
+                                  "[3000], [1], 8, 2, 128, 16, torch.bfloat16"])
+def test_a_first_call_may_be_captured(case):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", _FIRST_CALL, case], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "the same" in r.stdout, r.stderr[-2000:]
 
 
 @pytest.mark.gpu
