@@ -142,7 +142,7 @@ int check_query(const kcg_paged_cache* c, const kcg_paged_query* q) {
   if (q->q_heads < 1 || q->q_heads % c->kv_heads || q->q_heads / c->kv_heads > 64)
     return fail(KCG_E_BAD_ARG, "attention_paged: 1 to 64 query heads share a key head");
   if (q->window < 0 || q->sinks < 0) return fail(KCG_E_BAD_ARG, "attention_paged: negative window or sinks");
-  if (!(q->scale > 0.f) || !(q->scale <= 3e38f)) return fail(KCG_E_BAD_ARG, "scale must be positive and finite");
+  if (!(q->scale > 0.f) || !(q->scale <= 2e38f)) return fail(KCG_E_BAD_ARG, "scale must be positive and finite");  // (times log2 e, too)
   if (static_cast<long long>(q->rows) * q->q_heads > 0x7fffff00LL) return fail(KCG_E_TOO_LARGE, "attention_paged: too many rows");
   return 0;
 }

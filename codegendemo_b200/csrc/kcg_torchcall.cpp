@@ -480,7 +480,7 @@ PyObject* attention_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!PyFloat_CheckExact(args[6])) Py_RETURN_NONE;
     const double scale = PyFloat_AS_DOUBLE(args[6]);
     a.scale = static_cast<float>(scale);
-    if (!(scale > 0.0 && scale < 3e38) || !(a.scale > 0.f)) Py_RETURN_NONE;
+    if (!(scale > 0.0 && scale <= 2e38) || !(a.scale > 0.f)) Py_RETURN_NONE;
   }
   auto size_of = [](PyObject* o, long least, int32_t* out) {
     if (!PyLong_CheckExact(o)) return false;

@@ -44,7 +44,7 @@ def _launched(status):
 
 def rotary_table(positions, dim, base=10000.0, device="cuda"):
     """(cos, sin) of the angles ``p * base ** (-2 i / dim)`` of positions p = 0 .. positions - 1, each (positions, dim / 2) in fp32; the
-    angles are taken in 64 bits (in 32 they lose 2^-8 of a turn at a position of 100 000)."""
+    angles are taken in 64 bits (in 32 they are off by 2^-8 of a radian at a position of 100 000)."""
     import torch
     if dim < 2 or dim % 2 or positions < 1:
         raise ValueError("a table of at least one position, of an even number of values")
@@ -198,7 +198,7 @@ def attention_paged(q, k_cache, v_cache, page_table, lengths, starts=None, scale
     a.Q, a.O = q.data_ptr(), out.data_ptr()
     if scale is None:
         scale = 1.0 / math.sqrt(c.d)
-    if not 0.0 < scale < 3e38:
+    if not 0.0 < scale <= 2e38:
         raise ValueError("scale must be positive and finite")
     if window is not None and window < 1:
         raise ValueError("a window sees at least the row's own key")

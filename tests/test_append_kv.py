@@ -1,5 +1,7 @@
 """Storing a step's rows in a paged cache, and the rotation on the way, against 64 bits."""
 import ctypes
+import os
+import re
 
 import pytest
 import torch
@@ -213,6 +215,16 @@ def test_generating_token_by_token_is_the_prompt_at_once():
     # each off by the weights' rounding (2^-8 of the largest |v| at most) and its own, twice
     for a, b in zip(got, want):
         assert float((a.float() - b.float()).abs().max()) <= 4 * 2.0 ** -8 * float(v.abs().max())
+
+
+SOURCES = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "codegendemo_b200", "csrc")
+
+
+@pytest.mark.parametrize("file", ["kcg_paged.cu", "paged.cuh", "paged_tokens.cuh", "paged_prompt.cuh", "attn_common.cuh"])
+def test_no_load_asks_for_memory_that_is_read_only_for_the_kernels_life(file):
+    """The kernel before in the stream may still write what these read (programmatic dependent launch)."""
+    text = re.sub(r"//[^\n]*", "", open(os.path.join(SOURCES, file)).read())
+    assert re.findall(r"__ldg\s*\(|ld\.global\.nc|__restrict__", text) == []
 
 
 def test_table_of_angles():

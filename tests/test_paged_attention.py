@@ -25,7 +25,7 @@ TOKENS = [
 PROMPTS = [
     ([1], [1], 1, 1, 64, 16, BF), ([127], [127], 1, 1, 128, 16, BF), ([128, 1, 129], [128, 1, 129], 8, 8, 64, 8, FP), ([300, 0, 257], [300, 0, 257], 32, 8, 128, 32, BF),
     ([1000], [1000], 14, 2, 64, 64, FP), ([777, 40], [100, 40], 5, 1, 128, 16, BF), ([2500], [3], 32, 8, 128, 128, FP), ([50, 60, 9], [60, 60, 12], 12, 4, 64, 16, BF),
-    ([640, 2, 700], [640, 0, 1], 63, 1, 128, 256, BF), ([3000, 1500], [513, 1500], 4, 4, 128, 64, BF), ([400] * 9, [400] * 9, 3, 1, 64, 32, FP),
+    ([700, 300], 100, 8, 2, 128, 16, BF), ([64, 500, 2], 65, 1, 1, 64, 32, FP), ([640, 2, 700], [640, 0, 1], 63, 1, 128, 256, BF), ([3000, 1500], [513, 1500], 4, 4, 128, 64, BF), ([400] * 9, [400] * 9, 3, 1, 64, 32, FP),
     ([5 * i + 1 for i in range(33)], [(7 * i) % (5 * i + 1) for i in range(33)], 8, 8, 64, 16, BF), ([90 - i for i in range(64)], [90 - i for i in range(64)], 4, 1, 128, 16, FP),
     ([i % 50 for i in range(65)], [i % 50 for i in range(65)], 8, 2, 64, 8, BF), ([(37 * i) % 200 + 1 for i in range(150)], [(i * i) % ((37 * i) % 200 + 1) for i in range(150)], 32, 8, 128, 32, BF),
 ]
@@ -55,7 +55,7 @@ def test_prompts(case):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("case", [TOKENS[4], TOKENS[6], TOKENS[8], TOKENS[13], PROMPTS[4], PROMPTS[5], PROMPTS[6], PROMPTS[9], PROMPTS[7]], ids=ids)
+@pytest.mark.parametrize("case", [TOKENS[4], TOKENS[6], TOKENS[8], TOKENS[13], PROMPTS[4], PROMPTS[5], PROMPTS[6], PROMPTS[8], PROMPTS[11], PROMPTS[7]], ids=ids)
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (16, 4), (100, 0), (128, 64), (129, 130), (1000, 3), (100000, 5)])
 def test_window_and_sinks(case, window, sinks):
     """What no row sees is NaN, and pages of nothing else are not in the table."""
@@ -298,7 +298,7 @@ def _call(q=None, k=None, v=None, table=None, lengths=None, starts=None, **how):
     (dict(q=_fake(2, 8, 128, dtype=FP)), "q must be"), (dict(q=_fake(2, 8, 256)[..., ::2]), "contiguous"), (dict(q=_fake(2, 8, 132)[..., :128]), "multiples of 8"),
     (dict(q=_fake(2, 1, 128).expand(2, 8, 128)), "strides"), (dict(q=_fake(16, 128)), "rows x heads"), (dict(table=_fake(2, 3, dtype=torch.int64)), "page_table"),
     (dict(table=_fake(3, dtype=torch.int32)), "page_table"), (dict(lengths=_fake(3, dtype=torch.int32)), "lengths"), (dict(starts=_fake(2, dtype=torch.int32)), "starts"),
-    (dict(window=0), "window"), (dict(sinks=-1), "sinks"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(out=_fake(2, 8, 64)), "out"),
+    (dict(window=0), "window"), (dict(sinks=-1), "sinks"), (dict(scale=0.0), "scale"), (dict(scale=3e38), "scale"), (dict(scale=float("nan")), "scale"), (dict(out=_fake(2, 8, 64)), "out"),
     (dict(k=_fake(4, 2, 16, 129)[..., 1:], v=_fake(4, 2, 16, 128)), "k_cache"),
 ])
 def test_wrong_arguments_are_refused(how, message):
