@@ -317,9 +317,7 @@ int attention_prompt(int device, cudaStream_t st, const kcg_paged_cache* c, cons
   p.tile_tokens = 128 / p.group;
   p.scale_log2 = q->scale * 1.4426950408889634f;
   const int pair = 2 * p.tile_tokens;
-  // Pairs of tiles, at most: a sequence has one that is not full.
-  const long long pairs = c->starts ? (static_cast<long long>(q->rows) + pair - 1) / pair + c->sequences - 1
-                                    : static_cast<long long>((p.seq.each + pair - 1) / pair) * c->sequences;
+  const long long pairs = AttnPrompt<128, true, false>::places(p.seq, pair);
   if (pairs > 0x7fffffffLL) return fail(KCG_E_TOO_LARGE, "attention_paged: too many rows");
   p.pairs = static_cast<int>(pairs);
   // Keys of a box: of a page, or of 32 where a window's keys begin anywhere and are laid out from a box's border on.

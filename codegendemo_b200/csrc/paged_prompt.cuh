@@ -101,6 +101,11 @@ struct AttnPrompt {
   // the pairs of sequence b take the places from (its first row) / (tokens of a pair) + b on, of which there are enough (some have no
   // tokens), so a search over the first rows alone finds the sequence; the last ones first.
   static constexpr int kOrdered = 64;
+  // Places in the row, at most.
+  static long long places(const Sequences& s, int pair) {
+    if (!s.starts && s.count <= kOrdered) return static_cast<long long>((s.each + pair - 1) / pair) * s.count;
+    return (static_cast<long long>(s.rows) + pair - 1) / pair + s.count - 1;  // (a sequence has one pair that is not full)
+  }
   struct Row {
     int first[2], rows[2], length[2];  // of sequences lane and lane + 32: first row, rows, tokens
     int pairs[2], level[2];            // pairs of tiles, level of the last one

@@ -27,6 +27,7 @@ PROMPTS = [
     ([1000], [1000], 14, 2, 64, 64, FP), ([777, 40], [100, 40], 5, 1, 128, 16, BF), ([2500], [3], 32, 8, 128, 128, FP), ([50, 60, 9], [60, 60, 12], 12, 4, 64, 16, BF),
     ([700, 300], 100, 8, 2, 128, 16, BF), ([64, 500, 2], 65, 1, 1, 64, 32, FP), ([640, 2, 700], [640, 0, 1], 63, 1, 128, 256, BF), ([3000, 1500], [513, 1500], 4, 4, 128, 64, BF), ([400] * 9, [400] * 9, 3, 1, 64, 32, FP),
     ([5 * i + 1 for i in range(33)], [(7 * i) % (5 * i + 1) for i in range(33)], 8, 8, 64, 16, BF), ([90 - i for i in range(64)], [90 - i for i in range(64)], 4, 1, 128, 16, FP),
+    ([40] * 70, 20, 8, 2, 64, 16, BF), ([65 + i for i in range(100)], 65, 1, 1, 128, 16, FP), ([90] * 64, 33, 8, 4, 64, 16, BF),
     ([i % 50 for i in range(65)], [i % 50 for i in range(65)], 8, 2, 64, 8, BF), ([(37 * i) % 200 + 1 for i in range(150)], [(i * i) % ((37 * i) % 200 + 1) for i in range(150)], 32, 8, 128, 32, BF),
 ]
 
