@@ -269,6 +269,36 @@ def test_queries_and_scores_that_are_no_numbers(case):
 
 
 @pytest.mark.gpu
+def test_a_refused_call_leaves_nothing_for_the_next():
+    """Calls for a device that is not there, then right ones."""
+    lib, gone = _lib.get_lib(), 63
+    for case in (([300, 20], 1, 8, 2, 128, 16, BF), ([300, 200], [300, 20], 8, 2, 128, 16, BF)):
+        step = Step(*case)
+        c = _lib.PagedCache(step.k_cache.data_ptr(), step.v_cache.data_ptr(), (ctypes.c_int64 * 3)(*step.k_cache.stride()[:3]),
+                            (ctypes.c_int64 * 3)(*step.v_cache.stride()[:3]), step.table.data_ptr(), step.lengths.data_ptr(),
+                            0 if step.starts is None else step.starts.data_ptr(), step.table.stride(0), step.k_cache.shape[0], 16, step.table.shape[1], 2, 2, 128, 62)
+        out, room = torch.empty_like(step.q), torch.empty(1 << 23, dtype=torch.uint8, device="cuda")
+        a = _lib.PagedQuery(step.q.data_ptr(), out.data_ptr(), (ctypes.c_int64 * 2)(1024, 128), (ctypes.c_int64 * 2)(1024, 128), room.data_ptr(), room.numel(),
+                            step.q.shape[0], 8, 0, 0, 128 ** -0.5)
+        k = torch.zeros(step.q.shape[0], 2, 128, dtype=BF, device="cuda")
+        r = _lib.NewRows(k.data_ptr(), k.data_ptr(), 0, 0, (ctypes.c_int64 * 2)(256, 128), (ctypes.c_int64 * 2)(256, 128))
+        r.rows = step.q.shape[0]
+        stream = torch.cuda.current_stream().cuda_stream
+        assert lib.kcg_attention_paged(gone, stream, ctypes.byref(c), ctypes.byref(a)) != 0
+        assert lib.kcg_attention_paged(0, stream, ctypes.byref(c), ctypes.byref(a)) == 0, lib.kcg_last_error()
+        assert lib.kcg_append_kv(gone, stream, ctypes.byref(c), ctypes.byref(r)) != 0
+        assert lib.kcg_attention_paged_status(gone, (ctypes.c_uint32 * 4)()) != 0
+        assert_close(out, *step.oracle())
+        a.workspace_bytes = 16
+        if step.starts is None:
+            assert lib.kcg_attention_paged(0, stream, ctypes.byref(c), ctypes.byref(a)) == _lib.E_BAD_ARG
+            assert lib.kcg_attention_paged_workspace(0, ctypes.byref(c), ctypes.byref(a)) > 16
+        else:
+            assert lib.kcg_attention_paged_workspace(0, ctypes.byref(c), ctypes.byref(a)) == 0
+        assert bool(torch.isfinite(matmul_op.attention_paged(*step.args())[:1]).all())
+
+
+@pytest.mark.gpu
 def test_no_rows():
     step = Step([10, 20], 1, 8, 2, 128, 16, BF)
     got = matmul_op.attention_paged(step.q[:0], *step.args()[1:5])
