@@ -540,283 +540,283 @@ struct AttnPrompt {
       uint32_t scores = 0, results = 0;  // of this tile so far
       bool alive = true;                 // no wait of this warp has run out
       while (unit_there()) {
-      const Unit& unit = bars->unit[taken & 1];
-      if (unit.end) {
-        unit_read();
-        break;
-      }
-      const Unit x = unit;
-      const bool live = token < x.tokens;
-      // places of keys below `see`, of those from `near` on and the sinks; rows without a token (whose scores are of whatever lies there) are not masked
-      const int position = x.p_lo + (live ? token : 0);
-      const int see = live ? x.list.place(min(position + 1, x.keys)) : 0x7fffffff;
-      const int near = live && p.window > 0 && position >= p.window ? position - p.window + 1 - x.list.shift : 0;
-      // m: what the exponentials of a step are taken against, in the exp2 domain: the row's running maximum as it was when some row of the warp last
-      // passed its own by 8. Weights are up to 2^8 then, which 16 bits hold as exactly as any (P's relative rounding is the same everywhere), and
-      // the sums in 32 bits; what is lost is that the largest weight is no longer exactly 1. Error against 64 bits, 2048 tokens, bf16: normal scores 2.02e-3
-      // -> 2.05e-3, scores of 4 times that 1.72e-3 -> 1.95e-3, of 16 times 1.44e-3 -> 1.45e-3. A window's nine steps would nearly all rescale O:
-      // 16384 tokens with a window of 1024 303 -> 283 us, 8192 without one 472 -> 451.
-      float m = -INFINITY;
-      uint64_t sum2[2] = {f32x2(0.f, 0.f), f32x2(0.f, 0.f)};
-      const int mine = t < x.tiles ? x.steps : 0;
-      int j = 0;
-      for (; j < mine && alive; ++j) {
-        alive = __all_sync(0xffffffffu, mbar_wait_for(&bars->s_full[t], scores & 1u, 4 * KCG_WAIT_LIMIT_NS));
-        if (!alive) {
-          if (lane == 0) report(bars, PAGED_TIMEOUT_ATTENTION, 3u, static_cast<uint32_t>(j));
+        const Unit& unit = bars->unit[taken & 1];
+        if (unit.end) {
+          unit_read();
           break;
         }
-        ++scores;
-        tc_fence_after_sync();
-        uint32_t sr[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(col_s + c * 32, sr[c]);
-        const int v0 = x.v0 + j * BC;
-        const int end = see - v0, gap0 = p.sinks - v0, gap1 = near - v0;
-        const bool masked = __any_sync(0xffffffffu, end < BC || (gap1 > 0 && gap0 < BC));
-        tmem_ld_wait();
-#pragma unroll
-        for (int c = 0; c < 4; ++c) pin_32(sr[c]);
-        if (masked) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            // a bit a key that the row sees (a test of a bit and a select each, where 32 comparisons with three borders are five)
-            const uint32_t bits = below(end - c * 32) & (below(gap0 - c * 32) | ~below(gap1 - c * 32));
-            if (__any_sync(0xffffffffu, bits != 0xffffffffu)) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (!(bits >> i & 1u)) sr[c][i] = __float_as_uint(-INFINITY);
-            }
+        const Unit x = unit;
+        const bool live = token < x.tokens;
+        // places of keys below `see`, of those from `near` on and the sinks; rows without a token (whose scores are of whatever lies there) are not masked
+        const int position = x.p_lo + (live ? token : 0);
+        const int see = live ? x.list.place(min(position + 1, x.keys)) : 0x7fffffff;
+        const int near = live && p.window > 0 && position >= p.window ? position - p.window + 1 - x.list.shift : 0;
+        // m: what the exponentials of a step are taken against, in the exp2 domain: the row's running maximum as it was when some row of the warp last
+        // passed its own by 8. Weights are up to 2^8 then, which 16 bits hold as exactly as any (P's relative rounding is the same everywhere), and
+        // the sums in 32 bits; what is lost is that the largest weight is no longer exactly 1. Error against 64 bits, 2048 tokens, bf16: normal scores 2.02e-3
+        // -> 2.05e-3, scores of 4 times that 1.72e-3 -> 1.95e-3, of 16 times 1.44e-3 -> 1.45e-3. A window's nine steps would nearly all rescale O:
+        // 16384 tokens with a window of 1024 303 -> 283 us, 8192 without one 472 -> 451.
+        float m = -INFINITY;
+        uint64_t sum2[2] = {f32x2(0.f, 0.f), f32x2(0.f, 0.f)};
+        const int mine = t < x.tiles ? x.steps : 0;
+        int j = 0;
+        for (; j < mine && alive; ++j) {
+          alive = __all_sync(0xffffffffu, mbar_wait_for(&bars->s_full[t], scores & 1u, 4 * KCG_WAIT_LIMIT_NS));
+          if (!alive) {
+            if (lane == 0) report(bars, PAGED_TIMEOUT_ATTENTION, 3u, static_cast<uint32_t>(j));
+            break;
           }
-        }
-        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        auto max_of = [&](int c) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 2)
-            mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(sr[c][i]), __uint_as_float(sr[c][i + 1]));
-        };
-#pragma unroll
-        for (int c = 0; c < 4; ++c) max_of(c);
-        // (the scale is positive: checked by the host)
-        const float highest = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;
-        const bool moved = __any_sync(0xffffffffu, live && highest > m + 8.f);
-        const float mx = moved ? fmaxf(m, highest) : m;
-        // (without a finite score so far the probabilities are 0, not -inf - -inf)
-        const float base = mx == -INFINITY ? 0.f : mx;
-        const float alpha = ex2(m - base);
-        m = mx;
-        const uint64_t alpha2 = f32x2(alpha, alpha), zero2 = f32x2(0.f, 0.f), base2 = f32x2(-base, -base);
-        sum2[0] = fma_f32x2(sum2[0], alpha2, zero2);
-        sum2[1] = fma_f32x2(sum2[1], alpha2, zero2);
-        // Exponentials and P of 32 keys: packed pairs over the S columns this thread has read.
-        auto exponentials = [&](int c) {
-          uint32_t w[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float2 e = f32x2_split(fma_f32x2(f32x2(__uint_as_float(sr[c][2 * i]), __uint_as_float(sr[c][2 * i + 1])), scale2, base2));
-            e.x = ex2(e.x);
-            e.y = ex2(e.y);
-            sum2[i & 1] = add_f32x2(sum2[i & 1], f32x2(e.x, e.y));
-            w[i] = pack_pair<kBf16>(e.x, e.y);
-          }
-          tmem_st_32x32b_x16(col_s + c * 16, w);
-        };
-        // O_t <- alpha * O_t, where the warp's rows have another m (the previous P_t V has retired: the scores just read were issued
-        // behind it).
-        if (j > 0 && moved) {
-          auto scale_store = [&](uint32_t (&o)[32], int c) {
-            pin_32(o);
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const float2 v = f32x2_split(mul_f32x2(f32x2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), alpha2));
-              o[i] = __float_as_uint(v.x);
-              o[i + 1] = __float_as_uint(v.y);
-            }
-            tmem_st_32x32b_x32(col_o + c * 32, o);
-          };
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t o[32];
-            tmem_ld_32x32b_x32(col_o + c * 32, o);
-            exponentials(c);
-            tmem_ld_wait();
-            scale_store(o, c);
-          }
-          if constexpr (kD == 128) {
-            static_assert(P_PART == 96, "the third piece of 32 keys comes before the publication");
-            uint32_t o[2][32];
-            tmem_ld_32x32b_x32(col_o + 64, o[0]);
-            tmem_ld_32x32b_x32(col_o + 96, o[1]);
-            exponentials(2);
-            tmem_ld_wait();
-            scale_store(o[0], 2);
-            scale_store(o[1], 3);
-          }
-        } else {
-          exponentials(0);
-          exponentials(1);
-          if constexpr (P_PART == 96) exponentials(2);
-        }
-        auto publish = [&](uint32_t bar) {
-          tmem_st_wait();
-          tc_fence_before_sync();
-          named_bar_arrive(bar, PT_THREADS);
-        };
-        publish(BAR_PART + t);
-        if constexpr (P_PART == 64) exponentials(2);
-        exponentials(3);
-        publish(BAR_FULL + t);
-      }
-      for (; j < mine; ++j) {  // (given up)
-        __syncwarp();
-        named_bar_sync(BAR_PART + t, PT_THREADS);
-        named_bar_sync(BAR_FULL + t, PT_THREADS);
-      }
-      const float2 s01 = f32x2_split(add_f32x2(sum2[0], sum2[1]));
-      const float l = s01.x + s01.y;
-      if (mine > 0 && alive) {
-        alive = __all_sync(0xffffffffu, mbar_wait(&bars->o_full[t], results & 1u, &bars->abort_flag));
-        if (!alive && lane == 0) report(bars, PAGED_TIMEOUT_ATTENTION, 4u, 0u);
-        ++results;
-      }
-      const bool gave_up = mine > 0 && !alive;
-      if constexpr (kKeySplit) {
-        // Partial results: once the products of both tiles have retired, the operand ring holds this CTA's O rows (fp32, not normalised,
-        // 16-byte units XOR-swizzled by the row: a warp writes 32 rows at a time) and their {maximum, sum}; then each CTA joins an equal
-        // share of the output over the cluster's shared memories.
-        constexpr int UNITS = kD / 4;  // 16-byte units of a row
-        constexpr int OFF_ML = TILES * BR * kD * 4;
-        static_assert(OFF_ML + TILES * BR * 8 <= RING_BYTES, "the partial result must fit the ring");
-        bool both = true;
-        if (mine > 0 && !gave_up && x.tiles == 2) {
-          both = __all_sync(0xffffffffu, mbar_wait(&bars->o_full[t ^ 1], 0u, &bars->abort_flag));
-          if (!both && lane == 0) report(bars, PAGED_TIMEOUT_ATTENTION, 5u, 0u);
-        }
-        if (t < x.tiles && both && !gave_up) {
+          ++scores;
           tc_fence_after_sync();
-          const int r = t * BR + row;
-          uint8_t* to = smem + r * kD * 4;
+          uint32_t sr[4][32];
 #pragma unroll
-          for (int c = 0; c < kD / 32; ++c) {
-            uint32_t o[32];
-            if (mine > 0) {
-              tmem_ld_32x32b_x32(col_o + c * 32, o);
-              tmem_ld_wait();
-              pin_32(o);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = 0u;
-            }
-#pragma unroll
-            for (int u = 0; u < 8; ++u)
-              *reinterpret_cast<uint4*>(to + (((c * 8 + u) ^ (r & (UNITS - 1))) << 4)) = make_uint4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
-          }
-          reinterpret_cast<float2*>(smem + OFF_ML)[r] = make_float2(m, l);
-        }
-        __syncwarp();
-        cluster_sync_all();
-        {
-          // This CTA's rows, as many to a warp: a lane first takes the weights of one of them, then the warp whole rows (d = 64: two), four loads of other CTAs'
-          // rows in flight for each of them. (An element at a time, with its row's weights each time, was 13 us of latency for two CTAs.)
-          const int all = x.tiles * BR, r0 = all * rank / p.splits, r1 = all * (rank + 1) / p.splits;
-          const int per = (r1 - r0 + 7) / 8, first = r0 + (warp - 4) * per, mine_rows = max(0, min(per, r1 - first));  // (at most 16)
-          const uint32_t base_addr = smem_u32(smem);
-          float f[8], inv = 0.f;
-          {
-            const uint32_t ml_addr = base_addr + OFF_ML + (first + min(lane, max(mine_rows - 1, 0))) * 8;
-            float2 ml[8];
-            float top = -INFINITY, sum = 0.f;
-#pragma unroll
-            for (int c = 0; c < 8; ++c) ml[c] = c < p.splits && mine_rows > 0 ? ld_cluster_f2(map_to_cta(ml_addr, c)) : make_float2(-INFINITY, 0.f);
-#pragma unroll
-            for (int c = 0; c < 8; ++c) top = fmaxf(top, ml[c].x);
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              f[c] = ml[c].y == 0.f ? 0.f : ex2(ml[c].x - top);  // (a part of no key; a sum of NaN has to reach the result)
-              sum = fmaf(f[c], ml[c].y, sum);
-            }
-            inv = sum == 0.f ? 0.f : 1.f / sum;
-          }
-          constexpr int ROWS = 128 / kD, AT_ONCE = 4;  // rows a warp takes with one load, loads in flight
-          const int u = lane % UNITS;
-          for (int k0 = 0; k0 < mine_rows; k0 += ROWS * AT_ONCE) {
-            float4 sums[AT_ONCE];
-#pragma unroll
-            for (int i = 0; i < AT_ONCE; ++i) sums[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              if (c >= p.splits) break;
-              float4 v[AT_ONCE];
-#pragma unroll
-              for (int i = 0; i < AT_ONCE; ++i) {
-                const int r = first + min(k0 + i * ROWS + lane / UNITS, mine_rows - 1);
-                v[i] = ld_cluster_f4(map_to_cta(base_addr + r * kD * 4 + ((u ^ (r & (UNITS - 1))) << 4), c));
-              }
-#pragma unroll
-              for (int i = 0; i < AT_ONCE; ++i) {
-                const float w = __shfl_sync(0xffffffffu, f[c], min(k0 + i * ROWS + lane / UNITS, mine_rows - 1));
-                if (w == 0.f) continue;  // (what a part of no key holds)
-                sums[i].x = fmaf(w, v[i].x, sums[i].x), sums[i].y = fmaf(w, v[i].y, sums[i].y);
-                sums[i].z = fmaf(w, v[i].z, sums[i].z), sums[i].w = fmaf(w, v[i].w, sums[i].w);
-              }
-            }
-#pragma unroll
-            for (int i = 0; i < AT_ONCE; ++i) {
-              const int k = k0 + i * ROWS + lane / UNITS, r = first + k, in_tile = r % BR;
-              const float scale = __shfl_sync(0xffffffffu, inv, min(k, mine_rows - 1));
-              const int tok = r / BR * p.tile_tokens + in_tile / p.group;
-              if (k >= mine_rows || in_tile >= p.tile_tokens * p.group || tok >= x.tokens) continue;
-              T* out = reinterpret_cast<T*>(p.o) + static_cast<long long>(unit.row0 + tok) * p.o_row +
-                       static_cast<long long>(unit.head * p.group + in_tile % p.group) * p.o_head + u * 4;
-              *reinterpret_cast<uint2*>(out) = make_uint2(pack_pair<kBf16>(sums[i].x * scale, sums[i].y * scale), pack_pair<kBf16>(sums[i].z * scale, sums[i].w * scale));
-            }
-          }
-        }
-        __syncwarp();
-        cluster_sync_all();  // the other CTAs read this one's shared memory until here
-      } else {
-        tc_fence_after_sync();
-        const float inv = mine == 0 || l == 0.f ? 0.f : 1.f / l;
-        // (this thread's row, from the result's first byte on; -1: none)
-        const long long at = live ? static_cast<long long>(unit.row0 + token) * p.o_row + static_cast<long long>(unit.head * p.group + head_row) * p.o_head : -1;
-        uint8_t* stage = smem + RING_BYTES + (warp - 4) * (32 * 128);
-        uint32_t o[kD / 32][32];
-        if (mine > 0 && !gave_up) {
-#pragma unroll
-          for (int c = 0; c < kD / 32; ++c) tmem_ld_32x32b_x32(col_o + c * 32, o[c]);
+          for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(col_s + c * 32, sr[c]);
+          const int v0 = x.v0 + j * BC;
+          const int end = see - v0, gap0 = p.sinks - v0, gap1 = near - v0;
+          const bool masked = __any_sync(0xffffffffu, end < BC || (gap1 > 0 && gap0 < BC));
           tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < kD / 32; ++c) pin_32(o[c]);
-        } else {
+          for (int c = 0; c < 4; ++c) pin_32(sr[c]);
+          if (masked) {
 #pragma unroll
-          for (int i = 0; i < kD; ++i) o[i / 32][i % 32] = 0u;
+            for (int c = 0; c < 4; ++c) {
+              // a bit a key that the row sees (a test of a bit and a select each, where 32 comparisons with three borders are five)
+              const uint32_t bits = below(end - c * 32) & (below(gap0 - c * 32) | ~below(gap1 - c * 32));
+              if (__any_sync(0xffffffffu, bits != 0xffffffffu)) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (!(bits >> i & 1u)) sr[c][i] = __float_as_uint(-INFINITY);
+              }
+            }
+          }
+          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          auto max_of = [&](int c) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 2)
+              mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(sr[c][i]), __uint_as_float(sr[c][i + 1]));
+          };
+#pragma unroll
+          for (int c = 0; c < 4; ++c) max_of(c);
+          // (the scale is positive: checked by the host)
+          const float highest = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;
+          const bool moved = __any_sync(0xffffffffu, live && highest > m + 8.f);
+          const float mx = moved ? fmaxf(m, highest) : m;
+          // (without a finite score so far the probabilities are 0, not -inf - -inf)
+          const float base = mx == -INFINITY ? 0.f : mx;
+          const float alpha = ex2(m - base);
+          m = mx;
+          const uint64_t alpha2 = f32x2(alpha, alpha), zero2 = f32x2(0.f, 0.f), base2 = f32x2(-base, -base);
+          sum2[0] = fma_f32x2(sum2[0], alpha2, zero2);
+          sum2[1] = fma_f32x2(sum2[1], alpha2, zero2);
+          // Exponentials and P of 32 keys: packed pairs over the S columns this thread has read.
+          auto exponentials = [&](int c) {
+            uint32_t w[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float2 e = f32x2_split(fma_f32x2(f32x2(__uint_as_float(sr[c][2 * i]), __uint_as_float(sr[c][2 * i + 1])), scale2, base2));
+              e.x = ex2(e.x);
+              e.y = ex2(e.y);
+              sum2[i & 1] = add_f32x2(sum2[i & 1], f32x2(e.x, e.y));
+              w[i] = pack_pair<kBf16>(e.x, e.y);
+            }
+            tmem_st_32x32b_x16(col_s + c * 16, w);
+          };
+          // O_t <- alpha * O_t, where the warp's rows have another m (the previous P_t V has retired: the scores just read were issued
+          // behind it).
+          if (j > 0 && moved) {
+            auto scale_store = [&](uint32_t (&o)[32], int c) {
+              pin_32(o);
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                const float2 v = f32x2_split(mul_f32x2(f32x2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), alpha2));
+                o[i] = __float_as_uint(v.x);
+                o[i + 1] = __float_as_uint(v.y);
+              }
+              tmem_st_32x32b_x32(col_o + c * 32, o);
+            };
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              uint32_t o[32];
+              tmem_ld_32x32b_x32(col_o + c * 32, o);
+              exponentials(c);
+              tmem_ld_wait();
+              scale_store(o, c);
+            }
+            if constexpr (kD == 128) {
+              static_assert(P_PART == 96, "the third piece of 32 keys comes before the publication");
+              uint32_t o[2][32];
+              tmem_ld_32x32b_x32(col_o + 64, o[0]);
+              tmem_ld_32x32b_x32(col_o + 96, o[1]);
+              exponentials(2);
+              tmem_ld_wait();
+              scale_store(o[0], 2);
+              scale_store(o[1], 3);
+            }
+          } else {
+            exponentials(0);
+            exponentials(1);
+            if constexpr (P_PART == 96) exponentials(2);
+          }
+          auto publish = [&](uint32_t bar) {
+            tmem_st_wait();
+            tc_fence_before_sync();
+            named_bar_arrive(bar, PT_THREADS);
+          };
+          publish(BAR_PART + t);
+          if constexpr (P_PART == 64) exponentials(2);
+          exponentials(3);
+          publish(BAR_FULL + t);
         }
+        for (; j < mine; ++j) {  // (given up)
+          __syncwarp();
+          named_bar_sync(BAR_PART + t, PT_THREADS);
+          named_bar_sync(BAR_FULL + t, PT_THREADS);
+        }
+        const float2 s01 = f32x2_split(add_f32x2(sum2[0], sum2[1]));
+        const float l = s01.x + s01.y;
+        if (mine > 0 && alive) {
+          alive = __all_sync(0xffffffffu, mbar_wait(&bars->o_full[t], results & 1u, &bars->abort_flag));
+          if (!alive && lane == 0) report(bars, PAGED_TIMEOUT_ATTENTION, 4u, 0u);
+          ++results;
+        }
+        const bool gave_up = mine > 0 && !alive;
+        if constexpr (kKeySplit) {
+          // Partial results: once the products of both tiles have retired, the operand ring holds this CTA's O rows (fp32, not normalised,
+          // 16-byte units XOR-swizzled by the row: a warp writes 32 rows at a time) and their {maximum, sum}; then each CTA joins an equal
+          // share of the output over the cluster's shared memories.
+          constexpr int UNITS = kD / 4;  // 16-byte units of a row
+          constexpr int OFF_ML = TILES * BR * kD * 4;
+          static_assert(OFF_ML + TILES * BR * 8 <= RING_BYTES, "the partial result must fit the ring");
+          bool both = true;
+          if (mine > 0 && !gave_up && x.tiles == 2) {
+            both = __all_sync(0xffffffffu, mbar_wait(&bars->o_full[t ^ 1], 0u, &bars->abort_flag));
+            if (!both && lane == 0) report(bars, PAGED_TIMEOUT_ATTENTION, 5u, 0u);
+          }
+          if (t < x.tiles && both && !gave_up) {
+            tc_fence_after_sync();
+            const int r = t * BR + row;
+            uint8_t* to = smem + r * kD * 4;
 #pragma unroll
-        for (int c2 = 0; c2 < HALVES; ++c2) {
-          __syncwarp();  // (the warp has read what the last round left here)
+            for (int c = 0; c < kD / 32; ++c) {
+              uint32_t o[32];
+              if (mine > 0) {
+                tmem_ld_32x32b_x32(col_o + c * 32, o);
+                tmem_ld_wait();
+                pin_32(o);
+              } else {
 #pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            uint32_t w[4];
+                for (int i = 0; i < 32; ++i) o[i] = 0u;
+              }
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              w[e] = pack_pair<kBf16>(__uint_as_float(o[c2 * 2 + u / 4][u % 4 * 8 + 2 * e]) * inv, __uint_as_float(o[c2 * 2 + u / 4][u % 4 * 8 + 2 * e + 1]) * inv);
-            *reinterpret_cast<uint4*>(stage + lane * 128 + ((u ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+              for (int u = 0; u < 8; ++u)
+                *reinterpret_cast<uint4*>(to + (((c * 8 + u) ^ (r & (UNITS - 1))) << 4)) = make_uint4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
+            }
+            reinterpret_cast<float2*>(smem + OFF_ML)[r] = make_float2(m, l);
           }
           __syncwarp();
-          uint4 v[8];
+          cluster_sync_all();
+          {
+            // This CTA's rows, as many to a warp: a lane first takes the weights of one of them, then the warp whole rows (d = 64: two), four loads of other CTAs'
+            // rows in flight for each of them. (An element at a time, with its row's weights each time, was 13 us of latency for two CTAs.)
+            const int all = x.tiles * BR, r0 = all * rank / p.splits, r1 = all * (rank + 1) / p.splits;
+            const int per = (r1 - r0 + 7) / 8, first = r0 + (warp - 4) * per, mine_rows = max(0, min(per, r1 - first));  // (at most 16)
+            const uint32_t base_addr = smem_u32(smem);
+            float f[8], inv = 0.f;
+            {
+              const uint32_t ml_addr = base_addr + OFF_ML + (first + min(lane, max(mine_rows - 1, 0))) * 8;
+              float2 ml[8];
+              float top = -INFINITY, sum = 0.f;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int r = k * 4 + lane / 8, u = lane & 7;
-            v[k] = *reinterpret_cast<const uint4*>(stage + r * 128 + ((u ^ (r & 7)) << 4));
+              for (int c = 0; c < 8; ++c) ml[c] = c < p.splits && mine_rows > 0 ? ld_cluster_f2(map_to_cta(ml_addr, c)) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+              for (int c = 0; c < 8; ++c) top = fmaxf(top, ml[c].x);
+#pragma unroll
+              for (int c = 0; c < 8; ++c) {
+                f[c] = ml[c].y == 0.f ? 0.f : ex2(ml[c].x - top);  // (a part of no key; a sum of NaN has to reach the result)
+                sum = fmaf(f[c], ml[c].y, sum);
+              }
+              inv = sum == 0.f ? 0.f : 1.f / sum;
+            }
+            constexpr int ROWS = 128 / kD, AT_ONCE = 4;  // rows a warp takes with one load, loads in flight
+            const int u = lane % UNITS;
+            for (int k0 = 0; k0 < mine_rows; k0 += ROWS * AT_ONCE) {
+              float4 sums[AT_ONCE];
+#pragma unroll
+              for (int i = 0; i < AT_ONCE; ++i) sums[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+              for (int c = 0; c < 8; ++c) {
+                if (c >= p.splits) break;
+                float4 v[AT_ONCE];
+#pragma unroll
+                for (int i = 0; i < AT_ONCE; ++i) {
+                  const int r = first + min(k0 + i * ROWS + lane / UNITS, mine_rows - 1);
+                  v[i] = ld_cluster_f4(map_to_cta(base_addr + r * kD * 4 + ((u ^ (r & (UNITS - 1))) << 4), c));
+                }
+#pragma unroll
+                for (int i = 0; i < AT_ONCE; ++i) {
+                  const float w = __shfl_sync(0xffffffffu, f[c], min(k0 + i * ROWS + lane / UNITS, mine_rows - 1));
+                  if (w == 0.f) continue;  // (what a part of no key holds)
+                  sums[i].x = fmaf(w, v[i].x, sums[i].x), sums[i].y = fmaf(w, v[i].y, sums[i].y);
+                  sums[i].z = fmaf(w, v[i].z, sums[i].z), sums[i].w = fmaf(w, v[i].w, sums[i].w);
+                }
+              }
+#pragma unroll
+              for (int i = 0; i < AT_ONCE; ++i) {
+                const int k = k0 + i * ROWS + lane / UNITS, r = first + k, in_tile = r % BR;
+                const float scale = __shfl_sync(0xffffffffu, inv, min(k, mine_rows - 1));
+                const int tok = r / BR * p.tile_tokens + in_tile / p.group;
+                if (k >= mine_rows || in_tile >= p.tile_tokens * p.group || tok >= x.tokens) continue;
+                T* out = reinterpret_cast<T*>(p.o) + static_cast<long long>(unit.row0 + tok) * p.o_row +
+                         static_cast<long long>(unit.head * p.group + in_tile % p.group) * p.o_head + u * 4;
+                *reinterpret_cast<uint2*>(out) = make_uint2(pack_pair<kBf16>(sums[i].x * scale, sums[i].y * scale), pack_pair<kBf16>(sums[i].z * scale, sums[i].w * scale));
+              }
+            }
+          }
+          __syncwarp();
+          cluster_sync_all();  // the other CTAs read this one's shared memory until here
+        } else {
+          tc_fence_after_sync();
+          const float inv = mine == 0 || l == 0.f ? 0.f : 1.f / l;
+          // (this thread's row, from the result's first byte on; -1: none)
+          const long long at = live ? static_cast<long long>(unit.row0 + token) * p.o_row + static_cast<long long>(unit.head * p.group + head_row) * p.o_head : -1;
+          uint8_t* stage = smem + RING_BYTES + (warp - 4) * (32 * 128);
+          uint32_t o[kD / 32][32];
+          if (mine > 0 && !gave_up) {
+#pragma unroll
+            for (int c = 0; c < kD / 32; ++c) tmem_ld_32x32b_x32(col_o + c * 32, o[c]);
+            tmem_ld_wait();
+#pragma unroll
+            for (int c = 0; c < kD / 32; ++c) pin_32(o[c]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < kD; ++i) o[i / 32][i % 32] = 0u;
           }
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const long long to = __shfl_sync(0xffffffffu, at, k * 4 + lane / 8);
-            if (to >= 0) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.o) + to + c2 * 64 + (lane & 7) * 8) = v[k];
+          for (int c2 = 0; c2 < HALVES; ++c2) {
+            __syncwarp();  // (the warp has read what the last round left here)
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                w[e] = pack_pair<kBf16>(__uint_as_float(o[c2 * 2 + u / 4][u % 4 * 8 + 2 * e]) * inv, __uint_as_float(o[c2 * 2 + u / 4][u % 4 * 8 + 2 * e + 1]) * inv);
+              *reinterpret_cast<uint4*>(stage + lane * 128 + ((u ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            __syncwarp();
+            uint4 v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const int r = k * 4 + lane / 8, u = lane & 7;
+              v[k] = *reinterpret_cast<const uint4*>(stage + r * 128 + ((u ^ (r & 7)) << 4));
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const long long to = __shfl_sync(0xffffffffu, at, k * 4 + lane / 8);
+              if (to >= 0) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.o) + to + c2 * 64 + (lane & 7) * 8) = v[k];
+            }
           }
         }
-      }
-      unit_read();
+        unit_read();
       }  // (units; a cluster has one, and its meetings are in it)
     }
 

@@ -156,48 +156,48 @@ struct AttnTokens {
       __syncthreads();
       g0 = sh->begin, g1 = sh->before[0];
     } else {
-    // All sequences' places, and where this CTA's range begins: a thread counts those of its run of sequences.
-    const int per = (p.seq.count + NUM_THREADS - 1) / NUM_THREADS;
-    const int b0 = min(static_cast<int>(threadIdx.x) * per, p.seq.count), b1 = min(b0 + per, p.seq.count);
-    long long mine = 0;
-    for (int b = b0; b < b1; ++b) mine += Keys(p, p.seq.lengths[b]).count + kTokensPause;
-    mine *= p.kv_heads;
-    long long upto = mine;
+      // All sequences' places, and where this CTA's range begins: a thread counts those of its run of sequences.
+      const int per = (p.seq.count + NUM_THREADS - 1) / NUM_THREADS;
+      const int b0 = min(static_cast<int>(threadIdx.x) * per, p.seq.count), b1 = min(b0 + per, p.seq.count);
+      long long mine = 0;
+      for (int b = b0; b < b1; ++b) mine += Keys(p, p.seq.lengths[b]).count + kTokensPause;
+      mine *= p.kv_heads;
+      long long upto = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += v;
-    }
-    if (lane == 31) sh->before[warp] = upto;
-    __syncthreads();
-    long long base = 0;
-#pragma unroll
-    for (int w = 0; w < 5; ++w) {
-      if (w < warp) base += sh->before[w];
-      total += sh->before[w];
-    }
-    const Ranges ranges(total, gridDim.x);
-    if (cta < ranges.ctas) g0 = ranges.begin(cta), g1 = ranges.begin(cta + 1);
-    base += upto - mine;
-    if (g0 < g1 && g0 >= base && g0 < base + mine) {
-      long long at = g0 - base;
-      for (int b = b0; b < b1; ++b) {
-        const int n = Keys(p, p.seq.lengths[b]).count, places = n + kTokensPause;
-        if (at < static_cast<long long>(places) * p.kv_heads) {
-          int h = static_cast<int>(at / places), t = static_cast<int>(at % places), to = b;
-          long long begin = g0;
-          if (t >= n) {  // behind the last tile: the next (sequence, head)'s first one
-            begin += places - t;
-            t = 0;
-            if (++h == p.kv_heads) h = 0, ++to;
-          }
-          if (begin < g1) sh->found[0] = to, sh->found[1] = h, sh->found[2] = t, sh->begin = begin;
-          break;
-        }
-        at -= static_cast<long long>(places) * p.kv_heads;
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
       }
-    }
-    __syncthreads();
+      if (lane == 31) sh->before[warp] = upto;
+      __syncthreads();
+      long long base = 0;
+#pragma unroll
+      for (int w = 0; w < 5; ++w) {
+        if (w < warp) base += sh->before[w];
+        total += sh->before[w];
+      }
+      const Ranges ranges(total, gridDim.x);
+      if (cta < ranges.ctas) g0 = ranges.begin(cta), g1 = ranges.begin(cta + 1);
+      base += upto - mine;
+      if (g0 < g1 && g0 >= base && g0 < base + mine) {
+        long long at = g0 - base;
+        for (int b = b0; b < b1; ++b) {
+          const int n = Keys(p, p.seq.lengths[b]).count, places = n + kTokensPause;
+          if (at < static_cast<long long>(places) * p.kv_heads) {
+            int h = static_cast<int>(at / places), t = static_cast<int>(at % places), to = b;
+            long long begin = g0;
+            if (t >= n) {  // behind the last tile: the next (sequence, head)'s first one
+              begin += places - t;
+              t = 0;
+              if (++h == p.kv_heads) h = 0, ++to;
+            }
+            if (begin < g1) sh->found[0] = to, sh->found[1] = h, sh->found[2] = t, sh->begin = begin;
+            break;
+          }
+          at -= static_cast<long long>(places) * p.kv_heads;
+        }
+      }
+      __syncthreads();
     }
     const bool any = sh->found[0] >= 0;
 
