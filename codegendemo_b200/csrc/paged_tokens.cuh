@@ -524,8 +524,8 @@ struct AttnTokens {
               if (c0 + c < p.splits) x[c] = ld_cluster_f4(map_to_cta(o_addr + i * 16, c0 + c));
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
-              const float f = weight(ml[c0 + c], top);
-              if (f == 0.f) continue;  // (no part, or one of no key: whatever lies there)
+              if (ml[c0 + c].y == 0.f) continue;  // (no part, or one of no key: whatever lies there)
+              const float f = weight(ml[c0 + c], top);  // (0 too: 0 x NaN is one)
               a.x = fmaf(f, x[c].x, a.x), a.y = fmaf(f, x[c].y, a.y), a.z = fmaf(f, x[c].z, a.z), a.w = fmaf(f, x[c].w, a.w);
               sum = fmaf(f, ml[c0 + c].y, sum);
             }
