@@ -57,7 +57,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 4) append_kv_kernel(const A
   const int b = sequence_of(a.seq, row);
   if (b < 0) return;
   const int n = a.seq.start(b + 1) - a.seq.start(b);
-  const int position = a.seq.lengths[b] - n + (row - a.seq.start(b));
+  const int position = max(a.seq.lengths[b], 0) - n + (row - a.seq.start(b));  // (of any length below 0 a negative one)
   const int page = position >= 0 && position < a.seq.capacity() ? a.seq.page_of(b, position) : -1;
   float c[8], s[8];
   if (turned) {
