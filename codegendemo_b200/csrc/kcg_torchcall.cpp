@@ -441,7 +441,7 @@ bool like_cache(const at::Tensor& t, const at::Tensor& cache) {
 }
 
 // The cache of args: k_cache, v_cache, page_table, lengths, starts. False: not this path's.
-bool paged_cache(PyObject* const* args, int64_t rows, kcg_paged_cache* c, const at::Tensor** k) {
+bool paged_cache(PyObject* const* args, int64_t rows, kcg_paged_cache* c, const at::Tensor** k, const at::Tensor** v = nullptr) {
   const at::Tensor *kc = heads(args[0], 4, c->k_stride), *vc = heads(args[1], 4, c->v_stride);
   if (!kc || !vc || vc->sizes() != kc->sizes() || !like_cache(*vc, *kc)) return false;
   const at::Tensor *table = ints(args[2], *kc, 2), *lengths = ints(args[3], *kc, 1), *starts = nullptr;
@@ -462,6 +462,7 @@ bool paged_cache(PyObject* const* args, int64_t rows, kcg_paged_cache* c, const 
   c->pages = static_cast<int32_t>(kc->size(0)), c->page = static_cast<int32_t>(page), c->width = static_cast<int32_t>(width);
   c->sequences = static_cast<int32_t>(sequences), c->kv_heads = static_cast<int32_t>(kc->size(1)), c->d = static_cast<int32_t>(kc->size(3));
   *k = kc;
+  if (v) *v = vc;
   return true;
 }
 
@@ -516,9 +517,9 @@ PyObject* append_kv(PyObject*, PyObject* const* args, Py_ssize_t n) {
   kcg_new_rows r{};
   if (n != 11 || !g_paged.append || !PyTuple_CheckExact(args[8]) || PyTuple_GET_SIZE(args[8]) != 2 || (args[9] != Py_False && args[9] != Py_True))
     Py_RETURN_NONE;
-  const at::Tensor *k = heads(args[0], 3, r.k_stride), *v = heads(args[1], 3, r.v_stride), *q = heads(args[7], 3, r.q_stride), *cache;
+  const at::Tensor *k = heads(args[0], 3, r.k_stride), *v = heads(args[1], 3, r.v_stride), *q = heads(args[7], 3, r.q_stride), *cache, *v_cache;
   const at::Tensor *cos = plain(PyTuple_GET_ITEM(args[8], 0), 2), *sin = plain(PyTuple_GET_ITEM(args[8], 1), 2);
-  if (!k || !v || !q || !cos || !sin || !paged_cache(args + 2, k->size(0), &c, &cache) || !like_cache(*k, *cache) || !like_cache(*v, *cache) ||
+  if (!k || !v || !q || !cos || !sin || !paged_cache(args + 2, k->size(0), &c, &cache, &v_cache) || !like_cache(*k, *cache) || !like_cache(*v, *cache) ||
       !like_cache(*q, *cache) || k->size(1) != c.kv_heads || v->size(1) != c.kv_heads || v->size(0) != k->size(0) || q->size(0) != k->size(0) || watched())
     Py_RETURN_NONE;
   const int64_t half = cos->size(1);
@@ -532,6 +533,7 @@ PyObject* append_kv(PyObject*, PyObject* const* args, Py_ssize_t n) {
     r.positions = address(*positions);
   }
   at::Tensor o = empty_like_on(*q, q->sizes(), q->scalar_type());
+  c.K = out_address(*cache), c.V = out_address(*v_cache);  // (written: memory that others share until then becomes the cache's own)
   r.K = address(*k), r.V = address(*v), r.Q = address(*q), r.QO = out_address(o);
   r.qo_stride[0] = q->size(1) * q->size(2), r.qo_stride[1] = q->size(2);
   r.cos = address(*cos), r.sin = address(*sin), r.angles = cos->size(0);
