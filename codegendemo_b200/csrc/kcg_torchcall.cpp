@@ -104,6 +104,9 @@ PyObject* finish(int status, at::Tensor&& result) {
   return nullptr;
 }
 
+// The same where the caller has the result already.
+PyObject* finish_given(int status, PyObject* result) { return status == 0 ? Py_NewRef(result) : finish(status, at::Tensor()); }
+
 // Launches the product if its kernel is known; None if it is not.
 PyObject* product(const Shape& shape, const at::Tensor& a, const at::Tensor& b, at::IntArrayRef sizes, PyObject* bias,
                   PyObject* relu_arg) {
@@ -440,6 +443,12 @@ bool like_cache(const at::Tensor& t, const at::Tensor& cache) {
   return t.scalar_type() == cache.scalar_type() && t.device() == cache.device() && t.size(t.dim() - 1) == cache.size(3);
 }
 
+// Rows x heads that the caller gave for the result of rows like `like`, and their strides.
+const at::Tensor* result_like(PyObject* o, const at::Tensor& like, int64_t* strides) {
+  const at::Tensor* t = heads(o, 3, strides);
+  return t && t->sizes() == like.sizes() && t->scalar_type() == like.scalar_type() && t->device() == like.device() ? t : nullptr;
+}
+
 // The cache of args: k_cache, v_cache, page_table, lengths, starts. False: not this path's.
 bool paged_cache(PyObject* const* args, int64_t rows, kcg_paged_cache* c, const at::Tensor** k, const at::Tensor** v = nullptr) {
   const at::Tensor *kc = heads(args[0], 4, c->k_stride), *vc = heads(args[1], 4, c->v_stride);
@@ -466,12 +475,13 @@ bool paged_cache(PyObject* const* args, int64_t rows, kcg_paged_cache* c, const 
   return true;
 }
 
-// attention_paged(q, k_cache, v_cache, page_table, lengths, starts, scale, window, sinks) -> tensor or None
+// attention_paged(q, k_cache, v_cache, page_table, lengths, starts, scale, window, sinks[, out]) -> tensor or None
 PyObject* attention_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   kcg_paged_cache c{};
   kcg_paged_query a{};
-  if (n != 9 || !g_paged.attention) Py_RETURN_NONE;
+  if ((n != 9 && n != 10) || !g_paged.attention) Py_RETURN_NONE;
+  PyObject* const given = n == 10 ? args[9] : Py_None;
   const at::Tensor *q = heads(args[0], 3, a.q_stride), *k;
   if (!q || !paged_cache(args + 1, q->size(0), &c, &k) || !like_cache(*q, *k) || watched()) Py_RETURN_NONE;
   a.rows = static_cast<int32_t>(q->size(0)), a.q_heads = static_cast<int32_t>(q->size(1));
@@ -492,9 +502,16 @@ PyObject* attention_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
   };
   if ((args[7] != Py_None && !size_of(args[7], 1, &a.window)) || !size_of(args[8], 0, &a.sinks)) Py_RETURN_NONE;
   const int device = q->device().index();
-  at::Tensor o = empty_like_on(*q, q->sizes(), q->scalar_type()), workspace;
-  a.Q = address(*q), a.O = out_address(o);
-  a.o_stride[0] = q->size(1) * q->size(2), a.o_stride[1] = q->size(2);
+  at::Tensor o, workspace;
+  const at::Tensor* out = &o;
+  if (given != Py_None) {
+    out = result_like(given, *q, a.o_stride);
+    if (!out) Py_RETURN_NONE;
+  } else {
+    o = empty_like_on(*q, q->sizes(), q->scalar_type());
+    a.o_stride[0] = q->size(1) * q->size(2), a.o_stride[1] = q->size(2);
+  }
+  a.O = out_address(*out), a.Q = address(*q);
   const int64_t bytes = g_paged.workspace(device, &c, &a);
   if (bytes < 0) Py_RETURN_NONE;
   if (bytes > 0) {
@@ -506,46 +523,61 @@ PyObject* attention_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Py_BEGIN_ALLOW_THREADS
   status = g_paged.attention(device, stream, &c, &a);
   Py_END_ALLOW_THREADS
-  return finish(status, std::move(o));
+  return given != Py_None ? finish_given(status, given) : finish(status, std::move(o));
   END_HANDLE_TH_ERRORS
 }
 
-// append_kv(k, v, k_cache, v_cache, page_table, lengths, starts, q, (cos, sin), interleaved, positions) -> the turned queries, or None
+// append_kv(k, v, k_cache, v_cache, page_table, lengths, starts, q, (cos, sin), interleaved, positions[, q_out]) -> the turned queries, True where
+// there are none (q is None), or None. Without rotation the pair is None.
 PyObject* append_kv(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   kcg_paged_cache c{};
   kcg_new_rows r{};
-  if (n != 11 || !g_paged.append || !PyTuple_CheckExact(args[8]) || PyTuple_GET_SIZE(args[8]) != 2 || (args[9] != Py_False && args[9] != Py_True))
+  if ((n != 11 && n != 12) || !g_paged.append || (args[9] != Py_False && args[9] != Py_True)) Py_RETURN_NONE;
+  PyObject* const given = n == 12 ? args[11] : Py_None;
+  const bool queries = args[7] != Py_None, rotated = args[8] != Py_None;
+  if ((!queries && given != Py_None) || (rotated ? !PyTuple_CheckExact(args[8]) || PyTuple_GET_SIZE(args[8]) != 2 : args[10] != Py_None)) Py_RETURN_NONE;
+  const at::Tensor *k = heads(args[0], 3, r.k_stride), *v = heads(args[1], 3, r.v_stride), *q = queries ? heads(args[7], 3, r.q_stride) : nullptr;
+  const at::Tensor *cache, *v_cache;
+  if (!k || !v || (queries && !q) || !paged_cache(args + 2, k->size(0), &c, &cache, &v_cache) || !like_cache(*k, *cache) || !like_cache(*v, *cache) ||
+      k->size(1) != c.kv_heads || v->size(1) != c.kv_heads || v->size(0) != k->size(0) || watched())
     Py_RETURN_NONE;
-  const at::Tensor *k = heads(args[0], 3, r.k_stride), *v = heads(args[1], 3, r.v_stride), *q = heads(args[7], 3, r.q_stride), *cache, *v_cache;
-  const at::Tensor *cos = plain(PyTuple_GET_ITEM(args[8], 0), 2), *sin = plain(PyTuple_GET_ITEM(args[8], 1), 2);
-  if (!k || !v || !q || !cos || !sin || !paged_cache(args + 2, k->size(0), &c, &cache, &v_cache) || !like_cache(*k, *cache) || !like_cache(*v, *cache) ||
-      !like_cache(*q, *cache) || k->size(1) != c.kv_heads || v->size(1) != c.kv_heads || v->size(0) != k->size(0) || q->size(0) != k->size(0) || watched())
-    Py_RETURN_NONE;
-  const int64_t half = cos->size(1);
-  if (cos->scalar_type() != at::kFloat || sin->scalar_type() != at::kFloat || cos->device() != k->device() || sin->device() != k->device() ||
-      cos->sizes() != sin->sizes() || cos->size(0) < 1 || half < 8 || half % 8 || half > c.d / 2 || address(*cos) % 16 || address(*sin) % 16 ||
-      q->size(1) > 65535)
-    Py_RETURN_NONE;
+  if (queries && (!like_cache(*q, *cache) || q->size(0) != k->size(0) || q->size(1) > 65535)) Py_RETURN_NONE;
+  if (rotated) {
+    const at::Tensor *cos = plain(PyTuple_GET_ITEM(args[8], 0), 2), *sin = plain(PyTuple_GET_ITEM(args[8], 1), 2);
+    if (!cos || !sin || cos->scalar_type() != at::kFloat || sin->scalar_type() != at::kFloat || cos->device() != k->device() || sin->device() != k->device() ||
+        cos->sizes() != sin->sizes())
+      Py_RETURN_NONE;
+    const int64_t half = cos->size(1);
+    if (cos->size(0) < 1 || half < 8 || half % 8 || half > c.d / 2 || address(*cos) % 16 || address(*sin) % 16) Py_RETURN_NONE;
+    r.cos = address(*cos), r.sin = address(*sin), r.angles = cos->size(0), r.rotary = static_cast<int32_t>(2 * half);
+    r.interleaved = args[9] == Py_True ? 1 : 0;
+  }
   if (args[10] != Py_None) {
     const at::Tensor* positions = ints(args[10], *k, 1);
     if (!positions || positions->size(0) != k->size(0)) Py_RETURN_NONE;
     r.positions = address(*positions);
   }
-  at::Tensor o = empty_like_on(*q, q->sizes(), q->scalar_type());
-  c.K = out_address(*cache), c.V = out_address(*v_cache);  // (written: memory that others share until then becomes the cache's own)
-  r.K = address(*k), r.V = address(*v), r.Q = address(*q), r.QO = out_address(o);
-  r.qo_stride[0] = q->size(1) * q->size(2), r.qo_stride[1] = q->size(2);
-  r.cos = address(*cos), r.sin = address(*sin), r.angles = cos->size(0);
-  r.rows = static_cast<int32_t>(k->size(0)), r.q_heads = static_cast<int32_t>(q->size(1)), r.rotary = static_cast<int32_t>(2 * half);
-  r.interleaved = args[9] == Py_True ? 1 : 0;
+  at::Tensor o;
+  const at::Tensor* out = &o;
+  if (given != Py_None) {
+    out = result_like(given, *q, r.qo_stride);
+    if (!out) Py_RETURN_NONE;
+  } else if (queries) {
+    o = empty_like_on(*q, q->sizes(), q->scalar_type());
+    r.qo_stride[0] = q->size(1) * q->size(2), r.qo_stride[1] = q->size(2);
+  }
+  // (what is written first: memory that others share until then becomes the tensor's own)
+  c.K = out_address(*cache), c.V = out_address(*v_cache);
+  if (queries) r.QO = out_address(*out), r.Q = address(*q), r.q_heads = static_cast<int32_t>(q->size(1));
+  r.K = address(*k), r.V = address(*v), r.rows = static_cast<int32_t>(k->size(0));
   const int device = k->device().index();
   const uint64_t stream = stream_of(*k);
   int status;
   Py_BEGIN_ALLOW_THREADS
   status = g_paged.append(device, stream, &c, &r);
   Py_END_ALLOW_THREADS
-  return finish(status, std::move(o));
+  return !queries ? finish_given(status, Py_True) : given != Py_None ? finish_given(status, given) : finish(status, std::move(o));
   END_HANDLE_TH_ERRORS
 }
 

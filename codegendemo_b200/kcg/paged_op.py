@@ -132,10 +132,10 @@ def append_kv(k, v, k_cache, v_cache, page_table, lengths, starts=None, q=None, 
     (x cos - y sin, y cos + x sin), rounded once. ``positions`` (rows, int32): angles of other positions than the cache's. k, v and q may be parts of
     one projection's result. Where two rows have one place in the cache, it holds values of either. A position without angles gives NaN.
     Rows of the queries whose position is negative become zeros, those behind the last sequence's are not written."""
-    if _warm and q is not None and rotary is not None and q_out is None:
-        turned = _warm.append_kv(k, v, k_cache, v_cache, page_table, lengths, starts, q, rotary, interleaved, positions)
+    if _warm:
+        turned = _warm.append_kv(k, v, k_cache, v_cache, page_table, lengths, starts, q, rotary, interleaved, positions, q_out)
         if turned is not None:
-            return turned
+            return turned if q is not None else None
     import torch
     cache_rows = k.shape[0] if k.dim() == 3 else 0
     c = _cache(k_cache, v_cache, page_table, lengths, starts, cache_rows)
@@ -181,10 +181,10 @@ def attention_paged(q, k_cache, v_cache, page_table, lengths, starts=None, scale
     any key gives zeros (a negative position: an empty place of the batch); rows behind the last sequence's are not written. Sums and
     softmax in fp32, the weights rounded to the inputs' type in front of their product with the values. Values of keys that no row of the
     sequence sees may be anything; those of keys that some row sees have to be finite."""
-    if _warm and out is None:
-        out = _warm.attention_paged(q, k_cache, v_cache, page_table, lengths, starts, scale, window, sinks)
-        if out is not None:
-            return out
+    if _warm:
+        found = _warm.attention_paged(q, k_cache, v_cache, page_table, lengths, starts, scale, window, sinks, out)
+        if found is not None:
+            return found
     if q.dim() != 3:
         raise ValueError("q must be rows x heads x d")
     c = _cache(k_cache, v_cache, page_table, lengths, starts, q.shape[0])
