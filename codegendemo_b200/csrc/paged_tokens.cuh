@@ -400,12 +400,26 @@ struct AttnTokens {
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[n][e] *= alpha[e >> 1];
         }
+        // Rows of large scores (see kLargeScores), whose products are rounded first. (The question costs 0.13 us of one sequence's 12.8; the same without
+        // a branch, two products a score, 0.16.)
+        float times[2] = {p.scale_log2, p.scale_log2};
+        if (__builtin_expect(__any_sync(0xffffffffu, fmaxf(fabsf(base_[0]), fabsf(base_[1])) >= kLargeScores), 0)) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const bool large = fabsf(base_[h]) >= kLargeScores;
+#pragma unroll
+            for (int n = 0; n < WKEYS / 8; ++n)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) c[n][2 * h + e] = __fmul_rn(c[n][2 * h + e], large ? p.scale_log2 : 1.f);
+            times[h] = large ? 1.f : p.scale_log2;
+          }
+        }
         float sum[2] = {0.f, 0.f};
 #pragma unroll
         for (int n = 0; n < WKEYS / 8; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            c[n][e] = ex2(fmaf(c[n][e], p.scale_log2, -base_[e >> 1]));
+            c[n][e] = ex2(fmaf(c[n][e], times[e >> 1], -base_[e >> 1]));
             sum[e >> 1] += c[n][e];
           }
         l[0] = l[0] * alpha[0] + sum[0];

@@ -180,7 +180,8 @@ def attention_paged(q, k_cache, v_cache, page_table, lengths, starts=None, scale
     last that many (itself among them), and the first ``sinks`` of the sequence. ``scale`` is 1 / sqrt(d) if not given. A row without
     any key gives zeros (a negative position: an empty place of the batch); rows behind the last sequence's are not written. Sums and
     softmax in fp32, the weights rounded to the inputs' type in front of their product with the values. Values of keys that no row of the
-    sequence sees may be anything; those of keys that some row sees have to be finite."""
+    sequence sees may be anything; those of keys that some row sees have to be finite. A row that sees a key whose score is NaN, or +inf (by the
+    scale, too: products are held in fp32), is NaN."""
     if _warm:
         found = _warm.attention_paged(q, k_cache, v_cache, page_table, lengths, starts, scale, window, sinks, out)
         if found is not None:

@@ -321,7 +321,8 @@ int kcg_append_kv(int device, uint64_t stream, const kcg_paged_cache* cache, con
 /* O = sum over keys of softmax(scale * q k^T) v, row by row: the query heads q_heads / kv_heads at a time share a key head; a row
  * at position p sees the keys of its sequence up to p, of those (window > 0) the last `window` and the first `sinks`. A row that sees none is zeros;
  * rows behind the last sequence's are left as they were. Values of keys that no row of the sequence sees may be anything, NaN
- * too; those of keys that some row sees have to be finite. Q and O: rows x q_heads x d, strides as above; O may be Q. scale positive, at most 2e38. `workspace`: device memory, 16-byte
+ * too; those of keys that some row sees have to be finite. Scores are held in fp32, times the scale too; a row that sees one of
+ * NaN or +inf is NaN. Q and O: rows x q_heads x d, strides as above; O may be Q. scale positive, at most 2e38. `workspace`: device memory, 16-byte
  * aligned, as many bytes as the function below says for the same cache and rows (0: none needed), free again when the call's work is done. */
 typedef struct kcg_paged_query {
   uint64_t Q, O;
