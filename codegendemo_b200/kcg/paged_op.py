@@ -98,6 +98,8 @@ def _cache(k_cache, v_cache, table, lengths, starts, rows):
     if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
         raise ValueError("page_table must be sequences x pages")
     sequences, width = table.shape
+    if sequences > 2 ** 24:
+        raise ValueError(f"at most 2^24 sequences, not {sequences}")
     _ints(table, "page_table", k_cache.device, sequences, width)
     ld = table.stride(0) if sequences > 1 else width
     if ld < width:
