@@ -10,6 +10,23 @@ import math
 import sys
 
 
+def append_errors(q, k, v, turned, k_cache, v_cache, table_row, first, rotary):
+    """What ``append_kv`` made of one sequence's rows at positions first, first + 1, ..: the relative errors of its turned queries and of the keys in its
+    pages (halves of a head in pairs) against 64 bits, and whether its values lie there as they were."""
+    import torch
+    cos, sin = (t[first:first + q.shape[0], None].double() for t in rotary)
+    half = cos.shape[-1]
+
+    def relative(x, got):
+        x = x.double()
+        want = torch.cat([x[..., :half] * cos - x[..., half:2 * half] * sin, x[..., half:2 * half] * cos + x[..., :half] * sin, x[..., 2 * half:]], -1)
+        return ((got.double() - want).norm() / want.norm()).item()
+    p = torch.arange(first, first + q.shape[0], device=q.device)
+    page = k_cache.shape[2]
+    at, slot = table_row.long()[p // page], p % page
+    return relative(q, turned), relative(k, k_cache[at, :, slot]), torch.equal(v_cache[at, :, slot], v)
+
+
 def main(argv=None) -> int:
     import torch
     from codegendemo_b200.kcg.matmul_op import append_kv, attention_paged, attention_paged_status, rotary_table
@@ -73,6 +90,13 @@ def main(argv=None) -> int:
     attention_paged_status(a.device)
     if not a.no_check:
         b, n, group = a.batch // 2, min(a.tokens, 128), a.heads // a.kv_heads
+        own = slice(b * a.tokens, (b + 1) * a.tokens)
+        off_q, off_k, same = append_errors(q[own], k[own], v[own], turned[own], k_cache, v_cache, table[b], first, rotary)
+        # each value rounded to 16 bits once, of products and a sum in fp32
+        most = torch.finfo(tdt).eps / 2 + 2.0 ** -20
+        right = max(off_q, off_k) <= most and same
+        print(f"relative error, sequence {b}, turned queries {off_q:.3e} and keys in their pages {off_k:.3e}  tolerance {most:.1e}, values "
+              f"{'as they were' if same else 'elsewhere'}  {'OK' if right else 'FAIL'}")
         kf, vf = (c[table[b].long()].transpose(0, 1).reshape(a.kv_heads, -1, a.d)[:, :a.length].double() for c in (k_cache, v_cache))
         x = turned[(b + 1) * a.tokens - n:(b + 1) * a.tokens].double().view(n, a.kv_heads, group, a.d).permute(1, 2, 0, 3)
         p, j = torch.arange(a.length - n, a.length, device=dev)[:, None], torch.arange(a.length, device=dev)[None]
@@ -82,7 +106,7 @@ def main(argv=None) -> int:
         err = ((out[(b + 1) * a.tokens - n:(b + 1) * a.tokens].double() - ref).norm() / ref.norm()).item()
         # weights and result rounded to 16 bits, at most 2^-8 each of values that average to less than the largest
         print(f"relative error, sequence {b}, last {n} tokens, against 64 bits {err:.3e}  tolerance 0.01  {'OK' if err <= 0.01 else 'FAIL'}")
-        return 0 if err <= 0.01 else 1
+        return 0 if right and err <= 0.01 else 1
     return 0
 
 
