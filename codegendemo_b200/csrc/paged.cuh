@@ -64,10 +64,11 @@ struct KeyList {
 };
 
 // Weights are 2^(score * scale - maximum), in one operation whose product is not rounded, where the maximum is that product rounded: half a unit of
-// its last place stands in the exponent of all of a row's weights, and their sum divides it out again. Below this magnitude that is a factor of 2^0.5 at
-// most; from 2^27 on it would be 2^8 and more, which with the prompts' lagging maximum passes fp16's range, and from 2^31 on fp32's. So from here on a
-// row's products are rounded first: its largest weight is 1, and what is infinite gives NaN.
-constexpr float kLargeScores = 16777216.f;
+// its last place stands in the exponent of all of a row's weights, and their sum divides it out again. From 2^27 on that would be a factor of 2^8 and more,
+// which with the prompts' lagging maximum passes fp16's range, and from 2^31 on fp32's. So from this magnitude on products are rounded first, as the
+// maximum is: the largest weight is 1, and what is infinite gives NaN. The two ways differ by 2^-13 of the exponent at most below it (a row's tiles
+// may go either way: with 2^24, a factor of 2^0.5, equal scores had unequal weights).
+constexpr float kLargeScores = 4096.f;
 
 // The sequence whose rows hold `row`, or -1; asked by a whole (converged) warp, 32 places at a time. (The last sequence that starts at
 // or before the row, if it has not ended there: empty ones start where the next one does.)

@@ -67,3 +67,34 @@ def test_a_row_with_a_score_of_infinity_is_nan(case):
     got[:, 0] = 0
     want[:, 0] = 0
     assert_close(got, want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", CASES[4:] + [([283, 163, 157], 70, 16, 4, 128, 64, BF)], ids=lambda c: f"{len(c[0])}x{max(c[0])}")
+@pytest.mark.parametrize("power", [5, 6, 7, 12, 17, 18, 19, 20])
+def test_equal_scores_weigh_the_same_wherever_they_lie(case, power):
+    """Every other row has one score many times all over its sequence, its neighbours only late a large one: equal scores share the weight evenly, in the
+    tiles before the neighbours' and after. (The two ways to a weight differ by 2^-13 of its exponent; the other terms as above.)"""
+    step = Step(*case, seed=power)
+    row, group, half_d = 0, step.q_heads // step.kv_heads, step.d // 2
+    r = torch.arange(step.q.shape[0] * step.q_heads, device="cuda").view(step.q.shape[0], step.q_heads, 1)
+    at = torch.arange(step.d, device="cuda")
+    step.q = torch.where(r % 2 == 0, at < 3 + r * 7 % (half_d // 2), at >= half_d).to(step.dtype)
+    for b, n in enumerate(step.lens):
+        j = torch.arange(n, device="cuda")[:, None]
+        step.k[b][:] = torch.where(at < half_d, j % 3 != 1, j >= n - n // 3).to(step.dtype)
+        step.put(b)
+    got = matmul_op.attention_paged(*step.args(), scale=2.0 ** power)
+    matmul_op.attention_paged_status(0)
+    half = torch.finfo(step.dtype).eps / 2
+    for b, (n, new) in enumerate(zip(step.lens, step.new)):
+        q = step.q[row:row + new].double().view(new, step.kv_heads, group, step.d).permute(1, 2, 0, 3)
+        s = (q @ step.k[b].double()[:, None].transpose(-1, -2)) * 2.0 ** power
+        sees = torch.arange(n, device="cuda")[None] <= torch.arange(n - new, n, device="cuda")[:, None]
+        s = torch.where(sees, s, float("-inf"))
+        w = torch.softmax(s, -1)
+        v = step.v[b].double()[:, None]
+        want, size = (x.permute(2, 0, 1, 3).reshape(new, step.q_heads, step.d) for x in (w @ v, w @ v.abs()))
+        tol = half * want.abs() + (half + 2 * 2.0 ** -13 + 2.0 ** -16) * size + 2.0 ** -24
+        assert_close(got[row:row + new], want, tol)
+        row += new
