@@ -220,8 +220,11 @@ int clusters_at_once(int device, int threads, int smem, int size) {
 
 // CTAs of a cluster that share the keys of one (sequence, key head) of `units`, where each has one of its own, and no second kernel joins their
 // parts: where the table is so short that each has four tiles at most, and all clusters run at once; two tiles at least, if there are
-// four. 0: the keys of all sequences are cut into ranges. Bf16, 32 heads over 8 of 128 values, cluster against ranges: 1 sequence of 128 keys 7.2 us /
-// 9.6, of 1024 8.7 / 10.1, of 2048 9.9 / 11.4, 4 of 512 9.1 / 11.3; with eight tiles each and more 4 of 4096 16.8 / 15.7, 1 of 32768 46 / 32.
+// four. 0: the keys of all sequences are cut into ranges. Bf16, 32 heads over 8 of 128 values, keys that are not in L2, cluster against ranges: 1 sequence of
+// 128 keys 6.5 us / 8.6, of 1024 8.8 / 10.3, of 2048 (two tiles each) 9.6 / 11.7, of 4096 (four) 11.4 / 13.4, of 5120 (five) 12.6 / 14.8, of 8192 (eight) 15.0 / 16.5, of
+// 16384 22.2 / 21.0, of 32768 36 / 31; 4 of 2048 (four) 13.0 / 17.1, of 8192 28.2 / 32.1; 16 of 512 (four) 12.7 / 17.7. So four is a border on the safe side: with sequences as
+// long as the table clusters win up to some eight tiles. What it keeps out is a table much wider than most of its sequences are long, whose longest one
+// a cluster has to itself (and keys in L2: 1 of 8192 14.0 / 13.7).
 template <typename Active>
 int tokens_cluster(long long units, int max_tiles, Active&& active) {
   if (max_tiles <= 4) return 1;

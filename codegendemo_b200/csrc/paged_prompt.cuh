@@ -10,19 +10,20 @@
 //   warp 2    waits for K and V in the issuer's place, and overwrites values that no row sees with zeros (0 x NaN would not vanish)
 //   warp 3    loads V tiles in the same way; finds the next pair of tiles when the loads of this one end
 //   warps 4-7 softmax of tile 0, warps 8-11 of tile 1, a row a thread
-// Bound by what bounds that kernel, the chain scores - softmax - product of a tile against the other tile's (1.8 us for both tiles' steps), and the
-// power cap: 8192 tokens, 32 heads over 8 of 128 values, bf16, 451 us (1220 TFLOP/s of the pairs seen). A window makes a pair of tiles short,
-// nine steps at a window of 1024: then what comes before the first step and behind the last one counts. So a CTA stays where it is and
-// takes over a CTA that has not been launched yet (cluster launch control) as its next pair: the queries and keys of that one are loaded, and
-// its first scores computed, while this one's rows are finished. 16384 tokens, a window of 1024, 4 sinks: 408 us with a launch a pair, then 340, 314 with
-// first scores ahead and fewer registers in the control warps, 283 with weights against a lagging maximum. In what is left a pair has 16 us of
-// steps and 4.5 of ends: masked steps at both of them, the results' stores, the first step's wait for its scores.
+// Bound by what bounds that kernel, the chain scores - softmax - product of a tile against the other tile's (1.8 us for both tiles' steps), and, where calls
+// follow one another, the power cap: 8192 tokens, 32 heads over 8 of 128 values, bf16, 525 us then, 1047 TFLOP/s of the pairs seen and 75 % of what
+// a library product sustains under the cap; in short bursts, before it sets in, 451, 74 % of such a product's burst. So a quarter is the chain. A window
+// makes a pair of tiles short, nine steps at a window of 1024: then what comes before the first step and behind the last one counts. So a CTA stays where
+// it is and takes over a CTA that has not been launched yet (cluster launch control) as its next pair: the queries and keys of that one are loaded, and
+// its first scores computed, while this one's rows are finished. 16384 tokens, a window of 1024, 4 sinks, short bursts: 408 us with a launch a pair, then 340,
+// 314 with first scores ahead and fewer registers in the control warps, 283 with weights against a lagging maximum; in a row 329 (812 TFLOP/s). In what is
+// left a pair has 16 us of steps and 4.5 of ends: masked steps at both of them, the results' stores, the first step's wait for its scores.
 // kKeySplit: where the tiles do not fill the GPU, the CTAs of a cluster share the keys of one pair, and join their results in shared memory.
 #pragma once
 
 struct PromptArgs {
   CUtensorMap tmQ;       // {d, head, row}, boxes of {64, group, tokens of a tile}
-  CUtensorMap tmK, tmV;  // {d, token of a page, head, page}, boxes of {64, min(page, 128), 1, 1}; 128-byte swizzle all
+  CUtensorMap tmK, tmV;  // {d, token of a page, head, page}, boxes of {64, min(page, 128; with a window 32), 1, 1}; 128-byte swizzle all
   Sequences seq;
   void* o;
   long long o_row, o_head;
@@ -95,7 +96,7 @@ struct AttnPrompt {
 
   // The row of units, as warp 3 walks it. A sequence's pairs of tiles are counted from its last token, whose pair sees the most keys; the first may
   // have fewer tokens. Up to kOrdered sequences: pairs with the most keys come first, over all sequences, so that none of the long ones begins
-  // last (6 prompts of up to 1501 tokens, 14 heads over 2 of 64 values: 37 us in the order of the sequences, 31); a pair's level is the keys of its last
+  // last (6 prompts of up to 1501 tokens, 14 heads over 2 of 64 values: 37 us in the order of the sequences, 31, and 28 with the steps after it); a pair's level is the keys of its last
   // token over a pair's tokens. For a place in the row the warp bisects its level, a lane one or two
   // sequences, whose facts it has read once (read and divided for every step of it, a place took 6 us). Of more sequences that would take longer than a unit, and many short units even out by themselves:
   // the pairs of sequence b take the places from (its first row) / (tokens of a pair) + b on, of which there are enough (some have no
@@ -555,7 +556,7 @@ struct AttnPrompt {
         // passed its own by 8. Weights are up to 2^8 then, which 16 bits hold as exactly as any (P's relative rounding is the same everywhere), and
         // the sums in 32 bits; what is lost is that the largest weight is no longer exactly 1. Error against 64 bits, 2048 tokens, bf16: normal scores 2.02e-3
         // -> 2.05e-3, scores of 4 times that 1.72e-3 -> 1.95e-3, of 16 times 1.44e-3 -> 1.45e-3. A window's nine steps would nearly all rescale O:
-        // 16384 tokens with a window of 1024 303 -> 283 us, 8192 without one 472 -> 451.
+        // 16384 tokens with a window of 1024 303 -> 283 us in short bursts, 8192 without one 472 -> 451.
         float m = -INFINITY;
         uint64_t sum2[2] = {f32x2(0.f, 0.f), f32x2(0.f, 0.f)};
         const int mine = t < x.tiles ? x.steps : 0;

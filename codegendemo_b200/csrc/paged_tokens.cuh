@@ -7,16 +7,18 @@
 // beginning of others. What a range covers whole leaves as a result, a part as
 // unnormalised fp32 rows with their maximum and sum in a workspace; a second kernel, already on the GPU when the first one ends, joins the
 // parts of a (sequence, head) in the order of its keys. No atomics: the order of every sum follows from the lengths.
+// 16 sequences of 16384 keys, 8 key heads of 128 values, bf16: 174 us for 4 rows a key head (6.2 TB/s), 177 for 24, 178 for 32, but 230 for 40 (4.7 TB/s; d = 64
+// 94 for 24, 137 for 40): in the form of up to 64 rows each warp reads all of K and V from shared memory, four times in all.
 //   warp 4     loads: a lane a box of a page (16 keys of K, say), its page's number fetched while the tile before is waited for; tells the others
 //              through the stage which rows and keys it holds
-//   warps 0-3  mma.sync m16n8k16 with 16 rows each. kRowGroups = 1 (up to 16 rows): each warp 16 of a tile's 64 keys; 2 (up to 32): two groups
-//              of rows, 32 keys each; 4 (up to 64): all 64 keys. (tcgen05 needs 128 rows: see kernels/attn_decode.cuh.)
+//   warps 0-3  mma.sync m16n8k16 with 16 rows each. kRowGroups = 1 (up to 16 rows): each warp a quarter of a tile's keys; 2 (up to 32): two groups
+//              of rows, half of the keys each; 4 (up to 64): all of them. (tcgen05 needs 128 rows: see kernels/attn_decode.cuh.)
 // Keys that no row sees, but a box holds (behind the last token of a page, before a window), may be anything: their scores are replaced
 // and their values overwritten with zeros, as 0 x NaN would not vanish.
 #pragma once
 
 struct TokensArgs {
-  CUtensorMap tmK, tmV;  // {d, token of a page, head, page}, boxes of {64, min(page, tile), 1, 1}, 128-byte swizzle
+  CUtensorMap tmK, tmV;  // {d, token of a page, head, page}, boxes of {64, min(page, tile; with a window 16), 1, 1}, 128-byte swizzle
   Sequences seq;
   const void* q;
   void* o;
@@ -567,7 +569,7 @@ __global__ void __launch_bounds__(160, 2) attention_tokens_kernel(const __grid_c
 }
 
 // The parts of the (sequence, key head) whose keys came into CTA blockIdx.x of the kernel above from the one before. A unit of n parts has n - 1 such
-// blocks, which share out its rows (one (sequence, head) of 65536 keys x 32 rows: 97 -> 22 us, in one block before); the 16 warps of a block share out a row's parts, if
+// blocks, which share out its rows (one (sequence, head) of 65536 keys x 32 rows: 97 -> 22 us, in one block before; 19 in a graph); the 16 warps of a block share out a row's parts, if
 // there are not as many rows, eight at a time. (Blocks of 256 threads and 40 registers, small enough to wait beside the kernel above, were slower, 18
 // against 14 us for one sequence of 4097: they take what the next call's CTAs need.)
 template <int kD, bool kBf16>

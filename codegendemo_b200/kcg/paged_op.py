@@ -21,7 +21,8 @@ captured graph follows what they say at its replay. The rows of a sequence are i
 + i. Without ``starts`` every sequence has as many rows as every other. A length of 0 is an empty place of the batch.
 
 All work on CUDA tensors of any device, fp16 or bf16, head dimension 64 or 128, on torch's current stream of that device; results come
-from torch's allocator. No autograd functions: what they serve is inference.
+from torch's allocator. No autograd functions: what they serve is inference. After the first call, calls with right arguments take one step in C++
+(3 to 5 us of host time, where the way through Python takes 19 to 31), results into given places among them.
 """
 import ctypes
 import math
